@@ -462,6 +462,74 @@ int pk_linear_add_rmsnorm(const void* x, int64_t x_row_stride, const void* weigh
                           int64_t out_row_stride, void* residual_out, int64_t residual_out_row_stride,
                           void* workspace, size_t workspace_bytes, pk_stream_t stream);
 
+/*
+ * Pages of the cache: copied, and for sequences that live on the device forked, grown, freed and
+ * compacted. They have the roles of the reference's BlockManager (src/engine/block_manager.py:
+ * 75-246) for a caller whose block tables, lengths and reference counts are on the device (a
+ * captured decode loop, candidates of one prompt); none has a counterpart on the device there.
+ *
+ * Caches: num_layers layers of num_blocks blocks of block_size token rows of row_elems 16-bit
+ * elements. A block is contiguous; block and layer strides are free (multiples of 8 elements,
+ * bases 16-byte aligned), so (L, NB, BS, Hkv, D) tensors and views of them both fit.
+ * Tables: block_tables (num_rows, table_width), row stride block_table_stride; context_lens
+ * (num_rows,) tokens of every row, 0: the row is empty; ref_counts (num_blocks,) the number of
+ * holders of every block, 0: free. A row of length n holds its first ceil(n / block_size) entries.
+ * Entries outside [0, num_blocks) are passed over, lengths beyond the table's width end there.
+ * Blocks are given out lowest number first in the order of the list. No call reads back to the
+ * host; calls on one pool must be ordered (one stream).
+ *
+ * pk_copy_blocks -- for every pair i: the first num_tokens[i] token rows (num_tokens NULL: all) of
+ *   block src_blocks[i] to block dst_blocks[i], K and V, in every layer. Pairs with a block
+ *   outside [0, num_blocks), the same block twice or no tokens are passed over. A target may
+ *   be neither the target nor the source of another pair of the call.
+ * pk_fork_sequences -- row children[i] becomes a copy of row parents[i]: it shares the parent's full
+ *   blocks (one more holder each) and gets a new block with the tokens of a last block that is not
+ *   full, copied in every layer, so both can grow. new_blocks[i] is that block, -1 if none was
+ *   needed, -2 if the pool had none left, -3 if children[i] is no row, is not empty or was listed
+ *   before; with -2 and -3 the child stays as it was. A parent that is no row is an empty one. At
+ *   most 1024 forks a call; workspace: pk_fork_workspace_bytes(num_forks).
+ * pk_extend_sequences -- one more token for every listed row: slot_mapping[i] is its cache slot
+ *   (block * block_size + offset), in a new block where the row's last one is full, and the
+ *   length grows by one. -1 and nothing changed where the row is no row or was listed before, its
+ *   table is full or the pool has no block left. At most 1024 rows a call; num_blocks *
+ *   block_size must fit 31 bits.
+ * pk_free_sequences -- the listed rows' blocks lose a holder, their entries become -1, their lengths 0
+ *   (a row that is listed twice is freed once).
+ * pk_compact_blocks -- with M live blocks, the live ones at M and above move, in order, to the free ones
+ *   below M, K and V in every layer; ref_counts and the entries of block_tables in use follow.
+ *   block_map[b] is block b's new number (-1: free), num_live[0] = M. Tables held elsewhere are
+ *   the caller's to rename by the map. workspace: pk_compact_workspace_bytes(num_blocks).
+ */
+int pk_copy_blocks(void* k_caches, void* v_caches, int64_t k_layer_stride, int64_t v_layer_stride,
+                   int64_t k_block_stride, int64_t v_block_stride, int32_t num_layers,
+                   int32_t num_blocks, int32_t block_size, int32_t row_elems,
+                   const int32_t* src_blocks, const int32_t* dst_blocks, const int32_t* num_tokens,
+                   int32_t num_pairs, pk_stream_t stream);
+size_t pk_fork_workspace_bytes(int32_t num_forks);
+int pk_fork_sequences(void* k_caches, void* v_caches, int64_t k_layer_stride, int64_t v_layer_stride,
+                      int64_t k_block_stride, int64_t v_block_stride, int32_t num_layers,
+                      int32_t num_blocks, int32_t block_size, int32_t row_elems,
+                      int32_t* block_tables, int64_t block_table_stride, int32_t num_rows,
+                      int32_t table_width, int32_t* context_lens, int32_t* ref_counts,
+                      const int32_t* parents, const int32_t* children, int32_t num_forks,
+                      int32_t* new_blocks, void* workspace, size_t workspace_bytes, pk_stream_t stream);
+int pk_extend_sequences(int32_t* block_tables, int64_t block_table_stride, int32_t num_rows,
+                        int32_t table_width, int32_t* context_lens, int32_t* ref_counts,
+                        int32_t num_blocks, int32_t block_size, const int32_t* rows,
+                        int32_t num_listed, int32_t* slot_mapping, pk_stream_t stream);
+int pk_free_sequences(int32_t* block_tables, int64_t block_table_stride, int32_t num_rows,
+                      int32_t table_width, int32_t* context_lens, int32_t* ref_counts,
+                      int32_t num_blocks, int32_t block_size, const int32_t* rows,
+                      int32_t num_listed, pk_stream_t stream);
+size_t pk_compact_workspace_bytes(int32_t num_blocks);
+int pk_compact_blocks(void* k_caches, void* v_caches, int64_t k_layer_stride, int64_t v_layer_stride,
+                      int64_t k_block_stride, int64_t v_block_stride, int32_t num_layers,
+                      int32_t num_blocks, int32_t block_size, int32_t row_elems,
+                      int32_t* block_tables, int64_t block_table_stride, int32_t num_rows,
+                      int32_t table_width, const int32_t* context_lens, int32_t* ref_counts,
+                      int32_t* block_map, int32_t* num_live, void* workspace, size_t workspace_bytes,
+                      pk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

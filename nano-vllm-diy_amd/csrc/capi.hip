@@ -143,11 +143,65 @@ int check_linear(const char* what, const void* x, int64_t x_row_stride, const vo
   return PK_OK;
 }
 
+// ---- pages of the cache ------------------------------------------------------------------
+
+// Caches of the page operators: a block is block_size * row_elems contiguous elements.
+int page_caches(const char* what, pk::PageCaches* c, void* k, void* v, int64_t k_layer, int64_t v_layer,
+                int64_t k_block, int64_t v_block, int32_t layers, int32_t num_blocks, int32_t block_size,
+                int32_t row_elems, int64_t pairs) {
+  if (layers <= 0 || num_blocks <= 0 || block_size <= 0 || row_elems <= 0)
+    return fail(PK_ERR_INVALID_ARG, "%s: layers=%d, num_blocks=%d, block_size=%d, row_elems=%d", what, layers,
+                num_blocks, block_size, row_elems);
+  if (row_elems % 8) return fail(PK_ERR_UNSUPPORTED, "%s: row_elems=%d must be a multiple of 8", what, row_elems);
+  if (!k || !v || !aligned16(k) || !aligned16(v))
+    return fail(PK_ERR_INVALID_ARG, "%s: caches must be non-null and 16-byte aligned", what);
+  const int64_t block = (int64_t)block_size * row_elems;
+  if (block > INT32_MAX) return fail(PK_ERR_UNSUPPORTED, "%s: block of %lld elements", what, (long long)block);
+  if (k_block < block || v_block < block || k_block % 8 || v_block % 8 || k_layer % 8 || v_layer % 8 ||
+      (layers > 1 && (k_layer < block || v_layer < block)))
+    return fail(PK_ERR_INVALID_ARG, "%s: block and layer strides must be >= block_size * row_elems and multiples of 8",
+                what);
+  *c = pk::PageCaches{static_cast<uint4*>(k), static_cast<uint4*>(v), k_layer / 8, v_layer / 8, k_block / 8,
+                      v_block / 8, layers, num_blocks, block_size, row_elems / 8};
+  if (pk::copy_pieces(*c, pairs) > pk::kCopyMaxPieces)
+    return fail(PK_ERR_UNSUPPORTED, "%s: %lld pages of %d layers in one call", what, (long long)pairs, layers);
+  return PK_OK;
+}
+
+int page_tables(const char* what, pk::PageTables* t, int32_t* tables, int64_t stride, int32_t rows, int32_t width,
+                int32_t* lens, int32_t* ref_counts, int32_t num_blocks, int32_t block_size) {
+  if (rows < 0 || width < 0 || num_blocks <= 0 || block_size <= 0)
+    return fail(PK_ERR_INVALID_ARG, "%s: rows=%d, table_width=%d, num_blocks=%d, block_size=%d", what, rows, width,
+                num_blocks, block_size);
+  if (rows > 0 && width > 0 && (!tables || stride < width))
+    return fail(PK_ERR_INVALID_ARG, "%s: block_tables null, or its row stride %lld below the width %d", what,
+                (long long)stride, width);
+  if ((rows > 0 && !lens) || !ref_counts)
+    return fail(PK_ERR_INVALID_ARG, "%s: null context_lens / ref_counts", what);
+  *t = pk::PageTables{tables, stride, rows, width, lens, ref_counts, num_blocks, block_size,
+                      (int32_t)std::min<int64_t>((int64_t)width * block_size, INT32_MAX)};
+  return PK_OK;
+}
+
+int check_list(const char* what, int32_t n) {
+  if (n < 0) return fail(PK_ERR_INVALID_ARG, "%s: %d sequences listed", what, n);
+  if (n > pk::kPoolMaxList)
+    return fail(PK_ERR_UNSUPPORTED, "%s: %d sequences in one call (at most %d)", what, n, pk::kPoolMaxList);
+  return PK_OK;
+}
+
+int check_scratch(const char* what, const void* ws, size_t bytes, size_t need) {
+  if (bytes < need || (need > 0 && !ws))
+    return fail(PK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, bytes, need);
+  if (need > 0 && !aligned16(ws)) return fail(PK_ERR_WORKSPACE, "%s: workspace must be 16-byte aligned", what);
+  return PK_OK;
+}
+
 }  // namespace
 
 extern "C" {
 
-int pk_abi_version(void) { return 10; }
+int pk_abi_version(void) { return 11; }
 
 const char* pk_last_error(void) { return g_last_error.c_str(); }
 
@@ -700,6 +754,110 @@ int pk_linear_add_rmsnorm(const void* x, int64_t x_row_stride, const void* weigh
                                                   out_row_stride, residual_out, residual_out_row_stride,
                                                   workspace, reinterpret_cast<hipStream_t>(stream)),
                     "linear_add_rmsnorm launch");
+}
+
+int pk_copy_blocks(void* k_caches, void* v_caches, int64_t k_layer_stride, int64_t v_layer_stride,
+                   int64_t k_block_stride, int64_t v_block_stride, int32_t num_layers, int32_t num_blocks,
+                   int32_t block_size, int32_t row_elems, const int32_t* src_blocks, const int32_t* dst_blocks,
+                   const int32_t* num_tokens, int32_t num_pairs, pk_stream_t stream) {
+  g_last_error.clear();
+  if (num_pairs < 0) return fail(PK_ERR_INVALID_ARG, "copy_blocks: num_pairs=%d < 0", num_pairs);
+  pk::PageCaches c{};
+  if (int rc = page_caches("copy_blocks", &c, k_caches, v_caches, k_layer_stride, v_layer_stride, k_block_stride,
+                           v_block_stride, num_layers, num_blocks, block_size, row_elems, num_pairs))
+    return rc;
+  if (num_pairs == 0) return PK_OK;
+  if (!src_blocks || !dst_blocks) return fail(PK_ERR_INVALID_ARG, "copy_blocks: null src_blocks / dst_blocks");
+  return hip_status(pk::launch_copy_blocks(c, src_blocks, dst_blocks, num_tokens, num_pairs,
+                                           reinterpret_cast<hipStream_t>(stream)),
+                    "copy_blocks launch");
+}
+
+size_t pk_fork_workspace_bytes(int32_t num_forks) { return num_forks <= 0 ? 0 : (size_t)num_forks * sizeof(int4); }
+
+int pk_fork_sequences(void* k_caches, void* v_caches, int64_t k_layer_stride, int64_t v_layer_stride,
+                      int64_t k_block_stride, int64_t v_block_stride, int32_t num_layers, int32_t num_blocks,
+                      int32_t block_size, int32_t row_elems, int32_t* block_tables, int64_t block_table_stride,
+                      int32_t num_rows, int32_t table_width, int32_t* context_lens, int32_t* ref_counts,
+                      const int32_t* parents, const int32_t* children, int32_t num_forks, int32_t* new_blocks,
+                      void* workspace, size_t workspace_bytes, pk_stream_t stream) {
+  g_last_error.clear();
+  if (int rc = check_list("fork_sequences", num_forks)) return rc;
+  pk::PageCaches c{};
+  pk::PageTables t{};
+  if (int rc = page_caches("fork_sequences", &c, k_caches, v_caches, k_layer_stride, v_layer_stride, k_block_stride,
+                           v_block_stride, num_layers, num_blocks, block_size, row_elems, num_forks))
+    return rc;
+  if (int rc = page_tables("fork_sequences", &t, block_tables, block_table_stride, num_rows, table_width,
+                           context_lens, ref_counts, num_blocks, block_size))
+    return rc;
+  if (num_forks == 0) return PK_OK;
+  if (!parents || !children || !new_blocks)
+    return fail(PK_ERR_INVALID_ARG, "fork_sequences: null parents / children / new_blocks");
+  if (int rc = check_scratch("fork_sequences", workspace, workspace_bytes, pk_fork_workspace_bytes(num_forks)))
+    return rc;
+  return hip_status(pk::launch_fork_sequences(t, c, parents, children, num_forks, new_blocks, workspace,
+                                              reinterpret_cast<hipStream_t>(stream)),
+                    "fork_sequences launch");
+}
+
+int pk_extend_sequences(int32_t* block_tables, int64_t block_table_stride, int32_t num_rows, int32_t table_width,
+                        int32_t* context_lens, int32_t* ref_counts, int32_t num_blocks, int32_t block_size,
+                        const int32_t* rows, int32_t num_listed, int32_t* slot_mapping, pk_stream_t stream) {
+  g_last_error.clear();
+  if (int rc = check_list("extend_sequences", num_listed)) return rc;
+  pk::PageTables t{};
+  if (int rc = page_tables("extend_sequences", &t, block_tables, block_table_stride, num_rows, table_width,
+                           context_lens, ref_counts, num_blocks, block_size))
+    return rc;
+  if ((int64_t)num_blocks * block_size > INT32_MAX)
+    return fail(PK_ERR_UNSUPPORTED, "extend_sequences: %lld slots do not fit 32-bit slot numbers",
+                (long long)num_blocks * block_size);
+  if (num_listed == 0) return PK_OK;
+  if (!rows || !slot_mapping) return fail(PK_ERR_INVALID_ARG, "extend_sequences: null rows / slot_mapping");
+  return hip_status(pk::launch_extend_sequences(t, rows, num_listed, slot_mapping,
+                                                reinterpret_cast<hipStream_t>(stream)),
+                    "extend_sequences launch");
+}
+
+int pk_free_sequences(int32_t* block_tables, int64_t block_table_stride, int32_t num_rows, int32_t table_width,
+                      int32_t* context_lens, int32_t* ref_counts, int32_t num_blocks, int32_t block_size,
+                      const int32_t* rows, int32_t num_listed, pk_stream_t stream) {
+  g_last_error.clear();
+  if (num_listed < 0) return fail(PK_ERR_INVALID_ARG, "free_sequences: %d sequences listed", num_listed);
+  pk::PageTables t{};
+  if (int rc = page_tables("free_sequences", &t, block_tables, block_table_stride, num_rows, table_width,
+                           context_lens, ref_counts, num_blocks, block_size))
+    return rc;
+  if (num_listed == 0) return PK_OK;
+  if (!rows) return fail(PK_ERR_INVALID_ARG, "free_sequences: null rows");
+  return hip_status(pk::launch_free_sequences(t, rows, num_listed, reinterpret_cast<hipStream_t>(stream)),
+                    "free_sequences launch");
+}
+
+size_t pk_compact_workspace_bytes(int32_t num_blocks) { return pk::compact_workspace_bytes(num_blocks); }
+
+int pk_compact_blocks(void* k_caches, void* v_caches, int64_t k_layer_stride, int64_t v_layer_stride,
+                      int64_t k_block_stride, int64_t v_block_stride, int32_t num_layers, int32_t num_blocks,
+                      int32_t block_size, int32_t row_elems, int32_t* block_tables, int64_t block_table_stride,
+                      int32_t num_rows, int32_t table_width, const int32_t* context_lens, int32_t* ref_counts,
+                      int32_t* block_map, int32_t* num_live, void* workspace, size_t workspace_bytes,
+                      pk_stream_t stream) {
+  g_last_error.clear();
+  pk::PageCaches c{};
+  pk::PageTables t{};
+  if (int rc = page_caches("compact_blocks", &c, k_caches, v_caches, k_layer_stride, v_layer_stride, k_block_stride,
+                           v_block_stride, num_layers, num_blocks, block_size, row_elems, num_blocks))
+    return rc;
+  if (int rc = page_tables("compact_blocks", &t, block_tables, block_table_stride, num_rows, table_width,
+                           const_cast<int32_t*>(context_lens), ref_counts, num_blocks, block_size))
+    return rc;
+  if (!block_map || !num_live) return fail(PK_ERR_INVALID_ARG, "compact_blocks: null block_map / num_live");
+  if (int rc = check_scratch("compact_blocks", workspace, workspace_bytes, pk_compact_workspace_bytes(num_blocks)))
+    return rc;
+  return hip_status(pk::launch_compact_blocks(t, c, block_map, num_live, workspace,
+                                              reinterpret_cast<hipStream_t>(stream)),
+                    "compact_blocks launch");
 }
 
 }  // extern "C"

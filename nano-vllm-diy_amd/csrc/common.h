@@ -260,6 +260,41 @@ hipError_t launch_linear_add_rmsnorm(const void* x, int64_t x_stride, const void
                                      int64_t res_stride, const void* norm_weight, float eps, void* out,
                                      int64_t out_stride, void* residual_out, int64_t res_out_stride, void* ws,
                                      hipStream_t stream);
+// Pages of the cache (kv_pages.hip). Strides of the caches in 16-byte vectors.
+struct PageCaches {
+  uint4* k;
+  uint4* v;
+  int64_t k_layer_vec, v_layer_vec;
+  int64_t k_block_vec, v_block_vec;
+  int32_t layers;
+  int32_t num_blocks;
+  int32_t block_size;
+  int32_t row_vec;               // vectors of one token row
+};
+struct PageTables {
+  int32_t* tables;               // (rows, width)
+  int64_t stride;
+  int32_t rows, width;
+  int32_t* lens;                 // tokens of every row
+  int32_t* ref_counts;           // holders of every block, 0: free
+  int32_t num_blocks;
+  int32_t block_size;
+  int32_t max_len;               // width * block_size, or INT32_MAX
+};
+constexpr int kPoolMaxList = 1024;  // sequences of one fork / extend call (one work-group decides)
+constexpr int64_t kCopyMaxPieces = 0x7ffff000;  // pieces of a copy are counted in 32 bits
+int64_t copy_pieces(const PageCaches& c, int64_t pairs);
+hipError_t launch_copy_blocks(const PageCaches& c, const int32_t* src, const int32_t* dst, const int32_t* tokens,
+                              int32_t num_pairs, hipStream_t stream);
+hipError_t launch_fork_sequences(const PageTables& t, const PageCaches& c, const int32_t* parents,
+                                 const int32_t* children, int32_t n, int32_t* new_blocks, void* workspace,
+                                 hipStream_t stream);
+hipError_t launch_extend_sequences(const PageTables& t, const int32_t* rows, int32_t n, int32_t* slots,
+                                   hipStream_t stream);
+hipError_t launch_free_sequences(const PageTables& t, const int32_t* rows, int32_t n, hipStream_t stream);
+size_t compact_workspace_bytes(int32_t num_blocks);
+hipError_t launch_compact_blocks(const PageTables& t, const PageCaches& c, int32_t* block_map, int32_t* num_live,
+                                 void* workspace, hipStream_t stream);
 hipError_t launch_lm_head_greedy(const void* x, int64_t x_stride, const int32_t* cu_rows,
                                  const void* w, int64_t w_stride, int32_t rows, int32_t vocab,
                                  int32_t k_dim, unsigned long long* keys, int32_t* ids,

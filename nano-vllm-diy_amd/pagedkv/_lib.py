@@ -125,9 +125,33 @@ SIGNATURES = {
         _c_void_p, _i64, _c_void_p, ctypes.c_float,  # residual, its row stride, norm weight, eps
         _c_void_p, _i64, _c_void_p, _i64,   # out, its row stride, residual_out, its row stride
         _c_void_p, _size_t, _c_void_p]),    # workspace, workspace_bytes, stream
+    "pk_copy_blocks": (ctypes.c_int, [
+        _c_void_p, _c_void_p,               # k_caches, v_caches
+        _i64, _i64, _i64, _i64,             # k/v layer strides, k/v block strides
+        _i32, _i32, _i32, _i32,             # num_layers, num_blocks, block_size, row_elems
+        _c_void_p, _c_void_p, _c_void_p,    # src_blocks, dst_blocks, num_tokens
+        _i32, _c_void_p]),                  # num_pairs, stream
+    "pk_fork_workspace_bytes": (_size_t, [_i32]),
+    "pk_fork_sequences": (ctypes.c_int, [
+        _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32,
+        _c_void_p, _i64, _i32, _i32,        # block_tables, its row stride, num_rows, table_width
+        _c_void_p, _c_void_p,               # context_lens, ref_counts
+        _c_void_p, _c_void_p, _i32, _c_void_p,  # parents, children, num_forks, new_blocks
+        _c_void_p, _size_t, _c_void_p]),    # workspace, workspace_bytes, stream
+    "pk_extend_sequences": (ctypes.c_int, [
+        _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _i32, _i32,
+        _c_void_p, _i32, _c_void_p, _c_void_p]),  # rows, num_listed, slot_mapping, stream
+    "pk_free_sequences": (ctypes.c_int, [
+        _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i32, _c_void_p]),
+    "pk_compact_workspace_bytes": (_size_t, [_i32]),
+    "pk_compact_blocks": (ctypes.c_int, [
+        _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32,
+        _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p,
+        _c_void_p, _c_void_p,               # block_map, num_live
+        _c_void_p, _size_t, _c_void_p]),    # workspace, workspace_bytes, stream
 }
 
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
