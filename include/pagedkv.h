@@ -463,6 +463,43 @@ int pk_linear_add_rmsnorm(const void* x, int64_t x_row_stride, const void* weigh
                           void* workspace, size_t workspace_bytes, pk_stream_t stream);
 
 /*
+ * Low-rank adapters of many requests beside a shared projection (no counterpart in the reference,
+ * whose layers have one set of weights, src/layers/linear.py:74-75, :169-170). Token row m has
+ * the adapter a = adapter_ids[m] of its own, any value outside [0, num_adapters) meaning none:
+ *   t[m, i]   = scales[a] * sum_k x[m, k] lora_a[a, i, k]         i < num_slices * rank
+ *   out[m, c] = bf16(base[m, c] + sum_j t[m, q rank + j] lora_b[a, c, j]),   j < rank
+ * with c in slice q: a merged projection (the reference's MergedColumnParallelLinear and qkv layers,
+ * linear.py:77-143, :145-228) has slices[0..num_slices) output columns for each of the layers
+ * merged in it, which have their own rows of lora_a and share lora_b's layout. Sums are fp32,
+ * t is not rounded, the output is rounded once. scales (num_adapters,) fp32, NULL: 1. slices is a
+ * HOST array (read before the call returns); NULL with num_slices 1: one slice of n_out.
+ * x (rows, k), lora_a (num_adapters, num_slices * rank, k), lora_b (num_adapters, n_out, rank) bf16;
+ * adapters of smaller rank are padded with zeros. k and rank multiples of 8, rank up to 128, up
+ * to 4 slices of multiples of 32 columns; pointers 16-byte aligned, strides multiples of 8. A
+ * row's result does not depend on the other rows' values.
+ *
+ * pk_lora_linear -- base = x W^T in fp32 (a decode step's projection, pk_linear's weight and limits:
+ *   at most 128 rows, k a multiple of 256); out must not overlap x.
+ * pk_lora_add -- base = y (rows, n_out) bf16, the output of a projection computed elsewhere. out may be
+ *   y (in place, rows without an adapter are then not written), or must not overlap y or x. Up to
+ *   2^22 rows; above 512 rows up to 8191 adapters.
+ */
+size_t pk_lora_linear_workspace_bytes(int32_t rows, int32_t n_out, int32_t k, int32_t rank, int32_t num_slices);
+int pk_lora_linear(const void* x, int64_t x_row_stride, const void* weight, int64_t weight_row_stride,
+                   int32_t rows, int32_t n_out, int32_t k, const void* lora_a, int64_t a_adapter_stride,
+                   int64_t a_row_stride, const void* lora_b, int64_t b_adapter_stride, int64_t b_row_stride,
+                   int32_t num_adapters, int32_t rank, const int32_t* adapter_ids, const float* scales,
+                   const int32_t* slices, int32_t num_slices, void* out, int64_t out_row_stride,
+                   void* workspace, size_t workspace_bytes, pk_stream_t stream);
+size_t pk_lora_add_workspace_bytes(int32_t rows, int32_t rank, int32_t num_slices, int32_t num_adapters);
+int pk_lora_add(const void* y, int64_t y_row_stride, const void* x, int64_t x_row_stride, int32_t rows,
+                int32_t n_out, int32_t k, const void* lora_a, int64_t a_adapter_stride, int64_t a_row_stride,
+                const void* lora_b, int64_t b_adapter_stride, int64_t b_row_stride, int32_t num_adapters,
+                int32_t rank, const int32_t* adapter_ids, const float* scales, const int32_t* slices,
+                int32_t num_slices, void* out, int64_t out_row_stride, void* workspace,
+                size_t workspace_bytes, pk_stream_t stream);
+
+/*
  * Pages of the cache: copied, and for sequences that live on the device forked, grown, freed and
  * compacted. They have the roles of the reference's BlockManager (src/engine/block_manager.py:
  * 75-246) for a caller whose block tables, lengths and reference counts are on the device (a

@@ -197,6 +197,65 @@ int check_scratch(const char* what, const void* ws, size_t bytes, size_t need) {
   return PK_OK;
 }
 
+// ---- adapters beside a projection ---------------------------------------------------------
+
+int lora_args(const char* what, pk::LoraArgs* p, const void* x, int64_t x_row_stride, int32_t rows, int32_t n_out,
+              int32_t k, const void* lora_a, int64_t a_adapter_stride, int64_t a_row_stride, const void* lora_b,
+              int64_t b_adapter_stride, int64_t b_row_stride, int32_t num_adapters, int32_t rank,
+              const int32_t* adapter_ids, const float* scales, const int32_t* slices, int32_t num_slices, void* out,
+              int64_t out_row_stride) {
+  if (rows < 0 || n_out <= 0 || k <= 0 || num_adapters < 0)
+    return fail(PK_ERR_INVALID_ARG, "%s: rows=%d, n_out=%d, k=%d, num_adapters=%d", what, rows, n_out, k, num_adapters);
+  if (k % 8) return fail(PK_ERR_UNSUPPORTED, "%s: k=%d must be a multiple of 8", what, k);
+  if (rank <= 0 || rank % 8 || rank > pk::kLoraMaxRank)
+    return fail(PK_ERR_UNSUPPORTED, "%s: rank=%d must be a multiple of 8 up to %d", what, rank, pk::kLoraMaxRank);
+  if (num_slices < 1 || num_slices > pk::kLoraMaxSlices || (num_slices > 1 && !slices))
+    return fail(PK_ERR_INVALID_ARG, "%s: num_slices=%d (1 to %d, with their widths)", what, num_slices,
+                pk::kLoraMaxSlices);
+  *p = pk::LoraArgs{};
+  int64_t sum = 0;
+  for (int q = 0; q < num_slices; ++q) {
+    const int32_t w = slices ? slices[q] : n_out;
+    if (w <= 0) return fail(PK_ERR_INVALID_ARG, "%s: slice %d has %d columns", what, q, w);
+    if (w % 32) return fail(PK_ERR_UNSUPPORTED, "%s: slice of %d columns, must be a multiple of 32", what, w);
+    sum += w;
+    if (sum > n_out) break;
+    p->slice_begin[q + 1] = (int32_t)sum;
+  }
+  if (sum != n_out) return fail(PK_ERR_INVALID_ARG, "%s: the slices' widths do not add up to n_out=%d", what, n_out);
+  if (rows > 0) {
+    if (!x || !out || !adapter_ids || (num_adapters > 0 && (!lora_a || !lora_b)))
+      return fail(PK_ERR_INVALID_ARG, "%s: null pointer argument", what);
+    if (!aligned16(x) || !aligned16(out) || (num_adapters > 0 && (!aligned16(lora_a) || !aligned16(lora_b))))
+      return fail(PK_ERR_INVALID_ARG, "%s: x, lora_a, lora_b and out must be 16-byte aligned", what);
+    if (x_row_stride < k || x_row_stride % 8 || out_row_stride < n_out || out_row_stride % 8)
+      return fail(PK_ERR_INVALID_ARG, "%s: row strides must cover a row and be multiples of 8", what);
+    if (num_adapters > 0 && (a_row_stride < k || a_row_stride % 8 || b_row_stride < rank || b_row_stride % 8 ||
+                             a_adapter_stride < 0 || a_adapter_stride % 8 || b_adapter_stride < 0 ||
+                             b_adapter_stride % 8))
+      return fail(PK_ERR_INVALID_ARG, "%s: adapter strides must cover a row and be multiples of 8", what);
+  }
+  p->x = static_cast<const uint16_t*>(x);
+  p->x_stride = x_row_stride;
+  p->rows = rows;
+  p->n_out = n_out;
+  p->k = k;
+  p->a = static_cast<const uint16_t*>(lora_a);
+  p->a_adapter = a_adapter_stride;
+  p->a_row = a_row_stride;
+  p->b = static_cast<const uint16_t*>(lora_b);
+  p->b_adapter = b_adapter_stride;
+  p->b_row = b_row_stride;
+  p->num_adapters = num_adapters;
+  p->rank = rank;
+  p->ids = adapter_ids;
+  p->scales = scales;
+  p->num_slices = num_slices;
+  p->out = static_cast<uint16_t*>(out);
+  p->out_stride = out_row_stride;
+  return PK_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -754,6 +813,75 @@ int pk_linear_add_rmsnorm(const void* x, int64_t x_row_stride, const void* weigh
                                                   out_row_stride, residual_out, residual_out_row_stride,
                                                   workspace, reinterpret_cast<hipStream_t>(stream)),
                     "linear_add_rmsnorm launch");
+}
+
+size_t pk_lora_linear_workspace_bytes(int32_t rows, int32_t n_out, int32_t k, int32_t rank, int32_t num_slices) {
+  if (rows <= 0 || rows > pk::kLinearMaxRows || n_out <= 0 || n_out % 32 || k <= 0 || k % 256 || rank <= 0 ||
+      rank > pk::kLoraMaxRank || num_slices <= 0 || num_slices > pk::kLoraMaxSlices)
+    return 0;
+  pk::LoraArgs p{};
+  p.rows = rows, p.n_out = n_out, p.k = k, p.rank = rank, p.num_slices = num_slices;
+  return pk::lora_linear_workspace_bytes(p);
+}
+
+int pk_lora_linear(const void* x, int64_t x_row_stride, const void* weight, int64_t weight_row_stride, int32_t rows,
+                   int32_t n_out, int32_t k, const void* lora_a, int64_t a_adapter_stride, int64_t a_row_stride,
+                   const void* lora_b, int64_t b_adapter_stride, int64_t b_row_stride, int32_t num_adapters,
+                   int32_t rank, const int32_t* adapter_ids, const float* scales, const int32_t* slices,
+                   int32_t num_slices, void* out, int64_t out_row_stride, void* workspace, size_t workspace_bytes,
+                   pk_stream_t stream) {
+  g_last_error.clear();
+  pk::LoraArgs p;
+  if (int rc = lora_args("lora_linear", &p, x, x_row_stride, rows, n_out, k, lora_a, a_adapter_stride, a_row_stride,
+                         lora_b, b_adapter_stride, b_row_stride, num_adapters, rank, adapter_ids, scales, slices,
+                         num_slices, out, out_row_stride))
+    return rc;
+  if (rows == 0) return PK_OK;
+  const size_t need = pk_lora_linear_workspace_bytes(rows, n_out, k, rank, num_slices);
+  if (int rc = check_linear("lora_linear", x, x_row_stride, weight, weight_row_stride, rows, n_out, k, out,
+                            out_row_stride, workspace, workspace_bytes, need))
+    return rc;
+  return hip_status(pk::launch_lora_linear(p, weight, weight_row_stride, workspace,
+                                           reinterpret_cast<hipStream_t>(stream)),
+                    "lora_linear launch");
+}
+
+size_t pk_lora_add_workspace_bytes(int32_t rows, int32_t rank, int32_t num_slices, int32_t num_adapters) {
+  if (rows <= 0 || rank <= 0 || rank > pk::kLoraMaxRank || num_slices <= 0 || num_slices > pk::kLoraMaxSlices ||
+      num_adapters < 0)
+    return 0;
+  pk::LoraArgs p{};
+  p.rows = rows, p.rank = rank, p.num_slices = num_slices, p.num_adapters = num_adapters;
+  return pk::lora_add_workspace_bytes(p);
+}
+
+int pk_lora_add(const void* y, int64_t y_row_stride, const void* x, int64_t x_row_stride, int32_t rows, int32_t n_out,
+                int32_t k, const void* lora_a, int64_t a_adapter_stride, int64_t a_row_stride, const void* lora_b,
+                int64_t b_adapter_stride, int64_t b_row_stride, int32_t num_adapters, int32_t rank,
+                const int32_t* adapter_ids, const float* scales, const int32_t* slices, int32_t num_slices, void* out,
+                int64_t out_row_stride, void* workspace, size_t workspace_bytes, pk_stream_t stream) {
+  g_last_error.clear();
+  pk::LoraArgs p;
+  if (int rc = lora_args("lora_add", &p, x, x_row_stride, rows, n_out, k, lora_a, a_adapter_stride, a_row_stride,
+                         lora_b, b_adapter_stride, b_row_stride, num_adapters, rank, adapter_ids, scales, slices,
+                         num_slices, out, out_row_stride))
+    return rc;
+  if (rows == 0) return PK_OK;
+  if (!y || !aligned16(y) || y_row_stride < n_out || y_row_stride % 8)
+    return fail(PK_ERR_INVALID_ARG, "lora_add: y null, not 16-byte aligned, or its row stride no multiple of 8 >= n_out");
+  if (y == out && y_row_stride != out_row_stride)
+    return fail(PK_ERR_INVALID_ARG, "lora_add: out may be y only with y's row stride");
+  if (rows > pk::kLoraSmallRows && num_adapters > pk::kLoraMaxAdapters)
+    return fail(PK_ERR_UNSUPPORTED, "lora_add: %d adapters for more than %d rows (at most %d)", num_adapters,
+                pk::kLoraSmallRows, pk::kLoraMaxAdapters);
+  if (rows > (1 << 22) || n_out > (1 << 20))
+    return fail(PK_ERR_UNSUPPORTED, "lora_add: rows=%d, n_out=%d (at most 2^22 and 2^20)", rows, n_out);
+  if (int rc = check_scratch("lora_add", workspace, workspace_bytes,
+                             pk_lora_add_workspace_bytes(rows, rank, num_slices, num_adapters)))
+    return rc;
+  p.y = static_cast<const uint16_t*>(y);
+  p.y_stride = y_row_stride;
+  return hip_status(pk::launch_lora_add(p, workspace, reinterpret_cast<hipStream_t>(stream)), "lora_add launch");
 }
 
 int pk_copy_blocks(void* k_caches, void* v_caches, int64_t k_layer_stride, int64_t v_layer_stride,

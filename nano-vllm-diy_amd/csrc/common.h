@@ -260,6 +260,41 @@ hipError_t launch_linear_add_rmsnorm(const void* x, int64_t x_stride, const void
                                      int64_t res_stride, const void* norm_weight, float eps, void* out,
                                      int64_t out_stride, void* residual_out, int64_t res_out_stride, void* ws,
                                      hipStream_t stream);
+// Low-rank adapters beside a projection (lora.hip).
+constexpr int kLoraMaxSlices = 4;
+constexpr int kLoraMaxRank = 128;
+constexpr int kLoraMaxAdapters = 8191;  // of an addition to more than kLoraSmallRows rows: its sort's LDS
+constexpr int kLoraSmallRows = 512;
+struct LoraArgs {
+  const uint16_t* x;
+  int64_t x_stride;
+  int32_t rows, n_out, k;
+  const uint16_t* a;             // (num_adapters, num_slices * rank, k)
+  int64_t a_adapter, a_row;
+  const uint16_t* b;             // (num_adapters, n_out, rank)
+  int64_t b_adapter, b_row;
+  int32_t num_adapters, rank;
+  const int32_t* ids;            // adapter of every row
+  const float* scales;           // of every adapter, or nullptr: 1
+  int32_t num_slices;
+  int32_t slice_begin[kLoraMaxSlices + 1];  // output columns of the slices
+  const uint16_t* y;             // the sums' base (lora_add)
+  int64_t y_stride;
+  uint16_t* out;
+  int64_t out_stride;
+  // set by the launches
+  float* t;                      // [rows][num_slices * rank], scaled
+  float* part;                   // [ks][rows][n_out] partial sums of the projection (lora_linear)
+  int32_t ks;
+  int32_t group_cols, col_groups;  // columns of an expand work-group; groups over all slices
+  int4* tiles;                   // sorted tiles: (adapter or -1, first position, rows, 0)
+  int32_t* num_tiles;
+  int32_t* perm;                 // row at every sorted position
+};
+size_t lora_linear_workspace_bytes(const LoraArgs& p);
+size_t lora_add_workspace_bytes(const LoraArgs& p);
+hipError_t launch_lora_linear(const LoraArgs& p, const void* w, int64_t w_stride, void* ws, hipStream_t stream);
+hipError_t launch_lora_add(const LoraArgs& p, void* ws, hipStream_t stream);
 // Pages of the cache (kv_pages.hip). Strides of the caches in 16-byte vectors.
 struct PageCaches {
   uint4* k;

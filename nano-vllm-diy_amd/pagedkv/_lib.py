@@ -125,6 +125,20 @@ SIGNATURES = {
         _c_void_p, _i64, _c_void_p, ctypes.c_float,  # residual, its row stride, norm weight, eps
         _c_void_p, _i64, _c_void_p, _i64,   # out, its row stride, residual_out, its row stride
         _c_void_p, _size_t, _c_void_p]),    # workspace, workspace_bytes, stream
+    "pk_lora_linear_workspace_bytes": (_size_t, [_i32, _i32, _i32, _i32, _i32]),
+    "pk_lora_linear": (ctypes.c_int, [
+        _c_void_p, _i64, _c_void_p, _i64,   # x, its row stride, weight, its row stride
+        _i32, _i32, _i32,                   # rows, n_out, k
+        _c_void_p, _i64, _i64,              # lora_a, its adapter and row strides
+        _c_void_p, _i64, _i64,              # lora_b, its adapter and row strides
+        _i32, _i32, _c_void_p, _c_void_p,   # num_adapters, rank, adapter_ids, scales
+        ctypes.POINTER(_i32), _i32,         # slices (host), num_slices
+        _c_void_p, _i64, _c_void_p, _size_t, _c_void_p]),  # out, its row stride, workspace, its bytes, stream
+    "pk_lora_add_workspace_bytes": (_size_t, [_i32, _i32, _i32, _i32]),
+    "pk_lora_add": (ctypes.c_int, [
+        _c_void_p, _i64, _c_void_p, _i64,   # y, its row stride, x, its row stride
+        _i32, _i32, _i32, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i32, _i32, _c_void_p, _c_void_p,
+        ctypes.POINTER(_i32), _i32, _c_void_p, _i64, _c_void_p, _size_t, _c_void_p]),
     "pk_copy_blocks": (ctypes.c_int, [
         _c_void_p, _c_void_p,               # k_caches, v_caches
         _i64, _i64, _i64, _i64,             # k/v layer strides, k/v block strides
