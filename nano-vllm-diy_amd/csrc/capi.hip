@@ -901,7 +901,7 @@ int pk_copy_blocks(void* k_caches, void* v_caches, int64_t k_layer_stride, int64
                     "copy_blocks launch");
 }
 
-size_t pk_fork_workspace_bytes(int32_t num_forks) { return num_forks <= 0 ? 0 : (size_t)num_forks * sizeof(int4); }
+size_t pk_fork_workspace_bytes(int32_t num_forks) { return pk::fork_workspace_bytes(num_forks); }
 
 int pk_fork_sequences(void* k_caches, void* v_caches, int64_t k_layer_stride, int64_t v_layer_stride,
                       int64_t k_block_stride, int64_t v_block_stride, int32_t num_layers, int32_t num_blocks,

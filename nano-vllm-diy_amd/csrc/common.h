@@ -263,8 +263,11 @@ hipError_t launch_linear_add_rmsnorm(const void* x, int64_t x_stride, const void
 // Low-rank adapters beside a projection (lora.hip).
 constexpr int kLoraMaxSlices = 4;
 constexpr int kLoraMaxRank = 128;
-constexpr int kLoraMaxAdapters = 8191;  // of an addition to more than kLoraSmallRows rows: its sort's LDS
-constexpr int kLoraSmallRows = 512;
+constexpr int kLoraMaxAdapters = 4095;  // of an addition to more than kLoraSmallRows rows: its sort's LDS
+#ifndef PK_SMALL
+#define PK_SMALL 512
+#endif
+constexpr int kLoraSmallRows = PK_SMALL;
 struct LoraArgs {
   const uint16_t* x;
   int64_t x_stride;
@@ -286,10 +289,11 @@ struct LoraArgs {
   float* t;                      // [rows][num_slices * rank], scaled
   float* part;                   // [ks][rows][n_out] partial sums of the projection (lora_linear)
   int32_t ks;
-  int32_t group_cols, col_groups;  // columns of an expand work-group; groups over all slices
-  int4* tiles;                   // sorted tiles: (adapter or -1, first position, rows, 0)
-  int32_t* num_tiles;
-  int32_t* perm;                 // row at every sorted position
+  int32_t col_groups;            // column groups of an expand launch over all slices
+  int32_t max_tiles;
+  int2* tiles;                   // sorted tiles of 64 rows: (adapter or -1, rows)
+  int32_t* perm;                 // [tile][64] their rows
+  int32_t* place;                // of every row among the rows of its adapter
 };
 size_t lora_linear_workspace_bytes(const LoraArgs& p);
 size_t lora_add_workspace_bytes(const LoraArgs& p);
@@ -321,6 +325,7 @@ constexpr int64_t kCopyMaxPieces = 0x7ffff000;  // pieces of a copy are counted 
 int64_t copy_pieces(const PageCaches& c, int64_t pairs);
 hipError_t launch_copy_blocks(const PageCaches& c, const int32_t* src, const int32_t* dst, const int32_t* tokens,
                               int32_t num_pairs, hipStream_t stream);
+size_t fork_workspace_bytes(int32_t num_forks);
 hipError_t launch_fork_sequences(const PageTables& t, const PageCaches& c, const int32_t* parents,
                                  const int32_t* children, int32_t n, int32_t* new_blocks, void* workspace,
                                  hipStream_t stream);

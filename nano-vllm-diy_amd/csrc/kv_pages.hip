@@ -27,13 +27,16 @@ struct CopyList {
   const int32_t* src;
   const int32_t* dst;
   const int32_t* tokens;     // nullptr: whole pages
-  const int4* plan;          // forks: (src, dst, tokens, length); dst < 0: nothing to copy
-  const int32_t* num_pairs;  // on the device (compaction), or nullptr: max_pairs
+  const int4* heads;         // forks: (src, tokens, first target in dst, -) of every run of targets; the entry
+                             // after the last one has their end
+  const int32_t* num_pairs;  // on the device (forks, compaction), or nullptr: max_pairs
   int32_t max_pairs;
 };
 
 // Pieces of 16 KiB of one page of one layer's K or V, dealt to the work-groups round robin, all
-// loads of a piece before its stores. A copy is bound by HBM: each byte is read and written once.
+// loads of a piece before its stores; a fork's piece is read once for all targets in a row that
+// want it. A copy is bound by HBM: each byte is read once and written once.
+template <bool kHeads>
 __device__ __forceinline__ void copy_pages(const PageCaches& c, const CopyList& list, int32_t group,
                                            int32_t groups) {
   const int32_t pairs = list.num_pairs ? min(*list.num_pairs, list.max_pairs) : list.max_pairs;
@@ -47,38 +50,40 @@ __device__ __forceinline__ void copy_pages(const PageCaches& c, const CopyList& 
     rem -= layer * 2 * pieces;
     const bool is_v = rem >= pieces;
     const int32_t piece = is_v ? rem - pieces : rem;
-    int32_t src, dst, tokens = c.block_size;
-    if (list.plan) {
-      const int4 p = list.plan[i];
-      src = p.x; dst = p.y; tokens = p.z;
+    int32_t src, tokens = c.block_size, first = i, last = i + 1;
+    if constexpr (kHeads) {
+      const int4 head = list.heads[i];
+      src = head.x;
+      tokens = head.y;
+      first = head.z;
+      last = list.heads[i + 1].z;
     } else {
       src = list.src[i];
-      dst = list.dst[i];
       if (list.tokens) tokens = min(list.tokens[i], c.block_size);
     }
     const int32_t n = tokens * c.row_vec;
     const int32_t base = piece * kCopyVecs + (int32_t)threadIdx.x;
-    if (src < 0 || src >= c.num_blocks || dst < 0 || dst >= c.num_blocks || src == dst || piece * kCopyVecs >= n)
-      continue;
-    uint4* cache = is_v ? c.v : c.k;
-    const int64_t at = layer * (is_v ? c.v_layer_vec : c.k_layer_vec);
+    if (src < 0 || src >= c.num_blocks || piece * kCopyVecs >= n) continue;
+    u32x4* cache = reinterpret_cast<u32x4*>(is_v ? c.v : c.k) + layer * (is_v ? c.v_layer_vec : c.k_layer_vec);
     const int64_t block_vec = is_v ? c.v_block_vec : c.k_block_vec;
-    const uint4* from = cache + at + src * block_vec;
-    uint4* to = cache + at + dst * block_vec;
-    if (piece * kCopyVecs + kCopyVecs <= n) {
-      uint4 v[kCopyUnroll];
+    const u32x4* from = cache + src * block_vec;
+    u32x4 v[kCopyUnroll];
 #pragma unroll
-      for (int j = 0; j < kCopyUnroll; ++j) v[j] = from[base + j * kCopyThreads];
+    for (int j = 0; j < kCopyUnroll; ++j)
+      if (base + j * kCopyThreads < n) v[j] = from[base + j * kCopyThreads];
+    for (int32_t t = first; t < last; ++t) {
+      const int32_t dst = list.dst[t];
+      if (dst < 0 || dst >= c.num_blocks || src == dst) continue;
+      u32x4* to = cache + dst * block_vec;
 #pragma unroll
-      for (int j = 0; j < kCopyUnroll; ++j) to[base + j * kCopyThreads] = v[j];
-    } else {
-      for (int32_t e = base; e < n; e += kCopyThreads) to[e] = from[e];
+      for (int j = 0; j < kCopyUnroll; ++j)
+        if (base + j * kCopyThreads < n) __builtin_nontemporal_store(v[j], to + base + j * kCopyThreads);
     }
   }
 }
 
 __global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(const PageCaches c, const CopyList list) {
-  copy_pages(c, list, blockIdx.x, gridDim.x);
+  copy_pages<false>(c, list, blockIdx.x, gridDim.x);
 }
 
 int32_t copy_groups(const PageCaches& c, int64_t pairs) {
@@ -138,20 +143,44 @@ __device__ __forceinline__ int32_t pool_take(const int32_t* ref_counts, int32_t 
   return need && nth < min(have, kPoolThreads) ? found[nth] : -1;
 }
 
-// Whether entry i of the list (held in LDS) names a row that an earlier entry names too.
-__device__ __forceinline__ bool listed_before(const int32_t* rows, int32_t i, int32_t row) {
-  for (int32_t j = 0; j < i; ++j)
-    if (rows[j] == row) return true;
-  return false;
+// Whether entry i of the list (n entries in LDS, 16-byte aligned) names a row that an earlier entry
+// names too: every thread reads the same four entries at a time, none waits for a comparison.
+__device__ __forceinline__ bool listed_before(const int32_t* rows, int32_t n, int32_t i, int32_t row) {
+  bool found = false;
+#pragma unroll 4
+  for (int32_t j = 0; j < n; j += 4) {
+    const int4 r = *reinterpret_cast<const int4*>(rows + j);
+    found |= (r.x == row && j < i) | (r.y == row && j + 1 < i) | (r.z == row && j + 2 < i) | (r.w == row && j + 3 < i);
+  }
+  return found;
 }
 
-// Who gets which block in a fork: new_blocks[i] and the plan (source page, target page, tokens to
-// copy, child's length; length -1: the child is left as it was). The children's lengths and the
-// new blocks' counts are written here, tables and shared counts by the launch that copies.
+// What a fork leaves for the launch that applies it.
+struct ForkPlan {
+  int4* heads;       // runs of children in a row that copy the same tokens (CopyList::heads), and the end
+  int32_t* targets;  // their new blocks
+  int32_t* blocks;   // of every child: its new block, or -1
+  int32_t* lens;     // of every child: its length, -1: it stays as it was
+  int32_t* runs;     // number of runs
+};
+
+ForkPlan fork_plan(void* ws, int32_t n) {
+  ForkPlan f;
+  f.heads = static_cast<int4*>(ws);
+  f.targets = reinterpret_cast<int32_t*>(f.heads + n + 1);
+  f.blocks = f.targets + n;
+  f.lens = f.blocks + n;
+  f.runs = f.lens + n;
+  return f;
+}
+
+// Who gets which block in a fork. The children's lengths and the new blocks' counts are written
+// here, tables and shared counts by the launch that copies.
 __global__ __launch_bounds__(kPoolThreads) void fork_plan_kernel(const PageTables t, const int32_t* parents,
                                                                  const int32_t* children, int32_t n,
-                                                                 int32_t* new_blocks, int4* plan) {
-  __shared__ int32_t rows[kPoolThreads], found[kPoolThreads], part[kPoolWaves];
+                                                                 int32_t* new_blocks, const ForkPlan f) {
+  __shared__ __attribute__((aligned(16))) int32_t rows[kPoolThreads];
+  __shared__ int32_t found[kPoolThreads], part[kPoolWaves];
   const int32_t i = threadIdx.x;
   int32_t parent = -1, child = -1, length = 0;
   if (i < n) {
@@ -161,35 +190,55 @@ __global__ __launch_bounds__(kPoolThreads) void fork_plan_kernel(const PageTable
   }
   rows[i] = child;
   __syncthreads();
-  const bool ok = i < n && child >= 0 && child < t.rows && t.lens[child] == 0 && !listed_before(rows, i, child);
+  const bool listed = listed_before(rows, n, i, child);
+  const bool ok = i < n && child >= 0 && child < t.rows && t.lens[child] == 0 && !listed;
   const int32_t full = length / t.block_size, tail = length - full * t.block_size;
   const bool need = ok && tail > 0;
+  const int32_t src = need ? t.tables[parent * t.stride + full] : -1;
   int32_t want;
   const int32_t nth = pool_scan(need, part, &want);
   // (pool_take's barriers order every read of the lengths before the writes below)
   const int32_t block = pool_take(t.ref_counts, t.num_blocks, need, nth, want, part, found);
+  const bool done = ok && (!need || block >= 0), copies = need && done;
+  // The copies, in order (blocks run out for the last ones, so nth counts those that got one),
+  // and the runs of one source and length among them.
+  __syncthreads();  // `found` has been read
+  rows[i] = copies ? src : -2;
+  found[i] = tail;
+  __syncthreads();
+  const bool head = copies && (i == 0 || rows[i - 1] != src || found[i - 1] != tail);
+  int32_t runs, copied;
+  const int32_t run = pool_scan(head, part, &runs);
+  pool_scan(copies, part, &copied);
+  if (i == 0) {
+    *f.runs = runs;
+    f.heads[runs] = make_int4(-1, 0, copied, 0);
+  }
   if (i >= n) return;
-  const bool done = ok && (!need || block >= 0);
   new_blocks[i] = !ok ? -3 : !need ? -1 : block >= 0 ? block : -2;
-  plan[i] = make_int4(need && done ? t.tables[parent * t.stride + full] : -1, need && done ? block : -1, tail,
-                      done ? length : -1);
+  f.blocks[i] = copies ? block : -1;
+  f.lens[i] = done ? length : -1;
+  if (head) f.heads[run] = make_int4(src, tail, nth, 0);
+  if (copies) {
+    f.targets[nth] = block;
+    t.ref_counts[block] = 1;
+  }
   if (done) t.lens[child] = length;
-  if (done && need) t.ref_counts[block] = 1;
 }
 
 // Work-groups [0, n): child i's table row, and one more holder for the pages it shares. The
 // others copy the new pages' tokens.
 __global__ __launch_bounds__(kCopyThreads) void fork_apply_kernel(const PageTables t, const PageCaches c,
                                                                   const int32_t* parents, const int32_t* children,
-                                                                  int32_t n, const int4* plan) {
+                                                                  int32_t n, const ForkPlan f) {
   if ((int32_t)blockIdx.x >= n) {
-    copy_pages(c, CopyList{nullptr, nullptr, nullptr, plan, nullptr, n}, blockIdx.x - n, gridDim.x - n);
+    copy_pages<true>(c, CopyList{nullptr, f.targets, nullptr, f.heads, f.runs, n}, blockIdx.x - n, gridDim.x - n);
     return;
   }
   const int32_t i = blockIdx.x;
-  const int4 p = plan[i];
-  if (p.w < 0) return;
-  const int32_t full = p.w / t.block_size;
+  const int32_t length = f.lens[i];
+  if (length < 0) return;
+  const int32_t full = length / t.block_size;
   const int32_t* from = t.tables + parents[i] * t.stride;  // read only where full > 0: the parent is a row then
   int32_t* to = t.tables + children[i] * t.stride;
   for (int32_t j = threadIdx.x; j < t.width; j += kCopyThreads) {
@@ -198,7 +247,7 @@ __global__ __launch_bounds__(kCopyThreads) void fork_apply_kernel(const PageTabl
       b = from[j];
       if (b >= 0 && b < t.num_blocks) atomicAdd(t.ref_counts + b, 1);
     } else if (j == full) {
-      b = p.y;
+      b = f.blocks[i];
     }
     to[j] = b;
   }
@@ -208,14 +257,16 @@ __global__ __launch_bounds__(kCopyThreads) void fork_apply_kernel(const PageTabl
 // nothing changed where the row is no row, is listed before, its table is full or the pool empty.
 __global__ __launch_bounds__(kPoolThreads) void extend_kernel(const PageTables t, const int32_t* list, int32_t n,
                                                               int32_t* slots) {
-  __shared__ int32_t rows[kPoolThreads], found[kPoolThreads], part[kPoolWaves];
+  __shared__ __attribute__((aligned(16))) int32_t rows[kPoolThreads];
+  __shared__ int32_t found[kPoolThreads], part[kPoolWaves];
   const int32_t i = threadIdx.x;
   int32_t row = -1;
   if (i < n) row = list[i];
   rows[i] = row;
   __syncthreads();
   int32_t length = -1;
-  if (row >= 0 && row < t.rows && !listed_before(rows, i, row)) length = t.lens[row];
+  const bool listed = listed_before(rows, n, i, row);
+  if (row >= 0 && row < t.rows && !listed) length = t.lens[row];
   const bool ok = length >= 0 && length < t.max_len;
   const int32_t page = ok ? length / t.block_size : 0, off = ok ? length - page * t.block_size : 0;
   const bool need = ok && off == 0;
@@ -307,7 +358,7 @@ __global__ __launch_bounds__(kCopyThreads) void compact_apply_kernel(const PageT
                                                                      const int32_t* block_map, const CopyList list,
                                                                      int32_t table_groups) {
   if ((int32_t)blockIdx.x >= table_groups) {
-    copy_pages(c, list, blockIdx.x - table_groups, gridDim.x - table_groups);
+    copy_pages<false>(c, list, blockIdx.x - table_groups, gridDim.x - table_groups);
     return;
   }
   const int64_t total = (int64_t)t.rows * t.width;
@@ -339,15 +390,19 @@ hipError_t launch_copy_blocks(const PageCaches& c, const int32_t* src, const int
   return hipGetLastError();
 }
 
+size_t fork_workspace_bytes(int32_t n) {
+  return n <= 0 ? 0 : (size_t)(n + 1) * sizeof(int4) + (size_t)(3 * n + 1) * sizeof(int32_t);
+}
+
 hipError_t launch_fork_sequences(const PageTables& t, const PageCaches& c, const int32_t* parents,
                                  const int32_t* children, int32_t n, int32_t* new_blocks, void* workspace,
                                  hipStream_t stream) {
-  int4* plan = static_cast<int4*>(workspace);
+  const ForkPlan f = fork_plan(workspace, n);
   hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kPoolThreads), 0, stream, t, parents, children, n, new_blocks,
-                     plan);
+                     f);
   if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
   hipLaunchKernelGGL(fork_apply_kernel, dim3(n + copy_groups(c, n)), dim3(kCopyThreads), 0, stream, t, c, parents,
-                     children, n, plan);
+                     children, n, f);
   return hipGetLastError();
 }
 

@@ -36,7 +36,7 @@ namespace {
 template <int NP, int MT, int NB, int EPI>
 __global__ __launch_bounds__(kLinThreads) void linear_kernel(const LinArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[lin_smem_bytes(NP, MT)];
-  linear_tile<NP, MT, NB, EPI>(a, blockIdx.x, smem);
+  linear_tile<NP, MT, NB, EPI>(a, blockIdx.x, smem, NoAddend{});
 }
 
 // Sum of the KS partials, then the store or SiLU * mul epilogue; 8 output columns per thread.

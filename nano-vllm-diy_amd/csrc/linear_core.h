@@ -79,13 +79,23 @@ __device__ __forceinline__ void lin_lds_barrier() {
 // (16 lanes = 16 rows of one column) are free of bank conflicts. Two LDS stages: chunk c
 // is stored in stage c & 1 while the other stage may still be read for chunk c - 1.
 // Wavefront w multiplies the 64 columns [64 w, 64 w + 64) of every chunk.
+// What an epilogue adds to the sums of a work-group's 32 x 32 outputs (NP = MT = 1) before they are
+// rounded: load is called before the K walk, put and add after it, with a barrier between them and
+// LDS of their own. Thread (c, q) adds to row c, columns 4 q .. 4 q + 3. Here: nothing.
+struct NoAddend {
+  __device__ __forceinline__ void load(int row0, int n0) {}
+  __device__ __forceinline__ void put(char* lds) const {}
+  __device__ __forceinline__ void add(const char* lds, float4& v) const {}
+};
+
 // `block` is the work-group's index in the launch shape of choose_config, `smem` its
 // lin_smem_bytes(NP, MT) bytes of LDS.
-template <int NP, int MT, int NB, int EPI>
-__device__ __forceinline__ void linear_tile(const LinArgs a, const int block, char* smem) {
+template <int NP, int MT, int NB, int EPI, class Addend>
+__device__ __forceinline__ void linear_tile(const LinArgs a, const int block, char* smem, Addend addend) {
   constexpr int kOps = NP + MT;               // operand tiles per chunk
   constexpr int kTileBytes = 32 * kLinChunk * 2;
   constexpr int kStage = kOps * kTileBytes;
+  constexpr int kSumBytes = 4 * NP * 4 * kWave * 16;  // the four wavefronts' sums of one x tile
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = threadIdx.x / kWave;
   const int r = lane & 31, h = lane >> 5;
@@ -120,6 +130,8 @@ __device__ __forceinline__ void linear_tile(const LinArgs a, const int block, ch
     const int cc = 8 * wave + 4 * h + i;  // MFMA step i reads 16-byte column cc of row r
     rofs[i] = r * (2 * kLinChunk) + ((cc ^ r) & 31) * 16;
   }
+
+  addend.load(row0, n0);
 
   f32x16 acc[NP][MT];
 #pragma unroll
@@ -182,6 +194,7 @@ __device__ __forceinline__ void linear_tile(const LinArgs a, const int block, ch
       for (int j = 0; j < 4; ++j)
         red[wave][p][j][lane] = make_float4(acc[p][t][4 * j], acc[p][t][4 * j + 1], acc[p][t][4 * j + 2],
                                             acc[p][t][4 * j + 3]);
+    addend.put(smem + kSumBytes);
     __syncthreads();
     const int m = row0 + 32 * t + c;
     float4 v[NP];
@@ -194,6 +207,7 @@ __device__ __forceinline__ void linear_tile(const LinArgs a, const int block, ch
     }
     if (m < a.rows) {
       if constexpr (EPI == kEpiStore) {
+        addend.add(smem + kSumBytes, v[0]);
         *reinterpret_cast<uint2*>(a.y + (int64_t)m * a.y_stride + n) =
             make_uint2(pack_bf16x2(v[0].x, v[0].y), pack_bf16x2(v[0].z, v[0].w));
       } else if constexpr (EPI == kEpiSiluMul) {

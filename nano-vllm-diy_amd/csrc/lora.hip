@@ -24,6 +24,8 @@
 // >> 4) supplies row r of both operands at k = 8 h .. 8 h + 7 and holds D[4 h .. 4 h + 3][r]. The
 // token rows are the second operand, so a lane's four values are neighbours in one row of t
 // or out.
+#include <type_traits>
+
 #include "linear_core.h"
 
 namespace pk {
@@ -32,8 +34,10 @@ namespace {
 constexpr int kLoraThreads = 256;
 constexpr int kLoraWaves = kLoraThreads / kWave;
 constexpr int kLoraTile = 64;        // rows of a sorted tile
+constexpr int kLoraShrinkRows = 32;  // of which a shrink work-group takes
 constexpr int kLoraSmallTile = 16;   // rows of a tile that is not sorted
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanTurns = 4;        // turns of 4096 rows whose ids are loaded together
 
 __device__ __forceinline__ f32x4 mfma16(const u32x4 a, const u32x4 b, const f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
@@ -63,70 +67,106 @@ __device__ __forceinline__ bool small_tile(const LoraArgs& p, int32_t slot, int3
   return true;
 }
 
-__device__ __forceinline__ bool sorted_tile(const LoraArgs& p, int32_t tile, int32_t* rows, int32_t* id) {
-  if (tile >= *p.num_tiles) return false;
-  const int4 t = p.tiles[tile];  // adapter, first position, rows
+// Sorted: R rows of the tile from its row `first` on (its record and its rows are loaded together;
+// an unused tile has no rows).
+template <int R>
+__device__ __forceinline__ bool sorted_tile(const LoraArgs& p, int32_t tile, int32_t first, int32_t* rows,
+                                            int32_t* id) {
+  if (tile >= p.max_tiles) return false;
+  const int32_t i = first + threadIdx.x;
+  const int2 t = p.tiles[tile];  // adapter, rows
+  const int32_t row = threadIdx.x < R ? p.perm[(int64_t)tile * kLoraTile + i] : -1;
   *id = t.x;
-  if (threadIdx.x < kLoraTile) rows[threadIdx.x] = (int)threadIdx.x < t.z ? p.perm[t.y + threadIdx.x] : -1;
+  if (first >= t.y) return false;
+  if (threadIdx.x < R) rows[threadIdx.x] = i < t.y ? row : -1;
   __syncthreads();
   return true;
 }
 
 // ---------------------------------------------------------------- shrink ----------------
 
-constexpr int shrink_smem_bytes(int r, int cb) { return kLoraWaves * r * (cb * 16 + 4) * 4; }
+// A chunk is 64 elements of k: 128 contiguous bytes of every row, in LDS with 16 bytes between rows.
+constexpr int kChunk = 64;
+constexpr int kChunkStride = kChunk * 2 + 16;
+constexpr int shrink_smem_bytes(int r, int cb) {
+  const int chunks = kLoraWaves * (r + cb * 16) * kChunkStride, sums = kLoraWaves * r * (cb * 16 + 4) * 4;
+  return chunks > sums ? chunks : sums;
+}
 
-// t of R rows of one adapter at its columns [c0, c0 + 16 CB). The four wavefronts take the k range
-// in turns of 64 (128 contiguous bytes of every row), U turns' loads before their products,
-// and add up in LDS.
-template <int R, int CB, int U>
+// This wavefront's LDS writes before its reads and its reads before its next writes: a
+// wavefront's LDS operations run in order, so only the compiler has to be told.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// t of R rows of one adapter at its columns [c0, c0 + 16 CB). The four wavefronts take the chunks of
+// k in turn (each its own: no barrier) and add up in LDS at the end. A chunk's x and A rows are
+// loaded 8 rows an instruction and put into the MFMA's order through LDS: loaded in that
+// order, four neighbouring lanes would hold four rows, four cache lines instead of one, and
+// the L1 would be the bound. The loads are U chunks ahead.
+// store(i, c, v): t of the tile's row i at columns c0 + c .. + 3, scaled.
+template <int R, int CB, int U, class Store>
 __device__ __forceinline__ void shrink_tile(const LoraArgs& p, const int32_t id, const int32_t c0, const int32_t* rows,
-                                            char* smem) {
-  constexpr int kSubs = R / 16, kStride = CB * 16 + 4;
+                                            char* smem, const Store& store) {
+  constexpr int kSubs = R / 16, kLoads = (R + 16 * CB) / 8, kStride = CB * 16 + 4;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int r = lane & 15, h = lane >> 4;
   const int32_t width = p.num_slices * p.rank;
-  const uint16_t *xr[kSubs], *ar[CB];
+  const uint16_t* src[kLoads];
 #pragma unroll
-  for (int s = 0; s < kSubs; ++s) {
-    const int32_t row = rows[16 * s + r];
-    xr[s] = p.x + (int64_t)max(row, 0) * p.x_stride;  // (what the missing rows give is not stored)
+  for (int i = 0; i < kLoads; ++i) {
+    const int m = 8 * i + (lane >> 3);
+    if (8 * i < R)
+      src[i] = p.x + (int64_t)max(rows[m], 0) * p.x_stride;  // (what the missing rows give is not stored)
+    else
+      src[i] = p.a + id * p.a_adapter + (int64_t)min(c0 + m - R, width - 1) * p.a_row;
+    src[i] += 8 * (lane & 7);
   }
-#pragma unroll
-  for (int c = 0; c < CB; ++c)
-    ar[c] = p.a + id * p.a_adapter + (int64_t)min(c0 + 16 * c + r, width - 1) * p.a_row;
+  char* mine = smem + wave * (R + 16 * CB) * kChunkStride;
+  char* put = mine + (lane >> 3) * kChunkStride + 16 * (lane & 7);
+  const char* get = mine + r * kChunkStride + 16 * h;
   f32x4 acc[kSubs][CB];
 #pragma unroll
   for (int s = 0; s < kSubs; ++s)
 #pragma unroll
     for (int c = 0; c < CB; ++c) acc[s][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  constexpr int kTurn = kLoraWaves * 64;
-  for (int32_t k0 = wave * 64; k0 < p.k; k0 += U * kTurn) {
-    u32x4 xv[2 * U][kSubs], av[2 * U][CB];
+  constexpr int32_t kTurn = kLoraWaves * kChunk;
+  u32x4 st[U][kLoads];
+  const auto load = [&](int u, int32_t at) {
+    const bool in = at + 8 * (lane & 7) < p.k;  // k is a multiple of 8
 #pragma unroll
-    for (int u = 0; u < 2 * U; ++u) {
-      const int32_t kp = k0 + (u >> 1) * kTurn + (u & 1) * 32 + 8 * h;
-      const bool in = kp < p.k;  // k is a multiple of 8
-      const int32_t at = in ? kp : 0;
-      const u32x4 zero = {0u, 0u, 0u, 0u};
-#pragma unroll
-      for (int s = 0; s < kSubs; ++s) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(xr[s] + at);
-        xv[u][s] = in ? v : zero;
-      }
-#pragma unroll
-      for (int c = 0; c < CB; ++c) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(ar[c] + at);
-        av[u][c] = in ? v : zero;
-      }
+    for (int i = 0; i < kLoads; ++i) {
+      st[u][i] = u32x4{0u, 0u, 0u, 0u};
+      if (in) st[u][i] = *reinterpret_cast<const u32x4*>(src[i] + at);
     }
+  };
 #pragma unroll
-    for (int u = 0; u < 2 * U; ++u)
+  for (int u = 0; u < U; ++u) load(u, wave * kChunk + u * kTurn);
+  for (int32_t k0 = wave * kChunk; k0 < p.k; k0 += U * kTurn) {
 #pragma unroll
-      for (int s = 0; s < kSubs; ++s)
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
-        for (int c = 0; c < CB; ++c) acc[s][c] = mfma16(av[u][c], xv[u][s], acc[s][c]);
+      for (int i = 0; i < kLoads; ++i) *reinterpret_cast<u32x4*>(put + i * 8 * kChunkStride) = st[u][i];
+      if (k0 + U * kTurn < p.k) load(u, k0 + (U + u) * kTurn);
+      wave_lds_fence();
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        u32x4 xv[kSubs];
+#pragma unroll
+        for (int s = 0; s < kSubs; ++s)
+          xv[s] = *reinterpret_cast<const u32x4*>(get + 16 * s * kChunkStride + 64 * q);
+#pragma unroll
+        for (int c = 0; c < CB; ++c) {
+          const u32x4 av = *reinterpret_cast<const u32x4*>(get + (R + 16 * c) * kChunkStride + 64 * q);
+#pragma unroll
+          for (int s = 0; s < kSubs; ++s) acc[s][c] = mfma16(av, xv[s], acc[s][c]);
+        }
+      }
+      wave_lds_fence();
+    }
   }
+  __syncthreads();  // every wavefront is done with its chunks before they hold the sums
   float* red = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int s = 0; s < kSubs; ++s)
@@ -137,61 +177,131 @@ __device__ __forceinline__ void shrink_tile(const LoraArgs& p, const int32_t id,
   const float scale = p.scales ? p.scales[id] : 1.0f;
   for (int e = threadIdx.x; e < R * CB * 4; e += kLoraThreads) {
     const int i = e / (CB * 4), c = (e - i * (CB * 4)) * 4;
-    const int32_t row = rows[i];
-    if (row < 0 || c0 + c >= width) continue;
     f32x4 v[kLoraWaves];
 #pragma unroll
     for (int w = 0; w < kLoraWaves; ++w) v[w] = *reinterpret_cast<const f32x4*>(red + (w * R + i) * kStride + c);
     f32x4 sum;
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[j] = ((v[0][j] + v[1][j]) + (v[2][j] + v[3][j])) * scale;
-    *reinterpret_cast<f32x4*>(p.t + (int64_t)row * width + c0 + c) = sum;
+    store(i, c, sum);
   }
 }
 
-// Work-group = (row, 16 columns of t).
+// shrink_tile's sums to p.t, for the expand's launch.
+template <int R, int CB, int U>
+__device__ __forceinline__ void shrink_to_memory(const LoraArgs& p, const int32_t id, const int32_t c0,
+                                                 const int32_t* rows, char* smem) {
+  const int32_t width = p.num_slices * p.rank;
+  shrink_tile<R, CB, U>(p, id, c0, rows, smem, [&](int i, int c, const f32x4 v) {
+    const int32_t row = rows[i];
+    if (row >= 0 && c0 + c < width) *reinterpret_cast<f32x4*>(p.t + (int64_t)row * width + c0 + c) = v;
+  });
+}
+
+// Work-group = (row, 16 CB columns of t).
+template <int CB>
 __device__ __forceinline__ void shrink_small(const LoraArgs& p, int32_t group, int32_t* rows, char* smem) {
-  const int32_t blocks = (p.num_slices * p.rank + 15) / 16;
+  const int32_t blocks = (p.num_slices * p.rank + 16 * CB - 1) / (16 * CB);
   const int32_t slot = group / blocks;
   int32_t id;
   if (!small_tile(p, slot, rows, &id) || id < 0) return;
-  shrink_tile<kLoraSmallTile, 1, 4>(p, id, (group - slot * blocks) * 16, rows, smem);
+  shrink_to_memory<kLoraSmallTile, CB, 4>(p, id, (group - slot * blocks) * 16 * CB, rows, smem);
 }
 
 __global__ __launch_bounds__(kLoraThreads) void lora_shrink_small_kernel(const LoraArgs p) {
   __shared__ __attribute__((aligned(16))) char smem[shrink_smem_bytes(kLoraSmallTile, 1)];
   __shared__ int32_t rows[kLoraSmallTile];
-  shrink_small(p, blockIdx.x, rows, smem);
+  shrink_small<1>(p, blockIdx.x, rows, smem);
 }
 
-// Work-group = (sorted tile, 64 columns of t).
+// Work-group = (32 rows of a sorted tile, 16 CB columns of t).
+template <int CB>
 __global__ __launch_bounds__(kLoraThreads) void lora_shrink_kernel(const LoraArgs p) {
-  __shared__ __attribute__((aligned(16))) char smem[shrink_smem_bytes(kLoraTile, 4)];
-  __shared__ int32_t rows[kLoraTile];
-  const int32_t blocks = (p.num_slices * p.rank + 63) / 64;
-  const int32_t tile = blockIdx.x / blocks;
+  __shared__ __attribute__((aligned(16))) char smem[shrink_smem_bytes(kLoraShrinkRows, CB)];
+  __shared__ int32_t rows[kLoraShrinkRows];
+  const int32_t blocks = (p.num_slices * p.rank + 16 * CB - 1) / (16 * CB);
+  // the blocks of one tile's rows are 8 work-groups apart: one XCD, whose L2 gives the rows to all
+  const int32_t part = blockIdx.x / (8 * blocks) * 8 + blockIdx.x % 8, block = blockIdx.x % (8 * blocks) / 8;
   int32_t id;
-  if (!sorted_tile(p, tile, rows, &id) || id < 0) return;
-  shrink_tile<kLoraTile, 4, 2>(p, id, (blockIdx.x - tile * blocks) * 64, rows, smem);
+  if (!sorted_tile<kLoraShrinkRows>(p, part / (kLoraTile / kLoraShrinkRows),
+                                    part % (kLoraTile / kLoraShrinkRows) * kLoraShrinkRows, rows, &id) || id < 0)
+    return;
+  shrink_to_memory<kLoraShrinkRows, CB, 1>(p, id, block * 16 * CB, rows, smem);
 }
 
-// The sums of a decode step's projection (work-groups [0, lin_groups)) and the shrink of its
-// adapters, which need nothing of each other, in one launch.
-template <int NB>
+// The partial sums of a decode step's projection (work-groups [0, lin_groups)) and the shrink of its
+// adapters, which need nothing of each other, in one launch; the expand adds the partial sums.
+template <int NB, int CB>
 __global__ __launch_bounds__(kLinThreads) void lora_linear_kernel(const LinArgs a, const LoraArgs p,
                                                                   const int32_t lin_groups) {
   __shared__ __attribute__((aligned(16))) char smem[lin_smem_bytes(1, 1)];
   __shared__ int32_t rows[kLoraSmallTile];
   if ((int32_t)blockIdx.x < lin_groups)
-    linear_tile<1, 1, NB, kEpiPartial>(a, blockIdx.x, smem);
+    linear_tile<1, 1, NB, kEpiPartial>(a, blockIdx.x, smem, NoAddend{});
   else
-    shrink_small(p, blockIdx.x - lin_groups, rows, smem);
+    shrink_small<CB>(p, blockIdx.x - lin_groups, rows, smem);
+}
+
+// A projection whose K is not split, after the shrink's launch: the work-group adds its rows' adapters
+// to its sums, products in fp32, for ranks up to 16. A row's B is 64 pieces of 16 bytes (two a
+// column), one after the other in memory; the row's eight threads take them in turn, whole cache
+// lines, before the K walk, which hides them. Their products with t go through LDS to the threads
+// that have the columns.
+struct LoraAddend {
+  const LoraArgs& p;
+  bool any;
+  u32x4 b[8];
+  f32x4 t[2];
+  __device__ __forceinline__ void load(int row0, int n0) {
+    const int32_t m = row0 + (threadIdx.x >> 3), piece = threadIdx.x & 7, half = piece & 1;
+    const int32_t id = m < p.rows ? adapter_of(p, m) : -1;
+    any = id >= 0;
+    if (!any) return;
+    int32_t q = 0;
+    while (q < p.num_slices - 1 && n0 >= p.slice_begin[q + 1]) ++q;  // (slices are multiples of 32 columns)
+    const uint16_t* bp = p.b + id * p.b_adapter + (n0 + (piece >> 1)) * p.b_row + 8 * half;
+    const float* tp = p.t + (int64_t)m * (p.num_slices * p.rank) + q * p.rank + 8 * half;
+    const bool in = 8 * half < p.rank;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      b[i] = u32x4{0u, 0u, 0u, 0u};
+      if (in) b[i] = *reinterpret_cast<const u32x4*>(bp + 4 * i * p.b_row);
+    }
+    t[0] = t[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (in) {
+      t[0] = *reinterpret_cast<const f32x4*>(tp);
+      t[1] = *reinterpret_cast<const f32x4*>(tp + 4);
+    }
+  }
+  // [row][64] products of the pieces, 4 floats between rows
+  __device__ __forceinline__ void put(char* lds) const {
+    float* at = reinterpret_cast<float*>(lds) + (threadIdx.x >> 3) * 68 + (threadIdx.x & 7);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float d = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        d = fmaf(bf16_lo(b[i][e]), t[e >> 1][2 * (e & 1)], d);
+        d = fmaf(bf16_hi(b[i][e]), t[e >> 1][2 * (e & 1) + 1], d);
+      }
+      at[8 * i] = d;
+    }
+  }
+  __device__ __forceinline__ void add(const char* lds, float4& v) const {
+    if (!any) return;
+    const float* at = reinterpret_cast<const float*>(lds) + (threadIdx.x >> 3) * 68 + 8 * (threadIdx.x & 7);
+    const f32x4 d0 = *reinterpret_cast<const f32x4*>(at), d1 = *reinterpret_cast<const f32x4*>(at + 4);
+    v = make_float4(v.x + (d0[0] + d0[1]), v.y + (d0[2] + d0[3]), v.z + (d1[0] + d1[1]), v.w + (d1[2] + d1[3]));
+  }
+};
+
+template <int NB>
+__global__ __launch_bounds__(kLinThreads) void lora_linear_expand_kernel(const LinArgs a, const LoraArgs p) {
+  __shared__ __attribute__((aligned(16))) char smem[lin_smem_bytes(1, 1)];
+  linear_tile<1, 1, NB, kEpiStore>(a, blockIdx.x, smem, LoraAddend{p});
 }
 
 // ---------------------------------------------------------------- expand ----------------
-
-constexpr int lora_rank32(int rank) { return (rank + 31) / 32 * 32; }
-constexpr int expand_row_bytes(int rank) { return lora_rank32(rank) * 4 + 16; }  // hi, lo, and 16 against bank conflicts
 
 __device__ __forceinline__ void split_bf16(float v, uint32_t* hi, uint32_t* lo) {
   const uint32_t b = f32_to_bf16(v);
@@ -201,219 +311,416 @@ __device__ __forceinline__ void split_bf16(float v, uint32_t* hi, uint32_t* lo) 
   *lo = (b & 0x7f80u) == 0x7f80u ? 0u : f32_to_bf16(v - head);
 }
 
-// out of R rows of one adapter at columns [begin, end) of slice q: 64 columns a wavefront and turn.
-// MFMA row i of tile u is column 32 (u >> 1) + 8 (i >> 2) + 4 (u & 1) + (i & 3) of the turn, so a lane
-// holds 8 neighbouring columns of a row in two tiles: 16-byte loads and stores, 64 contiguous
-// bytes of every row in one instruction. NCH: 32-wide pieces of the rank.
-// kPartial: base is the sum of p.ks fp32 partial products, else bf16 rows of y.
-template <int R, int NCH, bool kPartial>
-__device__ __forceinline__ void expand_tile(const LoraArgs& p, const int32_t id, const int32_t q, const int32_t begin,
-                                            const int32_t end, const int32_t* rows, char* smem) {
-  constexpr int kSubs = R / 16;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const int r = lane & 15, h = lane >> 4;
-  const int row_bytes = expand_row_bytes(p.rank), lo_at = lora_rank32(p.rank) * 2;
-  if (id >= 0) {
-    const int quads = lora_rank32(p.rank) / 4;
-    const int64_t width = p.num_slices * p.rank;
-    for (int e = threadIdx.x; e < R * quads; e += kLoraThreads) {
-      const int i = e / quads, j = (e - i * quads) * 4;
-      const int32_t row = rows[i];
-      f32x4 v = {0.f, 0.f, 0.f, 0.f};
-      if (row >= 0 && j < p.rank) v = *reinterpret_cast<const f32x4*>(p.t + row * width + q * p.rank + j);
-      uint32_t hi[4], lo[4];
+// How both expand kernels multiply. A wavefront has 16 rows and 128 columns: t's rows are the
+// MFMA's first operand, B's the second, and row j of MFMA tile u is column 8 j + u, so that a lane's
+// eight tiles give 8 neighbouring columns of a row and 16 lanes 256 contiguous bytes of it: whole
+// cache lines of base and out. B is loaded along its rows and ordered through LDS, KP elements of
+// the rank at a time with 16 bytes between rows. Of t both halves are multiplied; with KP = 16
+// they fit one MFMA (k 0-15 hi, 16-31 lo).
+template <int KP>
+struct ExpandShape {
+  static constexpr int kRowBytes = KP * 2 + 16;
+  static constexpr int kChunks = KP / 8;                   // 16-byte pieces of a B row
+  static constexpr int kSteps = KP > 32 ? KP / 32 : 1;     // MFMA steps
+  // LDS row of a column: column 8 j + u of 128 at 16 u + j, so a tile's rows are neighbours
+  __device__ static __forceinline__ int at(int c) { return (c & ~127) | (c & 7) << 4 | (c & 127) >> 3; }
+};
+
+// A lane's part of t, both halves: row t_row (of one slice), elements j0 + 32 n + 8 h of KP.
+template <int KP>
+__device__ __forceinline__ void load_t(const float* t_row, int32_t rank, int32_t j0, int h,
+                                       u32x4 (&hi)[ExpandShape<KP>::kSteps], u32x4 (&lo)[ExpandShape<KP>::kSteps]) {
 #pragma unroll
-      for (int n = 0; n < 4; ++n) split_bf16(v[n], &hi[n], &lo[n]);
-      char* to = smem + i * row_bytes + j * 2;
-      *reinterpret_cast<u32x2*>(to) = u32x2{hi[0] | hi[1] << 16, hi[2] | hi[3] << 16};
-      *reinterpret_cast<u32x2*>(to + lo_at) = u32x2{lo[0] | lo[1] << 16, lo[2] | lo[3] << 16};
-    }
-    __syncthreads();
-  }
-  const uint16_t* bp = p.b + max(id, 0) * p.b_adapter;
-  for (int32_t c0 = begin + 64 * wave; c0 < end; c0 += 64 * kLoraWaves) {
-    const bool both = c0 + 32 < end;  // ranges are multiples of 32 columns
-    u32x4 bv[NCH][4];
-    if (id >= 0) {
-#pragma unroll
-      for (int ch = 0; ch < NCH; ++ch)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int32_t col = c0 + (both ? 32 * (u >> 1) : 0) + 8 * (r >> 2) + 4 * (u & 1) + (r & 3);
-          const int32_t j = 32 * ch + 8 * h;
-          bv[ch][u] = u32x4{0u, 0u, 0u, 0u};
-          if (j < p.rank) bv[ch][u] = *reinterpret_cast<const u32x4*>(bp + col * p.b_row + j);
-        }
+  for (int n = 0; n < ExpandShape<KP>::kSteps; ++n) {
+    const int32_t j = j0 + 32 * n + 8 * (KP == 16 ? h & 1 : h);
+    f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    if (j < rank) {
+      v[0] = *reinterpret_cast<const f32x4*>(t_row + j);
+      v[1] = *reinterpret_cast<const f32x4*>(t_row + j + 4);
     }
 #pragma unroll
-    for (int s = 0; s < kSubs; ++s) {
-      const int32_t row = rows[16 * s + r];
-      // the base's 2 x 8 columns
-      f32x4 acc[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-      u32x4 yv[2];
-      if constexpr (!kPartial) {
-#pragma unroll
-        for (int v = 0; v < 2; ++v)
-          if (row >= 0 && (v == 0 || both))
-            yv[v] = *reinterpret_cast<const u32x4*>(p.y + row * p.y_stride + c0 + 32 * v + 8 * h);
-      }
-      if (id >= 0) {
-#pragma unroll
-        for (int ch = 0; ch < NCH; ++ch) {
-          const char* at = smem + (16 * s + r) * row_bytes + 64 * ch + 16 * h;
-          const bool in = 32 * ch < lo_at / 2;
-          u32x4 hi = {0u, 0u, 0u, 0u}, lo = hi;
-          if (in) {
-            hi = *reinterpret_cast<const u32x4*>(at);
-            lo = *reinterpret_cast<const u32x4*>(at + lo_at);
-          }
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            acc[u] = mfma16(bv[ch][u], lo, acc[u]);
-            acc[u] = mfma16(bv[ch][u], hi, acc[u]);
-          }
-        }
-      }
-#pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        if (row < 0 || (v == 1 && !both)) continue;
-        const int32_t col = c0 + 32 * v + 8 * h;
-        float base[8];
-        if constexpr (kPartial) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) base[e] = 0.f;
-          for (int k = 0; k < p.ks; ++k) {
-            const float* pp = p.part + ((int64_t)k * p.rows + row) * p.n_out + col;
-            const f32x4 a = *reinterpret_cast<const f32x4*>(pp), b = *reinterpret_cast<const f32x4*>(pp + 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              base[e] += a[e];
-              base[4 + e] += b[e];
-            }
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            base[2 * e] = bf16_lo(yv[v][e]);
-            base[2 * e + 1] = bf16_hi(yv[v][e]);
-          }
-        }
-        if (id >= 0) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            base[e] += acc[2 * v][e];
-            base[4 + e] += acc[2 * v + 1][e];
-          }
-        }
-        u32x4 o;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = pack_bf16x2(base[2 * e], base[2 * e + 1]);
-        *reinterpret_cast<u32x4*>(p.out + row * p.out_stride + col) = o;
-      }
+    for (int e = 0; e < 4; ++e) {
+      uint32_t ha, la, hb, lb;
+      split_bf16(v[e >> 1][2 * (e & 1)], &ha, &la);
+      split_bf16(v[e >> 1][2 * (e & 1) + 1], &hb, &lb);
+      hi[n][e] = ha | hb << 16;
+      lo[n][e] = la | lb << 16;
+      if (KP == 16 && h >= 2) hi[n][e] = lo[n][e];
     }
   }
 }
 
-// Work-group = (row or sorted tile, p.group_cols columns of one slice).
-template <bool kSorted, int NCH, bool kPartial>
-__global__ __launch_bounds__(kLoraThreads) void lora_expand_kernel(const LoraArgs p) {
-  constexpr int R = kSorted ? kLoraTile : kLoraSmallTile;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ int32_t rows[R];
-  const int32_t tile = blockIdx.x / p.col_groups;
-  int32_t g = blockIdx.x - tile * p.col_groups, q = 0;
+// acc[u] += t B^T over KP elements; b: LDS row of the wavefront's first column.
+template <int KP>
+__device__ __forceinline__ void expand_mfma(const char* b, int r, int h, const u32x4 (&hi)[ExpandShape<KP>::kSteps],
+                                            const u32x4 (&lo)[ExpandShape<KP>::kSteps], f32x4 (&acc)[8]) {
+  constexpr int kRowBytes = ExpandShape<KP>::kRowBytes;
+#pragma unroll
+  for (int n = 0; n < ExpandShape<KP>::kSteps; ++n) {
+    const char* get = b + r * kRowBytes + 64 * n + 16 * (KP == 16 ? h & 1 : h);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const u32x4 bv = *reinterpret_cast<const u32x4*>(get + 16 * u * kRowBytes);
+      if constexpr (KP != 16) acc[u] = mfma16(lo[n], bv, acc[u]);
+      acc[u] = mfma16(hi[n], bv, acc[u]);
+    }
+  }
+}
+
+// The slice of column group g (of `cols` columns each) and its first column.
+__device__ __forceinline__ int32_t group_slice(const LoraArgs& p, int32_t g, int32_t cols, int32_t* begin) {
+  int32_t q = 0;
   for (; q < p.num_slices - 1; ++q) {
-    const int32_t n = (p.slice_begin[q + 1] - p.slice_begin[q] + p.group_cols - 1) / p.group_cols;
+    const int32_t n = (p.slice_begin[q + 1] - p.slice_begin[q] + cols - 1) / cols;
     if (g < n) break;
     g -= n;
   }
-  int32_t id;
-  if constexpr (kSorted) {
-    if (!sorted_tile(p, tile, rows, &id)) return;
-  } else {
-    if (!small_tile(p, tile, rows, &id)) return;
-  }
+  *begin = p.slice_begin[q] + g * cols;
+  return q;
+}
+
+// Work-group = (row, up to 512 columns of a slice): the rows of 16 with that row's adapter, 128
+// columns a wavefront. Everything is asked for before the first wait.
+// kBase: where base is from -- kBasePartial: the sum of p.ks fp32 partial products, kBaseRows: bf16
+// rows of y, kBaseRowsShrink: those, and t is computed here, by every work-group of the row again, instead of
+// by a launch before (the rank is KP at most then).
+constexpr int kSmallCols = 512;
+enum Base { kBasePartial = 0, kBaseRows = 1, kBaseRowsShrink = 2 };
+
+template <int KP, int kBase>
+__global__ __launch_bounds__(kLoraThreads) void lora_expand_small_kernel(const LoraArgs p) {
+  using S = ExpandShape<KP>;
+  constexpr bool kPartial = kBase == kBasePartial, kShrink = kBase == kBaseRowsShrink;
+  constexpr int kLoads = kSmallCols * S::kChunks / kLoraThreads, CB = (KP + 15) / 16;
+  constexpr int kBBytes = kSmallCols * S::kRowBytes, kShrinkBytes = kShrink ? shrink_smem_bytes(kLoraSmallTile, CB) : 0;
+  __shared__ __attribute__((aligned(16))) char smem[kBBytes > kShrinkBytes ? kBBytes : kShrinkBytes];
+  __shared__ __attribute__((aligned(16))) float t_here[kShrink ? kLoraSmallTile * KP : 4];
+  __shared__ int32_t rows[kLoraSmallTile];
+  const int32_t slot = blockIdx.x / p.col_groups;
+  int32_t id, begin;
+  if (!small_tile(p, slot, rows, &id)) return;
   if (!kPartial && id < 0 && p.out == p.y) return;  // rows without an adapter stay as they are
-  const int32_t begin = p.slice_begin[q] + g * p.group_cols;
-  expand_tile<R, NCH, kPartial>(p, id, q, begin, min(begin + p.group_cols, p.slice_begin[q + 1]), rows, smem);
+  const int32_t q = group_slice(p, blockIdx.x - slot * p.col_groups, kSmallCols, &begin);
+  const int32_t end = min(begin + kSmallCols, p.slice_begin[q + 1]);
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int r = lane & 15, h = lane >> 4;
+  const int32_t col = begin + 128 * wave + 8 * r;  // this lane's columns
+  const bool in = col < end;                       // ranges are multiples of 32 columns
+  int32_t row[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) row[i] = rows[4 * h + i];
+  u32x4 yv[4];
+  if constexpr (!kPartial) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (in && row[i] >= 0) yv[i] = *reinterpret_cast<const u32x4*>(p.y + row[i] * p.y_stride + col);
+  }
+  f32x4 acc[8];
+#pragma unroll
+  for (int u = 0; u < 8; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (id >= 0) {
+    const uint16_t* bp = p.b + id * p.b_adapter;
+    const float* tp = kShrink ? t_here + r * KP
+                              : p.t + (int64_t)max(rows[r], 0) * (p.num_slices * p.rank) + q * p.rank;
+#pragma unroll 1
+    for (int32_t j0 = 0; j0 < p.rank; j0 += KP) {
+      u32x4 st[kLoads], hi[S::kSteps], lo[S::kSteps];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int e = i * kLoraThreads + threadIdx.x, c = e / S::kChunks, j = j0 + e % S::kChunks * 8;
+        st[i] = u32x4{0u, 0u, 0u, 0u};
+        if (begin + c < end && j < p.rank) st[i] = *reinterpret_cast<const u32x4*>(bp + (begin + c) * p.b_row + j);
+      }
+      if constexpr (kShrink) {
+        shrink_tile<kLoraSmallTile, CB, 4 / CB>(p, id, q * p.rank, rows, smem, [&](int i, int c, const f32x4 v) {
+          *reinterpret_cast<f32x4*>(t_here + i * KP + c) = v;
+        });
+        __syncthreads();  // t is there, and the sums it was added from are free for B
+      }
+      load_t<KP>(tp, p.rank, j0, h, hi, lo);
+      if (j0) __syncthreads();  // the previous piece has been read
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int e = i * kLoraThreads + threadIdx.x;
+        *reinterpret_cast<u32x4*>(smem + S::at(e / S::kChunks) * S::kRowBytes + e % S::kChunks * 16) = st[i];
+      }
+      __syncthreads();
+      expand_mfma<KP>(smem + 128 * wave * S::kRowBytes, r, h, hi, lo, acc);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (!in || row[i] < 0) continue;
+    float f[8];
+    if constexpr (kPartial) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = 0.f;
+      const float* pp = p.part + (int64_t)row[i] * p.n_out + col;
+      for (int k0 = 0; k0 < p.ks; k0 += 4) {  // four splits' loads together, added in order
+        f32x4 a[4], b[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float* at = pp + (int64_t)min(k0 + k, p.ks - 1) * p.rows * p.n_out;
+          a[k] = *reinterpret_cast<const f32x4*>(at);
+          b[k] = *reinterpret_cast<const f32x4*>(at + 4);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k0 + k < p.ks)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              f[e] += a[k][e];
+              f[4 + e] += b[k][e];
+            }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[2 * e] = bf16_lo(yv[i][e]);
+        f[2 * e + 1] = bf16_hi(yv[i][e]);
+      }
+    }
+    if (id >= 0) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) f[u] += acc[u][i];
+    }
+    u32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = pack_bf16x2(f[2 * e], f[2 * e + 1]);
+    if constexpr (!kPartial)
+      if (id < 0) o = yv[i];
+    *reinterpret_cast<u32x4*>(p.out + row[i] * p.out_stride + col) = o;
+  }
+}
+
+// Work-group = (sorted tile, up to kSortedCols columns of a slice): 16 rows a wavefront, all four the
+// same columns, which they walk 128 at a time. The walk's loads are one turn ahead of its
+// products: B's next rows and the base's next columns are in flight while this turn multiplies
+// and stores. t stays in registers: NP pieces of KP elements of the rank.
+constexpr int kSortedCols = 512;
+
+template <int KP, int NP>
+__global__ __launch_bounds__(kLoraThreads) void lora_expand_kernel(const LoraArgs p) {
+  using S = ExpandShape<KP>;
+  constexpr int kLoads = 128 * S::kChunks / kLoraThreads;
+  constexpr int kBuf = 128 * S::kRowBytes;
+  __shared__ __attribute__((aligned(16))) char smem[2 * kBuf];
+  __shared__ int32_t rows[kLoraTile];
+  const int32_t tile = blockIdx.x / p.col_groups;
+  int32_t id, begin;
+  if (!sorted_tile<kLoraTile>(p, tile, 0, rows, &id)) return;
+  if (id < 0 && p.out == p.y) return;  // rows without an adapter stay as they are
+  const int32_t q = group_slice(p, blockIdx.x - tile * p.col_groups, kSortedCols, &begin);
+  const int32_t end = min(begin + kSortedCols, p.slice_begin[q + 1]);
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int r = lane & 15, h = lane >> 4;
+  int32_t row[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) row[i] = rows[16 * wave + 4 * h + i];
+  const uint16_t* bp = p.b + max(id, 0) * p.b_adapter;
+  u32x4 st[kLoads], yv[4], hi[NP][S::kSteps], lo[NP][S::kSteps];
+  const auto load_b = [&](int32_t c0, int32_t j0) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int e = i * kLoraThreads + threadIdx.x, c = e / S::kChunks, j = j0 + e % S::kChunks * 8;
+      st[i] = u32x4{0u, 0u, 0u, 0u};
+      if (c0 + c < end && j < p.rank) st[i] = *reinterpret_cast<const u32x4*>(bp + (c0 + c) * p.b_row + j);
+    }
+  };
+  const auto load_y = [&](int32_t c0, u32x4 (&y)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c0 + 8 * r < end && row[i] >= 0)
+        y[i] = *reinterpret_cast<const u32x4*>(p.y + row[i] * p.y_stride + c0 + 8 * r);
+  };
+  if (id >= 0) load_b(begin, 0);
+  load_y(begin, yv);
+  if (id >= 0) {
+    const float* tp = p.t + (int64_t)max(rows[16 * wave + r], 0) * (p.num_slices * p.rank) + q * p.rank;
+#pragma unroll
+    for (int n = 0; n < NP; ++n) load_t<KP>(tp, p.rank, n * KP, h, hi[n], lo[n]);
+  }
+  int buf = 0;
+  for (int32_t c0 = begin; c0 < end; c0 += 128) {
+    u32x4 next[4];
+    f32x4 acc[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (c0 + 128 < end) load_y(c0 + 128, next);
+    if (id >= 0) {
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const int e = i * kLoraThreads + threadIdx.x;
+          *reinterpret_cast<u32x4*>(smem + buf * kBuf + S::at(e / S::kChunks) * S::kRowBytes + e % S::kChunks * 16) =
+              st[i];
+        }
+        if (n + 1 < NP) load_b(c0, (n + 1) * KP);
+        else if (c0 + 128 < end) load_b(c0 + 128, 0);
+        // one barrier a turn: the buffer written next was last read before it
+        lin_lds_barrier();
+        expand_mfma<KP>(smem + buf * kBuf, r, h, hi[n], lo[n], acc);
+        buf ^= 1;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (c0 + 8 * r >= end || row[i] < 0) continue;
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[2 * e] = bf16_lo(yv[i][e]) + acc[2 * e][i];
+        f[2 * e + 1] = bf16_hi(yv[i][e]) + acc[2 * e + 1][i];
+      }
+      u32x4 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = pack_bf16x2(f[2 * e], f[2 * e + 1]);
+      if (id < 0) o = yv[i];
+      // non-temporal: the lines are whole and nothing here reads them again
+      __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(p.out + row[i] * p.out_stride + c0 + 8 * r));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) yv[i] = next[i];
+  }
 }
 
 // ---------------------------------------------------------------- sorting ---------------
 
-// One work-group: rows per adapter (bucket num_adapters: none), the buckets' first positions and
-// tiles, then every row's position. A wavefront whose rows have one adapter, the common case
-// of a prefill step, counts them in one LDS atomic. Rows of one adapter come in any order.
+// One work-group: every row's place among the rows of its adapter (bucket num_adapters: none), the
+// buckets' first tiles, then every row's position. A lane has 4 neighbouring rows, a wavefront 256
+// at a time; 256 rows of one adapter, the common case of a prefill step, count as one entry, and the
+// entries of all kPlanTurns turns ask the counters in one LDS atomic, lane i for turn i. The work is
+// instructions on one CU, so what is done per row is what counts: 16384 rows of 8 adapters
+// 9.3 us with one row a lane.
+// Rows of one adapter come in any order, which no result shows: a row's sums are its own.
+typedef int32_t i32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+
 __global__ __launch_bounds__(kPlanThreads) void lora_plan_kernel(const LoraArgs p) {
-  extern __shared__ int32_t count[];  // num_adapters + 1
-  __shared__ int32_t part[2][kPlanThreads / kWave];
+  extern __shared__ int32_t count[];  // rows of every bucket, and behind them its first tile
+  __shared__ int32_t part[kPlanThreads / kWave];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int32_t buckets = p.num_adapters + 1;
+  int32_t* first_tile = count + buckets;
   for (int32_t b = threadIdx.x; b < buckets; b += kPlanThreads) count[b] = 0;
   __syncthreads();
-  const auto take = [&](int32_t row) -> int32_t {  // the row's place in its bucket's counter
-    const bool is_row = row < p.rows;
-    int32_t b = is_row ? adapter_of(p, row) : -1;
-    if (b < 0) b = p.num_adapters;
-    const uint64_t live = __ballot(is_row);
-    if (live == 0) return 0;
-    const int32_t first = __builtin_amdgcn_readfirstlane(b);  // (rows ascend with the lane: lane 0 is one)
-    if (__ballot(is_row && b != first) == 0) {
-      int32_t at = 0;
-      if (lane == 0) at = atomicAdd(count + first, __popcll(live));
-      return __builtin_amdgcn_readfirstlane(at) + lane;
+  constexpr int kTurn = 4 * kPlanThreads, kStep = kPlanTurns * kTurn;
+  const bool one_step = p.rows <= kStep;  // then adapters and places stay in registers
+  int32_t b[kPlanTurns][4], place[kPlanTurns][4];
+  const int32_t my_row = 4 * (int32_t)threadIdx.x;
+  const auto load_ids = [&](int32_t row0) {
+#pragma unroll
+    for (int i = 0; i < kPlanTurns; ++i) {
+      const int32_t row = row0 + i * kTurn + my_row;
+      if (row + 3 < p.rows) {
+        const i32x4_u v = *reinterpret_cast<const i32x4_u*>(p.ids + row);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[i][e] = v[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[i][e] = p.ids[min(row + e, p.rows - 1)];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[i][e] = b[i][e] >= 0 && b[i][e] < p.num_adapters ? b[i][e] : p.num_adapters;
     }
-    return is_row ? atomicAdd(count + b, 1) : 0;
   };
-  for (int32_t row0 = 0; row0 < p.rows; row0 += kPlanThreads) take(row0 + threadIdx.x);
+  for (int32_t row0 = 0; row0 < p.rows; row0 += kStep) {
+    load_ids(row0);
+    uint32_t mixed = 0;
+    int32_t bucket = 0, n = 0;  // of turn `lane`
+#pragma unroll
+    for (int i = 0; i < kPlanTurns; ++i) {
+      const int32_t left = p.rows - (row0 + i * kTurn + 4 * kWave * wave);  // rows from the wavefront's first on
+      if (left <= 0) continue;
+      // (rows past the end repeat the last one's id: the same bucket as a row that counts)
+      const int32_t first = __builtin_amdgcn_readfirstlane(b[i][0]);
+      const bool other = b[i][0] != first || b[i][1] != first || b[i][2] != first || b[i][3] != first;
+      if (__ballot(other) != 0) mixed |= 1u << i;
+      else if (lane == i) {
+        bucket = first;
+        n = min(left, 4 * kWave);
+      }
+    }
+    int32_t at = 0;
+    if (n > 0) at = atomicAdd(count + bucket, n);
+#pragma unroll
+    for (int i = 0; i < kPlanTurns; ++i) {
+      const int32_t row = row0 + i * kTurn + my_row, mine = min(p.rows - row, 4);
+      int32_t first = __builtin_amdgcn_readlane(at, i) + 4 * lane;
+      const bool same = b[i][0] == b[i][1] && b[i][0] == b[i][2] && b[i][0] == b[i][3];
+      if ((mixed >> i & 1) && same && mine > 0) first = atomicAdd(count + b[i][0], mine);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) place[i][e] = first + e;
+      if ((mixed >> i & 1) && !same) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < mine) place[i][e] = atomicAdd(count + b[i][e], 1);
+      }
+      if (!one_step) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < mine) p.place[row + e] = place[i][e];
+      }
+    }
+  }
   __syncthreads();
-  // first positions and first tiles of the buckets: exclusive sums over them, a stretch of
-  // neighbouring buckets a thread
+  // the buckets' first tiles: an exclusive sum over them, a stretch of neighbours a thread
   const int32_t per = (buckets + kPlanThreads - 1) / kPlanThreads;
   const int32_t b0 = min((int32_t)threadIdx.x * per, buckets), b1 = min(b0 + per, buckets);
-  int32_t n = 0, t = 0;
-  for (int32_t b = b0; b < b1; ++b) {
-    n += count[b];
-    t += (count[b] + kLoraTile - 1) / kLoraTile;
-  }
-  int32_t in = n, it = t;
+  int32_t t = 0;
+  for (int32_t i = b0; i < b1; ++i) t += (count[i] + kLoraTile - 1) / kLoraTile;
+  int32_t it = t;
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) {
-    const int32_t on = __shfl_up(in, d, kWave), ot = __shfl_up(it, d, kWave);
-    if (lane >= d) {
-      in += on;
-      it += ot;
-    }
+    const int32_t o = __shfl_up(it, d, kWave);
+    if (lane >= d) it += o;
   }
-  if (lane == kWave - 1) {
-    part[0][wave] = in;
-    part[1][wave] = it;
-  }
+  if (lane == kWave - 1) part[wave] = it;
   __syncthreads();
-  in -= n;
   it -= t;
   int32_t tiles = 0;
+#pragma unroll
   for (int w = 0; w < kPlanThreads / kWave; ++w) {
-    if (w < wave) {
-      in += part[0][w];
-      it += part[1][w];
-    }
-    tiles += part[1][w];
+    if (w < wave) it += part[w];
+    tiles += part[w];
   }
-  for (int32_t b = b0; b < b1; ++b) {
-    const int32_t c = count[b];
-    for (int32_t i = 0; i < c; i += kLoraTile)
-      p.tiles[it++] = make_int4(b < p.num_adapters ? b : -1, in + i, min(c - i, kLoraTile), 0);
-    count[b] = in;  // from here on the bucket's next free position
-    in += c;
+  for (int32_t i = b0; i < b1; ++i) {
+    first_tile[i] = it;
+    it += (count[i] + kLoraTile - 1) / kLoraTile;
   }
-  if (threadIdx.x == 0) *p.num_tiles = tiles;
+  for (int32_t i = tiles + threadIdx.x; i < p.max_tiles; i += kPlanThreads) p.tiles[i] = make_int2(-1, 0);
   __syncthreads();
-  for (int32_t row0 = 0; row0 < p.rows; row0 += kPlanThreads) {
-    const int32_t row = row0 + threadIdx.x;
-    const int32_t at = take(row);
-    if (row < p.rows) p.perm[at] = row;
+  // row `row` of bucket c at place `at`: its position, and its tile's record if it is the tile's first
+  const auto record = [&](int32_t c, int32_t at) {
+    p.tiles[first_tile[c] + at / kLoraTile] =
+        make_int2(c < p.num_adapters ? c : -1, min(count[c] - at, kLoraTile));
+  };
+  for (int32_t row0 = 0; row0 < p.rows; row0 += kStep) {
+    if (!one_step) load_ids(row0);
+#pragma unroll
+    for (int i = 0; i < kPlanTurns; ++i) {
+      const int32_t row = row0 + i * kTurn + my_row;
+      if (!one_step) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) place[i][e] = p.place[min(row + e, p.rows - 1)];
+      }
+      if (row >= p.rows) continue;
+      if (row + 3 < p.rows && b[i][0] == b[i][1] && b[i][0] == b[i][2] && b[i][0] == b[i][3]) {
+        // four places in a row (counted together)
+        const int32_t at = place[i][0], first = (at + kLoraTile - 1) / kLoraTile * kLoraTile;
+        *reinterpret_cast<i32x4_u*>(p.perm + (int64_t)first_tile[b[i][0]] * kLoraTile + at) =
+            i32x4_u{row, row + 1, row + 2, row + 3};
+        if (first < at + 4) record(b[i][0], first);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (row + e >= p.rows) continue;
+          const int32_t c = b[i][e], at = place[i][e];
+          p.perm[(int64_t)first_tile[c] * kLoraTile + at] = row + e;
+          if (at % kLoraTile == 0) record(c, at);
+        }
+      }
+    }
   }
 }
 
@@ -423,28 +730,49 @@ int64_t lora_max_tiles(int32_t rows, int32_t num_adapters) {
   return rows / kLoraTile + std::min<int64_t>((int64_t)num_adapters + 1, rows);
 }
 
-int32_t lora_col_groups(LoraArgs& p, int32_t group_cols) {
-  p.group_cols = group_cols;
-  p.col_groups = 0;
-  for (int q = 0; q < p.num_slices; ++q)
-    p.col_groups += (p.slice_begin[q + 1] - p.slice_begin[q] + group_cols - 1) / group_cols;
-  return p.col_groups;
+int32_t col_groups(const LoraArgs& p, int32_t cols) {
+  int32_t n = 0;
+  for (int q = 0; q < p.num_slices; ++q) n += (p.slice_begin[q + 1] - p.slice_begin[q] + cols - 1) / cols;
+  return n;
 }
 
-template <bool kSorted, bool kPartial>
-hipError_t launch_expand(const LoraArgs& p, int64_t tiles, hipStream_t stream) {
-  const dim3 grid((unsigned)(tiles * p.col_groups)), block(kLoraThreads);
-  const unsigned lds = (kSorted ? kLoraTile : kLoraSmallTile) * expand_row_bytes(p.rank);
-  if (p.rank <= 32)
-    hipLaunchKernelGGL((lora_expand_kernel<kSorted, 1, kPartial>), grid, block, lds, stream, p);
-  else if (p.rank <= 64)
-    hipLaunchKernelGGL((lora_expand_kernel<kSorted, 2, kPartial>), grid, block, lds, stream, p);
+template <int kBase>
+hipError_t launch_expand_small(LoraArgs p, hipStream_t stream) {
+  p.col_groups = col_groups(p, kSmallCols);
+  const dim3 grid((unsigned)(p.rows * p.col_groups)), block(kLoraThreads);
+  if (p.rank <= 16)
+    hipLaunchKernelGGL((lora_expand_small_kernel<16, kBase>), grid, block, 0, stream, p);
   else
-    hipLaunchKernelGGL((lora_expand_kernel<kSorted, 4, kPartial>), grid, block, lds, stream, p);
+    hipLaunchKernelGGL((lora_expand_small_kernel<32, kBase>), grid, block, 0, stream, p);
   return hipGetLastError();
 }
 
-size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
+// Whether a small addition computes t in the expand's work-groups (one launch, but every group of
+// 512 columns reads its adapter's A again): where all of them are on the GPU at once, two a CU up to
+// rank 16, one up to 32. Measured on the 1024 x 2048 projection, one launch and two, us: 128 rows
+// (256 work-groups) rank 16 6.3 and 8.1, rank 32 9.3 and 9.0; 300 rows (600) 13.7 and 10.5, 25.1 and 14.4.
+bool shrink_in_expand(const LoraArgs& p) {
+  return p.rank <= 32 && (int64_t)p.rows * col_groups(p, kSmallCols) <= (p.rank <= 16 ? 512 : 256);
+}
+
+hipError_t launch_expand_sorted(LoraArgs p, int64_t tiles, hipStream_t stream) {
+  p.col_groups = col_groups(p, kSortedCols);
+  const dim3 grid((unsigned)(tiles * p.col_groups)), block(kLoraThreads);
+  if (p.rank <= 16)
+    hipLaunchKernelGGL((lora_expand_kernel<16, 1>), grid, block, 0, stream, p);
+  else if (p.rank <= 32)
+    hipLaunchKernelGGL((lora_expand_kernel<32, 1>), grid, block, 0, stream, p);
+  else if (p.rank <= 64)
+    hipLaunchKernelGGL((lora_expand_kernel<64, 1>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((lora_expand_kernel<64, 2>), grid, block, 0, stream, p);
+  return hipGetLastError();
+}
+
+// Whether the projection's work-groups add the adapters themselves (the shrink before them) rather
+// than leave partial sums to an expand. Measured, us of the two forms: 97 rows, 1024 x 6144, rank 16
+// XX and 16.8; 1 row, 1024 x 4096 XX and 9.7.
+bool expand_in_linear(const LoraArgs& p, const LinCfg& c) { return c.ks == 1 && p.rank <= 16; }
 
 size_t t_bytes(const LoraArgs& p) { return (size_t)p.rows * p.num_slices * p.rank * sizeof(float); }
 
@@ -452,13 +780,13 @@ size_t t_bytes(const LoraArgs& p) { return (size_t)p.rows * p.num_slices * p.ran
 
 size_t lora_linear_workspace_bytes(const LoraArgs& p) {
   const LinCfg c = choose_config(p.rows, p.n_out / kLinTile, p.k, 1);
-  return t_bytes(p) + (size_t)c.ks * p.rows * p.n_out * sizeof(float);
+  return t_bytes(p) + (expand_in_linear(p, c) ? 0 : (size_t)c.ks * p.rows * p.n_out * sizeof(float));
 }
 
 size_t lora_add_workspace_bytes(const LoraArgs& p) {
   if (p.rows <= kLoraSmallRows) return t_bytes(p);
-  return t_bytes(p) + 16 + (size_t)lora_max_tiles(p.rows, p.num_adapters) * sizeof(int4) +
-         round16((size_t)p.rows * sizeof(int32_t));
+  return t_bytes(p) + (size_t)lora_max_tiles(p.rows, p.num_adapters) * (kLoraTile * sizeof(int32_t) + sizeof(int2)) +
+         (size_t)p.rows * sizeof(int32_t);
 }
 
 hipError_t launch_lora_linear(const LoraArgs& args, const void* w, int64_t w_stride, void* ws, hipStream_t stream) {
@@ -478,16 +806,40 @@ hipError_t launch_lora_linear(const LoraArgs& args, const void* w, int64_t w_str
   a.ks = c.ks;
   a.part = p.part;
   const int32_t lin_groups = (p.n_out / kLinTile) * c.ks * c.mgroups;
-  const int32_t shrink = p.num_adapters > 0 ? p.rows * ((p.num_slices * p.rank + 15) / 16) : 0;
+  const int32_t cols16 = (p.num_slices * p.rank + 15) / 16;
+  if (expand_in_linear(p, c)) {
+    if (p.num_adapters > 0) {
+      hipLaunchKernelGGL(lora_shrink_small_kernel, dim3(p.rows * cols16), dim3(kLoraThreads), 0, stream, p);
+      if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
+    }
+    a.y = p.out;
+    a.y_stride = p.out_stride;
+    switch (c.nb) {
+      case 1: hipLaunchKernelGGL(lora_linear_expand_kernel<1>, dim3(lin_groups), dim3(kLinThreads), 0, stream, a, p); break;
+      case 2: hipLaunchKernelGGL(lora_linear_expand_kernel<2>, dim3(lin_groups), dim3(kLinThreads), 0, stream, a, p); break;
+      default: hipLaunchKernelGGL(lora_linear_expand_kernel<4>, dim3(lin_groups), dim3(kLinThreads), 0, stream, a, p); break;
+    }
+    return hipGetLastError();
+  }
+  // 32 columns of t a work-group where there would be too many of 16 to be resident beside the
+  // projection's (two a CU): 128 rows, rank 64, k = 3072 11.8 us instead of 13.4
+  const bool wide = p.rows * cols16 >= 512;
+  const int32_t shrink = p.num_adapters > 0 ? p.rows * (wide ? (cols16 + 1) / 2 : cols16) : 0;
   const dim3 grid(lin_groups + shrink), block(kLinThreads);
+  const auto launch = [&](auto nb, auto cb) {
+    hipLaunchKernelGGL((lora_linear_kernel<nb.value, cb.value>), grid, block, 0, stream, a, p, lin_groups);
+  };
+  const auto launch_nb = [&](auto nb) {
+    if (wide) launch(nb, std::integral_constant<int, 2>{});
+    else launch(nb, std::integral_constant<int, 1>{});
+  };
   switch (c.nb) {
-    case 1: hipLaunchKernelGGL(lora_linear_kernel<1>, grid, block, 0, stream, a, p, lin_groups); break;
-    case 2: hipLaunchKernelGGL(lora_linear_kernel<2>, grid, block, 0, stream, a, p, lin_groups); break;
-    default: hipLaunchKernelGGL(lora_linear_kernel<4>, grid, block, 0, stream, a, p, lin_groups); break;
+    case 1: launch_nb(std::integral_constant<int, 1>{}); break;
+    case 2: launch_nb(std::integral_constant<int, 2>{}); break;
+    default: launch_nb(std::integral_constant<int, 4>{}); break;
   }
   if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
-  lora_col_groups(p, 64 * kLoraWaves);
-  return launch_expand<false, true>(p, p.rows, stream);
+  return launch_expand_small<kBasePartial>(p, stream);
 }
 
 hipError_t launch_lora_add(const LoraArgs& args, void* ws, hipStream_t stream) {
@@ -495,28 +847,37 @@ hipError_t launch_lora_add(const LoraArgs& args, void* ws, hipStream_t stream) {
   p.t = static_cast<float*>(ws);
   const int32_t width = p.num_slices * p.rank;
   if (p.rows <= kLoraSmallRows) {
+    if (shrink_in_expand(p)) return launch_expand_small<kBaseRowsShrink>(p, stream);
     if (p.num_adapters > 0) {
       hipLaunchKernelGGL(lora_shrink_small_kernel, dim3(p.rows * ((width + 15) / 16)), dim3(kLoraThreads), 0, stream,
                          p);
       if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
     }
-    lora_col_groups(p, 64 * kLoraWaves);
-    return launch_expand<false, false>(p, p.rows, stream);
+    return launch_expand_small<kBaseRows>(p, stream);
   }
   const int64_t tiles = lora_max_tiles(p.rows, p.num_adapters);
   char* at = static_cast<char*>(ws) + t_bytes(p);
-  p.num_tiles = reinterpret_cast<int32_t*>(at);
-  p.tiles = reinterpret_cast<int4*>(at + 16);
-  p.perm = reinterpret_cast<int32_t*>(at + 16 + tiles * sizeof(int4));
-  hipLaunchKernelGGL(lora_plan_kernel, dim3(1), dim3(kPlanThreads), (p.num_adapters + 1) * sizeof(int32_t), stream, p);
+  p.max_tiles = (int32_t)tiles;
+  p.perm = reinterpret_cast<int32_t*>(at);
+  p.tiles = reinterpret_cast<int2*>(p.perm + tiles * kLoraTile);
+  p.place = reinterpret_cast<int32_t*>(p.tiles + tiles);
+  hipLaunchKernelGGL(lora_plan_kernel, dim3(1), dim3(kPlanThreads), 2 * (p.num_adapters + 1) * sizeof(int32_t), stream,
+                     p);
   if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
   if (p.num_adapters > 0) {
-    hipLaunchKernelGGL(lora_shrink_kernel, dim3((unsigned)(tiles * ((width + 63) / 64))), dim3(kLoraThreads), 0, stream,
-                       p);
+    // at most 64 columns of t a work-group, shared evenly
+    const int32_t cols16 = (width + 15) / 16, blocks = (cols16 + 3) / 4, cb = (cols16 + blocks - 1) / blocks;
+    const int64_t parts = (tiles * (kLoraTile / kLoraShrinkRows) + 7) / 8 * 8;  // whole rounds of the XCDs
+    const dim3 grid((unsigned)(parts * ((width + 16 * cb - 1) / (16 * cb))));
+    switch (cb) {
+      case 1: hipLaunchKernelGGL(lora_shrink_kernel<1>, grid, dim3(kLoraThreads), 0, stream, p); break;
+      case 2: hipLaunchKernelGGL(lora_shrink_kernel<2>, grid, dim3(kLoraThreads), 0, stream, p); break;
+      case 3: hipLaunchKernelGGL(lora_shrink_kernel<3>, grid, dim3(kLoraThreads), 0, stream, p); break;
+      default: hipLaunchKernelGGL(lora_shrink_kernel<4>, grid, dim3(kLoraThreads), 0, stream, p); break;
+    }
     if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
   }
-  lora_col_groups(p, 64 * kLoraWaves);
-  return launch_expand<true, false>(p, tiles, stream);
+  return launch_expand_sorted(p, tiles, stream);
 }
 
 }  // namespace pk

@@ -15,54 +15,51 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import check, lib
-from .ops import _req_i32, _stream
+from ._call import call, scratch
+from ._lib import lib
+from .ops import _req_i32
 
 
 def _list_i32(name: str, t: torch.Tensor, device: torch.device) -> int:
     _req_i32(name, t, device)
-    if t.dim() != 1 or not t.is_contiguous():
+    shape = t.shape
+    if len(shape) != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous 1-D tensor")
-    return t.numel()
+    return shape[0]
 
 
 def _cache_args(k: torch.Tensor, v: torch.Tensor):
-    """(pointers, strides, sizes) of the C-ABI, and the block size, for a pair of caches."""
-    if k.dim() == 4 and v.dim() == 4:
-        k, v = k.unsqueeze(0), v.unsqueeze(0)
-    if k.dim() != 5 or v.shape != k.shape:
+    """(pointers, strides, sizes) of the C-ABI for a pair of caches, and their device."""
+    shape, ks, vs = k.shape, k.stride(), v.stride()
+    if v.shape != shape or len(shape) not in (4, 5):
         raise ValueError("caches must be two (L, NB, BS, Hkv, D) or (NB, BS, Hkv, D) tensors of one shape")
     if k.dtype != v.dtype or k.element_size() != 2:
         raise TypeError("caches must share one 16-bit dtype")
-    if k.device != v.device or k.device.type != "cuda":
-        raise ValueError(f"caches must be on one GPU, got {k.device} and {v.device}")
-    layers, blocks, block_size, heads, head_dim = k.shape
+    dev = k.device
+    if v.device != dev or dev.type != "cuda":
+        raise ValueError(f"caches must be on one GPU, got {dev} and {v.device}")
+    if len(shape) == 4:
+        shape, ks, vs = (1, *shape), (0, *ks), (0, *vs)
+    layers, blocks, block_size, heads, head_dim = shape
     row = heads * head_dim
-    for c in (k, v):
-        if c.stride()[2:] != (row, head_dim, 1):
-            raise ValueError("a block's rows must be contiguous (block_size x heads x head_dim)")
-    return (k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), k.stride(1), v.stride(1), layers, blocks,
-            block_size, row), k.device
+    if ks[2:] != (row, head_dim, 1) or vs[2:] != (row, head_dim, 1):
+        raise ValueError("a block's rows must be contiguous (block_size x heads x head_dim)")
+    return (k.data_ptr(), v.data_ptr(), ks[0], vs[0], ks[1], vs[1], layers, blocks, block_size, row), dev
 
 
 def _pool_args(block_tables: torch.Tensor, context_lens: torch.Tensor, ref_counts: torch.Tensor,
                device: torch.device):
     _req_i32("block_tables", block_tables, device)
-    if block_tables.dim() != 2 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+    shape, stride = block_tables.shape, block_tables.stride()
+    if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
         raise ValueError("block_tables must be (R, W) with contiguous rows")
-    rows, width = block_tables.shape
-    if rows > 1 and block_tables.stride(0) < width:
+    rows, width = shape
+    if rows > 1 and stride[0] < width:
         raise ValueError("block_tables' rows must not overlap")
     if _list_i32("context_lens", context_lens, device) != rows:
         raise ValueError(f"context_lens must have one length per row of block_tables ({rows})")
     _list_i32("ref_counts", ref_counts, device)
-    return block_tables.data_ptr(), max(block_tables.stride(0), width), rows, width, context_lens.data_ptr(), \
-        ref_counts.data_ptr()
-
-
-def _scratch(nbytes: int, device: torch.device) -> torch.Tensor:
-    # one buffer per call, from the capture's own pool under capture: no two graphs share it
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return block_tables.data_ptr(), max(stride[0], width), rows, width, context_lens.data_ptr(), ref_counts.data_ptr()
 
 
 def copy_blocks(k_caches: torch.Tensor, v_caches: torch.Tensor, src_blocks: torch.Tensor,
@@ -79,10 +76,8 @@ def copy_blocks(k_caches: torch.Tensor, v_caches: torch.Tensor, src_blocks: torc
     if _list_i32("dst_blocks", dst_blocks, dev) != pairs or \
             (num_tokens is not None and _list_i32("num_tokens", num_tokens, dev) != pairs):
         raise ValueError("src_blocks, dst_blocks and num_tokens must have one entry per pair")
-    with torch.cuda.device(dev):
-        check(lib().pk_copy_blocks(*args, src_blocks.data_ptr(), dst_blocks.data_ptr(),
-                                   0 if num_tokens is None else num_tokens.data_ptr(), pairs, _stream(k_caches)),
-              "pk_copy_blocks")
+    call(lib().pk_copy_blocks, "pk_copy_blocks", dev, *args, src_blocks.data_ptr(), dst_blocks.data_ptr(),
+         0 if num_tokens is None else num_tokens.data_ptr(), pairs)
 
 
 def fork_sequences(k_caches: torch.Tensor, v_caches: torch.Tensor, block_tables: torch.Tensor,
@@ -106,11 +101,9 @@ def fork_sequences(k_caches: torch.Tensor, v_caches: torch.Tensor, block_tables:
         raise ValueError("parents and children must have one entry per fork")
     new_blocks = torch.empty(n, dtype=torch.int32, device=dev)
     nbytes = lib().pk_fork_workspace_bytes(n)
-    ws = _scratch(nbytes, dev)
-    with torch.cuda.device(dev):
-        check(lib().pk_fork_sequences(*args, *pool, parents.data_ptr(), children.data_ptr(), n,
-                                      new_blocks.data_ptr(), ws.data_ptr(), nbytes, _stream(k_caches)),
-              "pk_fork_sequences")
+    ws = scratch(nbytes, dev)
+    call(lib().pk_fork_sequences, "pk_fork_sequences", dev, *args, *pool, parents.data_ptr(), children.data_ptr(), n,
+         new_blocks.data_ptr(), ws.data_ptr(), nbytes)
     return new_blocks
 
 
@@ -127,9 +120,8 @@ def extend_sequences(block_tables: torch.Tensor, context_lens: torch.Tensor, ref
     pool = _pool_args(block_tables, context_lens, ref_counts, dev)
     n = _list_i32("rows", rows, dev)
     slots = torch.empty(n, dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
-        check(lib().pk_extend_sequences(*pool, ref_counts.numel(), int(block_size), rows.data_ptr(), n,
-                                        slots.data_ptr(), _stream(block_tables)), "pk_extend_sequences")
+    call(lib().pk_extend_sequences, "pk_extend_sequences", dev, *pool, ref_counts.numel(), int(block_size),
+         rows.data_ptr(), n, slots.data_ptr())
     return slots
 
 
@@ -141,9 +133,8 @@ def free_sequences(block_tables: torch.Tensor, context_lens: torch.Tensor, ref_c
     dev = block_tables.device
     pool = _pool_args(block_tables, context_lens, ref_counts, dev)
     n = _list_i32("rows", rows, dev)
-    with torch.cuda.device(dev):
-        check(lib().pk_free_sequences(*pool, ref_counts.numel(), int(block_size), rows.data_ptr(), n,
-                                      _stream(block_tables)), "pk_free_sequences")
+    call(lib().pk_free_sequences, "pk_free_sequences", dev, *pool, ref_counts.numel(), int(block_size),
+         rows.data_ptr(), n)
 
 
 def compact_blocks(k_caches: torch.Tensor, v_caches: torch.Tensor, block_tables: torch.Tensor,
@@ -159,8 +150,7 @@ def compact_blocks(k_caches: torch.Tensor, v_caches: torch.Tensor, block_tables:
     block_map = torch.empty_like(ref_counts)
     num_live = torch.empty(1, dtype=torch.int32, device=dev)
     nbytes = lib().pk_compact_workspace_bytes(args[7])
-    ws = _scratch(nbytes, dev)
-    with torch.cuda.device(dev):
-        check(lib().pk_compact_blocks(*args, *pool, block_map.data_ptr(), num_live.data_ptr(), ws.data_ptr(), nbytes,
-                                      _stream(k_caches)), "pk_compact_blocks")
+    ws = scratch(nbytes, dev)
+    call(lib().pk_compact_blocks, "pk_compact_blocks", dev, *args, *pool, block_map.data_ptr(), num_live.data_ptr(),
+         ws.data_ptr(), nbytes)
     return block_map, num_live

@@ -20,8 +20,9 @@ from functools import lru_cache
 
 import torch
 
-from ._lib import check, lib
-from .ops import LINEAR_MAX_ROWS, _given_workspace, _req_i32, _rows2d, _stream
+from ._call import call, scratch
+from ._lib import lib
+from .ops import LINEAR_MAX_ROWS, _given_workspace, _req_i32
 
 
 @lru_cache(maxsize=256)
@@ -32,54 +33,55 @@ def _slices(slices: tuple[int, ...] | None, n_out: int):
     return (ctypes.c_int32 * len(widths))(*widths), len(widths)
 
 
-def _adapter_args(x, n_out, lora_a, lora_b, adapter_ids, scales, slices):
+def _rows2d(name: str, t: torch.Tensor, device: torch.device) -> tuple[torch.Size, int]:
+    """(shape, row stride) of a 2-D bf16 tensor with contiguous rows on the device."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or t.dtype != torch.bfloat16 or stride[1] != 1:
+        raise ValueError(f"{name} must be a 2-D bf16 tensor with contiguous rows")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    return shape, stride[0]
+
+
+def _adapter_args(rows, k, n_out, dev, lora_a, lora_b, adapter_ids, scales, slices):
     """The adapter arguments of the C-ABI, after the checks both operators share."""
-    _rows2d("x", x)
-    rows, k = x.shape
-    dev = x.device
     arr, num_slices = _slices(None if slices is None else tuple(slices), n_out)
-    for name, t in (("lora_a", lora_a), ("lora_b", lora_b)):
-        if t.dim() != 3 or t.dtype != torch.bfloat16 or t.stride(2) != 1:
+    a_shape, a_stride, b_shape, b_stride = lora_a.shape, lora_a.stride(), lora_b.shape, lora_b.stride()
+    for name, t, stride in (("lora_a", lora_a, a_stride), ("lora_b", lora_b, b_stride)):
+        if len(stride) != 3 or t.dtype != torch.bfloat16 or stride[2] != 1:
             raise ValueError(f"{name} must be a 3-D bf16 tensor with contiguous rows")
         if t.device != dev:
             raise ValueError(f"{name} is on {t.device}, expected {dev}")
-    adapters, _, rank = lora_b.shape
-    if lora_b.shape[1] != n_out or lora_a.shape != (adapters, num_slices * rank, k):
-        raise ValueError(f"lora_a {tuple(lora_a.shape)} and lora_b {tuple(lora_b.shape)} must be (L, {num_slices} * r, "
-                         f"{k}) and (L, {n_out}, r)")
+    adapters, b_rows, rank = b_shape
+    if b_rows != n_out or a_shape != (adapters, num_slices * rank, k):
+        raise ValueError(f"lora_a {tuple(a_shape)} and lora_b {tuple(b_shape)} must be (L, {num_slices} * r, {k}) and "
+                         f"(L, {n_out}, r)")
     _req_i32("adapter_ids", adapter_ids, dev)
     if adapter_ids.shape != (rows,) or not adapter_ids.is_contiguous():
         raise ValueError(f"adapter_ids must be a contiguous ({rows},) tensor")
     if scales is not None and (scales.dtype != torch.float32 or scales.shape != (adapters,) or scales.device != dev or
                                not scales.is_contiguous()):
         raise ValueError(f"scales must be a contiguous ({adapters},) float32 tensor on {dev}")
-    return (lora_a.data_ptr(), lora_a.stride(0), lora_a.stride(1), lora_b.data_ptr(), lora_b.stride(0),
-            lora_b.stride(1), adapters, rank, adapter_ids.data_ptr(), 0 if scales is None else scales.data_ptr(), arr,
-            num_slices)
+    return (lora_a.data_ptr(), a_stride[0], a_stride[1], lora_b.data_ptr(), b_stride[0], b_stride[1], adapters, rank,
+            adapter_ids.data_ptr(), 0 if scales is None else scales.data_ptr(), arr, num_slices)
 
 
 def _out(out, rows, n_out, dev):
     if out is None:
-        return torch.empty(rows, n_out, dtype=torch.bfloat16, device=dev)
-    _rows2d("out", out)
-    if out.shape != (rows, n_out) or out.device != dev:
-        raise ValueError(f"out must be a ({rows}, {n_out}) tensor on {dev}")
-    return out
+        return torch.empty(rows, n_out, dtype=torch.bfloat16, device=dev), n_out
+    shape, stride = _rows2d("out", out, dev)
+    if shape != (rows, n_out):
+        raise ValueError(f"out must be a ({rows}, {n_out}) tensor")
+    return out, stride
 
 
+@lru_cache(maxsize=4096)
 def lora_workspace_bytes(rows: int, n_out: int, k: int, rank: int, num_slices: int = 1, num_adapters: int = 0,
                          linear: bool = False) -> int:
     """Scratch bytes of one lora_add call, or with linear=True of one lora_linear call."""
     if linear:
         return int(lib().pk_lora_linear_workspace_bytes(rows, n_out, k, rank, num_slices))
     return int(lib().pk_lora_add_workspace_bytes(rows, rank, num_slices, num_adapters))
-
-
-def _scratch(workspace, nbytes, dev):
-    # one buffer per call, from the capture's own pool under capture: no two graphs share it
-    if workspace is None:
-        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    return _given_workspace(workspace, nbytes, dev)
 
 
 def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
@@ -89,22 +91,19 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     weight (n_out, k) bf16, adapter_ids (rows,) int32. The projection's sums are not rounded before
     the adapter is added. workspace: optional caller-owned uint8 scratch of
     lora_workspace_bytes(..., linear=True) bytes; calls that may overlap must not share one."""
-    _rows2d("weight", weight)
-    n_out = weight.shape[0]
-    args = _adapter_args(x, n_out, lora_a, lora_b, adapter_ids, scales, slices)
-    rows, k = x.shape
     dev = x.device
-    if weight.shape[1] != k or weight.device != dev:
-        raise ValueError(f"weight {tuple(weight.shape)} on {weight.device} does not match x {tuple(x.shape)} on {dev}")
+    (rows, k), x_stride = _rows2d("x", x, dev)
+    (n_out, w_k), w_stride = _rows2d("weight", weight, dev)
+    if w_k != k:
+        raise ValueError(f"weight {tuple(weight.shape)} does not match x {tuple(x.shape)}")
     if rows > LINEAR_MAX_ROWS:
         raise ValueError(f"decode-step linear layers take at most {LINEAR_MAX_ROWS} rows, got {rows}")
-    out = _out(out, rows, n_out, dev)
-    nbytes = lib().pk_lora_linear_workspace_bytes(rows, n_out, k, args[7], args[11])
-    ws = _scratch(workspace, nbytes, dev)
-    with torch.cuda.device(dev):
-        check(lib().pk_lora_linear(x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), rows, n_out, k,
-                                   *args, out.data_ptr(), out.stride(0), ws.data_ptr(), nbytes, _stream(x)),
-              "pk_lora_linear")
+    args = _adapter_args(rows, k, n_out, dev, lora_a, lora_b, adapter_ids, scales, slices)
+    out, out_stride = _out(out, rows, n_out, dev)
+    nbytes = lora_workspace_bytes(rows, n_out, k, args[7], args[11], linear=True)
+    ws = scratch(nbytes, dev) if workspace is None else _given_workspace(workspace, nbytes, dev)
+    call(lib().pk_lora_linear, "pk_lora_linear", dev, x.data_ptr(), x_stride, weight.data_ptr(), w_stride, rows, n_out,
+         k, *args, out.data_ptr(), out_stride, ws.data_ptr(), nbytes)
     return out
 
 
@@ -114,17 +113,15 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: tor
     """y plus every row's own adapter applied to x: y (rows, n_out) bf16 is the projection's output,
     x (rows, k) bf16 its input. out may be y (in place); otherwise rows without an adapter are
     copied. workspace: optional caller-owned uint8 scratch of lora_workspace_bytes(...) bytes."""
-    _rows2d("y", y)
-    n_out = y.shape[1]
-    args = _adapter_args(x, n_out, lora_a, lora_b, adapter_ids, scales, slices)
-    rows, k = x.shape
     dev = x.device
-    if y.shape[0] != rows or y.device != dev:
-        raise ValueError(f"y {tuple(y.shape)} on {y.device} does not match x {tuple(x.shape)} on {dev}")
-    out = _out(out, rows, n_out, dev)
-    nbytes = lib().pk_lora_add_workspace_bytes(rows, args[7], args[11], args[6])
-    ws = _scratch(workspace, nbytes, dev)
-    with torch.cuda.device(dev):
-        check(lib().pk_lora_add(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), rows, n_out, k, *args,
-                                out.data_ptr(), out.stride(0), ws.data_ptr(), nbytes, _stream(x)), "pk_lora_add")
+    (rows, k), x_stride = _rows2d("x", x, dev)
+    (y_rows, n_out), y_stride = _rows2d("y", y, dev)
+    if y_rows != rows:
+        raise ValueError(f"y {tuple(y.shape)} does not match x {tuple(x.shape)}")
+    args = _adapter_args(rows, k, n_out, dev, lora_a, lora_b, adapter_ids, scales, slices)
+    out, out_stride = _out(out, rows, n_out, dev)
+    nbytes = lora_workspace_bytes(rows, n_out, k, args[7], args[11], args[6])
+    ws = scratch(nbytes, dev) if workspace is None else _given_workspace(workspace, nbytes, dev)
+    call(lib().pk_lora_add, "pk_lora_add", dev, y.data_ptr(), y_stride, x.data_ptr(), x_stride, rows, n_out, k, *args,
+         out.data_ptr(), out_stride, ws.data_ptr(), nbytes)
     return out

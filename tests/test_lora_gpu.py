@@ -95,7 +95,7 @@ def test_linear_against_formula(gpu, rows, proj, rank, adapters, ids):
     (1, QKV, 16, 4, 1), (2, (8, (32,)), 8, 2, "mixed"), (63, (40, (32, 32)), 16, 3, "mixed"),
     (64, (1000, (96,)), 32, 3, "mixed"), (65, (1032, (160, 32, 32, 64)), 128, 3, "mixed"), (300, O, 8, 24, "mixed"),
     (512, QKV, 16, 600, "mixed"), (513, QKV, 16, 8, "runs"), (513, (40, (32, 32)), 40, 1, 0),
-    (600, (264, (288,)), 72, 8191, "mixed"), (700, (1000, (96, 64)), 24, 3, "mixed"), (1025, DOWN, 64, 7, "runs"),
+    (600, (264, (288,)), 72, 4095, "mixed"), (700, (1000, (96, 64)), 24, 3, "mixed"), (1025, DOWN, 64, 7, "runs"),
     (2000, GATE_UP, 128, 5, "runs"), (3001, O, 16, 50, "mixed"), (1500, (64, (32,)), 8, 4, -1)])
 def test_add_against_formula(gpu, rows, proj, rank, adapters, ids):
     k, widths = proj

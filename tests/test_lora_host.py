@@ -59,7 +59,7 @@ def test_refusals_of_one():
     assert _call("pk_lora_add", y=None) == _lib.PK_ERR_INVALID_ARG
     assert _call("pk_lora_add", y_stride=56) == _lib.PK_ERR_INVALID_ARG
     assert _call("pk_lora_add", y_stride=72) == _lib.PK_ERR_INVALID_ARG             # out is y, other rows
-    assert _call("pk_lora_add", rows=513, adapters=8192) == _lib.PK_ERR_UNSUPPORTED
+    assert _call("pk_lora_add", rows=513, adapters=4096) == _lib.PK_ERR_UNSUPPORTED
     assert _call("pk_lora_add", rows=2 ** 22 + 1) == _lib.PK_ERR_UNSUPPORTED
     for name in ("pk_lora_linear", "pk_lora_add"):
         assert _call(name, rows=0, x=None, ids=None, out=None, ws=None, ws_bytes=0) == _lib.PK_OK
@@ -68,10 +68,13 @@ def test_refusals_of_one():
 def test_workspace_sizes():
     lib = _lib.lib()
     assert lib.pk_lora_add_workspace_bytes(100, 16, 3, 8) == 100 * 48 * 4
-    # sorted: t, the tiles' number and list, the rows' positions
-    assert lib.pk_lora_add_workspace_bytes(1000, 16, 3, 8) == 1000 * 48 * 4 + 16 + (15 + 9) * 16 + 4000
-    base = lib.pk_linear_workspace_bytes(100, 1024, 1024, 2)
-    assert lib.pk_lora_linear_workspace_bytes(100, 1024, 1024, 16, 1) == base + 100 * 16 * 4
+    # sorted: t, the rows of the tiles, their records, the rows' places
+    assert lib.pk_lora_add_workspace_bytes(1000, 16, 3, 8) == 1000 * 48 * 4 + (15 + 9) * (256 + 8) + 4000
+    # t, and the projection's partial sums where it leaves them (K split, or ranks above 16)
+    base = lib.pk_linear_workspace_bytes(100, 1024, 2048, 2)
+    assert lib.pk_lora_linear_workspace_bytes(100, 1024, 2048, 16, 1) == base + 100 * 16 * 4
+    assert lib.pk_lora_linear_workspace_bytes(100, 4096, 1024, 24, 3) == 100 * (4096 + 72) * 4
+    assert lib.pk_lora_linear_workspace_bytes(100, 4096, 1024, 16, 3) == 100 * 48 * 4
     assert lib.pk_lora_linear_workspace_bytes(129, 1024, 1024, 16, 1) == 0
 
 
