@@ -34,7 +34,6 @@ namespace {
 constexpr int kLoraThreads = 256;
 constexpr int kLoraWaves = kLoraThreads / kWave;
 constexpr int kLoraTile = 64;        // rows of a sorted tile
-constexpr int kLoraShrinkRows = 32;  // of which a shrink work-group takes
 constexpr int kLoraSmallTile = 16;   // rows of a tile that is not sorted
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanTurns = 4;        // turns of 4096 rows whose ids are loaded together
@@ -214,19 +213,18 @@ __global__ __launch_bounds__(kLoraThreads) void lora_shrink_small_kernel(const L
   shrink_small<1>(p, blockIdx.x, rows, smem);
 }
 
-// Work-group = (32 rows of a sorted tile, 16 CB columns of t).
-template <int CB>
+// Work-group = (R rows of a sorted tile, 16 CB columns of t).
+template <int R, int CB>
 __global__ __launch_bounds__(kLoraThreads) void lora_shrink_kernel(const LoraArgs p) {
-  __shared__ __attribute__((aligned(16))) char smem[shrink_smem_bytes(kLoraShrinkRows, CB)];
-  __shared__ int32_t rows[kLoraShrinkRows];
+  __shared__ __attribute__((aligned(16))) char smem[shrink_smem_bytes(R, CB)];
+  __shared__ int32_t rows[R];
   const int32_t blocks = (p.num_slices * p.rank + 16 * CB - 1) / (16 * CB);
   // the blocks of one tile's rows are 8 work-groups apart: one XCD, whose L2 gives the rows to all
   const int32_t part = blockIdx.x / (8 * blocks) * 8 + blockIdx.x % 8, block = blockIdx.x % (8 * blocks) / 8;
+  constexpr int kParts = kLoraTile / R;
   int32_t id;
-  if (!sorted_tile<kLoraShrinkRows>(p, part / (kLoraTile / kLoraShrinkRows),
-                                    part % (kLoraTile / kLoraShrinkRows) * kLoraShrinkRows, rows, &id) || id < 0)
-    return;
-  shrink_to_memory<kLoraShrinkRows, CB, 1>(p, id, block * 16 * CB, rows, smem);
+  if (!sorted_tile<R>(p, part / kParts, part % kParts * R, rows, &id) || id < 0) return;
+  shrink_to_memory<R, CB, 1>(p, id, block * 16 * CB, rows, smem);
 }
 
 // The partial sums of a decode step's projection (work-groups [0, lin_groups)) and the shrink of its
@@ -531,7 +529,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_kernel(const LoraArg
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (c0 + 8 * r < end && row[i] >= 0)
-        y[i] = *reinterpret_cast<const u32x4*>(p.y + row[i] * p.y_stride + c0 + 8 * r);
+        y[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p.y + row[i] * p.y_stride + c0 + 8 * r));
   };
   if (id >= 0) load_b(begin, 0);
   load_y(begin, yv);
@@ -577,7 +575,8 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_kernel(const LoraArg
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = pack_bf16x2(f[2 * e], f[2 * e + 1]);
       if (id < 0) o = yv[i];
-      // non-temporal: the lines are whole and nothing here reads them again
+      // base and out non-temporal: whole lines, used once (16384 rows on qkv, caches cold: 74.0 us for
+      // the three launches, 77.7 with ordinary loads, 81.7 with ordinary stores as well)
       __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(p.out + row[i] * p.out_stride + c0 + 8 * r));
     }
 #pragma unroll
@@ -755,6 +754,30 @@ bool shrink_in_expand(const LoraArgs& p) {
   return p.rank <= 32 && (int64_t)p.rows * col_groups(p, kSmallCols) <= (p.rank <= 16 ? 512 : 256);
 }
 
+template <int R>
+void launch_shrink_rows(const LoraArgs& p, int64_t tiles, int32_t cb, int32_t blocks, hipStream_t stream) {
+  const int64_t parts = (tiles * (kLoraTile / R) + 7) / 8 * 8;  // whole rounds of the XCDs
+  const dim3 grid((unsigned)(parts * blocks)), block(kLoraThreads);
+  switch (cb) {
+    case 1: hipLaunchKernelGGL((lora_shrink_kernel<R, 1>), grid, block, 0, stream, p); break;
+    case 2: hipLaunchKernelGGL((lora_shrink_kernel<R, 2>), grid, block, 0, stream, p); break;
+    case 3: hipLaunchKernelGGL((lora_shrink_kernel<R, 3>), grid, block, 0, stream, p); break;
+    default: hipLaunchKernelGGL((lora_shrink_kernel<R, 4>), grid, block, 0, stream, p); break;
+  }
+}
+
+// At most 64 columns of t a work-group, shared evenly. 64 rows a work-group read A half as often as
+// 32, where that still fills the GPU one and a half times: 13001 rows, t of 128 columns 13.8 us and
+// 16.5; 16384 rows, t of 48 columns (256 work-groups of 64 rows) 11.4 and 10.0.
+void launch_shrink_sorted(const LoraArgs& p, int64_t tiles, hipStream_t stream) {
+  const int32_t cols16 = (p.num_slices * p.rank + 15) / 16, n = (cols16 + 3) / 4, cb = (cols16 + n - 1) / n;
+  const int32_t blocks = (cols16 + cb - 1) / cb;
+  if ((int64_t)p.rows / 64 * blocks >= 384)
+    launch_shrink_rows<64>(p, tiles, cb, blocks, stream);
+  else
+    launch_shrink_rows<32>(p, tiles, cb, blocks, stream);
+}
+
 hipError_t launch_expand_sorted(LoraArgs p, int64_t tiles, hipStream_t stream) {
   p.col_groups = col_groups(p, kSortedCols);
   const dim3 grid((unsigned)(tiles * p.col_groups)), block(kLoraThreads);
@@ -865,16 +888,7 @@ hipError_t launch_lora_add(const LoraArgs& args, void* ws, hipStream_t stream) {
                      p);
   if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
   if (p.num_adapters > 0) {
-    // at most 64 columns of t a work-group, shared evenly
-    const int32_t cols16 = (width + 15) / 16, blocks = (cols16 + 3) / 4, cb = (cols16 + blocks - 1) / blocks;
-    const int64_t parts = (tiles * (kLoraTile / kLoraShrinkRows) + 7) / 8 * 8;  // whole rounds of the XCDs
-    const dim3 grid((unsigned)(parts * ((width + 16 * cb - 1) / (16 * cb))));
-    switch (cb) {
-      case 1: hipLaunchKernelGGL(lora_shrink_kernel<1>, grid, dim3(kLoraThreads), 0, stream, p); break;
-      case 2: hipLaunchKernelGGL(lora_shrink_kernel<2>, grid, dim3(kLoraThreads), 0, stream, p); break;
-      case 3: hipLaunchKernelGGL(lora_shrink_kernel<3>, grid, dim3(kLoraThreads), 0, stream, p); break;
-      default: hipLaunchKernelGGL(lora_shrink_kernel<4>, grid, dim3(kLoraThreads), 0, stream, p); break;
-    }
+    launch_shrink_sorted(p, tiles, stream);
     if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
   }
   return launch_expand_sorted(p, tiles, stream);

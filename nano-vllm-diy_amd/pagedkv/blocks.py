@@ -20,9 +20,13 @@ from ._lib import lib
 from .ops import _req_i32
 
 
+_I32 = torch.int32
+
+
 def _list_i32(name: str, t: torch.Tensor, device: torch.device) -> int:
-    _req_i32(name, t, device)
     shape = t.shape
+    if t.dtype is not _I32 or t.device != device:
+        _req_i32(name, t, device)
     if len(shape) != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous 1-D tensor")
     return shape[0]
@@ -49,7 +53,8 @@ def _cache_args(k: torch.Tensor, v: torch.Tensor):
 
 def _pool_args(block_tables: torch.Tensor, context_lens: torch.Tensor, ref_counts: torch.Tensor,
                device: torch.device):
-    _req_i32("block_tables", block_tables, device)
+    if block_tables.dtype is not _I32 or block_tables.device != device:
+        _req_i32("block_tables", block_tables, device)
     shape, stride = block_tables.shape, block_tables.stride()
     if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
         raise ValueError("block_tables must be (R, W) with contiguous rows")
