@@ -14,6 +14,8 @@ Context (src/utils/context.py:5-14), built by the runner (model_runner.py:174-23
   sequences that hold them (results within the attention tolerance of the plain path).
   0 states that no block is shared (and allows the one-launch store + decode); None keeps
   the library default.
+* adapter_ids (an addition): (N,) int32 adapter of every new token, -1 for none; read by a model
+  that has adapters bound (Qwen3Model.bind_adapters). None: the base model for every token.
 """
 from __future__ import annotations
 
@@ -33,3 +35,4 @@ class Context:
     context_lens: Tensor | None = None
     block_tables: Tensor | None = None
     cached_prefix_keys: int | None = None
+    adapter_ids: Tensor | None = None

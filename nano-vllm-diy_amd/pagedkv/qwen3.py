@@ -11,7 +11,8 @@ Per layer (qwen3.py:155-169):
     h = silu_and_mul(x W_gate_up^T) W_down^T                        qwen3.py:119-123
 and the final norm (qwen3.py:194). Weights are random (the serving benchmark runs a
 random-init model of the Qwen3-0.6B geometry); the LM head is tied to the embedding
-(qwen3.py:215-216).
+(qwen3.py:215-216). With adapters bound (an addition), every token's own low-rank adapter is
+added to each of the four projections.
 """
 from __future__ import annotations
 
@@ -20,7 +21,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
-from . import ops
+from . import lora, ops
 from .context import Context
 
 
@@ -62,6 +63,27 @@ class Qwen3Weights:
         self.final_norm = torch.ones(H, **bf)
 
 
+class Qwen3Adapters:
+    """Low-rank adapters for all four projections of every layer, as lora_linear / lora_add take them:
+    per layer and projection (A, B) of num_adapters adapters, bf16, random-normal; scales (alpha / r)
+    in fp32. The merged projections' slices are the layers merged in them (q, k, v; gate, up)."""
+
+    def __init__(self, cfg: Qwen3Config, num_adapters: int, rank: int, device: torch.device, seed: int = 6,
+                 std: float = 0.02, scale: float = 2.0):
+        g = torch.Generator(device=device).manual_seed(seed)
+        H, D, inter = cfg.hidden_size, cfg.head_dim, cfg.intermediate_size
+        qd, kvd = cfg.num_attention_heads * D, cfg.num_key_value_heads * D
+        self.slices = dict(qkv=(qd, kvd, kvd), o=(H,), gate_up=(inter, inter), down=(H,))
+        width = dict(qkv=H, o=qd, gate_up=H, down=inter)
+
+        def randn(*shape):
+            return (torch.randn(*shape, generator=g, device=device) * std).to(torch.bfloat16)
+
+        self.layers = [{name: (randn(num_adapters, len(s) * rank, width[name]), randn(num_adapters, sum(s), rank))
+                        for name, s in self.slices.items()} for _ in range(cfg.num_hidden_layers)]
+        self.scales = torch.full((num_adapters,), scale, dtype=torch.float32, device=device)
+
+
 class Qwen3Model:
     """Forward over one step's tokens; K/V caches are (L, NB, BS, Hkv, D) per operand."""
 
@@ -76,6 +98,11 @@ class Qwen3Model:
         dev = weights.embed.device
         self.cos_sin = ops.rope_cos_sin(max_position, cfg.head_dim, cfg.rope_theta, dev)
         self.scale = cfg.head_dim ** -0.5
+        self.adapters: Qwen3Adapters | None = None
+
+    def bind_adapters(self, adapters: Qwen3Adapters | None) -> None:
+        """Adapters for the tokens whose Context names one (ctx.adapter_ids); None: none."""
+        self.adapters = adapters
 
     def bind_caches(self, k_caches: torch.Tensor | None, v_caches: torch.Tensor | None) -> None:
         """Per-layer K/V cache views, (L, NB, BS, Hkv, D) per operand (model_runner.py:161-165)."""
@@ -103,7 +130,9 @@ class Qwen3Model:
         decode-step linear kernels, each fused with the op after it: qkv_proj; o_proj + the
         post-attention RMSNorm; gate_up_proj + SiluAndMul; down_proj + the next layer's input
         RMSNorm (the final norm after the last layer). Larger steps use F.linear (a library
-        GEMM) and the separate norm / activation kernels. Rounding points are the same."""
+        GEMM) and the separate norm / activation kernels. Rounding points are the same.
+        With adapters (bind_adapters and ctx.adapter_ids) every projection is lora_linear, or
+        F.linear and lora_add, followed by the separate kernels."""
         cfg, W = self.cfg, self.w
         Hq, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         eps = cfg.rms_norm_eps
@@ -112,6 +141,18 @@ class Qwen3Model:
         # a decode step: every sequence has one new token (cu_seqlens_q = arange), read
         # through block tables; the producer then runs inside the attention launch
         decode = not flat and ctx.max_seqlen_q == 1 and input_ids.shape[0] == ctx.cu_seqlens_q.numel() - 1
+        ad = self.adapters if ctx.adapter_ids is not None else None
+
+        def project(x, L, li, name):
+            """x through a projection and its adapters, or the projection alone"""
+            if ad is None:
+                return ops.linear(x, L[name]) if small else F.linear(x, L[name])
+            args = (*ad.layers[li][name], ctx.adapter_ids, ad.scales, ad.slices[name])
+            if small:
+                return lora.lora_linear(x, L[name], *args)
+            y = F.linear(x, L[name])
+            return lora.lora_add(y, x, *args, out=y)
+
         h = F.embedding(input_ids, W.embed)
         residual = None
         nl = len(W.layers)
@@ -121,7 +162,7 @@ class Qwen3Model:
                 residual = h
             elif not small:
                 x, residual = ops.add_rmsnorm(h, L["input_norm"], eps, residual=residual)
-            qkv = ops.linear(x, L["qkv"]) if small else F.linear(x, L["qkv"])
+            qkv = project(x, L, li, "qkv")
             kc, vc = (None, None) if self.k_caches is None else (self.k_caches[li], self.v_caches[li])
             if decode:
                 # one launch: q/k norm + RoPE, the K/V store and paged decode attention; no
@@ -140,17 +181,19 @@ class Qwen3Model:
                     o = ops.varlen_attention(q, kc, vc, ctx.cu_seqlens_q, ctx.cu_seqlens_k,
                                              ctx.max_seqlen_q, ctx.max_seqlen_k, self.scale, True,
                                              ctx.block_tables, cached_prefix_keys=0)
-            if small:
+            if small and ad is None:
                 x, residual = ops.linear_add_rmsnorm(o.view(-1, Hq * D), L["o"], residual,
                                                      L["post_norm"], eps, residual_out=residual)
                 nxt = W.layers[li + 1]["input_norm"] if li + 1 < nl else W.final_norm
                 x, residual = ops.linear_add_rmsnorm(ops.linear_silu_mul(x, L["gate_up"]), L["down"],
                                                      residual, nxt, eps, residual_out=residual)
             else:
-                h = F.linear(o.view(-1, Hq * D), L["o"])
+                h = project(o.view(-1, Hq * D), L, li, "o")
                 x, residual = ops.add_rmsnorm(h, L["post_norm"], eps, residual=residual)
-                h = F.linear(ops.silu_and_mul(F.linear(x, L["gate_up"])), L["down"])
-        if not small:
+                h = project(ops.silu_and_mul(project(x, L, li, "gate_up")), L, li, "down")
+                if small and li + 1 < nl:
+                    x, residual = ops.add_rmsnorm(h, W.layers[li + 1]["input_norm"], eps, residual=residual)
+        if not small or ad is not None:
             x, _ = ops.add_rmsnorm(h, W.final_norm, eps, residual=residual)
         return x
 
