@@ -491,7 +491,8 @@ int pk_lora_linear(const void* x, int64_t x_row_stride, const void* weight, int6
                    int32_t num_adapters, int32_t rank, const int32_t* adapter_ids, const float* scales,
                    const int32_t* slices, int32_t num_slices, void* out, int64_t out_row_stride,
                    void* workspace, size_t workspace_bytes, pk_stream_t stream);
-size_t pk_lora_add_workspace_bytes(int32_t rows, int32_t rank, int32_t num_slices, int32_t num_adapters);
+size_t pk_lora_add_workspace_bytes(int32_t rows, int32_t n_out, int32_t rank, const int32_t* slices,
+                                   int32_t num_slices, int32_t num_adapters);
 int pk_lora_add(const void* y, int64_t y_row_stride, const void* x, int64_t x_row_stride, int32_t rows,
                 int32_t n_out, int32_t k, const void* lora_a, int64_t a_adapter_stride, int64_t a_row_stride,
                 const void* lora_b, int64_t b_adapter_stride, int64_t b_row_stride, int32_t num_adapters,

@@ -199,20 +199,11 @@ int check_scratch(const char* what, const void* ws, size_t bytes, size_t need) {
 
 // ---- adapters beside a projection ---------------------------------------------------------
 
-int lora_args(const char* what, pk::LoraArgs* p, const void* x, int64_t x_row_stride, int32_t rows, int32_t n_out,
-              int32_t k, const void* lora_a, int64_t a_adapter_stride, int64_t a_row_stride, const void* lora_b,
-              int64_t b_adapter_stride, int64_t b_row_stride, int32_t num_adapters, int32_t rank,
-              const int32_t* adapter_ids, const float* scales, const int32_t* slices, int32_t num_slices, void* out,
-              int64_t out_row_stride) {
-  if (rows < 0 || n_out <= 0 || k <= 0 || num_adapters < 0)
-    return fail(PK_ERR_INVALID_ARG, "%s: rows=%d, n_out=%d, k=%d, num_adapters=%d", what, rows, n_out, k, num_adapters);
-  if (k % 8) return fail(PK_ERR_UNSUPPORTED, "%s: k=%d must be a multiple of 8", what, k);
-  if (rank <= 0 || rank % 8 || rank > pk::kLoraMaxRank)
-    return fail(PK_ERR_UNSUPPORTED, "%s: rank=%d must be a multiple of 8 up to %d", what, rank, pk::kLoraMaxRank);
+// The slices of an operator's output columns.
+int lora_slices(const char* what, pk::LoraArgs* p, int32_t n_out, const int32_t* slices, int32_t num_slices) {
   if (num_slices < 1 || num_slices > pk::kLoraMaxSlices || (num_slices > 1 && !slices))
     return fail(PK_ERR_INVALID_ARG, "%s: num_slices=%d (1 to %d, with their widths)", what, num_slices,
                 pk::kLoraMaxSlices);
-  *p = pk::LoraArgs{};
   int64_t sum = 0;
   for (int q = 0; q < num_slices; ++q) {
     const int32_t w = slices ? slices[q] : n_out;
@@ -223,6 +214,22 @@ int lora_args(const char* what, pk::LoraArgs* p, const void* x, int64_t x_row_st
     p->slice_begin[q + 1] = (int32_t)sum;
   }
   if (sum != n_out) return fail(PK_ERR_INVALID_ARG, "%s: the slices' widths do not add up to n_out=%d", what, n_out);
+  p->num_slices = num_slices;
+  return PK_OK;
+}
+
+int lora_args(const char* what, pk::LoraArgs* p, const void* x, int64_t x_row_stride, int32_t rows, int32_t n_out,
+              int32_t k, const void* lora_a, int64_t a_adapter_stride, int64_t a_row_stride, const void* lora_b,
+              int64_t b_adapter_stride, int64_t b_row_stride, int32_t num_adapters, int32_t rank,
+              const int32_t* adapter_ids, const float* scales, const int32_t* slices, int32_t num_slices, void* out,
+              int64_t out_row_stride) {
+  if (rows < 0 || n_out <= 0 || k <= 0 || num_adapters < 0)
+    return fail(PK_ERR_INVALID_ARG, "%s: rows=%d, n_out=%d, k=%d, num_adapters=%d", what, rows, n_out, k, num_adapters);
+  if (k % 8) return fail(PK_ERR_UNSUPPORTED, "%s: k=%d must be a multiple of 8", what, k);
+  if (rank <= 0 || rank % 8 || rank > pk::kLoraMaxRank)
+    return fail(PK_ERR_UNSUPPORTED, "%s: rank=%d must be a multiple of 8 up to %d", what, rank, pk::kLoraMaxRank);
+  *p = pk::LoraArgs{};
+  if (int rc = lora_slices(what, p, n_out, slices, num_slices)) return rc;
   if (rows > 0) {
     if (!x || !out || !adapter_ids || (num_adapters > 0 && (!lora_a || !lora_b)))
       return fail(PK_ERR_INVALID_ARG, "%s: null pointer argument", what);
@@ -250,7 +257,6 @@ int lora_args(const char* what, pk::LoraArgs* p, const void* x, int64_t x_row_st
   p->rank = rank;
   p->ids = adapter_ids;
   p->scales = scales;
-  p->num_slices = num_slices;
   p->out = static_cast<uint16_t*>(out);
   p->out_stride = out_row_stride;
   return PK_OK;
@@ -846,12 +852,13 @@ int pk_lora_linear(const void* x, int64_t x_row_stride, const void* weight, int6
                     "lora_linear launch");
 }
 
-size_t pk_lora_add_workspace_bytes(int32_t rows, int32_t rank, int32_t num_slices, int32_t num_adapters) {
-  if (rows <= 0 || rank <= 0 || rank > pk::kLoraMaxRank || num_slices <= 0 || num_slices > pk::kLoraMaxSlices ||
-      num_adapters < 0)
-    return 0;
+size_t pk_lora_add_workspace_bytes(int32_t rows, int32_t n_out, int32_t rank, const int32_t* slices,
+                                   int32_t num_slices, int32_t num_adapters) {
   pk::LoraArgs p{};
-  p.rows = rows, p.rank = rank, p.num_slices = num_slices, p.num_adapters = num_adapters;
+  if (rows <= 0 || rank <= 0 || rank > pk::kLoraMaxRank || num_adapters < 0 ||
+      lora_slices("lora_add", &p, n_out, slices, num_slices) != PK_OK)
+    return 0;
+  p.rows = rows, p.n_out = n_out, p.rank = rank, p.num_adapters = num_adapters;
   return pk::lora_add_workspace_bytes(p);
 }
 
@@ -877,7 +884,7 @@ int pk_lora_add(const void* y, int64_t y_row_stride, const void* x, int64_t x_ro
   if (rows > (1 << 22) || n_out > (1 << 20))
     return fail(PK_ERR_UNSUPPORTED, "lora_add: rows=%d, n_out=%d (at most 2^22 and 2^20)", rows, n_out);
   if (int rc = check_scratch("lora_add", workspace, workspace_bytes,
-                             pk_lora_add_workspace_bytes(rows, rank, num_slices, num_adapters)))
+                             pk::lora_add_workspace_bytes(p)))
     return rc;
   p.y = static_cast<const uint16_t*>(y);
   p.y_stride = y_row_stride;

@@ -80,10 +80,12 @@ __device__ __forceinline__ void lin_lds_barrier() {
 // is stored in stage c & 1 while the other stage may still be read for chunk c - 1.
 // Wavefront w multiplies the 64 columns [64 w, 64 w + 64) of every chunk.
 // What an epilogue adds to the sums of a work-group's 32 x 32 outputs (NP = MT = 1) before they are
-// rounded: load is called before the K walk, put and add after it, with a barrier between them and
-// LDS of their own. Thread (c, q) adds to row c, columns 4 q .. 4 q + 3. Here: nothing.
+// rounded: load is called before the K walk; after it prepare, which has all of the LDS, put and add, with
+// barriers between the three and LDS of their own for the last two. Thread (c, q) adds to row c,
+// columns 4 q .. 4 q + 3. Here: nothing.
 struct NoAddend {
   __device__ __forceinline__ void load(int row0, int n0) {}
+  __device__ __forceinline__ void prepare(char* lds) {}
   __device__ __forceinline__ void put(char* lds) const {}
   __device__ __forceinline__ void add(const char* lds, float4& v) const {}
 };
@@ -178,6 +180,7 @@ __device__ __forceinline__ void linear_tile(const LinArgs a, const int block, ch
     }
   }
   __syncthreads();  // every wavefront is done with the stages before they hold the sums
+  addend.prepare(smem);
   auto red = reinterpret_cast<float4 (*)[NP][4][kWave]>(smem);
 
   // Add the four wavefronts' accumulators one x-row tile at a time. Thread (c, q) then owns

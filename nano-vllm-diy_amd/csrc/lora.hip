@@ -245,35 +245,61 @@ __global__ __launch_bounds__(kLinThreads) void lora_linear_kernel(const LinArgs 
 // column), one after the other in memory; the row's eight threads take them in turn, whole cache
 // lines, before the K walk, which hides them. Their products with t go through LDS to the threads
 // that have the columns.
+//
+// kShrink: t is computed here too, after the K walk, by every work-group for its slice. One adapter's A
+// is read again by all of them in 1.4 us less than a launch of its own (1024 x 4096, rank 16, in a
+// graph: 1 row 7.1 and 8.5 us); every further adapter costs 1.7 us (2 rows 8.9 and 8.5, 4 rows 11.9 and
+// 8.4). Outside a graph the second launch is 3.3 us of host time, so two rows still gain.
+constexpr int kOneLaunchRows = 2;
+
+template <bool kShrink>
 struct LoraAddend {
   const LoraArgs& p;
-  bool any;
+  int32_t* rows;   // LDS, 16 (kShrink)
+  float* t_here;   // LDS, [16][16] (kShrink)
+  int32_t id, slice;
   u32x4 b[8];
   f32x4 t[2];
+  __device__ __forceinline__ int half() const { return threadIdx.x & 1; }
   __device__ __forceinline__ void load(int row0, int n0) {
-    const int32_t m = row0 + (threadIdx.x >> 3), piece = threadIdx.x & 7, half = piece & 1;
-    const int32_t id = m < p.rows ? adapter_of(p, m) : -1;
-    any = id >= 0;
-    if (!any) return;
-    int32_t q = 0;
-    while (q < p.num_slices - 1 && n0 >= p.slice_begin[q + 1]) ++q;  // (slices are multiples of 32 columns)
-    const uint16_t* bp = p.b + id * p.b_adapter + (n0 + (piece >> 1)) * p.b_row + 8 * half;
-    const float* tp = p.t + (int64_t)m * (p.num_slices * p.rank) + q * p.rank + 8 * half;
-    const bool in = 8 * half < p.rank;
+    const int32_t m = row0 + (threadIdx.x >> 3), piece = threadIdx.x & 7;
+    id = m < p.rows ? adapter_of(p, m) : -1;
+    slice = 0;
+    while (slice < p.num_slices - 1 && n0 >= p.slice_begin[slice + 1]) ++slice;  // (multiples of 32 columns)
+    if (id < 0) return;
+    const uint16_t* bp = p.b + id * p.b_adapter + (n0 + (piece >> 1)) * p.b_row + 8 * half();
+    const bool in = 8 * half() < p.rank;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       b[i] = u32x4{0u, 0u, 0u, 0u};
       if (in) b[i] = *reinterpret_cast<const u32x4*>(bp + 4 * i * p.b_row);
     }
+    if constexpr (!kShrink) load_t(p.t + (int64_t)m * (p.num_slices * p.rank) + slice * p.rank);
+  }
+  __device__ __forceinline__ void load_t(const float* row) {
     t[0] = t[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (in) {
-      t[0] = *reinterpret_cast<const f32x4*>(tp);
-      t[1] = *reinterpret_cast<const f32x4*>(tp + 4);
+    if (8 * half() < p.rank) {
+      t[0] = *reinterpret_cast<const f32x4*>(row + 8 * half());
+      t[1] = *reinterpret_cast<const f32x4*>(row + 8 * half() + 4);
+    }
+  }
+  __device__ __forceinline__ void prepare(char* lds) {
+    if constexpr (kShrink) {
+      for (int j = 0; j < p.rows; ++j) {  // the rows' adapters, each once
+        int32_t a;
+        if (!small_tile(p, j, rows, &a) || a < 0) continue;
+        shrink_tile<kLoraSmallTile, 1, 4>(p, a, slice * p.rank, rows, lds, [&](int i, int c, const f32x4 v) {
+          if (rows[i] >= 0) *reinterpret_cast<f32x4*>(t_here + 16 * i + c) = v;
+        });
+        __syncthreads();
+      }
+      if (id >= 0) load_t(t_here + 16 * (threadIdx.x >> 3));
     }
   }
   // [row][64] products of the pieces, 4 floats between rows
   __device__ __forceinline__ void put(char* lds) const {
     float* at = reinterpret_cast<float*>(lds) + (threadIdx.x >> 3) * 68 + (threadIdx.x & 7);
+    if (id < 0) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float d = 0.f;
@@ -286,17 +312,19 @@ struct LoraAddend {
     }
   }
   __device__ __forceinline__ void add(const char* lds, float4& v) const {
-    if (!any) return;
+    if (id < 0) return;
     const float* at = reinterpret_cast<const float*>(lds) + (threadIdx.x >> 3) * 68 + 8 * (threadIdx.x & 7);
     const f32x4 d0 = *reinterpret_cast<const f32x4*>(at), d1 = *reinterpret_cast<const f32x4*>(at + 4);
     v = make_float4(v.x + (d0[0] + d0[1]), v.y + (d0[2] + d0[3]), v.z + (d1[0] + d1[1]), v.w + (d1[2] + d1[3]));
   }
 };
 
-template <int NB>
+template <int NB, bool kShrink>
 __global__ __launch_bounds__(kLinThreads) void lora_linear_expand_kernel(const LinArgs a, const LoraArgs p) {
   __shared__ __attribute__((aligned(16))) char smem[lin_smem_bytes(1, 1)];
-  linear_tile<1, 1, NB, kEpiStore>(a, blockIdx.x, smem, LoraAddend{p});
+  __shared__ __attribute__((aligned(16))) float t_here[kShrink ? kLoraSmallTile * 16 : 4];
+  __shared__ int32_t rows[kLoraSmallTile];
+  linear_tile<1, 1, NB, kEpiStore>(a, blockIdx.x, smem, LoraAddend<kShrink>{p, rows, t_here});
 }
 
 // ---------------------------------------------------------------- expand ----------------
@@ -377,20 +405,21 @@ __device__ __forceinline__ int32_t group_slice(const LoraArgs& p, int32_t g, int
   return q;
 }
 
-// Work-group = (row, up to 512 columns of a slice): the rows of 16 with that row's adapter, 128
+// Work-group = (row, up to 128 WAVES columns of a slice): the rows of 16 with that row's adapter, 128
 // columns a wavefront. Everything is asked for before the first wait.
 // kBase: where base is from -- kBasePartial: the sum of p.ks fp32 partial products, kBaseRows: bf16
 // rows of y, kBaseRowsShrink: those, and t is computed here, by every work-group of the row again, instead of
 // by a launch before (the rank is KP at most then).
-constexpr int kSmallCols = 512;
 enum Base { kBasePartial = 0, kBaseRows = 1, kBaseRowsShrink = 2 };
 
-template <int KP, int kBase>
-__global__ __launch_bounds__(kLoraThreads) void lora_expand_small_kernel(const LoraArgs p) {
+template <int KP, int WAVES, int kBase>
+__global__ __launch_bounds__(WAVES* kWave) void lora_expand_small_kernel(const LoraArgs p) {
   using S = ExpandShape<KP>;
   constexpr bool kPartial = kBase == kBasePartial, kShrink = kBase == kBaseRowsShrink;
-  constexpr int kLoads = kSmallCols * S::kChunks / kLoraThreads, CB = (KP + 15) / 16;
-  constexpr int kBBytes = kSmallCols * S::kRowBytes, kShrinkBytes = kShrink ? shrink_smem_bytes(kLoraSmallTile, CB) : 0;
+  static_assert(!kShrink || WAVES == kLoraWaves, "shrink_tile's work-group");
+  constexpr int kThreads = WAVES * kWave, kCols = 128 * WAVES;
+  constexpr int kLoads = kCols * S::kChunks / kThreads, CB = (KP + 15) / 16;
+  constexpr int kBBytes = kCols * S::kRowBytes, kShrinkBytes = kShrink ? shrink_smem_bytes(kLoraSmallTile, CB) : 0;
   __shared__ __attribute__((aligned(16))) char smem[kBBytes > kShrinkBytes ? kBBytes : kShrinkBytes];
   __shared__ __attribute__((aligned(16))) float t_here[kShrink ? kLoraSmallTile * KP : 4];
   __shared__ int32_t rows[kLoraSmallTile];
@@ -398,8 +427,8 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_small_kernel(const L
   int32_t id, begin;
   if (!small_tile(p, slot, rows, &id)) return;
   if (!kPartial && id < 0 && p.out == p.y) return;  // rows without an adapter stay as they are
-  const int32_t q = group_slice(p, blockIdx.x - slot * p.col_groups, kSmallCols, &begin);
-  const int32_t end = min(begin + kSmallCols, p.slice_begin[q + 1]);
+  const int32_t q = group_slice(p, blockIdx.x - slot * p.col_groups, kCols, &begin);
+  const int32_t end = min(begin + kCols, p.slice_begin[q + 1]);
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int r = lane & 15, h = lane >> 4;
   const int32_t col = begin + 128 * wave + 8 * r;  // this lane's columns
@@ -425,7 +454,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_small_kernel(const L
       u32x4 st[kLoads], hi[S::kSteps], lo[S::kSteps];
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int e = i * kLoraThreads + threadIdx.x, c = e / S::kChunks, j = j0 + e % S::kChunks * 8;
+        const int e = i * kThreads + threadIdx.x, c = e / S::kChunks, j = j0 + e % S::kChunks * 8;
         st[i] = u32x4{0u, 0u, 0u, 0u};
         if (begin + c < end && j < p.rank) st[i] = *reinterpret_cast<const u32x4*>(bp + (begin + c) * p.b_row + j);
       }
@@ -439,7 +468,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_small_kernel(const L
       if (j0) __syncthreads();  // the previous piece has been read
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int e = i * kLoraThreads + threadIdx.x;
+        const int e = i * kThreads + threadIdx.x;
         *reinterpret_cast<u32x4*>(smem + S::at(e / S::kChunks) * S::kRowBytes + e % S::kChunks * 16) = st[i];
       }
       __syncthreads();
@@ -735,14 +764,20 @@ int32_t col_groups(const LoraArgs& p, int32_t cols) {
   return n;
 }
 
+template <int KP, int WAVES, int kBase>
+void launch_expand_waves(LoraArgs p, hipStream_t stream) {
+  p.col_groups = col_groups(p, 128 * WAVES);
+  hipLaunchKernelGGL((lora_expand_small_kernel<KP, WAVES, kBase>), dim3((unsigned)(p.rows * p.col_groups)),
+                     dim3(WAVES * kWave), 0, stream, p);
+}
+
+// Above rank 32 two wavefronts have all of B's 64 (of 128, twice 64) elements in flight: 128 rows on 3072
+// x 1024, rank 64 6.5 us; four wavefronts and twice 32 elements 7.2.
 template <int kBase>
-hipError_t launch_expand_small(LoraArgs p, hipStream_t stream) {
-  p.col_groups = col_groups(p, kSmallCols);
-  const dim3 grid((unsigned)(p.rows * p.col_groups)), block(kLoraThreads);
-  if (p.rank <= 16)
-    hipLaunchKernelGGL((lora_expand_small_kernel<16, kBase>), grid, block, 0, stream, p);
-  else
-    hipLaunchKernelGGL((lora_expand_small_kernel<32, kBase>), grid, block, 0, stream, p);
+hipError_t launch_expand_small(const LoraArgs& p, hipStream_t stream) {
+  if (p.rank <= 16) launch_expand_waves<16, 4, kBase>(p, stream);
+  else if (p.rank <= 32) launch_expand_waves<32, 4, kBase>(p, stream);
+  else if constexpr (kBase != kBaseRowsShrink) launch_expand_waves<64, 2, kBase>(p, stream);
   return hipGetLastError();
 }
 
@@ -751,7 +786,7 @@ hipError_t launch_expand_small(LoraArgs p, hipStream_t stream) {
 // rank 16, one up to 32. Measured on the 1024 x 2048 projection, one launch and two, us: 128 rows
 // (256 work-groups) rank 16 6.3 and 8.1, rank 32 9.3 and 9.0; 300 rows (600) 13.7 and 10.5, 25.1 and 14.4.
 bool shrink_in_expand(const LoraArgs& p) {
-  return p.rank <= 32 && (int64_t)p.rows * col_groups(p, kSmallCols) <= (p.rank <= 16 ? 512 : 256);
+  return p.rank <= 32 && (int64_t)p.rows * col_groups(p, 128 * kLoraWaves) <= (p.rank <= 16 ? 512 : 256);
 }
 
 template <int R>
@@ -793,8 +828,8 @@ hipError_t launch_expand_sorted(LoraArgs p, int64_t tiles, hipStream_t stream) {
 }
 
 // Whether the projection's work-groups add the adapters themselves (the shrink before them) rather
-// than leave partial sums to an expand. Measured, us of the two forms: 97 rows, 1024 x 6144, rank 16
-// XX and 16.8; 1 row, 1024 x 4096 XX and 9.7.
+// than leave partial sums to an expand. Measured, us of the two forms' kernels: 97 rows, 1024 x 6144, rank
+// 16 15.2 and 16.7; 1 row, 1024 x 4096 8.9 and 9.7 (in two launches).
 bool expand_in_linear(const LoraArgs& p, const LinCfg& c) { return c.ks == 1 && p.rank <= 16; }
 
 size_t t_bytes(const LoraArgs& p) { return (size_t)p.rows * p.num_slices * p.rank * sizeof(float); }
@@ -803,11 +838,12 @@ size_t t_bytes(const LoraArgs& p) { return (size_t)p.rows * p.num_slices * p.ran
 
 size_t lora_linear_workspace_bytes(const LoraArgs& p) {
   const LinCfg c = choose_config(p.rows, p.n_out / kLinTile, p.k, 1);
-  return t_bytes(p) + (expand_in_linear(p, c) ? 0 : (size_t)c.ks * p.rows * p.n_out * sizeof(float));
+  if (expand_in_linear(p, c)) return p.rows <= kOneLaunchRows ? 0 : t_bytes(p);
+  return t_bytes(p) + (size_t)c.ks * p.rows * p.n_out * sizeof(float);
 }
 
 size_t lora_add_workspace_bytes(const LoraArgs& p) {
-  if (p.rows <= kLoraSmallRows) return t_bytes(p);
+  if (p.rows <= kLoraSmallRows) return shrink_in_expand(p) ? 0 : t_bytes(p);
   return t_bytes(p) + (size_t)lora_max_tiles(p.rows, p.num_adapters) * (kLoraTile * sizeof(int32_t) + sizeof(int2)) +
          (size_t)p.rows * sizeof(int32_t);
 }
@@ -831,16 +867,25 @@ hipError_t launch_lora_linear(const LoraArgs& args, const void* w, int64_t w_str
   const int32_t lin_groups = (p.n_out / kLinTile) * c.ks * c.mgroups;
   const int32_t cols16 = (p.num_slices * p.rank + 15) / 16;
   if (expand_in_linear(p, c)) {
-    if (p.num_adapters > 0) {
+    a.y = p.out;
+    a.y_stride = p.out_stride;
+    const bool here = p.rows <= kOneLaunchRows;
+    if (p.num_adapters > 0 && !here) {
       hipLaunchKernelGGL(lora_shrink_small_kernel, dim3(p.rows * cols16), dim3(kLoraThreads), 0, stream, p);
       if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
     }
-    a.y = p.out;
-    a.y_stride = p.out_stride;
+    const auto launch = [&](auto nb) {
+      if (here)
+        hipLaunchKernelGGL((lora_linear_expand_kernel<nb.value, true>), dim3(lin_groups), dim3(kLinThreads), 0, stream,
+                           a, p);
+      else
+        hipLaunchKernelGGL((lora_linear_expand_kernel<nb.value, false>), dim3(lin_groups), dim3(kLinThreads), 0, stream,
+                           a, p);
+    };
     switch (c.nb) {
-      case 1: hipLaunchKernelGGL(lora_linear_expand_kernel<1>, dim3(lin_groups), dim3(kLinThreads), 0, stream, a, p); break;
-      case 2: hipLaunchKernelGGL(lora_linear_expand_kernel<2>, dim3(lin_groups), dim3(kLinThreads), 0, stream, a, p); break;
-      default: hipLaunchKernelGGL(lora_linear_expand_kernel<4>, dim3(lin_groups), dim3(kLinThreads), 0, stream, a, p); break;
+      case 1: launch(std::integral_constant<int, 1>{}); break;
+      case 2: launch(std::integral_constant<int, 2>{}); break;
+      default: launch(std::integral_constant<int, 4>{}); break;
     }
     return hipGetLastError();
   }

@@ -134,7 +134,7 @@ SIGNATURES = {
         _i32, _i32, _c_void_p, _c_void_p,   # num_adapters, rank, adapter_ids, scales
         ctypes.POINTER(_i32), _i32,         # slices (host), num_slices
         _c_void_p, _i64, _c_void_p, _size_t, _c_void_p]),  # out, its row stride, workspace, its bytes, stream
-    "pk_lora_add_workspace_bytes": (_size_t, [_i32, _i32, _i32, _i32]),
+    "pk_lora_add_workspace_bytes": (_size_t, [_i32, _i32, _i32, ctypes.POINTER(_i32), _i32, _i32]),
     "pk_lora_add": (ctypes.c_int, [
         _c_void_p, _i64, _c_void_p, _i64,   # y, its row stride, x, its row stride
         _i32, _i32, _i32, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i32, _i32, _c_void_p, _c_void_p,

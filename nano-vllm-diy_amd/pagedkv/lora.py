@@ -33,33 +33,41 @@ def _slices(slices: tuple[int, ...] | None, n_out: int):
     return (ctypes.c_int32 * len(widths))(*widths), len(widths)
 
 
+_BF16, _F32 = torch.bfloat16, torch.float32
+
+
 def _rows2d(name: str, t: torch.Tensor, device: torch.device) -> tuple[torch.Size, int]:
     """(shape, row stride) of a 2-D bf16 tensor with contiguous rows on the device."""
     shape, stride = t.shape, t.stride()
-    if len(shape) != 2 or t.dtype != torch.bfloat16 or stride[1] != 1:
+    if len(shape) != 2 or t.dtype is not _BF16 or stride[1] != 1:
         raise ValueError(f"{name} must be a 2-D bf16 tensor with contiguous rows")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
     return shape, stride[0]
 
 
+def _adapter(name: str, t: torch.Tensor, device: torch.device) -> tuple[torch.Size, tuple[int, ...]]:
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or t.dtype is not _BF16 or stride[2] != 1:
+        raise ValueError(f"{name} must be a 3-D bf16 tensor with contiguous rows")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    return shape, stride
+
+
 def _adapter_args(rows, k, n_out, dev, lora_a, lora_b, adapter_ids, scales, slices):
     """The adapter arguments of the C-ABI, after the checks both operators share."""
-    arr, num_slices = _slices(None if slices is None else tuple(slices), n_out)
-    a_shape, a_stride, b_shape, b_stride = lora_a.shape, lora_a.stride(), lora_b.shape, lora_b.stride()
-    for name, t, stride in (("lora_a", lora_a, a_stride), ("lora_b", lora_b, b_stride)):
-        if len(stride) != 3 or t.dtype != torch.bfloat16 or stride[2] != 1:
-            raise ValueError(f"{name} must be a 3-D bf16 tensor with contiguous rows")
-        if t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, expected {dev}")
-    adapters, b_rows, rank = b_shape
+    arr, num_slices = _slices(slices, n_out)
+    a_shape, a_stride = _adapter("lora_a", lora_a, dev)
+    (adapters, b_rows, rank), b_stride = _adapter("lora_b", lora_b, dev)
     if b_rows != n_out or a_shape != (adapters, num_slices * rank, k):
-        raise ValueError(f"lora_a {tuple(a_shape)} and lora_b {tuple(b_shape)} must be (L, {num_slices} * r, {k}) and "
-                         f"(L, {n_out}, r)")
-    _req_i32("adapter_ids", adapter_ids, dev)
+        raise ValueError(f"lora_a {tuple(a_shape)} and lora_b {tuple(lora_b.shape)} must be (L, {num_slices} * r, {k}) "
+                         f"and (L, {n_out}, r)")
+    if adapter_ids.dtype is not torch.int32 or adapter_ids.device != dev:
+        _req_i32("adapter_ids", adapter_ids, dev)
     if adapter_ids.shape != (rows,) or not adapter_ids.is_contiguous():
         raise ValueError(f"adapter_ids must be a contiguous ({rows},) tensor")
-    if scales is not None and (scales.dtype != torch.float32 or scales.shape != (adapters,) or scales.device != dev or
+    if scales is not None and (scales.dtype is not _F32 or scales.shape != (adapters,) or scales.device != dev or
                                not scales.is_contiguous()):
         raise ValueError(f"scales must be a contiguous ({adapters},) float32 tensor on {dev}")
     return (lora_a.data_ptr(), a_stride[0], a_stride[1], lora_b.data_ptr(), b_stride[0], b_stride[1], adapters, rank,
@@ -76,12 +84,21 @@ def _out(out, rows, n_out, dev):
 
 
 @lru_cache(maxsize=4096)
-def lora_workspace_bytes(rows: int, n_out: int, k: int, rank: int, num_slices: int = 1, num_adapters: int = 0,
-                         linear: bool = False) -> int:
-    """Scratch bytes of one lora_add call, or with linear=True of one lora_linear call."""
+def lora_workspace_bytes(rows: int, n_out: int, k: int, rank: int, slices: tuple[int, ...] | None = None,
+                         num_adapters: int = 0, linear: bool = False) -> int:
+    """Scratch bytes of one lora_add call, or with linear=True of one lora_linear call (0: none)."""
+    arr, num_slices = _slices(slices, n_out)
     if linear:
         return int(lib().pk_lora_linear_workspace_bytes(rows, n_out, k, rank, num_slices))
-    return int(lib().pk_lora_add_workspace_bytes(rows, rank, num_slices, num_adapters))
+    return int(lib().pk_lora_add_workspace_bytes(rows, n_out, rank, arr, num_slices, num_adapters))
+
+
+def _workspace(workspace, nbytes, dev):
+    """(pointer, bytes, the tensor) of the scratch of a call"""
+    if nbytes == 0:
+        return 0, 0, None
+    ws = scratch(nbytes, dev) if workspace is None else _given_workspace(workspace, nbytes, dev)
+    return ws.data_ptr(), nbytes, ws
 
 
 def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
@@ -98,12 +115,12 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
         raise ValueError(f"weight {tuple(weight.shape)} does not match x {tuple(x.shape)}")
     if rows > LINEAR_MAX_ROWS:
         raise ValueError(f"decode-step linear layers take at most {LINEAR_MAX_ROWS} rows, got {rows}")
+    slices = None if slices is None else tuple(slices)
     args = _adapter_args(rows, k, n_out, dev, lora_a, lora_b, adapter_ids, scales, slices)
     out, out_stride = _out(out, rows, n_out, dev)
-    nbytes = lora_workspace_bytes(rows, n_out, k, args[7], args[11], linear=True)
-    ws = scratch(nbytes, dev) if workspace is None else _given_workspace(workspace, nbytes, dev)
+    ws, nbytes, _keep = _workspace(workspace, lora_workspace_bytes(rows, n_out, k, args[7], slices, 0, True), dev)
     call(lib().pk_lora_linear, "pk_lora_linear", dev, x.data_ptr(), x_stride, weight.data_ptr(), w_stride, rows, n_out,
-         k, *args, out.data_ptr(), out_stride, ws.data_ptr(), nbytes)
+         k, *args, out.data_ptr(), out_stride, ws, nbytes)
     return out
 
 
@@ -118,10 +135,10 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: tor
     (y_rows, n_out), y_stride = _rows2d("y", y, dev)
     if y_rows != rows:
         raise ValueError(f"y {tuple(y.shape)} does not match x {tuple(x.shape)}")
+    slices = None if slices is None else tuple(slices)
     args = _adapter_args(rows, k, n_out, dev, lora_a, lora_b, adapter_ids, scales, slices)
     out, out_stride = _out(out, rows, n_out, dev)
-    nbytes = lora_workspace_bytes(rows, n_out, k, args[7], args[11], args[6])
-    ws = scratch(nbytes, dev) if workspace is None else _given_workspace(workspace, nbytes, dev)
+    ws, nbytes, _keep = _workspace(workspace, lora_workspace_bytes(rows, n_out, k, args[7], slices, args[6]), dev)
     call(lib().pk_lora_add, "pk_lora_add", dev, y.data_ptr(), y_stride, x.data_ptr(), x_stride, rows, n_out, k, *args,
-         out.data_ptr(), out_stride, ws.data_ptr(), nbytes)
+         out.data_ptr(), out_stride, ws, nbytes)
     return out

@@ -81,7 +81,8 @@ def _add(d, **kw):
     (1, QKV, 16, 4, 2), (1, DOWN, 8, 1, -1), (7, O, 64, 3, "mixed"), (16, QKV, 128, 5, "mixed"),
     (17, GATE_UP, 24, 2, "mixed"), (33, DOWN, 72, 40, "mixed"), (97, GATE_UP, 16, 8, "runs"), (128, QKV, 16, 1, 0),
     (128, DOWN, 64, 130, "mixed"), (128, O, 8, 3, -1), (65, (256, (32, 96, 64, 32)), 40, 6, "mixed"),
-    (100, (512, (64,)), 104, 300, "mixed")])
+    (100, (512, (64,)), 104, 300, "mixed"), (2, QKV, 16, 4, "mixed"), (2, GATE_UP, 8, 1, 0), (1, QKV, 8, 3, -1),
+    (3, QKV, 16, 4, "mixed"), (1, GATE_UP, 40, 2, 1)])
 def test_linear_against_formula(gpu, rows, proj, rank, adapters, ids):
     k, widths = proj
     c = _case(rows + rank, rows, k, widths, rank, adapters, ids)
@@ -96,7 +97,9 @@ def test_linear_against_formula(gpu, rows, proj, rank, adapters, ids):
     (64, (1000, (96,)), 32, 3, "mixed"), (65, (1032, (160, 32, 32, 64)), 128, 3, "mixed"), (300, O, 8, 24, "mixed"),
     (512, QKV, 16, 600, "mixed"), (513, QKV, 16, 8, "runs"), (513, (40, (32, 32)), 40, 1, 0),
     (600, (264, (288,)), 72, 4095, "mixed"), (700, (1000, (96, 64)), 24, 3, "mixed"), (1025, DOWN, 64, 7, "runs"),
-    (2000, GATE_UP, 128, 5, "runs"), (3001, O, 16, 50, "mixed"), (1500, (64, (32,)), 8, 4, -1)])
+    (2000, GATE_UP, 128, 5, "runs"), (30, QKV, 32, 7, "mixed"), (64, QKV, 24, 3, "runs"), (33, DOWN, 16, 9, "mixed"),
+    (128, O, 32, 2, "mixed"), (17000, (64, (32, 32)), 8, 3, "runs"), (33000, (64, (32,)), 16, 40, "mixed"),
+    (24700, (256, (64, 64)), 32, 2, "runs"), (3001, O, 16, 50, "mixed"), (1500, (64, (32,)), 8, 4, -1)])
 def test_add_against_formula(gpu, rows, proj, rank, adapters, ids):
     k, widths = proj
     c = _case(rows + rank, rows, k, widths, rank, adapters, ids)
@@ -274,13 +277,13 @@ def test_two_streams(gpu):
 
 def test_given_workspace(gpu):
     d = _gpu(_case(3, 700, 256, (64, 32), 16, 5), gpu)
-    need = pagedkv.lora_workspace_bytes(700, 96, 256, 16, 2, 5)
+    need = pagedkv.lora_workspace_bytes(700, 96, 256, 16, (64, 32), 5)
     ws = torch.full((need + 64,), 255, dtype=torch.uint8, device=gpu)
     print("[lora_add] workspace", flush=True)
     assert torch.equal(_add(d, workspace=ws[:need]), _add(d))
     assert bool((ws[need:] == 255).all())
     small = {n: d[n][:100] if n in ("x", "y", "ids") else d[n] for n in d}
-    need = pagedkv.lora_workspace_bytes(100, 96, 256, 16, 2, linear=True)
+    need = pagedkv.lora_workspace_bytes(100, 96, 256, 16, (64, 32), linear=True)
     ws = torch.full((need + 64,), 255, dtype=torch.uint8, device=gpu)
     assert torch.equal(_linear(small, workspace=ws[:need]), _linear(small))
     assert bool((ws[need:] == 255).all())

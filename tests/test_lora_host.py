@@ -44,8 +44,9 @@ def _call(name, **kw):
     (dict(x_stride=248), _lib.PK_ERR_INVALID_ARG), (dict(out_stride=60), _lib.PK_ERR_INVALID_ARG),
     (dict(a_row=255), _lib.PK_ERR_INVALID_ARG), (dict(b_row=8), _lib.PK_ERR_INVALID_ARG),
     (dict(a_adapter=-8), _lib.PK_ERR_INVALID_ARG), (dict(b_adapter=12), _lib.PK_ERR_INVALID_ARG),
-    (dict(ws_bytes=8), _lib.PK_ERR_WORKSPACE), (dict(ws=None), _lib.PK_ERR_WORKSPACE),
-    (dict(ws=PTR + 4), _lib.PK_ERR_WORKSPACE)])
+    (dict(ws_bytes=8, rank=64, b_row=64), _lib.PK_ERR_WORKSPACE),  # (rank 64: t is left in the workspace)
+    (dict(ws=None, rank=64, b_row=64), _lib.PK_ERR_WORKSPACE),
+    (dict(ws=PTR + 4, rank=64, b_row=64), _lib.PK_ERR_WORKSPACE)])
 def test_refusals(name, kw, code):
     assert _call(name, **kw) == code, _lib.lib().pk_last_error()
     assert name[3:].encode() in _lib.lib().pk_last_error()
@@ -67,15 +68,21 @@ def test_refusals_of_one():
 
 def test_workspace_sizes():
     lib = _lib.lib()
-    assert lib.pk_lora_add_workspace_bytes(100, 16, 3, 8) == 100 * 48 * 4
+    qkv = (ctypes.c_int32 * 3)(2048, 1024, 1024)
+    # one launch, no scratch, while all its work-groups are on the GPU at once
+    assert lib.pk_lora_add_workspace_bytes(64, 4096, 16, qkv, 3, 8) == 0
+    assert lib.pk_lora_add_workspace_bytes(100, 4096, 16, qkv, 3, 8) == 100 * 48 * 4
     # sorted: t, the rows of the tiles, their records, the rows' places
-    assert lib.pk_lora_add_workspace_bytes(1000, 16, 3, 8) == 1000 * 48 * 4 + (15 + 9) * (256 + 8) + 4000
+    assert lib.pk_lora_add_workspace_bytes(1000, 4096, 16, qkv, 3, 8) == 1000 * 48 * 4 + (15 + 9) * (256 + 8) + 4000
+    assert lib.pk_lora_add_workspace_bytes(1000, 4000, 16, qkv, 3, 8) == 0                # refused
     # t, and the projection's partial sums where it leaves them (K split, or ranks above 16)
     base = lib.pk_linear_workspace_bytes(100, 1024, 2048, 2)
     assert lib.pk_lora_linear_workspace_bytes(100, 1024, 2048, 16, 1) == base + 100 * 16 * 4
     assert lib.pk_lora_linear_workspace_bytes(100, 4096, 1024, 24, 3) == 100 * (4096 + 72) * 4
     assert lib.pk_lora_linear_workspace_bytes(100, 4096, 1024, 16, 3) == 100 * 48 * 4
+    assert lib.pk_lora_linear_workspace_bytes(2, 4096, 1024, 16, 3) == 0
     assert lib.pk_lora_linear_workspace_bytes(129, 1024, 1024, 16, 1) == 0
+    assert pagedkv.lora_workspace_bytes(100, 4096, 1024, 16, (2048, 1024, 1024), 8) == 100 * 48 * 4
 
 
 def test_python_refusals():
@@ -89,7 +96,7 @@ def test_python_refusals():
                           (dict(slices=(32, 16)), "add up"), (dict(slices=(32, 32)), "must be"),
                           (dict(adapter_ids=ids[:3]), "adapter_ids"), (dict(scales=torch.ones(3)), "scales"),
                           (dict(scales=torch.ones(2, dtype=torch.float64)), "scales"),
-                          (dict(out=torch.zeros(4, 32, **bf)), "out must be")]:
+                          (dict(slices=()), "add up"), (dict(out=torch.zeros(4, 32, **bf)), "out must be")]:
             with pytest.raises(ValueError, match=match):
                 call(**kw)
         with pytest.raises(TypeError, match="int32"):
