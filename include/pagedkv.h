@@ -475,14 +475,15 @@ int pk_linear_add_rmsnorm(const void* x, int64_t x_row_stride, const void* weigh
  * HOST array (read before the call returns); NULL with num_slices 1: one slice of n_out.
  * x (rows, k), lora_a (num_adapters, num_slices * rank, k), lora_b (num_adapters, n_out, rank) bf16;
  * adapters of smaller rank are padded with zeros. k and rank multiples of 8, rank up to 128, up
- * to 4 slices of multiples of 32 columns; pointers 16-byte aligned, strides multiples of 8. A
- * row's result does not depend on the other rows' values.
+ * to 4 slices of multiples of 32 columns, up to 2^22 rows of 2^20 columns (and what a launch of
+ * 2^24 work-groups covers); pointers 16-byte aligned, strides multiples of 8. A row's result does
+ * not depend on the other rows' values. An infinite weight gives NaN.
  *
  * pk_lora_linear -- base = x W^T in fp32 (a decode step's projection, pk_linear's weight and limits:
  *   at most 128 rows, k a multiple of 256); out must not overlap x.
  * pk_lora_add -- base = y (rows, n_out) bf16, the output of a projection computed elsewhere. out may be
- *   y (in place, rows without an adapter are then not written), or must not overlap y or x. Up to
- *   2^22 rows; above 512 rows up to 4095 adapters.
+ *   y (in place, rows without an adapter are then not written), or must not overlap y or x. Above
+ *   512 rows up to 4095 adapters.
  */
 size_t pk_lora_linear_workspace_bytes(int32_t rows, int32_t n_out, int32_t k, int32_t rank, int32_t num_slices);
 int pk_lora_linear(const void* x, int64_t x_row_stride, const void* weight, int64_t weight_row_stride,
@@ -528,8 +529,9 @@ int pk_lora_add(const void* y, int64_t y_row_stride, const void* x, int64_t x_ro
  *   most 1024 forks a call; workspace: pk_fork_workspace_bytes(num_forks).
  * pk_extend_sequences -- one more token for every listed row: slot_mapping[i] is its cache slot
  *   (block * block_size + offset), in a new block where the row's last one is full, and the
- *   length grows by one. -1 and nothing changed where the row is no row or was listed before, its
- *   table is full or the pool has no block left. At most 1024 rows a call; num_blocks *
+ *   length grows by one. A last block that is not full must be the row's alone (a fork leaves no
+ *   other). -1 and nothing changed where the row is no row or was listed before, its table is full
+ *   or the pool has no block left. At most 1024 rows a call; num_blocks *
  *   block_size must fit 31 bits.
  * pk_free_sequences -- the listed rows' blocks lose a holder, their entries become -1, their lengths 0
  *   (a row that is listed twice is freed once).

@@ -226,6 +226,9 @@ int lora_args(const char* what, pk::LoraArgs* p, const void* x, int64_t x_row_st
   if (rows < 0 || n_out <= 0 || k <= 0 || num_adapters < 0)
     return fail(PK_ERR_INVALID_ARG, "%s: rows=%d, n_out=%d, k=%d, num_adapters=%d", what, rows, n_out, k, num_adapters);
   if (k % 8) return fail(PK_ERR_UNSUPPORTED, "%s: k=%d must be a multiple of 8", what, k);
+  if (rows > pk::kLoraMaxRows || n_out > pk::kLoraMaxOut)
+    return fail(PK_ERR_UNSUPPORTED, "%s: rows=%d, n_out=%d (at most %d and %d)", what, rows, n_out, pk::kLoraMaxRows,
+                pk::kLoraMaxOut);
   if (rank <= 0 || rank % 8 || rank > pk::kLoraMaxRank)
     return fail(PK_ERR_UNSUPPORTED, "%s: rank=%d must be a multiple of 8 up to %d", what, rank, pk::kLoraMaxRank);
   *p = pk::LoraArgs{};
@@ -881,8 +884,8 @@ int pk_lora_add(const void* y, int64_t y_row_stride, const void* x, int64_t x_ro
   if (rows > pk::kLoraSmallRows && num_adapters > pk::kLoraMaxAdapters)
     return fail(PK_ERR_UNSUPPORTED, "lora_add: %d adapters for more than %d rows (at most %d)", num_adapters,
                 pk::kLoraSmallRows, pk::kLoraMaxAdapters);
-  if (rows > (1 << 22) || n_out > (1 << 20))
-    return fail(PK_ERR_UNSUPPORTED, "lora_add: rows=%d, n_out=%d (at most 2^22 and 2^20)", rows, n_out);
+  if (pk::lora_add_groups(p) > pk::kLoraMaxGroups)
+    return fail(PK_ERR_UNSUPPORTED, "lora_add: rows=%d of n_out=%d are too many for one launch", rows, n_out);
   if (int rc = check_scratch("lora_add", workspace, workspace_bytes,
                              pk::lora_add_workspace_bytes(p)))
     return rc;
@@ -960,6 +963,8 @@ int pk_free_sequences(int32_t* block_tables, int64_t block_table_stride, int32_t
                       const int32_t* rows, int32_t num_listed, pk_stream_t stream) {
   g_last_error.clear();
   if (num_listed < 0) return fail(PK_ERR_INVALID_ARG, "free_sequences: %d sequences listed", num_listed);
+  if (num_listed > (1 << 24))
+    return fail(PK_ERR_UNSUPPORTED, "free_sequences: %d sequences in one call (at most 2^24)", num_listed);
   pk::PageTables t{};
   if (int rc = page_tables("free_sequences", &t, block_tables, block_table_stride, num_rows, table_width,
                            context_lens, ref_counts, num_blocks, block_size))

@@ -263,6 +263,9 @@ hipError_t launch_linear_add_rmsnorm(const void* x, int64_t x_stride, const void
 // Low-rank adapters beside a projection (lora.hip).
 constexpr int kLoraMaxSlices = 4;
 constexpr int kLoraMaxRank = 128;
+constexpr int kLoraMaxRows = 1 << 22;
+constexpr int kLoraMaxOut = 1 << 20;
+constexpr int64_t kLoraMaxGroups = (1 << 24) - 1;  // work-groups of 256 threads in one launch
 constexpr int kLoraMaxAdapters = 4095;  // of an addition to more than kLoraSmallRows rows: its sort's LDS
 // Rows up to which an addition works on 16 rows in a row, unsorted. Measured, unsorted and sorted, us: 512
 // rows of qkv, 8 adapters of rank 16 18.4 and 21.9, 100 26.8 and 25.8; 384 rows 14.9 and 21.7, 21.8 and 25.5; 768
@@ -298,6 +301,7 @@ struct LoraArgs {
 };
 size_t lora_linear_workspace_bytes(const LoraArgs& p);
 size_t lora_add_workspace_bytes(const LoraArgs& p);
+int64_t lora_add_groups(const LoraArgs& p);  // of its largest launch
 hipError_t launch_lora_linear(const LoraArgs& p, const void* w, int64_t w_stride, void* ws, hipStream_t stream);
 hipError_t launch_lora_add(const LoraArgs& p, void* ws, hipStream_t stream);
 // Pages of the cache (kv_pages.hip). Strides of the caches in 16-byte vectors.

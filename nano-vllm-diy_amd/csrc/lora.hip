@@ -848,6 +848,14 @@ size_t lora_add_workspace_bytes(const LoraArgs& p) {
          (size_t)p.rows * sizeof(int32_t);
 }
 
+int64_t lora_add_groups(const LoraArgs& p) {
+  const bool small = p.rows <= kLoraSmallRows;
+  const int64_t tiles = small ? p.rows : lora_max_tiles(p.rows, p.num_adapters);
+  // (an unsorted expand has 256 columns or more a work-group; a shrink 32 rows and 64 columns of t)
+  return tiles * std::max<int64_t>(col_groups(p, small ? 256 : kSortedCols),
+                                   2 * ((p.num_slices * p.rank + (small ? 15 : 63)) / (small ? 16 : 64)));
+}
+
 hipError_t launch_lora_linear(const LoraArgs& args, const void* w, int64_t w_stride, void* ws, hipStream_t stream) {
   LoraArgs p = args;
   const LinCfg c = choose_config(p.rows, p.n_out / kLinTile, p.k, 1);

@@ -12,6 +12,8 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 def call(fn, what: str, device: torch.device, *args) -> None:
     """fn(*args, current stream of device) with device current; raises what it refuses."""
     index = device.index
+    if index is None:
+        raise ValueError(f"{what}: tensors must be on a GPU, not on {device}")
     if index == torch.cuda.current_device():
         code = fn(*args, _raw_stream(index))
     else:

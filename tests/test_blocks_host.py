@@ -63,6 +63,7 @@ def test_list_refusals():
         assert _call(name, n=-1) == _lib.PK_ERR_INVALID_ARG
         assert _call(name, n=1025) == _lib.PK_ERR_UNSUPPORTED
     assert _call("pk_free_sequences", n=-1) == _lib.PK_ERR_INVALID_ARG
+    assert _call("pk_free_sequences", n=2 ** 24 + 1) == _lib.PK_ERR_UNSUPPORTED
     assert _call("pk_fork_sequences", n=1, parents=None) == _lib.PK_ERR_INVALID_ARG
     assert _call("pk_extend_sequences", n=1, slots=None) == _lib.PK_ERR_INVALID_ARG
     assert _call("pk_extend_sequences", blocks=2 ** 24) == _lib.PK_ERR_UNSUPPORTED  # slots past 31 bits
@@ -95,6 +96,8 @@ def test_python_refusals():
         pagedkv.free_sequences(t, ln, rc, 8, torch.zeros(4, dtype=torch.int32)[::2])
     with pytest.raises(ValueError, match="contiguous rows"):
         pagedkv.free_sequences(t.t(), ln[:2], rc, 8, one)
+    with pytest.raises(ValueError, match="on a GPU"):
+        pagedkv.extend_sequences(t, ln, rc, 8, one)
 
 
 def test_oracle_pool_by_hand():

@@ -61,7 +61,14 @@ def test_refusals_of_one():
     assert _call("pk_lora_add", y_stride=56) == _lib.PK_ERR_INVALID_ARG
     assert _call("pk_lora_add", y_stride=72) == _lib.PK_ERR_INVALID_ARG             # out is y, other rows
     assert _call("pk_lora_add", rows=513, adapters=4096) == _lib.PK_ERR_UNSUPPORTED
-    assert _call("pk_lora_add", rows=2 ** 22 + 1) == _lib.PK_ERR_UNSUPPORTED
+    for name in ("pk_lora_linear", "pk_lora_add"):
+        assert _call(name, rows=2 ** 22 + 1) == _lib.PK_ERR_UNSUPPORTED
+        wide = dict(n_out=2 ** 20 + 32, out_stride=2 ** 20 + 32)
+        assert _call(name, **wide, **(dict(y_stride=2 ** 20 + 32) if name == "pk_lora_add" else {})) == \
+            _lib.PK_ERR_UNSUPPORTED
+    assert _call("pk_lora_add", rows=2 ** 22, n_out=2 ** 20, out_stride=2 ** 20, y_stride=2 ** 20) == \
+        _lib.PK_ERR_UNSUPPORTED
+    assert b"too many" in _lib.lib().pk_last_error()
     for name in ("pk_lora_linear", "pk_lora_add"):
         assert _call(name, rows=0, x=None, ids=None, out=None, ws=None, ws_bytes=0) == _lib.PK_OK
 
@@ -105,5 +112,7 @@ def test_python_refusals():
         pagedkv.lora_add(y[:3], x, a, b, ids)
     with pytest.raises(ValueError, match="does not match"):
         pagedkv.lora_linear(x, w[:, :128], a, b, ids)
+    with pytest.raises(ValueError, match="on a GPU"):  # tensors of one device, which is not a GPU
+        pagedkv.lora_add(y, x, a, b, ids)
     with pytest.raises(ValueError, match="at most 128"):
         pagedkv.lora_linear(torch.zeros(129, 256, **bf), w, a, b, torch.zeros(129, dtype=torch.int32))
