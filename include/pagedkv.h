@@ -482,8 +482,7 @@ int pk_linear_add_rmsnorm(const void* x, int64_t x_row_stride, const void* weigh
  * pk_lora_linear -- base = x W^T in fp32 (a decode step's projection, pk_linear's weight and limits:
  *   at most 128 rows, k a multiple of 256); out must not overlap x.
  * pk_lora_add -- base = y (rows, n_out) bf16, the output of a projection computed elsewhere. out may be
- *   y (in place, rows without an adapter are then not written), or must not overlap y or x. Above
- *   512 rows up to 4095 adapters.
+ *   y (in place, rows without an adapter are then not written), or must not overlap y or x.
  */
 size_t pk_lora_linear_workspace_bytes(int32_t rows, int32_t n_out, int32_t k, int32_t rank, int32_t num_slices);
 int pk_lora_linear(const void* x, int64_t x_row_stride, const void* weight, int64_t weight_row_stride,

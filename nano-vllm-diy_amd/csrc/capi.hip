@@ -881,9 +881,6 @@ int pk_lora_add(const void* y, int64_t y_row_stride, const void* x, int64_t x_ro
     return fail(PK_ERR_INVALID_ARG, "lora_add: y null, not 16-byte aligned, or its row stride no multiple of 8 >= n_out");
   if (y == out && y_row_stride != out_row_stride)
     return fail(PK_ERR_INVALID_ARG, "lora_add: out may be y only with y's row stride");
-  if (rows > pk::kLoraSmallRows && num_adapters > pk::kLoraMaxAdapters)
-    return fail(PK_ERR_UNSUPPORTED, "lora_add: %d adapters for more than %d rows (at most %d)", num_adapters,
-                pk::kLoraSmallRows, pk::kLoraMaxAdapters);
   if (pk::lora_add_groups(p) > pk::kLoraMaxGroups)
     return fail(PK_ERR_UNSUPPORTED, "lora_add: rows=%d of n_out=%d are too many for one launch", rows, n_out);
   if (int rc = check_scratch("lora_add", workspace, workspace_bytes,

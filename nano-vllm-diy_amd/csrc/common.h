@@ -266,12 +266,7 @@ constexpr int kLoraMaxRank = 128;
 constexpr int kLoraMaxRows = 1 << 22;
 constexpr int kLoraMaxOut = 1 << 20;
 constexpr int64_t kLoraMaxGroups = (1 << 24) - 1;  // work-groups of 256 threads in one launch
-constexpr int kLoraMaxAdapters = 4095;  // of an addition to more than kLoraSmallRows rows: its sort's LDS
-// Rows up to which an addition works on 16 rows in a row, unsorted. Measured, unsorted and sorted, us: 512
-// rows of qkv, 8 adapters of rank 16 18.4 and 21.9, 100 26.8 and 25.8; 384 rows 14.9 and 21.7, 21.8 and 25.5; 768
-// rows 24.5 and 22.5, 35.3 and 26.3.
-constexpr int kLoraSmallRows = 512;
-
+constexpr int kLoraMaxSorted = 4095;           // adapters of a sorted addition
 struct LoraArgs {
   const uint16_t* x;
   int64_t x_stride;
@@ -293,6 +288,7 @@ struct LoraArgs {
   float* t;                      // [rows][num_slices * rank], scaled
   float* part;                   // [ks][rows][n_out] partial sums of the projection (lora_linear)
   int32_t ks;
+  int32_t tile_slots;            // unsorted: groups that 16 rows can have
   int32_t col_groups;            // column groups of an expand launch over all slices
   int32_t max_tiles;
   int2* tiles;                   // sorted tiles of 64 rows: (adapter or -1, rows)

@@ -9,8 +9,9 @@
 // The work is reading: W or base once, out once, and the adapters in use once each; the products
 // are 16-64 wide and free next to that. So rows are brought together by adapter, and a group of
 // up to 16 or 64 rows of ONE adapter is an MFMA tile that reads A and B once for all of them:
-//   * up to kLoraSmallRows rows: the groups are the equal ids within 16 consecutive rows. Nothing is
-//     sorted: the work-group of a row that is not the first of its group has nothing to do.
+//   * few rows (small_add): the groups are the equal ids within 16 consecutive rows. Nothing is sorted:
+//     there is a work-group for every group that 16 rows can have, 16 or one for each adapter and one
+//     for none, and those without a group end.
 //   * more: one work-group sorts the rows by adapter (counts, offsets, positions) and lists the
 //     tiles of 64.
 // Every row's sums are taken in the same order whatever shares its tile, so a row's result does
@@ -50,17 +51,27 @@ __device__ __forceinline__ int32_t adapter_of(const LoraArgs& p, int32_t row) {
 }
 
 // A tile: its adapter, and each of its R rows' index in x (-1: not a row of the tile), in LDS.
-// Not sorted: the rows of [16 tile, 16 tile + 16) with the adapter of row `slot`; false if an
-// earlier row has that adapter. Every thread of the work-group calls it.
+// Not sorted: of the rows of [16 t, 16 t + 16) those with the jth group's adapter, t = slot /
+// tile_slots and j = slot % tile_slots; false if there is none. Every thread calls it.
 __device__ __forceinline__ bool small_tile(const LoraArgs& p, int32_t slot, int32_t* rows, int32_t* id) {
   const int lane = threadIdx.x & (kWave - 1);
-  const int32_t row = (slot & ~(kLoraSmallTile - 1)) + lane;
+  const int32_t tile = slot / p.tile_slots, row = tile * kLoraSmallTile + lane;
   const bool is_row = lane < kLoraSmallTile && row < p.rows;
   const int32_t mine = is_row ? adapter_of(p, row) : -2;
-  const int j = slot & (kLoraSmallTile - 1);
-  *id = __builtin_amdgcn_readlane(mine, j);
-  const uint64_t group = __ballot(mine == *id);
-  if (__builtin_ctzll(group) != j) return false;
+  const int32_t j = slot - tile * p.tile_slots;
+  if (p.tile_slots == kLoraSmallTile) {  // the group of row j, if that is its first row
+    if (tile * kLoraSmallTile + j >= p.rows) return false;
+    *id = __builtin_amdgcn_readlane(mine, j);
+    if (__builtin_ctzll(__ballot(mine == *id)) != j) return false;
+  } else {
+    uint64_t left = __ballot(is_row);
+    for (int i = 0;; ++i) {
+      if (left == 0) return false;
+      *id = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+      if (i == j) break;
+      left &= ~__ballot(mine == *id);
+    }
+  }
   if (threadIdx.x < kLoraSmallTile) rows[threadIdx.x] = mine == *id ? row : -1;
   __syncthreads();
   return true;
@@ -197,7 +208,7 @@ __device__ __forceinline__ void shrink_to_memory(const LoraArgs& p, const int32_
   });
 }
 
-// Work-group = (row, 16 CB columns of t).
+// Work-group = (group of rows, 16 CB columns of t).
 template <int CB>
 __device__ __forceinline__ void shrink_small(const LoraArgs& p, int32_t group, int32_t* rows, char* smem) {
   const int32_t blocks = (p.num_slices * p.rank + 16 * CB - 1) / (16 * CB);
@@ -405,8 +416,7 @@ __device__ __forceinline__ int32_t group_slice(const LoraArgs& p, int32_t g, int
   return q;
 }
 
-// Work-group = (row, up to 128 WAVES columns of a slice): the rows of 16 with that row's adapter, 128
-// columns a wavefront. Everything is asked for before the first wait.
+// Work-group = (group of rows of one adapter, up to 128 WAVES columns of a slice): 128 columns a wavefront. Everything is asked for before the first wait.
 // kBase: where base is from -- kBasePartial: the sum of p.ks fp32 partial products, kBaseRows: bf16
 // rows of y, kBaseRowsShrink: those, and t is computed here, by every work-group of the row again, instead of
 // by a launch before (the rank is KP at most then).
@@ -764,10 +774,14 @@ int32_t col_groups(const LoraArgs& p, int32_t cols) {
   return n;
 }
 
+// Groups that 16 rows can have, and groups of all rows.
+int32_t tile_slots(const LoraArgs& p) { return std::min(std::min(kLoraSmallTile, p.num_adapters + 1), p.rows); }
+int32_t small_slots(const LoraArgs& p) { return (p.rows + kLoraSmallTile - 1) / kLoraSmallTile * tile_slots(p); }
+
 template <int KP, int WAVES, int kBase>
 void launch_expand_waves(LoraArgs p, hipStream_t stream) {
   p.col_groups = col_groups(p, 128 * WAVES);
-  hipLaunchKernelGGL((lora_expand_small_kernel<KP, WAVES, kBase>), dim3((unsigned)(p.rows * p.col_groups)),
+  hipLaunchKernelGGL((lora_expand_small_kernel<KP, WAVES, kBase>), dim3((unsigned)(small_slots(p) * p.col_groups)),
                      dim3(WAVES * kWave), 0, stream, p);
 }
 
@@ -786,7 +800,7 @@ hipError_t launch_expand_small(const LoraArgs& p, hipStream_t stream) {
 // rank 16, one up to 32. Measured on the 1024 x 2048 projection, one launch and two, us: 128 rows
 // (256 work-groups) rank 16 6.3 and 8.1, rank 32 9.3 and 9.0; 300 rows (600) 13.7 and 10.5, 25.1 and 14.4.
 bool shrink_in_expand(const LoraArgs& p) {
-  return p.rank <= 32 && (int64_t)p.rows * col_groups(p, 128 * kLoraWaves) <= (p.rank <= 16 ? 512 : 256);
+  return p.rank <= 32 && (int64_t)small_slots(p) * col_groups(p, 128 * kLoraWaves) <= (p.rank <= 16 ? 512 : 256);
 }
 
 template <int R>
@@ -827,6 +841,18 @@ hipError_t launch_expand_sorted(LoraArgs p, int64_t tiles, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// Whether an addition works on groups of 16 rows, unsorted. What it costs grows with the groups that
+// there may be, each with its work-groups of the shrink and the expand and the time of about four more;
+// sorting costs 12 us whatever the rows. At the line of 20 a CU, sorted and unsorted, us: qkv (11 + 4 a
+// group at rank 16), 512 rows of 8 adapters (4320) 20.4 and 16.7, 768 (6480) 21.3 and 22.9; 2048 x 1024
+// (3 + 4), 768 rows of 100 (5376) 20.0 and 18.4, 1024 (7168) 21.5 and 20.8; rank 64 (8 + 4), 2048 rows of one
+// adapter (3072) 26.1 and 20.2, 4096 (6144) 28.2 and 37.4.
+bool small_add(const LoraArgs& p) {
+  if (p.num_adapters > kLoraMaxSorted) return true;  // the sort's counters would not fit its LDS
+  const int32_t each = 4 + col_groups(p, p.rank <= 32 ? 512 : 256) + (p.num_slices * p.rank + 15) / 16;
+  return (int64_t)small_slots(p) * each <= 20 * 256;
+}
+
 // Whether the projection's work-groups add the adapters themselves (the shrink before them) rather
 // than leave partial sums to an expand. Measured, us of the two forms' kernels: 97 rows, 1024 x 6144, rank
 // 16 15.2 and 16.7; 1 row, 1024 x 4096 8.9 and 9.7 (in two launches).
@@ -843,14 +869,14 @@ size_t lora_linear_workspace_bytes(const LoraArgs& p) {
 }
 
 size_t lora_add_workspace_bytes(const LoraArgs& p) {
-  if (p.rows <= kLoraSmallRows) return shrink_in_expand(p) ? 0 : t_bytes(p);
+  if (small_add(p)) return shrink_in_expand(p) ? 0 : t_bytes(p);
   return t_bytes(p) + (size_t)lora_max_tiles(p.rows, p.num_adapters) * (kLoraTile * sizeof(int32_t) + sizeof(int2)) +
          (size_t)p.rows * sizeof(int32_t);
 }
 
 int64_t lora_add_groups(const LoraArgs& p) {
-  const bool small = p.rows <= kLoraSmallRows;
-  const int64_t tiles = small ? p.rows : lora_max_tiles(p.rows, p.num_adapters);
+  const bool small = small_add(p);
+  const int64_t tiles = small ? small_slots(p) : lora_max_tiles(p.rows, p.num_adapters);
   // (an unsorted expand has 256 columns or more a work-group; a shrink 32 rows and 64 columns of t)
   return tiles * std::max<int64_t>(col_groups(p, small ? 256 : kSortedCols),
                                    2 * ((p.num_slices * p.rank + (small ? 15 : 63)) / (small ? 16 : 64)));
@@ -858,6 +884,7 @@ int64_t lora_add_groups(const LoraArgs& p) {
 
 hipError_t launch_lora_linear(const LoraArgs& args, const void* w, int64_t w_stride, void* ws, hipStream_t stream) {
   LoraArgs p = args;
+  p.tile_slots = tile_slots(p);
   const LinCfg c = choose_config(p.rows, p.n_out / kLinTile, p.k, 1);
   p.t = static_cast<float*>(ws);
   p.part = p.t + (size_t)p.rows * p.num_slices * p.rank;
@@ -879,7 +906,7 @@ hipError_t launch_lora_linear(const LoraArgs& args, const void* w, int64_t w_str
     a.y_stride = p.out_stride;
     const bool here = p.rows <= kOneLaunchRows;
     if (p.num_adapters > 0 && !here) {
-      hipLaunchKernelGGL(lora_shrink_small_kernel, dim3(p.rows * cols16), dim3(kLoraThreads), 0, stream, p);
+      hipLaunchKernelGGL(lora_shrink_small_kernel, dim3(small_slots(p) * cols16), dim3(kLoraThreads), 0, stream, p);
       if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
     }
     const auto launch = [&](auto nb) {
@@ -899,8 +926,8 @@ hipError_t launch_lora_linear(const LoraArgs& args, const void* w, int64_t w_str
   }
   // 32 columns of t a work-group where there would be too many of 16 to be resident beside the
   // projection's (two a CU): 128 rows, rank 64, k = 3072 11.8 us instead of 13.4
-  const bool wide = p.rows * cols16 >= 512;
-  const int32_t shrink = p.num_adapters > 0 ? p.rows * (wide ? (cols16 + 1) / 2 : cols16) : 0;
+  const bool wide = small_slots(p) * cols16 >= 512;
+  const int32_t shrink = p.num_adapters > 0 ? small_slots(p) * (wide ? (cols16 + 1) / 2 : cols16) : 0;
   const dim3 grid(lin_groups + shrink), block(kLinThreads);
   const auto launch = [&](auto nb, auto cb) {
     hipLaunchKernelGGL((lora_linear_kernel<nb.value, cb.value>), grid, block, 0, stream, a, p, lin_groups);
@@ -920,12 +947,13 @@ hipError_t launch_lora_linear(const LoraArgs& args, const void* w, int64_t w_str
 
 hipError_t launch_lora_add(const LoraArgs& args, void* ws, hipStream_t stream) {
   LoraArgs p = args;
+  p.tile_slots = tile_slots(p);
   p.t = static_cast<float*>(ws);
   const int32_t width = p.num_slices * p.rank;
-  if (p.rows <= kLoraSmallRows) {
+  if (small_add(p)) {
     if (shrink_in_expand(p)) return launch_expand_small<kBaseRowsShrink>(p, stream);
     if (p.num_adapters > 0) {
-      hipLaunchKernelGGL(lora_shrink_small_kernel, dim3(p.rows * ((width + 15) / 16)), dim3(kLoraThreads), 0, stream,
+      hipLaunchKernelGGL(lora_shrink_small_kernel, dim3(small_slots(p) * ((width + 15) / 16)), dim3(kLoraThreads), 0, stream,
                          p);
       if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
     }

@@ -96,7 +96,8 @@ def test_linear_against_formula(gpu, rows, proj, rank, adapters, ids):
     (1, QKV, 16, 4, 1), (2, (8, (32,)), 8, 2, "mixed"), (63, (40, (32, 32)), 16, 3, "mixed"),
     (64, (1000, (96,)), 32, 3, "mixed"), (65, (1032, (160, 32, 32, 64)), 128, 3, "mixed"), (300, O, 8, 24, "mixed"),
     (512, QKV, 16, 600, "mixed"), (513, QKV, 16, 8, "runs"), (513, (40, (32, 32)), 40, 1, 0),
-    (600, (264, (288,)), 72, 4095, "mixed"), (700, (1000, (96, 64)), 24, 3, "mixed"), (1025, DOWN, 64, 7, "runs"),
+    (600, (264, (288,)), 72, 4095, "mixed"), (700, (64, (288,)), 8, 5000, "mixed"), (2500, O, 16, 1, "runs"),
+    (1200, QKV, 16, 2, "mixed"), (1500, QKV, 16, 14, "runs"), (700, (1000, (96, 64)), 24, 3, "mixed"), (1025, DOWN, 64, 7, "runs"),
     (2000, GATE_UP, 128, 5, "runs"), (30, QKV, 32, 7, "mixed"), (64, QKV, 24, 3, "runs"), (33, DOWN, 16, 9, "mixed"),
     (128, O, 32, 2, "mixed"), (17000, (64, (32, 32)), 8, 3, "runs"), (33000, (64, (32,)), 16, 40, "mixed"),
     (24700, (256, (64, 64)), 32, 2, "runs"), (3001, O, 16, 50, "mixed"), (1500, (64, (32,)), 8, 4, -1)])
@@ -114,11 +115,13 @@ def test_add_against_formula(gpu, rows, proj, rank, adapters, ids):
     assert in_place is d["y"] and torch.equal(in_place.view(torch.int16), got.view(torch.int16))
 
 
-@pytest.mark.parametrize("rows", [100, 900])
+@pytest.mark.parametrize("rows", [100, 1900])
 def test_row_does_not_depend_on_the_batch(gpu, rows):
     """A row's bits are the same alone, in a batch and in another order of it, on both sides of the size
     at which rows are sorted."""
     d = _gpu(_case(rows, rows, 1024, (256, 64), 16, 5), gpu)
+    sorts = pagedkv.lora_workspace_bytes(rows, 320, 1024, 16, (256, 64), 5) > rows * 32 * 4
+    assert sorts == (rows == 1900)
     print(f"[lora_add] rows={rows} alone / together / reversed", flush=True)
     whole = _add(d)
     for m in (0, rows // 2, rows - 1):
@@ -128,7 +131,7 @@ def test_row_does_not_depend_on_the_batch(gpu, rows):
     assert torch.equal(_add(back).flip(0).view(torch.int16), whole.view(torch.int16))
 
 
-@pytest.mark.parametrize("rows", [40, 700])
+@pytest.mark.parametrize("rows", [40, 2700])
 def test_non_finite_values_stay_in_their_rows(gpu, rows):
     """NaN and infinity in one row's x or y, or in one adapter, reach only the rows they belong to."""
     c = _case(rows, rows, 512, (64, 64), 16, 4)
@@ -153,10 +156,11 @@ def test_non_finite_values_stay_in_their_rows(gpu, rows):
         assert float(got[7, 9]) == float("-inf") and torch.equal(got[7, 10:], clean[7, 10:])
 
 
-@pytest.mark.parametrize("rows", [70, 800])
-def test_strides_and_what_lies_around_the_output(gpu, rows):
-    """x, y, out, weight and both adapters as views of larger tensors; nothing beside out is written."""
-    k, n, rank, adapters = 256, 96, 16, 3
+@pytest.mark.parametrize("rows,adapters", [(1, 3), (17, 1), (33, 40), (70, 3), (125, 15), (800, 3), (900, 300), (2700, 5)])
+def test_strides_and_what_lies_around_the_output(gpu, rows, adapters):
+    """x, y, out, weight and both adapters as views of larger tensors; nothing beside out is written,
+    the rows behind the last one of a tile of 16 or 64 among it."""
+    k, n, rank = 256, 96, 16
     c = _case(rows, rows, k, (64, 32), rank, adapters)
     d = _gpu(c, gpu)
 
@@ -168,16 +172,17 @@ def test_strides_and_what_lies_around_the_output(gpu, rows):
     v = dict(d, x=view(d["x"], 24), y=view(d["y"], 40), w=view(d["w"], 16), b=view(d["b"], 8))
     layers = torch.stack([torch.zeros_like(d["a"]), d["a"]], 1)  # (L, layers, S r, k): this layer's slice
     v["a"] = layers[:, 1]
-    big = torch.full((rows + 2, n + 48), 7.0, dtype=torch.bfloat16, device=gpu)
-    print(f"[lora] rows={rows} strides", flush=True)
-    _add(v, out=big[1:-1, 16:16 + n])
-    assert torch.equal(big[1:-1, 16:16 + n], _add(d))
-    big[1:-1, 16:16 + n] = 7.0
+    big = torch.full((rows + 80, n + 48), 7.0, dtype=torch.bfloat16, device=gpu)
+    out = big[1:1 + rows, 16:16 + n]
+    print(f"[lora] rows={rows} adapters={adapters} strides", flush=True)
+    _add(v, out=out)
+    assert torch.equal(out, _add(d))
+    out.fill_(7.0)
     assert bool((big == 7.0).all())
     if rows <= 128:
-        _linear(v, out=big[1:-1, 16:16 + n])
-        assert torch.equal(big[1:-1, 16:16 + n], _linear(d))
-        big[1:-1, 16:16 + n] = 7.0
+        _linear(v, out=out)
+        assert torch.equal(out, _linear(d))
+        out.fill_(7.0)
         assert bool((big == 7.0).all())
 
 
@@ -223,7 +228,7 @@ def test_offsets_past_32_bits(gpu):
     assert y[rows - 1, n - 1].item() == 6.0 and y[7, 3].item() == 10.0 and y[7, n - 1].item() == 6.0
 
 
-@pytest.mark.parametrize("rows", [48, 640])
+@pytest.mark.parametrize("rows", [48, 640, 3000])
 def test_captured_call_replays_with_new_rows(gpu, rows):
     """A captured call replayed with other rows and other adapters in the same buffers, with eager calls
     of another shape between the replays."""
@@ -259,7 +264,7 @@ def test_captured_call_replays_with_new_rows(gpu, rows):
 
 def test_two_streams(gpu):
     """Calls on two streams at once, each with its own scratch."""
-    ds = [_gpu(_case(s, 900, 1024, (512,), 16, 4), gpu) for s in range(2)]
+    ds = [_gpu(_case(s, 4000, 1024, (512,), 16, 4), gpu) for s in range(2)]
     want = [_add(d) for d in ds]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in ds]
@@ -276,8 +281,9 @@ def test_two_streams(gpu):
 
 
 def test_given_workspace(gpu):
-    d = _gpu(_case(3, 700, 256, (64, 32), 16, 5), gpu)
-    need = pagedkv.lora_workspace_bytes(700, 96, 256, 16, (64, 32), 5)
+    d = _gpu(_case(3, 2700, 256, (64, 32), 16, 5), gpu)
+    need = pagedkv.lora_workspace_bytes(2700, 96, 256, 16, (64, 32), 5)
+    assert need > 2700 * 32 * 4  # sorted
     ws = torch.full((need + 64,), 255, dtype=torch.uint8, device=gpu)
     print("[lora_add] workspace", flush=True)
     assert torch.equal(_add(d, workspace=ws[:need]), _add(d))

@@ -60,7 +60,6 @@ def test_refusals_of_one():
     assert _call("pk_lora_add", y=None) == _lib.PK_ERR_INVALID_ARG
     assert _call("pk_lora_add", y_stride=56) == _lib.PK_ERR_INVALID_ARG
     assert _call("pk_lora_add", y_stride=72) == _lib.PK_ERR_INVALID_ARG             # out is y, other rows
-    assert _call("pk_lora_add", rows=513, adapters=4096) == _lib.PK_ERR_UNSUPPORTED
     for name in ("pk_lora_linear", "pk_lora_add"):
         assert _call(name, rows=2 ** 22 + 1) == _lib.PK_ERR_UNSUPPORTED
         wide = dict(n_out=2 ** 20 + 32, out_stride=2 ** 20 + 32)
@@ -78,7 +77,7 @@ def test_workspace_sizes():
     qkv = (ctypes.c_int32 * 3)(2048, 1024, 1024)
     # one launch, no scratch, while all its work-groups are on the GPU at once
     assert lib.pk_lora_add_workspace_bytes(64, 4096, 16, qkv, 3, 8) == 0
-    assert lib.pk_lora_add_workspace_bytes(100, 4096, 16, qkv, 3, 8) == 100 * 48 * 4
+    assert lib.pk_lora_add_workspace_bytes(200, 4096, 16, qkv, 3, 8) == 200 * 48 * 4
     # sorted: t, the rows of the tiles, their records, the rows' places
     assert lib.pk_lora_add_workspace_bytes(1000, 4096, 16, qkv, 3, 8) == 1000 * 48 * 4 + (15 + 9) * (256 + 8) + 4000
     assert lib.pk_lora_add_workspace_bytes(1000, 4000, 16, qkv, 3, 8) == 0                # refused
@@ -89,7 +88,7 @@ def test_workspace_sizes():
     assert lib.pk_lora_linear_workspace_bytes(100, 4096, 1024, 16, 3) == 100 * 48 * 4
     assert lib.pk_lora_linear_workspace_bytes(2, 4096, 1024, 16, 3) == 0
     assert lib.pk_lora_linear_workspace_bytes(129, 1024, 1024, 16, 1) == 0
-    assert pagedkv.lora_workspace_bytes(100, 4096, 1024, 16, (2048, 1024, 1024), 8) == 100 * 48 * 4
+    assert pagedkv.lora_workspace_bytes(200, 4096, 1024, 16, (2048, 1024, 1024), 8) == 200 * 48 * 4
 
 
 def test_python_refusals():
