@@ -224,7 +224,8 @@ __global__ __launch_bounds__(kLoraThreads) void lora_shrink_small_kernel(const L
   shrink_small<1>(p, blockIdx.x, rows, smem);
 }
 
-// Work-group = (R rows of a sorted tile, 16 CB columns of t).
+// Work-group = (R rows of a sorted tile, 16 CB columns of t). 16384 rows of k = 1024, 48 columns 10.0 us (x
+// alone 6.6 at a copy's rate): the rest is the chain from the tile's rows to their first loads.
 template <int R, int CB>
 __global__ __launch_bounds__(kLoraThreads) void lora_shrink_kernel(const LoraArgs p) {
   __shared__ __attribute__((aligned(16))) char smem[shrink_smem_bytes(R, CB)];
@@ -239,7 +240,8 @@ __global__ __launch_bounds__(kLoraThreads) void lora_shrink_kernel(const LoraArg
 }
 
 // The partial sums of a decode step's projection (work-groups [0, lin_groups)) and the shrink of its
-// adapters, which need nothing of each other, in one launch; the expand adds the partial sums.
+// adapters, which need nothing of each other, in one launch; the expand adds the partial sums. 128 rows,
+// 75 adapters of rank 64 on 3072 x 1024: 12.0 us for 34 MB.
 template <int NB, int CB>
 __global__ __launch_bounds__(kLinThreads) void lora_linear_kernel(const LinArgs a, const LoraArgs p,
                                                                   const int32_t lin_groups) {
@@ -533,7 +535,9 @@ __global__ __launch_bounds__(WAVES* kWave) void lora_expand_small_kernel(const L
 // Work-group = (sorted tile, up to kSortedCols columns of a slice): 16 rows a wavefront, all four the
 // same columns, which they walk 128 at a time. The walk's loads are one turn ahead of its
 // products: B's next rows and the base's next columns are in flight while this turn multiplies
-// and stores. t stays in registers: NP pieces of KP elements of the rank.
+// and stores. t stays in registers: NP pieces of KP elements of the rank. Bound by HBM: 16384 x 4096,
+// rank 16 56.8 us, 4.7 TB/s of base and out (a copy's rate); 13001 x 6144, rank 64 76 us, 4.2 TB/s.
+// 1024 columns a work-group 61 and 80, 256 and 384 within 2 %.
 constexpr int kSortedCols = 512;
 
 template <int KP, int NP>
@@ -629,8 +633,8 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_kernel(const LoraArg
 // buckets' first tiles, then every row's position. A lane has 4 neighbouring rows, a wavefront 256
 // at a time; 256 rows of one adapter, the common case of a prefill step, count as one entry, and the
 // entries of all kPlanTurns turns ask the counters in one LDS atomic, lane i for turn i. The work is
-// instructions on one CU, so what is done per row is what counts: 16384 rows of 8 adapters
-// 9.3 us with one row a lane.
+// instructions on one CU, so what is done per row is what counts: 16384 rows of 8 adapters 11.8 us
+// with one row a lane, 7.0 so.
 // Rows of one adapter come in any order, which no result shows: a row's sums are its own.
 typedef int32_t i32x4_u __attribute__((ext_vector_type(4), aligned(4)));
 

@@ -92,10 +92,10 @@ def fork_sequences(k_caches: torch.Tensor, v_caches: torch.Tensor, block_tables:
 
     A child shares its parent's full pages (ref_counts + 1) and, where the parent's last page is
     not full, gets a new page with that page's tokens, copied in every layer, so parent and child
-    both grow without seeing each other's tokens. Returns new_blocks (n,) int32: that page's number; -1 where none was
-    needed; -2 where the pool had none left; -3 where children[i] is no row of the tables, is not
-    empty or was listed before. With -2 and -3 the child stays as it was. At most 1024 forks a
-    call.
+    both grow without seeing each other's tokens. Returns new_blocks (n,) int32: that page's
+    number; -1 where none was needed; -2 where the pool had none left; -3 where children[i] is no
+    row of the tables, is not empty or was listed before. With -2 and -3 the child stays as it
+    was. At most 1024 forks a call.
     """
     args, dev = _cache_args(k_caches, v_caches)
     pool = _pool_args(block_tables, context_lens, ref_counts, dev)
@@ -117,7 +117,8 @@ def extend_sequences(block_tables: torch.Tensor, context_lens: torch.Tensor, ref
     """One more token for every listed row of the tables; returns slot_mapping (n,) int32.
 
     The token's slot is the one store_kvcache and the decode calls take; a row whose last page is
-    full gets a new page, and its length grows by one. -1, and nothing changed, where the row is
+    full gets a new page, and its length grows by one (a last page that is not full has to be the
+    row's alone, as forks leave it). -1, and nothing changed, where the row is
     no row of the tables or was listed before, its table is full or the pool has no page left.
     At most 1024 rows a call.
     """
