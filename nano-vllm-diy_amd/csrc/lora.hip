@@ -418,14 +418,16 @@ __device__ __forceinline__ int32_t group_slice(const LoraArgs& p, int32_t g, int
   return q;
 }
 
-// Work-group = (group of rows of one adapter, up to 128 WAVES columns of a slice): 128 columns a wavefront. Everything is asked for before the first wait.
+// Work-group = (group of rows of one adapter, up to 128 WAVES columns of a slice): 128 columns a
+// wavefront. Everything is asked for before the first wait.
 // kBase: where base is from -- kBasePartial: the sum of p.ks fp32 partial products, kBaseRows: bf16
 // rows of y, kBaseRowsShrink: those, and t is computed here, by every work-group of the row again, instead of
 // by a launch before (the rank is KP at most then).
 enum Base { kBasePartial = 0, kBaseRows = 1, kBaseRowsShrink = 2 };
 
 template <int KP, int WAVES, int kBase>
-__global__ __launch_bounds__(WAVES* kWave) void lora_expand_small_kernel(const LoraArgs p) {
+__global__ __launch_bounds__(WAVES* kWave, kBase == kBaseRowsShrink && KP == 16 ? 3 : 1) void
+lora_expand_small_kernel(const LoraArgs p) {
   using S = ExpandShape<KP>;
   constexpr bool kPartial = kBase == kBasePartial, kShrink = kBase == kBaseRowsShrink;
   static_assert(!kShrink || WAVES == kLoraWaves, "shrink_tile's work-group");
@@ -471,7 +473,7 @@ __global__ __launch_bounds__(WAVES* kWave) void lora_expand_small_kernel(const L
         if (begin + c < end && j < p.rank) st[i] = *reinterpret_cast<const u32x4*>(bp + (begin + c) * p.b_row + j);
       }
       if constexpr (kShrink) {
-        shrink_tile<kLoraSmallTile, CB, 4 / CB>(p, id, q * p.rank, rows, smem, [&](int i, int c, const f32x4 v) {
+        shrink_tile<kLoraSmallTile, CB, 2 / CB>(p, id, q * p.rank, rows, smem, [&](int i, int c, const f32x4 v) {
           *reinterpret_cast<f32x4*>(t_here + i * KP + c) = v;
         });
         __syncthreads();  // t is there, and the sums it was added from are free for B
@@ -800,11 +802,13 @@ hipError_t launch_expand_small(const LoraArgs& p, hipStream_t stream) {
 }
 
 // Whether a small addition computes t in the expand's work-groups (one launch, but every group of
-// 512 columns reads its adapter's A again): where all of them are on the GPU at once, two a CU up to
-// rank 16, one up to 32. Measured on the 1024 x 2048 projection, one launch and two, us: 128 rows
-// (256 work-groups) rank 16 6.3 and 8.1, rank 32 9.3 and 9.0; 300 rows (600) 13.7 and 10.5, 25.1 and 14.4.
+// 512 columns reads its adapter's A again): where all of them are on the GPU at once, three a CU up to
+// rank 16, two up to 32 (two chunks ahead in the shrink, not four, for that many). Measured, us in a
+// graph, one launch and two: 2048 x 1024, 300 rows of 100 adapters (608 work-groups) 10.7 and 10.6, 400 rows
+// (800) 14.3 and 11.7; qkv, 96 rows (768) 7.9 and 9.2, 128 rows (1024) 11.1 and 10.3; gate/up, rank 32, 64 rows of 8
+// adapters (432) 8.2 and 9.3, 96 rows (648) 11.6 and 9.7.
 bool shrink_in_expand(const LoraArgs& p) {
-  return p.rank <= 32 && (int64_t)small_slots(p) * col_groups(p, 128 * kLoraWaves) <= (p.rank <= 16 ? 512 : 256);
+  return p.rank <= 32 && (int64_t)small_slots(p) * col_groups(p, 128 * kLoraWaves) <= (p.rank <= 16 ? 768 : 512);
 }
 
 template <int R>
@@ -957,8 +961,8 @@ hipError_t launch_lora_add(const LoraArgs& args, void* ws, hipStream_t stream) {
   if (small_add(p)) {
     if (shrink_in_expand(p)) return launch_expand_small<kBaseRowsShrink>(p, stream);
     if (p.num_adapters > 0) {
-      hipLaunchKernelGGL(lora_shrink_small_kernel, dim3(small_slots(p) * ((width + 15) / 16)), dim3(kLoraThreads), 0, stream,
-                         p);
+      hipLaunchKernelGGL(lora_shrink_small_kernel, dim3(small_slots(p) * ((width + 15) / 16)), dim3(kLoraThreads), 0,
+                         stream, p);
       if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
     }
     return launch_expand_small<kBaseRows>(p, stream);

@@ -77,6 +77,7 @@ def test_workspace_sizes():
     qkv = (ctypes.c_int32 * 3)(2048, 1024, 1024)
     # one launch, no scratch, while all its work-groups are on the GPU at once
     assert lib.pk_lora_add_workspace_bytes(64, 4096, 16, qkv, 3, 8) == 0
+    assert lib.pk_lora_add_workspace_bytes(160, 4096, 16, qkv, 3, 8) == 0
     assert lib.pk_lora_add_workspace_bytes(200, 4096, 16, qkv, 3, 8) == 200 * 48 * 4
     # sorted: t, the rows of the tiles, their records, the rows' places
     assert lib.pk_lora_add_workspace_bytes(1000, 4096, 16, qkv, 3, 8) == 1000 * 48 * 4 + (15 + 9) * (256 + 8) + 4000
