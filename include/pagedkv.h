@@ -482,7 +482,8 @@ int pk_linear_add_rmsnorm(const void* x, int64_t x_row_stride, const void* weigh
  * pk_lora_linear -- base = x W^T in fp32 (a decode step's projection, pk_linear's weight and limits:
  *   at most 128 rows, k a multiple of 256); out must not overlap x.
  * pk_lora_add -- base = y (rows, n_out) bf16, the output of a projection computed elsewhere. out may be
- *   y (in place, rows without an adapter are then not written), or must not overlap y or x.
+ *   y (in place, rows without an adapter are then not written), or must not overlap y or x
+ *   (columns of one buffer, beside x's and y's with one row stride, do not).
  */
 size_t pk_lora_linear_workspace_bytes(int32_t rows, int32_t n_out, int32_t k, int32_t rank, int32_t num_slices);
 int pk_lora_linear(const void* x, int64_t x_row_stride, const void* weight, int64_t weight_row_stride,
@@ -511,8 +512,8 @@ int pk_lora_add(const void* y, int64_t y_row_stride, const void* x, int64_t x_ro
  * bases 16-byte aligned), so (L, NB, BS, Hkv, D) tensors and views of them both fit.
  * Tables: block_tables (num_rows, table_width), row stride block_table_stride; context_lens
  * (num_rows,) tokens of every row, 0: the row is empty; ref_counts (num_blocks,) the number of
- * holders of every block, 0: free. A row of length n holds its first ceil(n / block_size) entries.
- * Entries outside [0, num_blocks) are passed over, lengths beyond the table's width end there.
+ * holders of every block, 0: free (at most 2^30 blocks). A row of length n holds its first
+ * ceil(n / block_size) entries. Entries outside [0, num_blocks) are passed over, lengths beyond the table's width end there.
  * Blocks are given out lowest number first in the order of the list. No call reads back to the
  * host; calls on one pool must be ordered (one stream).
  *

@@ -173,6 +173,8 @@ int page_tables(const char* what, pk::PageTables* t, int32_t* tables, int64_t st
   if (rows < 0 || width < 0 || num_blocks <= 0 || block_size <= 0)
     return fail(PK_ERR_INVALID_ARG, "%s: rows=%d, table_width=%d, num_blocks=%d, block_size=%d", what, rows, width,
                 num_blocks, block_size);
+  if (num_blocks > (1 << 30))  // the kernels step over them in 32 bits
+    return fail(PK_ERR_UNSUPPORTED, "%s: num_blocks=%d (at most 2^30)", what, num_blocks);
   if (rows > 0 && width > 0 && (!tables || stride < width))
     return fail(PK_ERR_INVALID_ARG, "%s: block_tables null, or its row stride %lld below the width %d", what,
                 (long long)stride, width);
@@ -216,6 +218,20 @@ int lora_slices(const char* what, pk::LoraArgs* p, int32_t n_out, const int32_t*
   if (sum != n_out) return fail(PK_ERR_INVALID_ARG, "%s: the slices' widths do not add up to n_out=%d", what, n_out);
   p->num_slices = num_slices;
   return PK_OK;
+}
+
+// Whether the rows of two tensors of 16-bit elements share memory; with one stride, columns of one buffer
+// beside each other do not.
+bool rows_overlap(const void* a, int64_t a_stride, int64_t a_width, const void* b, int64_t b_stride, int64_t b_width,
+                  int64_t rows) {
+  const auto ab = reinterpret_cast<uintptr_t>(a), bb = reinterpret_cast<uintptr_t>(b);
+  const uintptr_t a_end = ab + ((uintptr_t)(rows - 1) * a_stride + a_width) * 2;
+  const uintptr_t b_end = bb + ((uintptr_t)(rows - 1) * b_stride + b_width) * 2;
+  if (ab >= b_end || bb >= a_end) return false;
+  if (a_stride != b_stride) return true;
+  const int64_t s = a_stride * 2, d = (int64_t)((intptr_t)(bb - ab) % s);
+  const int64_t at = d < 0 ? d + s : d;  // b's columns in a's row
+  return at < a_width * 2 || at + b_width * 2 > s;
 }
 
 int lora_args(const char* what, pk::LoraArgs* p, const void* x, int64_t x_row_stride, int32_t rows, int32_t n_out,
@@ -883,6 +899,11 @@ int pk_lora_add(const void* y, int64_t y_row_stride, const void* x, int64_t x_ro
     return fail(PK_ERR_INVALID_ARG, "lora_add: out may be y only with y's row stride");
   if (pk::lora_add_groups(p) > pk::kLoraMaxGroups)
     return fail(PK_ERR_UNSUPPORTED, "lora_add: rows=%d of n_out=%d are too many for one launch", rows, n_out);
+  // out is written while other work-groups still read x and y
+  if (rows_overlap(out, out_row_stride, n_out, x, x_row_stride, k, rows))
+    return fail(PK_ERR_INVALID_ARG, "lora_add: out overlaps x");
+  if (y != out && rows_overlap(out, out_row_stride, n_out, y, y_row_stride, n_out, rows))
+    return fail(PK_ERR_INVALID_ARG, "lora_add: out overlaps y without being y");
   if (int rc = check_scratch("lora_add", workspace, workspace_bytes,
                              pk::lora_add_workspace_bytes(p)))
     return rc;

@@ -6,7 +6,9 @@ import torch
 
 from ._lib import check
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# (not a public function: without it, through the stream object)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def call(fn, what: str, device: torch.device, *args) -> None:

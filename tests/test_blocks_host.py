@@ -67,6 +67,9 @@ def test_list_refusals():
     assert _call("pk_fork_sequences", n=1, parents=None) == _lib.PK_ERR_INVALID_ARG
     assert _call("pk_extend_sequences", n=1, slots=None) == _lib.PK_ERR_INVALID_ARG
     assert _call("pk_extend_sequences", blocks=2 ** 24) == _lib.PK_ERR_UNSUPPORTED  # slots past 31 bits
+    for name in ("pk_extend_sequences", "pk_free_sequences"):                       # steps over blocks past 31 bits
+        assert _call(name, blocks=2 ** 30 + 1, bs=1) == _lib.PK_ERR_UNSUPPORTED
+        assert _call(name, blocks=2 ** 30, bs=1) == _lib.PK_OK
     assert _call("pk_free_sequences", n=1, list=None) == _lib.PK_ERR_INVALID_ARG
     assert _call("pk_compact_blocks", map=None) == _lib.PK_ERR_INVALID_ARG
     need = _lib.lib().pk_fork_workspace_bytes(8)
@@ -80,7 +83,8 @@ def test_list_refusals():
 
 def test_python_refusals():
     k, v = torch.zeros(2, 4, 8, 1, 8, dtype=torch.bfloat16), torch.zeros(2, 4, 8, 1, 8, dtype=torch.bfloat16)
-    t, ln, rc = torch.full((3, 2), -1, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    t, ln = torch.full((3, 2), -1, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    rc = torch.zeros(4, dtype=torch.int32)
     one = torch.zeros(1, dtype=torch.int32)
     with pytest.raises(ValueError, match="one GPU"):
         pagedkv.copy_blocks(k, v, one, one)

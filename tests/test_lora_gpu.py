@@ -97,7 +97,8 @@ def test_linear_against_formula(gpu, rows, proj, rank, adapters, ids):
     (64, (1000, (96,)), 32, 3, "mixed"), (65, (1032, (160, 32, 32, 64)), 128, 3, "mixed"), (300, O, 8, 24, "mixed"),
     (512, QKV, 16, 600, "mixed"), (513, QKV, 16, 8, "runs"), (513, (40, (32, 32)), 40, 1, 0),
     (600, (264, (288,)), 72, 4095, "mixed"), (700, (64, (288,)), 8, 5000, "mixed"), (2500, O, 16, 1, "runs"),
-    (1200, QKV, 16, 2, "mixed"), (1500, QKV, 16, 14, "runs"), (700, (1000, (96, 64)), 24, 3, "mixed"), (1025, DOWN, 64, 7, "runs"),
+    (1200, QKV, 16, 2, "mixed"), (1500, QKV, 16, 14, "runs"), (700, (1000, (96, 64)), 24, 3, "mixed"),
+    (1025, DOWN, 64, 7, "runs"),
     (2000, GATE_UP, 128, 5, "runs"), (30, QKV, 32, 7, "mixed"), (64, QKV, 24, 3, "runs"), (33, DOWN, 16, 9, "mixed"),
     (128, O, 32, 2, "mixed"), (17000, (64, (32, 32)), 8, 3, "runs"), (33000, (64, (32,)), 16, 40, "mixed"),
     (24700, (256, (64, 64)), 32, 2, "runs"), (3001, O, 16, 50, "mixed"), (1500, (64, (32,)), 8, 4, -1)])
@@ -156,7 +157,8 @@ def test_non_finite_values_stay_in_their_rows(gpu, rows):
         assert float(got[7, 9]) == float("-inf") and torch.equal(got[7, 10:], clean[7, 10:])
 
 
-@pytest.mark.parametrize("rows,adapters", [(1, 3), (17, 1), (33, 40), (70, 3), (125, 15), (800, 3), (900, 300), (2700, 5)])
+@pytest.mark.parametrize("rows,adapters", [(1, 3), (17, 1), (33, 40), (70, 3), (125, 15), (800, 3), (900, 300),
+                                           (2700, 5)])
 def test_strides_and_what_lies_around_the_output(gpu, rows, adapters):
     """x, y, out, weight and both adapters as views of larger tensors; nothing beside out is written,
     the rows behind the last one of a tile of 16 or 64 among it."""
@@ -179,6 +181,9 @@ def test_strides_and_what_lies_around_the_output(gpu, rows, adapters):
     assert torch.equal(out, _add(d))
     out.fill_(7.0)
     assert bool((big == 7.0).all())
+    one = torch.cat([d["x"], d["y"], torch.zeros_like(d["y"])], 1)  # x, y and out as columns of one buffer
+    _add(dict(d, x=one[:, :k], y=one[:, k:k + n]), out=one[:, k + n:])
+    assert torch.equal(one, torch.cat([d["x"], d["y"], _add(d)], 1))
     if rows <= 128:
         _linear(v, out=out)
         assert torch.equal(out, _linear(d))

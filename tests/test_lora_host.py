@@ -14,8 +14,8 @@ PTR = (ctypes.addressof(BUF) + 255) // 256 * 256
 
 def _call(name, **kw):
     lora = dict(a=PTR, a_adapter=16 * 256, a_row=256, b=PTR, b_adapter=64 * 16, b_row=16, adapters=4, rank=16,
-                ids=PTR, scales=None, slices=None, num_slices=1, out=PTR + 8192, out_stride=64, ws=PTR, ws_bytes=1 << 20,
-                stream=None)
+                ids=PTR, scales=None, slices=None, num_slices=1, out=PTR + 8192, out_stride=64, ws=PTR,
+                ws_bytes=1 << 20, stream=None)
     if name == "pk_lora_linear":
         args = dict(x=PTR, x_stride=256, w=PTR, w_stride=256, rows=4, n_out=64, k=256, **lora)
     else:
@@ -57,9 +57,24 @@ def test_refusals_of_one():
     assert _call("pk_lora_linear", k=264, x_stride=264, w_stride=264, a_row=264) == _lib.PK_ERR_UNSUPPORTED
     assert _call("pk_lora_linear", w=None) == _lib.PK_ERR_INVALID_ARG
     assert _call("pk_lora_linear", out=PTR) == _lib.PK_ERR_INVALID_ARG              # out on x
+    assert _call("pk_lora_linear", out=PTR + 1024 + 16) == _lib.PK_ERR_INVALID_ARG  # on x's third row
+    assert b"overlaps x" in _lib.lib().pk_last_error()
     assert _call("pk_lora_add", y=None) == _lib.PK_ERR_INVALID_ARG
     assert _call("pk_lora_add", y_stride=56) == _lib.PK_ERR_INVALID_ARG
     assert _call("pk_lora_add", y_stride=72) == _lib.PK_ERR_INVALID_ARG             # out is y, other rows
+    # out on x or on part of y; a range of columns beside them is neither (refused for its scratch only)
+    assert _call("pk_lora_add", out=PTR, y=PTR + 16384) == _lib.PK_ERR_INVALID_ARG
+    assert b"overlaps x" in _lib.lib().pk_last_error()
+    assert _call("pk_lora_add", out=PTR + 8192 + 16) == _lib.PK_ERR_INVALID_ARG
+    assert b"overlaps y" in _lib.lib().pk_last_error()
+    beside = dict(x=PTR, x_stride=512, out=PTR + 512, out_stride=512, y=PTR + 640, y_stride=512, rank=64, b_row=64)
+    assert _call("pk_lora_add", **beside, ws_bytes=8) == _lib.PK_ERR_WORKSPACE
+    assert _call("pk_lora_add", **{**beside, "y": PTR + 624}, ws_bytes=8) == _lib.PK_ERR_INVALID_ARG
+    assert _call("pk_lora_add", **{**beside, "x": PTR + 16}, ws_bytes=8) == _lib.PK_ERR_INVALID_ARG
+    # (bytes of out's rows: 512..640, 1536..1664, ...; a row of x from 640 ends at 1152, one from 1040 at 1552)
+    at = dict(beside, y=PTR + 256 * 9, ws_bytes=8)
+    assert _call("pk_lora_add", **{**at, "x": PTR + 640}) == _lib.PK_ERR_WORKSPACE
+    assert _call("pk_lora_add", **{**at, "x": PTR + 1040}) == _lib.PK_ERR_INVALID_ARG
     for name in ("pk_lora_linear", "pk_lora_add"):
         assert _call(name, rows=2 ** 22 + 1) == _lib.PK_ERR_UNSUPPORTED
         wide = dict(n_out=2 ** 20 + 32, out_stride=2 ** 20 + 32)
@@ -98,8 +113,9 @@ def test_python_refusals():
     a, b, ids = torch.zeros(2, 16, 256, **bf), torch.zeros(2, 64, 16, **bf), torch.zeros(4, dtype=torch.int32)
     for call in (lambda **k: pagedkv.lora_add(**{**dict(y=y, x=x, lora_a=a, lora_b=b, adapter_ids=ids), **k}),
                  lambda **k: pagedkv.lora_linear(**{**dict(x=x, weight=w, lora_a=a, lora_b=b, adapter_ids=ids), **k})):
-        for kw, match in [(dict(x=x.float()), "bf16"), (dict(lora_a=a[:, :8]), "must be"), (dict(lora_a=a[:1]), "must be"),
-                          (dict(lora_b=b[:, :32]), "must be"), (dict(lora_b=b.transpose(1, 2)), "contiguous rows"),
+        for kw, match in [(dict(x=x.float()), "bf16"), (dict(lora_a=a[:, :8]), "must be"),
+                          (dict(lora_a=a[:1]), "must be"), (dict(lora_b=b[:, :32]), "must be"),
+                          (dict(lora_b=b.transpose(1, 2)), "contiguous rows"),
                           (dict(slices=(32, 16)), "add up"), (dict(slices=(32, 32)), "must be"),
                           (dict(adapter_ids=ids[:3]), "adapter_ids"), (dict(scales=torch.ones(3)), "scales"),
                           (dict(scales=torch.ones(2, dtype=torch.float64)), "scales"),
