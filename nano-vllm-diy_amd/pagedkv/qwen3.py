@@ -141,13 +141,14 @@ class Qwen3Model:
         # a decode step: every sequence has one new token (cu_seqlens_q = arange), read
         # through block tables; the producer then runs inside the attention launch
         decode = not flat and ctx.max_seqlen_q == 1 and input_ids.shape[0] == ctx.cu_seqlens_q.numel() - 1
-        ad = self.adapters if ctx.adapter_ids is not None else None
+        adapter_ids = getattr(ctx, "adapter_ids", None)  # absent on the reference Context
+        ad = self.adapters if adapter_ids is not None else None
 
         def project(x, L, li, name):
             """x through a projection and its adapters, or the projection alone"""
             if ad is None:
                 return ops.linear(x, L[name]) if small else F.linear(x, L[name])
-            args = (*ad.layers[li][name], ctx.adapter_ids, ad.scales, ad.slices[name])
+            args = (*ad.layers[li][name], adapter_ids, ad.scales, ad.slices[name])
             if small:
                 return lora.lora_linear(x, L[name], *args)
             y = F.linear(x, L[name])
