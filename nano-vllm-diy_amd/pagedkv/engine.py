@@ -60,6 +60,7 @@ class LLMEngine:
 
     def step(self):
         """One engine step; returns (step, number of sequences that finished) or None."""
+        self.runner.check_model()  # before the step's tokens are scheduled
         st = self.scheduler.schedule()
         if st is None:
             return None

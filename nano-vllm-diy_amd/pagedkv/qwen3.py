@@ -101,7 +101,8 @@ class Qwen3Model:
         self.adapters: Qwen3Adapters | None = None
 
     def bind_adapters(self, adapters: Qwen3Adapters | None) -> None:
-        """Adapters for the tokens whose Context names one (ctx.adapter_ids); None: none."""
+        """Adapters for the tokens whose Context names one (ctx.adapter_ids); None: none. For callers of
+        forward: the engine, whose requests name no adapters, refuses a step while some are bound."""
         self.adapters = adapters
 
     def bind_caches(self, k_caches: torch.Tensor | None, v_caches: torch.Tensor | None) -> None:

@@ -125,7 +125,15 @@ class ModelRunner:
     def _to_dev(self, t: torch.Tensor) -> torch.Tensor:
         return t.to(self.dev, non_blocking=True)
 
+    def check_model(self) -> None:
+        """A step names no adapters, and the captured graphs hold the base model: with adapters bound
+        they would answer every request with the base model."""
+        if self.model.adapters is not None:
+            raise RuntimeError("the engine's steps carry no adapter ids: unbind the model's adapters "
+                               "(bind_adapters(None)), or call the model with a Context that has adapter_ids")
+
     def run_eager(self, step: Step) -> torch.Tensor:
+        self.check_model()
         ctx = Context(is_prefill=step.is_prefill, cu_seqlens_q=self._to_dev(step.cu_seqlens_q),
                       cu_seqlens_k=self._to_dev(step.cu_seqlens_k), max_seqlen_q=step.max_seqlen_q,
                       max_seqlen_k=step.max_seqlen_k, slot_mapping=self._to_dev(step.slot_mapping),
@@ -187,6 +195,7 @@ class ModelRunner:
         torch.cuda.synchronize()
 
     def run_graph(self, step: Step) -> torch.Tensor:
+        self.check_model()
         S = step.num_seqs
         bs = next(b for b in self.graph_bs if b >= S)
         mb, off = self.max_blocks, self.off

@@ -7,6 +7,8 @@ import torch
 
 import pagedkv
 from pagedkv import lora, ops
+from pagedkv.engine import LLMEngine
+from pagedkv.runner import ModelRunner
 from pagedkv.qwen3 import Qwen3Adapters, Qwen3Config, Qwen3Model, Qwen3Weights
 
 CFG = Qwen3Config(vocab_size=32, hidden_size=64, num_hidden_layers=2, num_attention_heads=2, num_key_value_heads=1,
@@ -95,3 +97,26 @@ def test_adapter_ids_reach_all_four_projections(calls, kind):
     _forward(model, pagedkv.Context(**fields, adapter_ids=ids))
     assert sum(name == "lora_linear" for name, _ in calls) == 4 * CFG.num_hidden_layers
     assert not any(name in ("linear", "linear_silu_mul", "linear_add_rmsnorm") for name, _ in calls)
+
+
+def test_engine_refuses_adapters(calls):
+    """The engine's requests and steps name no adapters: with adapters bound to its model they would all be
+    answered by the base model, so a step is refused, before anything is scheduled, and goes on once
+    the adapters are unbound. The runner refuses both kinds of step by itself."""
+    runner = object.__new__(ModelRunner)
+    runner.model, runner.dev, runner.graphs = _model(), torch.device("cpu"), {}
+    runner.model.greedy = lambda hidden, ctx: torch.zeros(1, dtype=torch.int32)
+    done = []
+    eng = object.__new__(LLMEngine)
+    eng.runner = runner
+    step = SimpleNamespace(**_fields("prefill"), input_ids=torch.zeros(6, dtype=torch.int64),
+                           positions=torch.zeros(6, dtype=torch.int64), num_seqs=3)
+    eng.scheduler = SimpleNamespace(schedule=lambda: done.append("schedule") or step,
+                                    postprocess=lambda toks: done.append("postprocess") or 1)
+    runner.model.bind_adapters(Qwen3Adapters(CFG, 2, 8, torch.device("cpu")))
+    for refused in (eng.step, lambda: runner.run(step), lambda: runner.run_eager(step), lambda: runner.run_graph(step)):
+        with pytest.raises(RuntimeError, match="adapters"):
+            refused()
+    assert not done and not calls
+    runner.model.bind_adapters(None)
+    assert eng.step() == (step, 1) and done == ["schedule", "postprocess"]
