@@ -13,7 +13,7 @@ Context (src/utils/context.py:5-14), built by the runner (model_runner.py:174-23
   selects the shared-prefix decode path, which computes the shared blocks once for all the
   sequences that hold them (results within the attention tolerance of the plain path).
   0 states that no block is shared (and allows the one-launch store + decode); None keeps
-  the library default.
+  the library default in Attention, and is 0 to Qwen3Model.
 * adapter_ids (an addition): (N,) int32 adapter of every new token, -1 for none; read by a model
   that has adapters bound (Qwen3Model.bind_adapters). None: the base model for every token.
 """

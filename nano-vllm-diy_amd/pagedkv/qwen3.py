@@ -133,15 +133,22 @@ class Qwen3Model:
         RMSNorm (the final norm after the last layer). Larger steps use F.linear (a library
         GEMM) and the separate norm / activation kernels. Rounding points are the same.
         With adapters (bind_adapters and ctx.adapter_ids) every projection is lora_linear, or
-        F.linear and lora_add, followed by the separate kernels."""
+        F.linear and lora_add, followed by the separate kernels.
+        ctx.cached_prefix_keys has Attention.forward's meaning, and None states, as 0 does, that no
+        block is shared (the engine has no prefix cache): decode reads stream, and a decode step
+        stores inside the attention launch. Forks share full blocks, which the one launch may read
+        too; with the bound stated (above 0) they are computed once, after a store of its own."""
         cfg, W = self.cfg, self.w
         Hq, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         eps = cfg.rms_norm_eps
         flat = ctx.block_tables is None
         small = input_ids.shape[0] <= ops.LINEAR_MAX_ROWS
-        # a decode step: every sequence has one new token (cu_seqlens_q = arange), read
-        # through block tables; the producer then runs inside the attention launch
-        decode = not flat and ctx.max_seqlen_q == 1 and input_ids.shape[0] == ctx.cu_seqlens_q.numel() - 1
+        hint = getattr(ctx, "cached_prefix_keys", None) or 0  # absent on the reference Context
+        # a decode step without a stated shared prefix: every sequence has one new token
+        # (cu_seqlens_q = arange), read through block tables; the producer then runs inside the
+        # attention launch
+        decode = not flat and hint == 0 and ctx.max_seqlen_q == 1 and \
+            input_ids.shape[0] == ctx.cu_seqlens_q.numel() - 1
         adapter_ids = getattr(ctx, "adapter_ids", None)  # absent on the reference Context
         ad = self.adapters if adapter_ids is not None else None
 
@@ -168,7 +175,7 @@ class Qwen3Model:
             kc, vc = (None, None) if self.k_caches is None else (self.k_caches[li], self.v_caches[li])
             if decode:
                 # one launch: q/k norm + RoPE, the K/V store and paged decode attention; no
-                # block is shared (no prefix cache), so every decode read streams
+                # block is stated to be shared, so every decode read streams
                 o = ops.qkv_decode_attention(qkv, positions, self.cos_sin, Hq, Hkv, D, L["q_norm"], L["k_norm"],
                                              eps, kc, vc, ctx.slot_mapping, ctx.cu_seqlens_q, ctx.cu_seqlens_k,
                                              ctx.max_seqlen_k, self.scale, ctx.block_tables, cached_prefix_keys=0)
@@ -182,7 +189,8 @@ class Qwen3Model:
                 else:
                     o = ops.varlen_attention(q, kc, vc, ctx.cu_seqlens_q, ctx.cu_seqlens_k,
                                              ctx.max_seqlen_q, ctx.max_seqlen_k, self.scale, True,
-                                             ctx.block_tables, cached_prefix_keys=0)
+                                             ctx.block_tables, cached_prefix_keys=hint,
+                                             shared_prefix_keys=hint if hint > 0 else None)
             if small and ad is None:
                 x, residual = ops.linear_add_rmsnorm(o.view(-1, Hq * D), L["o"], residual,
                                                      L["post_norm"], eps, residual_out=residual)

@@ -120,3 +120,20 @@ def test_engine_refuses_adapters(calls):
     assert not done and not calls
     runner.model.bind_adapters(None)
     assert eng.step() == (step, 1) and done == ["schedule", "postprocess"]
+
+
+@pytest.mark.parametrize("kind", ["prefill", "mixed", "decode"])
+@pytest.mark.parametrize("hint", [None, 0, 8, -1])
+def test_cached_prefix_keys_reach_the_attention(calls, kind, hint):
+    """What a Context states of shared blocks (forks share their parent's full pages): the attention gets
+    the bound, a shared prefix (above 0) is computed once, and only a decode step without
+    shared blocks stores inside the launch that reads the cache."""
+    _forward(_model(), pagedkv.Context(**_fields(kind), cached_prefix_keys=hint))
+    attention = [(n, kw) for n, kw in calls if n in ("varlen_attention", "qkv_decode_attention")]
+    assert len(attention) == CFG.num_hidden_layers
+    want = hint or 0
+    for name, kw in attention:
+        assert (name == "qkv_decode_attention") == (kind == "decode" and want == 0)
+        if kind != "prefill":
+            assert kw.get("cached_prefix_keys") == want
+            assert (kw.get("shared_prefix_keys") or 0) == max(want, 0)
