@@ -83,10 +83,15 @@ def _out(out, rows, n_out, dev):
     return out, stride
 
 
-@lru_cache(maxsize=4096)
-def lora_workspace_bytes(rows: int, n_out: int, k: int, rank: int, slices: tuple[int, ...] | None = None,
-                         num_adapters: int = 0, linear: bool = False) -> int:
+def lora_workspace_bytes(rows: int, n_out: int, k: int, rank: int, slices=None, num_adapters: int = 0,
+                         linear: bool = False) -> int:
     """Scratch bytes of one lora_add call, or with linear=True of one lora_linear call (0: none)."""
+    return _workspace_bytes(rows, n_out, k, rank, None if slices is None else tuple(slices), num_adapters, linear)
+
+
+@lru_cache(maxsize=4096)
+def _workspace_bytes(rows: int, n_out: int, k: int, rank: int, slices: tuple[int, ...] | None, num_adapters: int,
+                     linear: bool) -> int:
     arr, num_slices = _slices(slices, n_out)
     if linear:
         return int(lib().pk_lora_linear_workspace_bytes(rows, n_out, k, rank, num_slices))
@@ -118,7 +123,7 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     slices = None if slices is None else tuple(slices)
     args = _adapter_args(rows, k, n_out, dev, lora_a, lora_b, adapter_ids, scales, slices)
     out, out_stride = _out(out, rows, n_out, dev)
-    ws, nbytes, _keep = _workspace(workspace, lora_workspace_bytes(rows, n_out, k, args[7], slices, 0, True), dev)
+    ws, nbytes, _keep = _workspace(workspace, _workspace_bytes(rows, n_out, k, args[7], slices, 0, True), dev)
     call(lib().pk_lora_linear, "pk_lora_linear", dev, x.data_ptr(), x_stride, weight.data_ptr(), w_stride, rows, n_out,
          k, *args, out.data_ptr(), out_stride, ws, nbytes)
     return out
@@ -138,7 +143,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: tor
     slices = None if slices is None else tuple(slices)
     args = _adapter_args(rows, k, n_out, dev, lora_a, lora_b, adapter_ids, scales, slices)
     out, out_stride = _out(out, rows, n_out, dev)
-    ws, nbytes, _keep = _workspace(workspace, lora_workspace_bytes(rows, n_out, k, args[7], slices, args[6]), dev)
+    ws, nbytes, _keep = _workspace(workspace, _workspace_bytes(rows, n_out, k, args[7], slices, args[6], False), dev)
     call(lib().pk_lora_add, "pk_lora_add", dev, y.data_ptr(), y_stride, x.data_ptr(), x_stride, rows, n_out, k, *args,
          out.data_ptr(), out_stride, ws, nbytes)
     return out

@@ -132,3 +132,16 @@ def test_python_refusals():
         pagedkv.lora_add(y, x, a, b, ids)
     with pytest.raises(ValueError, match="at most 128"):
         pagedkv.lora_linear(torch.zeros(129, 256, **bf), w, a, b, torch.zeros(129, dtype=torch.int32))
+
+
+def test_workspace_sizes_take_the_slices_of_the_operators():
+    """Any sequence of widths, as lora_linear and lora_add take them."""
+    for linear in (False, True):
+        want = pagedkv.lora_workspace_bytes(200, 4096, 1024, 24, (2048, 1024, 1024), 8, linear)
+        got = [pagedkv.lora_workspace_bytes(200, 4096, 1024, 24, s, 8, linear)
+               for s in ([2048, 1024, 1024], torch.Size((2048, 1024, 1024)), iter((2048, 1024, 1024)))]
+        assert got == [want] * 3
+        assert pagedkv.lora_workspace_bytes(200, 4096, 1024, 24, None, 8, linear) == \
+            pagedkv.lora_workspace_bytes(200, 4096, 1024, 24, [4096], 8, linear)
+    with pytest.raises(ValueError, match="add up"):
+        pagedkv.lora_workspace_bytes(200, 4096, 1024, 24, [2048, 1024], 8)
