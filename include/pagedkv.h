@@ -477,7 +477,8 @@ int pk_linear_add_rmsnorm(const void* x, int64_t x_row_stride, const void* weigh
  * adapters of smaller rank are padded with zeros. k and rank multiples of 8, rank up to 128, up
  * to 4 slices of multiples of 32 columns, up to 2^22 rows of 2^20 columns (and what a launch of
  * 2^24 work-groups covers); pointers 16-byte aligned, strides multiples of 8. A row's result does
- * not depend on the other rows' values. An infinite weight gives NaN.
+ * not depend on the other rows' values. Infinities and NaN give what the formula gives, in the rows and
+ * columns that they reach, but for an infinite element of lora_b: there NaN may stand for an infinity.
  *
  * pk_lora_linear -- base = x W^T in fp32 (a decode step's projection, pk_linear's weight and limits:
  *   at most 128 rows, k a multiple of 256); out must not overlap x.

@@ -19,7 +19,9 @@
 //
 // t is kept in fp32. For the expand it is split into two bf16, t = hi + lo with a remainder
 // below 2^-16 |t|, and both halves are multiplied (the products with bf16 B are exact in the
-// fp32 sum), so t costs no rounding of the output's size. The output is rounded once.
+// fp32 sum), so t costs no rounding of the output's size. The output is rounded once. An infinite B
+// gives NaN where lo is 0 or of the other sign, and the formula's infinity elsewhere and in the
+// epilogue that multiplies in fp32 (LoraAddend).
 //
 // MFMA: v_mfma_f32_16x16x32_bf16, D[i][j] = sum_k A[i][k] B[k][j]; lane (r = lane & 15, h = lane
 // >> 4) supplies row r of both operands at k = 8 h .. 8 h + 7 and holds D[4 h .. 4 h + 3][r]. The

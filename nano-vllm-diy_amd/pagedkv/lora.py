@@ -8,6 +8,7 @@ c. A merged projection (qkv, gate/up) has one slice per layer merged in it: its 
 `slices`, the layers' A matrices are stacked in lora_a (L, len(slices) * r, k), their B matrices,
 one after the other in lora_b (L, n_out, r). Adapters of smaller rank are padded with zeros;
 scales (L,) float32 holds alpha / r of each. Everything is bf16, summed in fp32 and rounded once.
+Infinities and NaN act as in the formula, but an infinite element of lora_b may give NaN for an infinity.
 
 lora_linear computes the projection as well (decode steps, at most 128 rows); lora_add adds to a
 projection's output, for prefill steps, whose projections are library products. No call reads
