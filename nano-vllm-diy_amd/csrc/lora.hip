@@ -345,10 +345,12 @@ __global__ __launch_bounds__(kLinThreads) void lora_linear_expand_kernel(const L
 // ---------------------------------------------------------------- expand ----------------
 
 __device__ __forceinline__ void split_bf16(float v, uint32_t* hi, uint32_t* lo) {
-  const uint32_t b = f32_to_bf16(v);
+  uint32_t b = f32_to_bf16(v);
+  // finite, but rounded to an infinity: the largest bf16, and what is above it in lo
+  if ((b & 0x7fffu) == 0x7f80u && fabsf(v) < INFINITY) --b;
   const float head = __uint_as_float(b << 16);
   *hi = b;
-  // an infinite head (t infinite, or beyond bf16) has no remainder
+  // an infinite t has no remainder
   *lo = (b & 0x7f80u) == 0x7f80u ? 0u : f32_to_bf16(v - head);
 }
 

@@ -87,3 +87,28 @@ def test_add(gpu, rows, proj, rank, scratch):
     assert (need == 0) == (scratch == "none") and (need == t) == (scratch == "t")
     _check(_add, lambda c: c["y"].double(), lambda: _inputs(rows, k, widths, rank), k, ROWS + ADAPTERS + ADD, gpu,
            f"add rows={rows} k={k} rank={rank}")
+
+
+@pytest.mark.parametrize("op,rows,rank", [
+    ("linear", 2, 16), ("linear", 40, 16), ("linear", 40, 24), ("linear", 40, 128), ("add", 40, 16), ("add", 33, 32),
+    ("add", 200, 40), ("add", 2700, 16), ("add", 2700, 128)])
+def test_t_beyond_the_largest_bf16(gpu, op, rows, rank):
+    """t = 3.4e38 fits fp32 but rounds to an infinity in bf16 (largest value 3.39e38): a tiny B brings it back
+    to an ordinary number, in every form. Every product but one is 0, so fp32 sums lose nothing:
+    half a bf16 step of the output and t's 2^-16."""
+    k, widths = 1024, (2048, 1024, 1024)
+    c = _case(1, rows, k, widths, rank, 3)
+    for name in ("x", "w", "y", "a", "b"):
+        c[name].zero_()
+    c["ids"].fill_(1)
+    c["ids"][1:] = torch.randint(-1, 3, (rows - 1,), generator=torch.Generator().manual_seed(1)).to(torch.int32)
+    c["x"][:, 9], c["a"][:, 3, 9] = 1.0, 1.0
+    c["x"][rows // 2:, 9] = -1.0
+    c["b"][:, :, 3] = 2.0 ** -126
+    c["scales"].fill_(3.4e38)
+    assert c["scales"].isfinite().all() and c["scales"].to(torch.bfloat16).isinf().all()
+    want = _exact(c, torch.zeros(rows, sum(widths), dtype=torch.float64), torch.zeros(1, dtype=torch.float64), k)[0]
+    assert want[c["ids"] >= 0, :2048].abs().min() > 3.9
+    print(f"[lora] {op} rows={rows} rank={rank} large t", flush=True)
+    got = (_linear if op == "linear" else _add)(_gpu(c, gpu)).cpu().double()
+    assert ((got - want).abs() <= (2.0 ** -8 + 2.0 ** -16) * want.abs()).all()
