@@ -14,8 +14,10 @@
 //     for none, and those without a group end.
 //   * more: one work-group sorts the rows by adapter (counts, offsets, positions) and lists the
 //     tiles of 64.
-// Every row's sums are taken in the same order whatever shares its tile, so a row's result does
-// not depend on the other rows of the batch beyond the choice between the two forms.
+// Every row's sums are taken in the same order whatever shares its tile. A row of lora_add has the same
+// bits alone and in any batch, sorted or not. For lora_linear the number of rows picks the projection's K
+// split and the form that adds the adapters, and with them the order of the sums; the other rows' values
+// and adapters change nothing.
 //
 // t is kept in fp32. For the expand it is split into two bf16, t = hi + lo with a remainder
 // below 2^-16 |t|, and both halves are multiplied (the products with bf16 B are exact in the
