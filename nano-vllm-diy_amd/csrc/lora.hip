@@ -346,14 +346,13 @@ __global__ __launch_bounds__(kLinThreads) void lora_linear_expand_kernel(const L
 
 // ---------------------------------------------------------------- expand ----------------
 
+// t = hi + lo. The head is within bf16's range, so that a finite t stays finite; an infinite or NaN t is
+// in lo.
 __device__ __forceinline__ void split_bf16(float v, uint32_t* hi, uint32_t* lo) {
-  uint32_t b = f32_to_bf16(v);
-  // finite, but rounded to an infinity: the largest bf16, and what is above it in lo
-  if ((b & 0x7fffu) == 0x7f80u && fabsf(v) < INFINITY) --b;
-  const float head = __uint_as_float(b << 16);
+  constexpr float kLargest = 0x1.fep127f;
+  const uint32_t b = f32_to_bf16(__builtin_amdgcn_fmed3f(v, -kLargest, kLargest));
   *hi = b;
-  // an infinite t has no remainder
-  *lo = (b & 0x7f80u) == 0x7f80u ? 0u : f32_to_bf16(v - head);
+  *lo = f32_to_bf16(v - __uint_as_float(b << 16));
 }
 
 // How both expand kernels multiply. A wavefront has 16 rows and 128 columns: t's rows are the
