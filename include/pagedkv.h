@@ -526,7 +526,8 @@ int pk_lora_add(const void* y, int64_t y_row_stride, const void* x, int64_t x_ro
  *   blocks (one more holder each) and gets a new block with the tokens of a last block that is not
  *   full, copied in every layer, so both can grow. new_blocks[i] is that block, -1 if none was
  *   needed, -2 if the pool had none left, -3 if children[i] is no row, is not empty or was listed
- *   before; with -2 and -3 the child stays as it was. A parent that is no row is an empty one. At
+ *   before; with -2 and -3 the child stays as it was. A parent that is no row is an empty one, and
+ *   parents are read as they are before the call (a row that the call makes a child is empty). At
  *   most 1024 forks a call; workspace: pk_fork_workspace_bytes(num_forks).
  * pk_extend_sequences -- one more token for every listed row: slot_mapping[i] is its cache slot
  *   (block * block_size + offset), in a new block where the row's last one is full, and the

@@ -6,9 +6,10 @@
 // computed next to the shrink (lora_linear, at most 128 rows), or given (lora_add). The reference
 // has no adapters; the projections are those of linear.hip.
 //
-// The work is reading: W or base once, out once, and the adapters in use once each; the products
-// are 16-64 wide and free next to that. So rows are brought together by adapter, and a group of
-// up to 16 or 64 rows of ONE adapter is an MFMA tile that reads A and B once for all of them:
+// The work is reading: W or base, out, and the adapters in use; the products are 16-64 wide and free
+// next to that. So rows are brought together by adapter, and a group of up to 16 or 64 rows of ONE
+// adapter is an MFMA tile that reads A and B once for all of them. An adapter whose rows are in several
+// groups is read by each, mostly from the caches:
 //   * few rows (small_add): the groups are the equal ids within 16 consecutive rows. Nothing is sorted:
 //     there is a work-group for every group that 16 rows can have, 16 or one for each adapter and one
 //     for none, and those without a group end.
@@ -245,7 +246,8 @@ __global__ __launch_bounds__(kLoraThreads) void lora_shrink_kernel(const LoraArg
 
 // The partial sums of a decode step's projection (work-groups [0, lin_groups)) and the shrink of its
 // adapters, which need nothing of each other, in one launch; the expand adds the partial sums. 128 rows,
-// 75 adapters of rank 64 on 3072 x 1024: 12.0 us for 34 MB.
+// 64 adapters of rank 64 in use on 3072 x 1024: 12.0 us. W, x and A read once are 32 MB; it reads 49,
+// since the 16-row groups hold 108 times one of the 64 adapters.
 template <int NB, int CB>
 __global__ __launch_bounds__(kLinThreads) void lora_linear_kernel(const LinArgs a, const LoraArgs p,
                                                                   const int32_t lin_groups) {
@@ -263,10 +265,11 @@ __global__ __launch_bounds__(kLinThreads) void lora_linear_kernel(const LinArgs 
 // lines, before the K walk, which hides them. Their products with t go through LDS to the threads
 // that have the columns.
 //
-// kShrink: t is computed here too, after the K walk, by every work-group for its slice. One adapter's A
-// is read again by all of them in 1.4 us less than a launch of its own (1024 x 4096, rank 16, in a
-// graph: 1 row 7.1 and 8.5 us); every further adapter costs 1.7 us (2 rows 8.9 and 8.5, 4 rows 11.9 and
-// 8.4). Outside a graph the second launch is 3.3 us of host time, so two rows still gain.
+// kShrink: t is computed here too, after the K walk, by every work-group for its slice, which saves the
+// shrink's launch and reads the rows' A in every work-group. Rank 16, every row an adapter of its own, one
+// launch and two, us in a graph over eight sets of weights in turn: 1024 x 4096 1 row 7.7 and 9.2, 2 rows 9.8
+// and 9.9, 3 rows 10.7 and 9.8, 4 rows 12.0 and 9.9; 1024 x 6144 1 row 8.6 and 10.3, 2 rows 10.1 and 10.4, 4
+// rows 12.3 and 10.3. Outside a graph the second launch also costs 3.3 us of host time.
 constexpr int kOneLaunchRows = 2;
 
 template <bool kShrink>
@@ -808,10 +811,12 @@ hipError_t launch_expand_small(const LoraArgs& p, hipStream_t stream) {
 
 // Whether a small addition computes t in the expand's work-groups (one launch, but every group of
 // 512 columns reads its adapter's A again): where all of them are on the GPU at once, three a CU up to
-// rank 16, two up to 32 (two chunks ahead in the shrink, not four, for that many). Measured, us in a
-// graph, one launch and two: 2048 x 1024, 300 rows of 100 adapters (608 work-groups) 10.7 and 10.6, 400 rows
-// (800) 14.3 and 11.7; qkv, 96 rows (768) 7.9 and 9.2, 128 rows (1024) 11.1 and 10.3; gate/up, rank 32, 64 rows of 8
-// adapters (432) 8.2 and 9.3, 96 rows (648) 11.6 and 9.7.
+// rank 16, two up to 32 (two chunks ahead in the shrink, not four, for that many). Measured, us in a graph over
+// eight sets of tensors in turn, one launch and two (work-groups): k = 2048, 1024 columns, rank 16, 300 rows of
+// 100 adapters (608) 11.5 and 12.4, 400 rows (800) 14.8 and 13.4; k = 3072, 300 rows of 20 (608) 11.8 and 12.9,
+// 400 rows (800) 15.6 and 13.3; qkv (k = 1024), 96 rows of 16 (768) 8.3 and 10.9, 128 rows (1024) 8.9 and 11.5: a
+// short k gains beyond the line too; rank 32, gate/up, 64 rows of 8 (432) 9.3 and 10.6, 96 rows (648) 12.6 and
+// 11.2; k = 2048, 900 rows of 3 (456) 12.5 and 14.3.
 bool shrink_in_expand(const LoraArgs& p) {
   return p.rank <= 32 && (int64_t)small_slots(p) * col_groups(p, 128 * kLoraWaves) <= (p.rank <= 16 ? 768 : 512);
 }
@@ -829,8 +834,11 @@ void launch_shrink_rows(const LoraArgs& p, int64_t tiles, int32_t cb, int32_t bl
 }
 
 // At most 64 columns of t a work-group, shared evenly. 64 rows a work-group read A half as often as
-// 32, where that still fills the GPU one and a half times: 13001 rows, t of 128 columns 13.8 us and
-// 16.5; 16384 rows, t of 48 columns (256 work-groups of 64 rows) 11.4 and 10.0.
+// 32, but are half as many. The line is where they fill the GPU one and a half times; around it the two
+// are within 4 % of a call, either way. Us a call in a graph, 32 and 64 rows (work-groups of 64): gate/up, rank 64,
+// 8192 rows (256) 76.8 and 76.0, 12288 (384) 97.1 and 95.8, 16384 (512) 122.1 and 121.5; qkv, rank 16, 16384 rows
+// (256) 77.1 and 77.4, 24576 (384) 115.6 and 114.6, 32768 (512) 144.3 and 146.6; 2048 x 1024, rank 16, 16384 rows
+// (256) 41.6 and 42.1, 24576 (384) 72.4 and 69.9, 32768 (512) 90.7 and 94.5.
 void launch_shrink_sorted(const LoraArgs& p, int64_t tiles, hipStream_t stream) {
   const int32_t cols16 = (p.num_slices * p.rank + 15) / 16, n = (cols16 + 3) / 4, cb = (cols16 + n - 1) / n;
   const int32_t blocks = (cols16 + cb - 1) / cb;
@@ -855,11 +863,16 @@ hipError_t launch_expand_sorted(LoraArgs p, int64_t tiles, hipStream_t stream) {
 }
 
 // Whether an addition works on groups of 16 rows, unsorted. What it costs grows with the groups that
-// there may be, each with its work-groups of the shrink and the expand and the time of about four more;
-// sorting costs 12 us whatever the rows. At the line of 20 a CU, sorted and unsorted, us: qkv (11 + 4 a
-// group at rank 16), 512 rows of 8 adapters (4320) 20.4 and 16.7, 768 (6480) 21.3 and 22.9; 2048 x 1024
-// (3 + 4), 768 rows of 100 (5376) 20.0 and 18.4, 1024 (7168) 21.5 and 20.8; rank 64 (8 + 4), 2048 rows of one
-// adapter (3072) 26.1 and 20.2, 4096 (6144) 28.2 and 37.4.
+// there may be, each with its work-groups of the shrink and the expand and the time of about four more. Sorting
+// costs a launch in front, 5-8 us up to 16384 rows and 9 for every 16384 more (one work-group does it). The line
+// of 20 a CU, 5120, is below the first place where sorting was the faster one. Unsorted and sorted, us a call in a
+// graph over eight sets of tensors in turn, ids at random (count): qkv, rank 16, 512 rows of 8 adapters (4320) 18.3
+// and 22.7, 768 (6480) 24.4 and 23.0; gate/up, rank 16, 768 rows of 4 (4320) 20.3 and 22.6, 1024 (5760) 24.2 and
+// 23.4; rank 64, 128 rows of 20 (4608) 22.4 and 24.1, 256 (9216) 35.7 and 24.7; 3072 x 1024, rank 32, 512 rows of 20
+// (4096) 22.8 and 25.4, 768 (6144) 28.8 and 26.5. Others cross later and lose up to 4 us between: 2048 x 1024, rank
+// 16, 768 rows of 100 (5376) 18.5 and 22.3, 1024 (7168) 20.8 and 22.7, 1280 (8960) 24.7 and 23.1. So do long runs
+// of one adapter, which leave most groups empty (qkv, 1024 rows of 8, 8640: 17.2 and 23.5), but the host does not
+// know the ids.
 bool small_add(const LoraArgs& p) {
   if (p.num_adapters > kLoraMaxSorted) return true;  // the sort's counters would not fit its LDS
   const int32_t each = 4 + col_groups(p, p.rank <= 32 ? 512 : 256) + (p.num_slices * p.rank + 15) / 16;

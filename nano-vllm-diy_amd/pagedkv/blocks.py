@@ -95,7 +95,8 @@ def fork_sequences(k_caches: torch.Tensor, v_caches: torch.Tensor, block_tables:
     both grow without seeing each other's tokens. Returns new_blocks (n,) int32: that page's
     number; -1 where none was needed; -2 where the pool had none left; -3 where children[i] is no
     row of the tables, is not empty or was listed before. With -2 and -3 the child stays as it
-    was. At most 1024 forks a call.
+    was. Parents are read as they are before the call: one that the call makes a child is empty.
+    At most 1024 forks a call.
     """
     args, dev = _cache_args(k_caches, v_caches)
     pool = _pool_args(block_tables, context_lens, ref_counts, dev)
