@@ -572,6 +572,70 @@ int pk_compact_blocks(void* k_caches, void* v_caches, int64_t k_layer_stride, in
                       int32_t* block_map, int32_t* num_live, void* workspace, size_t workspace_bytes,
                       pk_stream_t stream);
 
+/*
+ * Caches held in 4 bits (no counterpart in the reference, whose caches hold 16-bit elements,
+ * src/engine/model_runner.py:138-166): the same pages, tables and slots, 3.76 times the tokens in
+ * the same memory. A cache is bytes, (num_blocks, block_size, pk_fp4_row_bytes(num_kv_heads)), its rows
+ * contiguous; block strides are in bytes, multiples of 16. A token's row is
+ *   num_kv_heads * 64 bytes of values, two to a byte (dimension 2 i of a head in the low, 2 i + 1 in the
+ *   high four bits of its byte i), num_kv_heads * 4 scale bytes (one per 32 dimensions), and up to a
+ *   multiple of 16 bytes that are neither read nor written.
+ * Four bits are a sign, two of exponent and one of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6; the value is that
+ * times 2^(scale byte - 127). Of 32 values with the largest magnitude a the scale is the smallest power
+ * of two s with a <= 7 s, within 2^-126 .. 2^125; values are divided by it and rounded to nearest, ties to
+ * even, at most 6. An infinity or NaN among the 32 makes all of them NaN (scale byte 255). Every value is
+ * exact in bf16. A finite value is off by at most a / 5.
+ * To the page operators (pk_copy_blocks and those after it) such a cache is one of row_elems =
+ * pk_fp4_row_bytes / 2 16-bit elements where that is a multiple of 8, which it always is.
+ *
+ * pk_fp4_row_bytes -- bytes of a token's row: 68 * num_kv_heads rounded up to 16; 0 unless 1 .. 255 heads.
+ * pk_store_kvcache_fp4 -- pk_store_kvcache into such caches: key, value (num_tokens, num_kv_heads, head_dim)
+ *   bf16 with contiguous heads. Slots outside [0, num_slots) are passed over (-1: graph padding); of two
+ *   tokens with one slot, either's row may be the one that stays, or parts of both.
+ * pk_qk_norm_rope_store_fp4 -- pk_qk_norm_rope_store into such caches: q to q_out, k normalised, rotated,
+ *   rounded to bf16 and stored, v stored as it is. k_out, v_out (num_tokens, num_kv_heads, head_dim), NULL:
+ *   none: the values that the stored rows hold, of every token (slot or none), so a fresh prompt's attention
+ *   sees what later steps read. The norm's root is taken in 64 bits and no products are fused, so a key's
+ *   4-bit values follow from the formula alone. A row whose squares sum to no finite number is NaN.
+ * pk_gather_kv_fp4 -- pk_gather_kv of such a cache: the values of every sequence's rows in bf16, (sum Lk,
+ *   num_kv_heads, head_dim). Sequence b's rows begin at cu_seqlens_k[b]; rows at and past max_seqlen_k are not
+ *   written. Rows of table entries that are no block are 0.
+ * pk_varlen_attention_fp4 -- pk_varlen_attention in paged mode over such caches, in q's and out's layout, mask
+ *   and GQA groups: sequences with any number of query rows in one call (one, a few, chunks). The keys
+ *   of a table entry that is no block are seen by no row. Sequences without rows or keys are passed over, rows
+ *   past max_seqlen_q not written, keys past max_seqlen_k ignored; a row that sees no key (or none with a
+ *   score above -infinity) is written as 0.
+ *   num_rows: the rows of q, cu_seqlens_q[num_seqs] or more. Softmax, sums and partial results are fp32, the
+ *   weights rounded to bf16 for the product with V. NaN blocks reach the rows that see them and no
+ *   others. A row's result depends on the call's other sequences by the rounding of its partial sums; equal
+ *   calls give equal bits. At most 2^31 steps of 64 keys over the call's bounds.
+ *   workspace: pk_varlen_attention_fp4_workspace_bytes, 256-byte aligned (at most about 350 MB, 34 MB when
+ *   max_seqlen_q is 1); calls that may overlap must not share one.
+ */
+size_t pk_fp4_row_bytes(int32_t num_kv_heads);
+int pk_store_kvcache_fp4(const void* key, int64_t key_row_stride, const void* value, int64_t value_row_stride,
+                         void* k_cache, void* v_cache, const int32_t* slot_mapping, int32_t num_tokens,
+                         int32_t num_kv_heads, int32_t head_dim, int64_t num_slots, pk_stream_t stream);
+int pk_qk_norm_rope_store_fp4(const void* qkv, int64_t qkv_row_stride, const int64_t* positions, const float* cos_sin,
+                              int64_t max_position, const void* q_norm_weight, const void* k_norm_weight, float eps,
+                              int32_t num_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                              void* q_out, int64_t q_out_row_stride, void* k_out, int64_t k_out_row_stride,
+                              void* v_out, int64_t v_out_row_stride, void* k_cache, void* v_cache,
+                              const int32_t* slot_mapping, int64_t num_slots, pk_stream_t stream);
+int pk_gather_kv_fp4(const void* cache, int64_t block_stride, int32_t num_blocks, int32_t block_size,
+                     int32_t num_kv_heads, int32_t head_dim, const int32_t* block_table, int32_t block_table_stride,
+                     const int32_t* cu_seqlens_k, int32_t num_seqs, int32_t max_seqlen_k, void* dst,
+                     pk_stream_t stream);
+size_t pk_varlen_attention_fp4_workspace_bytes(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                               int32_t max_seqlen_q, int32_t max_seqlen_k);
+int pk_varlen_attention_fp4(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                            int64_t k_block_stride, int64_t v_block_stride, int32_t num_blocks, int32_t block_size,
+                            const int32_t* block_table, int32_t block_table_stride, const int32_t* cu_seqlens_q,
+                            const int32_t* cu_seqlens_k, int32_t num_seqs, int64_t num_rows, int32_t max_seqlen_q,
+                            int32_t max_seqlen_k, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                            float softmax_scale, int32_t causal, void* out, int64_t out_row_stride, void* workspace,
+                            size_t workspace_bytes, pk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,6 +15,7 @@
 
 #include "../../include/pagedkv.h"
 #include "common.h"
+#include "fp4.h"
 
 namespace {
 
@@ -285,7 +286,7 @@ int lora_args(const char* what, pk::LoraArgs* p, const void* x, int64_t x_row_st
 
 extern "C" {
 
-int pk_abi_version(void) { return 11; }
+int pk_abi_version(void) { return 12; }
 
 const char* pk_last_error(void) { return g_last_error.c_str(); }
 
@@ -1016,6 +1017,256 @@ int pk_compact_blocks(void* k_caches, void* v_caches, int64_t k_layer_stride, in
   return hip_status(pk::launch_compact_blocks(t, c, block_map, num_live, workspace,
                                               reinterpret_cast<hipStream_t>(stream)),
                     "compact_blocks launch");
+}
+
+// ---- caches held in 4 bits -----------------------------------------------------------------
+
+namespace {
+
+// A pair of 4-bit caches' head geometry; 0 when it is built.
+int fp4_heads(const char* what, int32_t num_kv_heads, int32_t head_dim) {
+  if (head_dim != pk::kHeadDim)
+    return fail(PK_ERR_UNSUPPORTED, "%s: head_dim=%d not built (only %d)", what, head_dim, pk::kHeadDim);
+  if (num_kv_heads <= 0 || num_kv_heads > pk::kFp4MaxHeads)
+    return fail(PK_ERR_UNSUPPORTED, "%s: num_kv_heads=%d (1 to %d)", what, num_kv_heads, pk::kFp4MaxHeads);
+  return PK_OK;
+}
+
+// Head rows are counted 16 to a work-group of 256 threads, in 32 bits.
+int fp4_tokens(const char* what, int64_t tokens, int64_t head_rows) {
+  if (tokens < 0) return fail(PK_ERR_INVALID_ARG, "%s: %lld tokens", what, (long long)tokens);
+  if (tokens * head_rows >= (1ll << 27))
+    return fail(PK_ERR_UNSUPPORTED, "%s: %lld tokens of %lld head rows in one call (below 2^27)", what,
+                (long long)tokens, (long long)head_rows);
+  return PK_OK;
+}
+
+// A (tokens, heads, 128) bf16 tensor with contiguous heads.
+int fp4_rows(const char* what, const char* name, const void* p, int64_t stride, int64_t heads) {
+  if (!p) return fail(PK_ERR_INVALID_ARG, "%s: null %s", what, name);
+  if (!aligned16(p) || stride < heads * pk::kHeadDim || stride % 8)
+    return fail(PK_ERR_INVALID_ARG, "%s: %s must be 16-byte aligned, its row stride %lld a multiple of 8 that covers a row",
+                what, name, (long long)stride);
+  return PK_OK;
+}
+
+int fp4_caches(const char* what, const void* k, const void* v) {
+  if (!k || !v || !aligned16(k) || !aligned16(v))
+    return fail(PK_ERR_INVALID_ARG, "%s: caches must be non-null and 16-byte aligned", what);
+  return PK_OK;
+}
+
+int fp4_blocks(const char* what, int64_t block_stride, int32_t num_blocks, int32_t block_size, int32_t row_bytes) {
+  if (num_blocks <= 0 || block_size <= 0)
+    return fail(PK_ERR_INVALID_ARG, "%s: num_blocks=%d, block_size=%d", what, num_blocks, block_size);
+  if (block_stride < (int64_t)block_size * row_bytes || block_stride % 16)
+    return fail(PK_ERR_INVALID_ARG, "%s: block stride of %lld bytes, must be a multiple of 16 and cover %d rows of %d",
+                what, (long long)block_stride, block_size, row_bytes);
+  return PK_OK;
+}
+
+}  // namespace
+
+size_t pk_fp4_row_bytes(int32_t num_kv_heads) {
+  return num_kv_heads > 0 && num_kv_heads <= pk::kFp4MaxHeads ? (size_t)pk::fp4_row_bytes(num_kv_heads) : 0;
+}
+
+int pk_store_kvcache_fp4(const void* key, int64_t key_row_stride, const void* value, int64_t value_row_stride,
+                         void* k_cache, void* v_cache, const int32_t* slot_mapping, int32_t num_tokens,
+                         int32_t num_kv_heads, int32_t head_dim, int64_t num_slots, pk_stream_t stream) {
+  g_last_error.clear();
+  const char* what = "store_kvcache_fp4";
+  if (int rc = fp4_heads(what, num_kv_heads, head_dim)) return rc;
+  if (int rc = fp4_tokens(what, num_tokens, 2 * num_kv_heads)) return rc;
+  if (num_slots < 0) return fail(PK_ERR_INVALID_ARG, "%s: num_slots < 0", what);
+  if (num_tokens == 0) return PK_OK;
+  if (int rc = fp4_rows(what, "key", key, key_row_stride, num_kv_heads)) return rc;
+  if (int rc = fp4_rows(what, "value", value, value_row_stride, num_kv_heads)) return rc;
+  if (int rc = fp4_caches(what, k_cache, v_cache)) return rc;
+  if (!slot_mapping) return fail(PK_ERR_INVALID_ARG, "%s: null slot_mapping", what);
+  pk::Fp4StoreArgs a{};
+  a.key = static_cast<const uint16_t*>(key);
+  a.key_stride = key_row_stride;
+  a.value = static_cast<const uint16_t*>(value);
+  a.value_stride = value_row_stride;
+  a.k_cache = static_cast<uint8_t*>(k_cache);
+  a.v_cache = static_cast<uint8_t*>(v_cache);
+  a.slot_mapping = slot_mapping;
+  a.num_tokens = num_tokens;
+  a.num_kv_heads = num_kv_heads;
+  a.row_bytes = pk::fp4_row_bytes(num_kv_heads);
+  a.num_slots = num_slots;
+  return hip_status(pk::launch_store_fp4(a, reinterpret_cast<hipStream_t>(stream)), "store_kvcache_fp4 launch");
+}
+
+int pk_qk_norm_rope_store_fp4(const void* qkv, int64_t qkv_row_stride, const int64_t* positions, const float* cos_sin,
+                              int64_t max_position, const void* q_norm_weight, const void* k_norm_weight, float eps,
+                              int32_t num_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                              void* q_out, int64_t q_out_row_stride, void* k_out, int64_t k_out_row_stride,
+                              void* v_out, int64_t v_out_row_stride, void* k_cache, void* v_cache,
+                              const int32_t* slot_mapping, int64_t num_slots, pk_stream_t stream) {
+  g_last_error.clear();
+  const char* what = "qk_norm_rope_store_fp4";
+  if (int rc = fp4_heads(what, num_kv_heads, head_dim)) return rc;
+  if (num_heads <= 0 || num_heads > 65535) return fail(PK_ERR_INVALID_ARG, "%s: num_heads=%d", what, num_heads);
+  if (int rc = fp4_tokens(what, num_tokens, num_heads + 2 * num_kv_heads)) return rc;
+  if (num_slots < 0 || max_position <= 0)
+    return fail(PK_ERR_INVALID_ARG, "%s: num_slots=%lld, max_position=%lld", what, (long long)num_slots,
+                (long long)max_position);
+  if (!(eps >= 0.f) || !std::isfinite(eps)) return fail(PK_ERR_INVALID_ARG, "%s: eps must be finite and not negative", what);
+  if (num_tokens == 0) return PK_OK;
+  if (int rc = fp4_rows(what, "qkv", qkv, qkv_row_stride, num_heads + 2 * num_kv_heads)) return rc;
+  if (int rc = fp4_rows(what, "q_out", q_out, q_out_row_stride, num_heads)) return rc;
+  if (k_out)
+    if (int rc = fp4_rows(what, "k_out", k_out, k_out_row_stride, num_kv_heads)) return rc;
+  if (v_out)
+    if (int rc = fp4_rows(what, "v_out", v_out, v_out_row_stride, num_kv_heads)) return rc;
+  if (int rc = fp4_caches(what, k_cache, v_cache)) return rc;
+  if (!positions || !cos_sin || !slot_mapping)
+    return fail(PK_ERR_INVALID_ARG, "%s: null positions / cos_sin / slot_mapping", what);
+  if (!aligned16(cos_sin) || (q_norm_weight && !aligned16(q_norm_weight)) || (k_norm_weight && !aligned16(k_norm_weight)))
+    return fail(PK_ERR_INVALID_ARG, "%s: cos_sin and norm weights must be 16-byte aligned", what);
+  pk::Fp4AppendArgs a{};
+  a.qkv = static_cast<const uint16_t*>(qkv);
+  a.qkv_stride = qkv_row_stride;
+  a.positions = positions;
+  a.cos_sin = cos_sin;
+  a.max_position = max_position;
+  a.q_weight = static_cast<const uint16_t*>(q_norm_weight);
+  a.k_weight = static_cast<const uint16_t*>(k_norm_weight);
+  a.eps = eps;
+  a.num_tokens = num_tokens;
+  a.num_heads = num_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.row_bytes = pk::fp4_row_bytes(num_kv_heads);
+  a.q_out = static_cast<uint16_t*>(q_out);
+  a.q_out_stride = q_out_row_stride;
+  a.k_out = static_cast<uint16_t*>(k_out);
+  a.k_out_stride = k_out_row_stride;
+  a.v_out = static_cast<uint16_t*>(v_out);
+  a.v_out_stride = v_out_row_stride;
+  a.k_cache = static_cast<uint8_t*>(k_cache);
+  a.v_cache = static_cast<uint8_t*>(v_cache);
+  a.slot_mapping = slot_mapping;
+  a.num_slots = num_slots;
+  return hip_status(pk::launch_append_fp4(a, reinterpret_cast<hipStream_t>(stream)), "qk_norm_rope_store_fp4 launch");
+}
+
+int pk_gather_kv_fp4(const void* cache, int64_t block_stride, int32_t num_blocks, int32_t block_size,
+                     int32_t num_kv_heads, int32_t head_dim, const int32_t* block_table, int32_t block_table_stride,
+                     const int32_t* cu_seqlens_k, int32_t num_seqs, int32_t max_seqlen_k, void* dst, pk_stream_t stream) {
+  g_last_error.clear();
+  const char* what = "gather_kv_fp4";
+  if (int rc = fp4_heads(what, num_kv_heads, head_dim)) return rc;
+  if (num_seqs < 0 || num_seqs > kMaxSeqs || max_seqlen_k < 0 || max_seqlen_k > kMaxSeqlen)
+    return fail(PK_ERR_INVALID_ARG, "%s: num_seqs=%d (at most %d), max_seqlen_k=%d (at most %d)", what, num_seqs,
+                kMaxSeqs, max_seqlen_k, kMaxSeqlen);
+  if (num_seqs == 0 || max_seqlen_k == 0) return PK_OK;
+  if (int rc = fp4_blocks(what, block_stride, num_blocks, block_size, pk::fp4_row_bytes(num_kv_heads))) return rc;
+  if (!cache || !block_table || !cu_seqlens_k || !dst) return fail(PK_ERR_INVALID_ARG, "%s: null pointer argument", what);
+  if (!aligned16(cache) || !aligned16(dst))
+    return fail(PK_ERR_INVALID_ARG, "%s: cache and dst must be 16-byte aligned", what);
+  if (block_table_stride < (max_seqlen_k - 1) / block_size + 1)
+    return fail(PK_ERR_INVALID_ARG, "%s: block_table_stride=%d does not cover max_seqlen_k=%d in blocks of %d", what,
+                block_table_stride, max_seqlen_k, block_size);
+  pk::Fp4GatherArgs a{};
+  a.cache = static_cast<const uint8_t*>(cache);
+  a.block_stride = block_stride;
+  a.num_blocks = num_blocks;
+  a.block_size = block_size;
+  a.num_kv_heads = num_kv_heads;
+  a.row_bytes = pk::fp4_row_bytes(num_kv_heads);
+  a.block_table = block_table;
+  a.bt_stride = block_table_stride;
+  a.cu_k = cu_seqlens_k;
+  a.num_seqs = num_seqs;
+  a.max_seqlen_k = max_seqlen_k;
+  a.dst = static_cast<uint16_t*>(dst);
+  return hip_status(pk::launch_gather_fp4(a, reinterpret_cast<hipStream_t>(stream)), "gather_kv_fp4 launch");
+}
+
+size_t pk_varlen_attention_fp4_workspace_bytes(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                               int32_t max_seqlen_q, int32_t max_seqlen_k) {
+  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || max_seqlen_q <= 0 ||
+      max_seqlen_k <= 0)
+    return 0;
+  const pk::Fp4AttnPlan p = pk::fp4_attention_plan(num_seqs, num_heads, num_kv_heads, max_seqlen_q, max_seqlen_k, 0);
+  return p.few_bytes + p.many_bytes;
+}
+
+int pk_varlen_attention_fp4(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                            int64_t k_block_stride, int64_t v_block_stride, int32_t num_blocks, int32_t block_size,
+                            const int32_t* block_table, int32_t block_table_stride, const int32_t* cu_seqlens_q,
+                            const int32_t* cu_seqlens_k, int32_t num_seqs, int64_t num_rows, int32_t max_seqlen_q,
+                            int32_t max_seqlen_k, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                            float softmax_scale, int32_t causal, void* out, int64_t out_row_stride, void* workspace,
+                            size_t workspace_bytes, pk_stream_t stream) {
+  g_last_error.clear();
+  const char* what = "varlen_attention_fp4";
+  if (int rc = fp4_heads(what, num_kv_heads, head_dim)) return rc;
+  if (num_seqs < 0 || num_rows < 0 || max_seqlen_q < 0 || max_seqlen_k < 0)
+    return fail(PK_ERR_INVALID_ARG, "%s: negative num_seqs / num_rows / max_seqlen", what);
+  if (num_seqs > kMaxSeqs) return fail(PK_ERR_INVALID_ARG, "%s: num_seqs=%d > %d", what, num_seqs, kMaxSeqs);
+  if (num_heads <= 0 || num_heads % num_kv_heads)
+    return fail(PK_ERR_INVALID_ARG, "%s: num_heads=%d not a multiple of num_kv_heads=%d", what, num_heads, num_kv_heads);
+  const int group = num_heads / num_kv_heads;
+  if (group != 1 && group != 2 && group != 4 && group != 8)
+    return fail(PK_ERR_UNSUPPORTED, "%s: GQA group %d not built (1, 2, 4, 8)", what, group);
+  if (num_seqs == 0 || num_rows == 0 || max_seqlen_q == 0 || max_seqlen_k == 0) return PK_OK;
+  if (max_seqlen_k > kMaxSeqlen || max_seqlen_q > kMaxSeqlen)
+    return fail(PK_ERR_UNSUPPORTED, "%s: max_seqlen_q=%d / max_seqlen_k=%d above %d", what, max_seqlen_q, max_seqlen_k,
+                kMaxSeqlen);
+  if (int rc = fp4_rows(what, "q", q, q_row_stride, num_heads)) return rc;
+  if (int rc = fp4_rows(what, "out", out, out_row_stride, num_heads)) return rc;
+  if (int rc = fp4_caches(what, k_cache, v_cache)) return rc;
+  if (!block_table || !cu_seqlens_q || !cu_seqlens_k)
+    return fail(PK_ERR_INVALID_ARG, "%s: null block_table / cu_seqlens", what);
+  const int32_t row_bytes = pk::fp4_row_bytes(num_kv_heads);
+  if (int rc = fp4_blocks(what, k_block_stride, num_blocks, block_size, row_bytes)) return rc;
+  if (int rc = fp4_blocks(what, v_block_stride, num_blocks, block_size, row_bytes)) return rc;
+  if (block_size % 64) return fail(PK_ERR_INVALID_ARG, "%s: block_size=%d must be a multiple of 64", what, block_size);
+  if (block_table_stride < (max_seqlen_k - 1) / block_size + 1)
+    return fail(PK_ERR_INVALID_ARG, "%s: block_table_stride=%d does not cover max_seqlen_k=%d in blocks of %d", what,
+                block_table_stride, max_seqlen_k, block_size);
+  if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale))
+    return fail(PK_ERR_INVALID_ARG, "%s: softmax_scale must be positive and finite", what);
+  const pk::Fp4AttnPlan p =
+      pk::fp4_attention_plan(num_seqs, num_heads, num_kv_heads, max_seqlen_q, max_seqlen_k, num_rows);
+  if (p.too_long)
+    return fail(PK_ERR_UNSUPPORTED, "%s: %d sequences of up to %d keys, %lld rows: more than 2^31 steps of 64 keys", what,
+                num_seqs, max_seqlen_k, (long long)num_rows);
+  const size_t need = p.few_bytes + p.many_bytes;
+  if (!workspace || workspace_bytes < need)
+    return fail(PK_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, need,
+                workspace ? workspace_bytes : (size_t)0);
+  if (reinterpret_cast<uintptr_t>(workspace) % kWorkspaceAlign)
+    return fail(PK_ERR_WORKSPACE, "%s: workspace must be %zu-byte aligned", what, kWorkspaceAlign);
+  pk::Fp4AttnArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_stride = q_row_stride;
+  a.k = static_cast<const uint8_t*>(k_cache);
+  a.v = static_cast<const uint8_t*>(v_cache);
+  a.k_block = k_block_stride;
+  a.v_block = v_block_stride;
+  a.row_bytes = row_bytes;
+  a.block_size = block_size;
+  a.num_blocks = num_blocks;
+  a.block_table = block_table;
+  a.bt_stride = block_table_stride;
+  a.cu_q = cu_seqlens_q;
+  a.cu_k = cu_seqlens_k;
+  a.num_seqs = num_seqs;
+  a.max_seqlen_q = max_seqlen_q;
+  a.max_seqlen_k = max_seqlen_k;
+  a.num_heads = num_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.group_shift = __builtin_ctz((unsigned)group);
+  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  a.causal = causal;
+  a.out = static_cast<uint16_t*>(out);
+  a.out_stride = out_row_stride;
+  a.workspace = workspace;
+  return hip_status(pk::launch_fp4_attention(a, p, reinterpret_cast<hipStream_t>(stream)), "varlen_attention_fp4 launch");
 }
 
 }  // extern "C"

@@ -1,0 +1,223 @@
+// Rows of 4-bit K/V caches (format: fp4.h): tokens stored as given, appended with q/k norm and rotation, and read
+// back as bf16 values.
+//
+// Reference: the 16-bit forms of the same steps, store_kvcache (src/layers/attention.py:10-61) and the producer in
+// Qwen3Attention.forward (src/models/qwen3.py:80-89); the reference has no quantised cache.
+//
+// Lanes: a 16-lane DPP row owns one head row of 128 values, lane c the values [8c, 8c + 8), so 32 values with one
+// scale are four neighbouring lanes (a quad): their largest magnitude is two quad permutes away, and a lane packs
+// its 8 values into one dword (16 lanes write the head's 64 bytes).
+//
+// What bounds them: HBM. A head row costs 256 bytes read and 68 written.
+#include "fp4.h"
+#include "norm_rope.h"
+
+namespace pk {
+namespace {
+
+constexpr int kRowThreads = 256;
+constexpr int kRowsPerGroup = kRowThreads / 16;
+
+// The largest magnitude (bf16 bits, sign cleared; infinities and NaN stay the largest) of the quad's 32 values.
+__device__ __forceinline__ uint32_t quad_top(const uint4 w) {
+  uint32_t m = 0;
+  const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max(m, max(x[i] & 0x7fffu, (x[i] >> 16) & 0x7fffu));
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, kDppXor1, 0xf, 0xf, false));
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, kDppXor2, 0xf, 0xf, false));
+  return m;
+}
+
+// A head row's 8 values of this lane into 4 bits: the lane's dword, and the quad's scale byte.
+__device__ __forceinline__ uint32_t quantise8(const uint4 w, uint32_t* scale_byte) {
+  *scale_byte = fp4_scale_byte(quad_top(w));
+  return fp4_pack8(w, *scale_byte);
+}
+
+// The dword and the scale byte of lane c into head h of a token's row.
+__device__ __forceinline__ void put_head(uint8_t* row, int heads, int h, int c, uint32_t data, uint32_t scale_byte) {
+  *reinterpret_cast<uint32_t*>(row + h * kFp4HeadBytes + c * 4) = data;
+  if ((c & 3) == 0) row[heads * kFp4HeadBytes + h * kFp4HeadScales + (c >> 2)] = (uint8_t)scale_byte;
+}
+
+__global__ __launch_bounds__(kRowThreads) void store_fp4_kernel(const Fp4StoreArgs a) {
+  const int c = threadIdx.x & 15;
+  const int per_token = 2 * a.num_kv_heads;
+  const int64_t i = (int64_t)blockIdx.x * kRowsPerGroup + (threadIdx.x >> 4);
+  if (i >= (int64_t)a.num_tokens * per_token) return;
+  const int32_t token = (int32_t)(i / per_token);
+  const int r = (int)(i - (int64_t)token * per_token);
+  const bool is_v = r >= a.num_kv_heads;
+  const int h = is_v ? r - a.num_kv_heads : r;
+  const int32_t slot = a.slot_mapping[token];
+  if (slot < 0 || slot >= a.num_slots) return;
+  const uint16_t* src = is_v ? a.value + (int64_t)token * a.value_stride : a.key + (int64_t)token * a.key_stride;
+  const uint4 w = *reinterpret_cast<const uint4*>(src + h * kHeadDim + c * 8);
+  uint32_t s;
+  const uint32_t d = quantise8(w, &s);
+  put_head((is_v ? a.v_cache : a.k_cache) + (int64_t)slot * a.row_bytes, a.num_kv_heads, h, c, d, s);
+}
+
+// Sum of a double over the 16 lanes of a DPP row, in every lane of it.
+template <int kCtrl>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, kCtrl, 0xf, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), kCtrl, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double row16_sum64(double v) {
+  v += dpp64<kDppXor1>(v);
+  v += dpp64<kDppXor2>(v);
+  v += dpp64<kDppHalfMirror>(v);
+  v += dpp64<kDppMirror>(v);
+  return v;
+}
+
+// 1 / sqrt(x) to the last bits of 64: the hardware's estimate and two steps of Newton's iteration.
+__device__ __forceinline__ float inverse_root(double x) {
+  double y = __builtin_amdgcn_rsq(x);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) y = y * (1.5 - 0.5 * x * y * y);
+  return x > 1.7e308 ? 0.f : (float)y;
+}
+
+// RMSNorm and rotation of one head row (norm_rope.h's steps and rounding points) with every operation rounded by
+// itself and the root taken in 64 bits: which of two neighbouring 4-bit values a key gets must not hang on how a
+// compiler fuses products, or on the order of a sum.
+__device__ __forceinline__ uint4 norm_rope_exact(const uint4 w, const uint16_t* wt, float eps, const float cv[8],
+                                                 const float sv[8], bool lower, int c) {
+#pragma clang fp contract(off)
+  float f[8];
+  unpack8(w, f);
+  if (wt != nullptr) {
+    double ss = 0.;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const double d = f[e];
+      ss = __builtin_fma(d, d, ss);
+    }
+    ss = row16_sum64(ss);
+    const float rs = inverse_root(ss * (1.0 / kHeadDim) + (double)eps);
+    float wf[8];
+    unpack8(*reinterpret_cast<const uint4*>(wt + c * 8), wf);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = round_bf16(wf[e] * (f[e] * rs));
+  }
+  float o[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float p = dpp_ror8(f[e]);  // element d +- 64
+    const float t1 = lower ? f[e] : p;
+    const float t2 = lower ? p : f[e];
+    const float a = t1 * (lower ? cv[e] : sv[e]);
+    const float b = t2 * (lower ? sv[e] : cv[e]);
+    o[e] = lower ? a - b : a + b;
+  }
+  return pack8(o);
+}
+
+// One wavefront per share of a token: its position, slot and cos/sin row are read once, DPP row j of it takes head
+// rows 4 (part + parts i) + j, with kAppendRows of them in flight.
+constexpr int kAppendRows = 8;
+__global__ __launch_bounds__(kRowThreads) void append_fp4_kernel(const Fp4AppendArgs a, int parts) {
+  constexpr int D = kHeadDim;
+  constexpr int kWaves = kRowThreads / kWave;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int c = lane & 15;
+  const bool lower = c < 8;
+  const int rows = a.num_heads + 2 * a.num_kv_heads;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t item = (int64_t)blockIdx.x * kWaves + wave;
+  if (item >= (int64_t)a.num_tokens * parts) return;
+  const int32_t token = (int32_t)(item / parts);
+  const int part = (int)(item - (int64_t)token * parts);
+  const uint16_t* src = a.qkv + (int64_t)token * a.qkv_stride + c * 8;
+  const int32_t slot = a.slot_mapping[token];
+  const bool stored = slot >= 0 && slot < a.num_slots;
+  float cv[8], sv[8];
+  rope_cos_sin_row(a.cos_sin, a.max_position, a.positions[token], c, cv, sv);
+  const int stride = 4 * parts;
+  for (int base = 4 * part + (lane >> 4); base < rows; base += stride * kAppendRows) {
+    uint4 w[kAppendRows];
+#pragma unroll
+    for (int i = 0; i < kAppendRows; ++i) {
+      const int r = base + stride * i;
+      w[i] = *reinterpret_cast<const uint4*>(src + (r < rows ? r : base) * D);
+    }
+#pragma unroll
+    for (int i = 0; i < kAppendRows; ++i) {
+      const int r = base + stride * i;
+      if (r >= rows) break;
+      if (r < a.num_heads) {
+        *reinterpret_cast<uint4*>(a.q_out + (int64_t)token * a.q_out_stride + r * D + c * 8) =
+            norm_rope_exact(w[i], a.q_weight, a.eps, cv, sv, lower, c);
+        continue;
+      }
+      const bool is_v = r >= a.num_heads + a.num_kv_heads;
+      const int h = r - a.num_heads - (is_v ? a.num_kv_heads : 0);
+      const uint4 x = is_v ? w[i] : norm_rope_exact(w[i], a.k_weight, a.eps, cv, sv, lower, c);
+      uint32_t s;
+      const uint32_t d = quantise8(x, &s);
+      if (stored)
+        put_head((is_v ? a.v_cache : a.k_cache) + (int64_t)slot * a.row_bytes, a.num_kv_heads, h, c, d, s);
+      uint16_t* out = is_v ? a.v_out : a.k_out;
+      if (out != nullptr)
+        *reinterpret_cast<uint4*>(out + (int64_t)token * (is_v ? a.v_out_stride : a.k_out_stride) + h * D + c * 8) =
+            fp4_unpack8(d, fp4_scale(s));
+    }
+  }
+}
+
+// Sequence blockIdx.y's rows through its table: 16 lanes a head row.
+__global__ __launch_bounds__(kRowThreads) void gather_fp4_kernel(const Fp4GatherArgs a) {
+  const int b = blockIdx.y;
+  const int c = threadIdx.x & 15;
+  const int k0 = a.cu_k[b];
+  const int len = min(a.cu_k[b + 1] - k0, a.max_seqlen_k);
+  const int64_t total = (int64_t)max(len, 0) * a.num_kv_heads;
+  const int64_t step = (int64_t)gridDim.x * kRowsPerGroup;
+  for (int64_t i = (int64_t)blockIdx.x * kRowsPerGroup + (threadIdx.x >> 4); i < total; i += step) {
+    const int t = (int)(i / a.num_kv_heads);
+    const int h = (int)(i - (int64_t)t * a.num_kv_heads);
+    const int blk = a.block_table[(int64_t)b * a.bt_stride + t / a.block_size];
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (blk >= 0 && blk < a.num_blocks) {
+      const uint8_t* row = a.cache + (int64_t)blk * a.block_stride + (int64_t)(t % a.block_size) * a.row_bytes;
+      const uint32_t d = *reinterpret_cast<const uint32_t*>(row + h * kFp4HeadBytes + c * 4);
+      const uint32_t s = row[a.num_kv_heads * kFp4HeadBytes + h * kFp4HeadScales + (c >> 2)];
+      x = fp4_unpack8(d, fp4_scale(s));
+    }
+    *reinterpret_cast<uint4*>(a.dst + ((int64_t)(k0 + t) * a.num_kv_heads + h) * kHeadDim + c * 8) = x;
+  }
+}
+
+}  // namespace
+
+hipError_t launch_store_fp4(const Fp4StoreArgs& a, hipStream_t stream) {
+  const int64_t rows = (int64_t)a.num_tokens * 2 * a.num_kv_heads;
+  hipLaunchKernelGGL(store_fp4_kernel, dim3((unsigned)((rows + kRowsPerGroup - 1) / kRowsPerGroup)), dim3(kRowThreads),
+                     0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_append_fp4(const Fp4AppendArgs& a, hipStream_t stream) {
+  const int quads = (a.num_heads + 2 * a.num_kv_heads + 3) / 4;  // 4 head rows per wavefront step
+  const int parts = a.num_tokens < 1024 ? (quads < 4 ? quads : 4) : 1;
+  const int64_t items = (int64_t)a.num_tokens * parts;
+  constexpr int kWaves = kRowThreads / kWave;
+  hipLaunchKernelGGL(append_fp4_kernel, dim3((unsigned)((items + kWaves - 1) / kWaves)), dim3(kRowThreads), 0, stream,
+                     a, parts);
+  return hipGetLastError();
+}
+
+hipError_t launch_gather_fp4(const Fp4GatherArgs& a, hipStream_t stream) {
+  const int64_t rows = (int64_t)a.max_seqlen_k * a.num_kv_heads;
+  const int64_t bx = (rows + kRowsPerGroup - 1) / kRowsPerGroup;
+  hipLaunchKernelGGL(gather_fp4_kernel, dim3((unsigned)(bx > 4096 ? 4096 : bx), (unsigned)a.num_seqs),
+                     dim3(kRowThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace pk

@@ -163,9 +163,35 @@ SIGNATURES = {
         _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p,
         _c_void_p, _c_void_p,               # block_map, num_live
         _c_void_p, _size_t, _c_void_p]),    # workspace, workspace_bytes, stream
+    "pk_fp4_row_bytes": (_size_t, [_i32]),
+    "pk_store_kvcache_fp4": (ctypes.c_int, [
+        _c_void_p, _i64, _c_void_p, _i64,   # key, its row stride, value, its row stride
+        _c_void_p, _c_void_p, _c_void_p,    # k_cache, v_cache, slot_mapping
+        _i32, _i32, _i32, _i64, _c_void_p]),  # num_tokens, num_kv_heads, head_dim, num_slots, stream
+    "pk_qk_norm_rope_store_fp4": (ctypes.c_int, [
+        _c_void_p, _i64,                    # qkv, qkv_row_stride
+        _c_void_p, _c_void_p, _i64,         # positions, cos_sin, max_position
+        _c_void_p, _c_void_p, ctypes.c_float,  # q/k norm weights, eps
+        _i32, _i32, _i32, _i32,             # num_tokens, num_heads, num_kv_heads, head_dim
+        _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64,  # q_out, k_out, v_out with their row strides
+        _c_void_p, _c_void_p, _c_void_p,    # k_cache, v_cache, slot_mapping
+        _i64, _c_void_p]),                  # num_slots, stream
+    "pk_gather_kv_fp4": (ctypes.c_int, [
+        _c_void_p, _i64, _i32, _i32,        # cache, block_stride, num_blocks, block_size
+        _i32, _i32, _c_void_p, _i32,        # num_kv_heads, head_dim, block_table, its row stride
+        _c_void_p, _i32, _i32, _c_void_p, _c_void_p]),  # cu_seqlens_k, num_seqs, max_seqlen_k, dst, stream
+    "pk_varlen_attention_fp4_workspace_bytes": (_size_t, [_i32, _i32, _i32, _i32, _i32]),
+    "pk_varlen_attention_fp4": (ctypes.c_int, [
+        _c_void_p, _i64, _c_void_p, _c_void_p,  # q, q_row_stride, k_cache, v_cache
+        _i64, _i64, _i32, _i32,             # k/v block strides, num_blocks, block_size
+        _c_void_p, _i32, _c_void_p, _c_void_p,  # block_table, its row stride, cu_seqlens_q, cu_seqlens_k
+        _i32, _i64, _i32, _i32,             # num_seqs, num_rows, max_seqlen_q, max_seqlen_k
+        _i32, _i32, _i32,                   # num_heads, num_kv_heads, head_dim
+        ctypes.c_float, _i32,               # softmax_scale, causal
+        _c_void_p, _i64, _c_void_p, _size_t, _c_void_p]),  # out, its row stride, workspace, its bytes, stream
 }
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
