@@ -6,7 +6,7 @@
 //     num_kv_heads x 4 scale bytes, one per 32 dimensions;
 //     0 to 15 bytes up to a multiple of 16, never read or written.
 // A value is a sign, two bits of exponent and one of mantissa -- 0, 0.5, 1, 1.5, 2, 3, 4 or 6 -- times
-// 2^(scale byte - 127); scale byte 255 makes its 32 values NaN. Two such products add up in bf16 without rounding,
+// 2^(scale byte - 127); scale byte 255 makes its 32 values NaN, 0, 253 and 254 do not occur. Two such products add up in bf16 without rounding,
 // so a value converts to bf16 exactly (v_cvt_scalef32_pk_bf16_fp4, which applies the scale's exponent as well).
 // Token-major rows keep a page one run of bytes whose first n tokens are its first n rows, which is what the page
 // operators (kv_pages.hip) copy.
@@ -18,6 +18,7 @@ namespace pk {
 
 constexpr int kFp4HeadBytes = kHeadDim / 2;   // values of one kv head
 constexpr int kFp4HeadScales = kHeadDim / 32;  // its scale bytes
+constexpr int kFp4MaxScale = 252;              // the largest scale byte of finite values
 constexpr int kFp4ScaleNaN = 255;
 constexpr int kFp4MaxHeads = 255;
 
@@ -32,7 +33,7 @@ inline int32_t fp4_row_bytes(int32_t num_kv_heads) {
 // 2^-126 .. 2^125: the smallest normal scale, and the largest one whose 6 s is finite. Infinities and NaN: 255.
 __device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t top) {
   const int e = (int)(top >> 7) - 2 + ((top & 0x7f) > 0x60 ? 1 : 0);  // 0x60: a mantissa of 1.75
-  return top >= 0x7f80 ? kFp4ScaleNaN : (uint32_t)min(max(e, 1), 252);
+  return top >= 0x7f80 ? kFp4ScaleNaN : (uint32_t)min(max(e, 1), kFp4MaxScale);
 }
 
 typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 fp4_bf16x2;
@@ -134,9 +135,11 @@ struct Fp4AttnArgs {
 // Launch shapes of a call, a function of its bounds; runs and columns of the partial results.
 struct Fp4AttnPlan {
   int32_t few_runs;              // work-groups over the sequences of few rows (per group of kv heads)
-  int32_t few_heads;             // kv heads (wavefronts) of one of them
+  int32_t few_heads;             // kv heads of one of them
+  int32_t few_slots;             // the next power of two
   int32_t few_cols;              // columns (rows x query heads) of a kv head's partial result
   int32_t many_runs;             // work-groups over the sequences of more rows, 0: there can be none
+  int64_t many_tiles;            // about as many tiles of rows (of all kv heads) as they have
   size_t few_bytes, many_bytes;  // partial results
   bool too_long;                 // the steps of a kv head may not fit 31 bits
 };

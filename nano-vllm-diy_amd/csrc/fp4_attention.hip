@@ -32,22 +32,30 @@
 //       work-group reads whole token rows.
 //   more rows: T = 2, a tile is 128 columns of one kv head, a wavefront 32 of them.
 #include <algorithm>
+#include <type_traits>
 
 #include "fp4.h"
 
 namespace pk {
 namespace {
 
-constexpr int kStep = 64;             // keys of a step
-constexpr int kManyWaves = 4;         // wavefronts of a work-group over sequences of more rows
-constexpr int kManyTiles = 2;         // tiles of 16 columns a wavefront of it holds
+constexpr int kFewWaves = 8;          // wavefronts of a work-group over sequences of few rows
+constexpr int kManyWaves = 4;         // ... of more rows
+constexpr int kManyTiles = 2;         // tiles of 16 columns a wavefront of the latter holds
 constexpr int kManyCols = kManyWaves * kManyTiles * 16;
+constexpr int kManyStep = 64;         // keys of its step
+constexpr int kSub = 32;              // keys a wavefront takes at once
 constexpr int kSlots = 8;             // sequences a lane keeps the steps of
 constexpr int kChunk = kSlots * kWave;
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kSlack = 8.f;         // the scores may exceed their reference by this (exp2 domain)
 
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 frag;
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef __attribute__((address_space(3))) uint32_t lds_u32;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) float lds_f32;
+typedef __attribute__((address_space(3))) f32x2 lds_f32x2;
 
 __device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(frag, a), __builtin_bit_cast(frag, b), c, 0, 0, 0);
@@ -69,6 +77,13 @@ __device__ __forceinline__ float quarters_sum(float v) {
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// An entry of a list that no kernel here writes, at a position that is the same for the wavefront: a scalar load,
+// which does not wait for the vector loads in flight as a vector load's use would.
+__device__ __forceinline__ int scalar_i32(const int32_t* p) {
+  typedef __attribute__((address_space(4))) const int32_t* constant;
+  return uniform(*(constant)reinterpret_cast<uintptr_t>(p));
+}
+
 // Inclusive sum over the wavefront.
 __device__ __forceinline__ int scan64(int v, int lane) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1, :2, :4, :8
@@ -86,8 +101,7 @@ __device__ __forceinline__ int scan64(int v, int lane) {
 struct Seq {
   int q0, rows, shift, keys;  // row r sees keys t <= r + shift
 };
-__device__ __forceinline__ Seq seq_of(const Fp4AttnArgs& a, int b) {
-  const int q0 = a.cu_q[b], q1 = a.cu_q[b + 1], k0 = a.cu_k[b], k1 = a.cu_k[b + 1];
+__device__ __forceinline__ Seq make_seq(const Fp4AttnArgs& a, int q0, int q1, int k0, int k1) {
   Seq s;
   s.q0 = q0;
   s.keys = min(k1 - k0, a.max_seqlen_k);
@@ -95,24 +109,32 @@ __device__ __forceinline__ Seq seq_of(const Fp4AttnArgs& a, int b) {
   s.shift = a.causal ? s.keys - (q1 - q0) : s.keys;
   return s;
 }
+__device__ __forceinline__ Seq seq_of(const Fp4AttnArgs& a, int b) {
+  return make_seq(a, a.cu_q[b], a.cu_q[b + 1], a.cu_k[b], a.cu_k[b + 1]);
+}
+__device__ __forceinline__ Seq uniform_seq(const Fp4AttnArgs& a, int b) {
+  const Seq s = make_seq(a, scalar_i32(a.cu_q + b), scalar_i32(a.cu_q + b + 1), scalar_i32(a.cu_k + b),
+                         scalar_i32(a.cu_k + b + 1));
+  return {uniform(s.q0), uniform(s.rows), uniform(s.shift), uniform(s.keys)};
+}
 
-// Steps of tile j of a sequence: up to the last key its last row sees, at least one.
-template <bool MANY>
+// Steps of STEP keys of tile j of a sequence: up to the last key its last row sees, at least one.
+template <bool MANY, int STEP>
 __device__ __forceinline__ int tile_steps(const Fp4AttnArgs& a, const Seq& s, int j) {
   const int per_tile = MANY ? kManyCols >> a.group_shift : s.rows;
   const int last = min(s.rows, (j + 1) * per_tile) - 1;
   const int end = min(s.keys, last + s.shift + 1);
-  return max(1, (end + kStep - 1) / kStep);
+  return max(1, (end + STEP - 1) / STEP);
 }
 
 // Steps of a sequence on the line of one kv head (MANY) or of all kv heads; 0 where it is on the other line.
-template <bool MANY>
+template <bool MANY, int STEP>
 __device__ __forceinline__ int seq_steps(const Fp4AttnArgs& a, const Seq& s) {
   if (s.rows <= 0 || (s.rows << a.group_shift > 16) != MANY) return 0;
-  if constexpr (!MANY) return tile_steps<false>(a, s, 0);
+  if constexpr (!MANY) return tile_steps<false, STEP>(a, s, 0);
   const int tiles = ((s.rows << a.group_shift) + kManyCols - 1) / kManyCols;
   int n = 0;
-  for (int j = 0; j < tiles; ++j) n += tile_steps<true>(a, s, j);
+  for (int j = 0; j < tiles; ++j) n += tile_steps<true, STEP>(a, s, j);
   return n;
 }
 
@@ -125,7 +147,7 @@ struct Tile {
 
 // The line of steps: MANY: kv head by kv head, sequence by sequence, tile by tile; otherwise the sequences' steps,
 // which the wavefronts take for a kv head each.
-template <bool MANY>
+template <bool MANY, int STEP>
 struct Line {
   int n[kSlots];     // steps of sequence `base` + 64 s + lane
   int base;
@@ -138,7 +160,7 @@ struct Line {
     for (int s = 0; s < kSlots; ++s) {
       n[s] = 0;
       const int b = first + 64 * s + lane;
-      if (first + 64 * s < a.num_seqs && b < a.num_seqs) n[s] = seq_steps<MANY>(a, seq_of(a, b));
+      if (first + 64 * s < a.num_seqs && b < a.num_seqs) n[s] = seq_steps<MANY, STEP>(a, seq_of(a, b));
     }
   }
   __device__ __forceinline__ void init(const Fp4AttnArgs& a, int lane) {
@@ -177,14 +199,13 @@ struct Line {
         }
       }
     }
-    t.b = b;
-    const Seq s = seq_of(a, b);
-    int start = seq_start, steps = tile_steps<MANY>(a, s, 0);
+    const Seq s = uniform_seq(a, b);
+    int start = seq_start, steps = tile_steps<MANY, STEP>(a, s, 0);
     if constexpr (MANY) {
       const int tiles = ((s.rows << a.group_shift) + kManyCols - 1) / kManyCols;
       for (int j0 = 0; j0 < tiles; j0 += kWave) {
         const int j = j0 + lane;
-        const int mine = j < tiles ? tile_steps<true>(a, s, j) : 0;
+        const int mine = j < tiles ? tile_steps<true, STEP>(a, s, j) : 0;
         const int incl = start + scan64(mine, lane);
         const uint64_t m = __builtin_amdgcn_ballot_w64(want < incl);
         if (m) {
@@ -197,8 +218,11 @@ struct Line {
         start = __builtin_amdgcn_readlane(incl, kWave - 1);
       }
     }
-    t.start = head_start + start;
-    t.steps = steps;
+    t.b = uniform(b);
+    t.head = uniform(t.head);
+    t.j = uniform(t.j);
+    t.start = head_start + uniform(start);
+    t.steps = uniform(steps);
     return t;
   }
 };
@@ -218,6 +242,9 @@ __device__ __forceinline__ Cuts cuts_of(int64_t total, int runs) { return {total
 struct Partials {
   float* o;       // [slot][head][column][128]
   float2* ml;     // [slot][head][column]
+  int32_t* live;  // runs that have work
+  int4* split;    // [run] the tile that begins in it and goes on: first row of out, columns, partial results (0: none),
+                  // kv head
   int heads, cols;
   __device__ __forceinline__ int64_t at(int64_t slot, int head, int col) const {
     return (slot * heads + head) * cols + col;
@@ -228,46 +255,155 @@ __host__ __device__ __forceinline__ size_t partial_rows(const Fp4AttnPlan& p, in
   return MANY ? (size_t)2 * p.many_runs * kManyCols : (size_t)2 * p.few_runs * num_kv_heads * p.few_cols;
 }
 
-// What a wavefront reads of a page's 64 rows. Four resources a cache, one for 16 rows: a row past the sequence's
-// end is out of its range and reads as zeros (the range check covers the lane's offset alone), so no key needs a
-// clamp, and a value behind the end is zero whatever the page holds.
-struct Offsets {
-  int k, ks;         // key l % 16: its 16 bytes, its scale
-  int v[4], vs[4];   // key 4 (l / 16) + i: its 4 bytes, their scale
-};
-struct Keys {
-  u32x4 d[4];
-  uint32_t s[4];
-};
-struct Vals {
-  uint32_t d[4][4];
-  uint32_t s[4][4];
-};
-
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const uint8_t* page, int rows, int row_bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(page), (short)0, max(rows, 0) * row_bytes, 0x00020000);
+// ---- rows in LDS ---------------------------------------------------------------------------
+//
+// A step's rows of the work-group's kv heads, HEADS slots a row: [K values | K scales | V values | V scales], a row's
+// values HEADS x 4 chunks of 16 bytes, its scales HEADS dwords. They come straight from memory (global_load_lds, 1
+// KiB an instruction for the values), two steps in turn. (With every wavefront reading its own head's bytes into
+// registers the kernel was bound by its load instructions: 40 a step of 64 keys and head, most of them of 16 to 256
+// bytes, 355 us for 256 sequences of 1k-8k keys.)
+//
+// Banks. Chunk c of row r lies in slot c ^ swizzle(r) of the row. 16 lanes read K chunk 4 h + g of 16 rows (16
+// bytes each), and 4 x 16 lanes 64 bytes each of four rows of V: with these swizzles, and the rows of a tile in the
+// order of row_of, both touch every bank once (twice for V with two heads).
+template <int HEADS>
+__device__ __forceinline__ int swizzle(int r) {
+  return HEADS >= 4 ? r & 15 : HEADS == 2 ? (r >> 1) & 7 : (r >> 2) & 3;
+}
+// The row (key) of a tile of 16 that is row m of its matrix product.
+template <int HEADS>
+__device__ __forceinline__ int row_of(int m) {
+  return HEADS == 1 ? 4 * (m & 3) + (m >> 2) : m;
 }
 
-__device__ __forceinline__ void load_keys(Keys& k, const uint8_t* page, int rows, int row_bytes, const Offsets& o) {
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const __amdgpu_buffer_rsrc_t r = rows_of(page + 16 * t * row_bytes, min(rows - 16 * t, 16), row_bytes);
-    k.d[t] = __builtin_amdgcn_raw_buffer_load_b128(r, o.k, 0, 0);
-    k.s[t] = __builtin_amdgcn_raw_buffer_load_b8(r, o.ks, 0, 0);
+template <int HEADS, int ROWS>
+struct Stage {
+  static constexpr int kValues = ROWS * HEADS * kFp4HeadBytes;
+  static constexpr int kScales = ROWS * HEADS * kFp4HeadScales;
+  static constexpr int kCache = kValues + kScales;
+  static constexpr int kBytes = 2 * kCache;
+};
+
+// Waits until this wavefront's loads have arrived, then for the other wavefronts.
+__device__ __forceinline__ void arrive_all() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// 16 or 4 bytes per active lane from base + off to lds + 16 or 4 lane, in flight until arrive_all.
+__device__ __forceinline__ void stage16(const uint8_t* base, int off, int lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds), "v"(off), "s"(base)
+               : "m0", "memory");
+}
+__device__ __forceinline__ void stage4(const uint8_t* base, int off, int lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+               :
+               : "s"(lds), "v"(off), "s"(base)
+               : "m0", "memory");
+}
+
+__device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
+  const uint64_t u = reinterpret_cast<uintptr_t>(p);
+  const uint64_t lo = (uint32_t)uniform((int)(uint32_t)u), hi = (uint32_t)uniform((int)(u >> 32));
+  return reinterpret_cast<const uint8_t*>(hi << 32 | lo);
+}
+
+// The place of a sequence's keys in the pages, from key t on in steps of `step` keys: the table's entry is read one
+// step ahead. An entry that is no block has no rows, and its keys are seen by nobody.
+struct Cursor {
+  const int32_t* table;
+  int t, entry, off, last, blk;
+
+  __device__ __forceinline__ void init(const Fp4AttnArgs& a, const int32_t* row, int first, int keys) {
+    table = row;
+    t = first;
+    entry = first / a.block_size;
+    off = first - entry * a.block_size;
+    last = (keys - 1) / a.block_size;
+    blk = scalar_i32(table + min(entry, last));
   }
-}
-
-__device__ __forceinline__ void load_vals(Vals& v, const uint8_t* page, int rows, int row_bytes, const Offsets& o) {
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const __amdgpu_buffer_rsrc_t r = rows_of(page + 16 * t * row_bytes, min(rows - 16 * t, 16), row_bytes);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v.d[t][i] = __builtin_amdgcn_raw_buffer_load_b32(r, o.v[i], 0, 0);
-      v.s[t][i] = __builtin_amdgcn_raw_buffer_load_b8(r, o.vs[i], 0, 0);
+  __device__ __forceinline__ bool good(const Fp4AttnArgs& a) const { return blk >= 0 && blk < a.num_blocks; }
+  __device__ __forceinline__ int rows(const Fp4AttnArgs& a, int keys) const { return good(a) ? keys - t : 0; }
+  // Rows from here on in a cache (any place of the cache where there are none).
+  __device__ __forceinline__ const uint8_t* at(const Fp4AttnArgs& a, const uint8_t* cache, int64_t block) const {
+    return good(a) ? cache + (blk * block + (int64_t)off * a.row_bytes) : cache;
+  }
+  __device__ __forceinline__ void next(const Fp4AttnArgs& a, int step) {
+    t += step;
+    off += step;
+    if (off >= a.block_size) {
+      do {
+        off -= a.block_size;
+        ++entry;
+      } while (off >= a.block_size);
+      blk = scalar_i32(table + min(entry, last));
     }
   }
-}
+};
+
+// One wavefront's share of a step's loads. Few rows (256 slots of a head and row, 8 wavefronts): of each cache two KiB
+// of values, of one cache a quarter of the scales. More rows (64 rows of one head, 4 wavefronts): one KiB of
+// each cache's values, the first two wavefronts a cache's scales.
+template <int HEADS, int ROWS, int WAVES>
+struct Loader {
+  typedef Stage<HEADS, ROWS> S;
+  static constexpr int kJobs = ROWS * HEADS / 16 / WAVES;   // KiB of values of a cache
+  static constexpr int kScaleJobs = ROWS * HEADS / 64;      // 256 bytes of scales of a cache
+  static_assert(kJobs * WAVES * 16 == ROWS * HEADS && 2 * kScaleJobs <= WAVES, "loads divide among the wavefronts");
+  int off[kJobs], row[kJobs];  // the lane's bytes and row after the cursor; no row where its slot is no head
+  int scale_off, scale_row;
+  int lds, scale_lds;
+  bool has_scales, scales_of_v;
+  Cursor at, scale_at;
+
+  __device__ __forceinline__ void init(const Fp4AttnArgs& a, const int32_t* table, int t0, int keys, int head0, int heads,
+                                       int wave, int lane) {
+    const int first = wave * kJobs * 64 / (4 * HEADS);  // the first row
+#pragma unroll
+    for (int j = 0; j < kJobs; ++j) {
+      const int slot = (wave * kJobs + j) * 64 + lane;
+      const int r = slot / (4 * HEADS), c = (slot % (4 * HEADS)) ^ swizzle<HEADS>(r);
+      row[j] = r - (first & ~31);
+      off[j] = row[j] * a.row_bytes + (head0 + (c >> 2)) * kFp4HeadBytes + 16 * (c & 3);
+      if ((c >> 2) >= heads) row[j] = INT32_MAX;
+    }
+    lds = wave * kJobs * 1024;
+    const int part = wave % (WAVES / 2 < kScaleJobs ? WAVES / 2 : kScaleJobs);
+    has_scales = wave < 2 * kScaleJobs;
+    scales_of_v = wave >= kScaleJobs;
+    const int s = part * 64 + lane, r = s / HEADS, h = s % HEADS;
+    const int scale_first = part * 64 / HEADS & ~31;
+    scale_row = r - scale_first;
+    scale_off = scale_row * a.row_bytes + a.num_kv_heads * kFp4HeadBytes + (head0 + h) * kFp4HeadScales;
+    if (h >= heads) scale_row = INT32_MAX;
+    scale_lds = (scales_of_v ? S::kCache : 0) + S::kValues + part * 256;
+    at.init(a, table, t0 + (first & ~31), keys);
+    scale_at.init(a, table, t0 + scale_first, keys);
+  }
+
+  // The next step's rows into a stage of LDS. (A row that is no key is not read: its place keeps what it has.)
+  __device__ __forceinline__ void issue(const Fp4AttnArgs& a, int keys, int stage) {
+    const int rows = at.rows(a, keys);
+    const uint8_t* k = uniform_ptr(at.at(a, a.k, a.k_block));
+    const uint8_t* v = uniform_ptr(at.at(a, a.v, a.v_block));
+#pragma unroll
+    for (int j = 0; j < kJobs; ++j)
+      if (row[j] < rows) {
+        stage16(k, off[j], stage + lds + 1024 * j);
+        stage16(v, off[j], stage + S::kCache + lds + 1024 * j);
+      }
+    at.next(a, ROWS);
+    if (has_scales) {
+      const int scale_rows = scale_at.rows(a, keys);
+      const uint8_t* c = uniform_ptr(scales_of_v ? scale_at.at(a, a.v, a.v_block) : scale_at.at(a, a.k, a.k_block));
+      if (scale_row < scale_rows) stage4(c, scale_off, stage + scale_lds);
+      scale_at.next(a, ROWS);
+    }
+  }
+};
+
+// ---- one wavefront's 32 keys -----------------------------------------------------------------
 
 // Running softmax of the wavefront's columns: lane l has column l % 16 of every tile.
 template <int T>
@@ -278,34 +414,74 @@ struct State {
   float l[T];        // this lane's keys' share of the sum
 };
 
-template <int T>
-__device__ __forceinline__ void scores(f32x4 (&s)[4][T], const State<T>& st, const Keys& k) {
+struct Vals {
+  uint32_t d[2][4];  // tile t, row row_of(4 (l / 16) + i): dimensions 8 (l % 16) .. + 7
+  uint32_t s[2][4];  // their scale byte
+};
+
+// Where a lane's rows lie in a stage.
+template <int HEADS, int ROWS>
+struct Lanes {
+  typedef Stage<HEADS, ROWS> S;
+  static constexpr int kTile = 16 * HEADS * kFp4HeadBytes, kScaleTile = 16 * HEADS * kFp4HeadScales;
+  int k, ks, v[4], vs;
+
+  // first: the wavefront's first row, slot: its head's.
+  __device__ __forceinline__ void init(int first, int slot, int lane) {
+    const int n = lane & 15, g = lane >> 4;
+    int r = row_of<HEADS>(n);
+    k = ((first + r) * 4 * HEADS + ((4 * slot + g) ^ swizzle<HEADS>(r))) * 16;
+    ks = S::kValues + ((first + r) * HEADS + slot) * 4 + g;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const float scale = fp4_scale(k.s[t]);
+    for (int i = 0; i < 4; ++i) {
+      r = row_of<HEADS>(4 * g + i);
+      v[i] = S::kCache + ((first + r) * 4 * HEADS + ((4 * slot + (n >> 2)) ^ swizzle<HEADS>(r))) * 16 + 4 * (n & 3);
+    }
+    vs = S::kCache + S::kValues + ((first + row_of<HEADS>(4 * g)) * HEADS + slot) * 4 + (n >> 2);
+  }
+  // Rows 16 tile0 on of the wavefront's.
+  template <int TILE0>
+  __device__ __forceinline__ void values(Vals& x, const lds_u8* stage) const {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x.d[t][i] = *(const lds_u32*)(stage + v[i] + (TILE0 + t) * kTile);
+        x.s[t][i] = *(const lds_u8*)(stage + vs + (TILE0 + t) * kScaleTile + row_of<HEADS>(i) * HEADS * 4);
+      }
+  }
+};
+
+// S^T of two tiles of 16 keys.
+template <int TILE0, int T, int HEADS, int ROWS>
+__device__ __forceinline__ void scores(f32x4 (&s)[2][T], const State<T>& st, const lds_u8* stage,
+                                       const Lanes<HEADS, ROWS>& at) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const u32x4 d = *(const lds_u32x4*)(stage + at.k + (TILE0 + t) * at.kTile);
+    const float scale = fp4_scale(*(const lds_u8*)(stage + at.ks + (TILE0 + t) * at.kScaleTile));
 #pragma unroll
     for (int x = 0; x < T; ++x) s[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const uint4 w = fp4_unpack8(k.d[t][c], scale);
+      const uint4 w = fp4_unpack8(d[c], scale);
 #pragma unroll
       for (int x = 0; x < T; ++x) s[t][x] = mfma(u32x4{w.x, w.y, w.z, w.w}, st.q[x][c], s[t][x]);
     }
   }
 }
 
-// The step's weights of the columns, in bf16 pairs: p[x][h] are keys 16 (2 h + t) + 4 (l / 16) + i in the order t, i.
+// The weights of the columns, in bf16 pairs, as the operand of the product with V: tile by tile, i by i.
 template <int T>
-__device__ __forceinline__ void weights(u32x4 (&p)[T][2], f32x4 (&s)[4][T], State<T>& st, float c2) {
+__device__ __forceinline__ void weights(u32x4 (&p)[T], const f32x4 (&s)[2][T], State<T>& st, float c2) {
   float top[T];
   bool over = false;
 #pragma unroll
   for (int x = 0; x < T; ++x) {
     float mx = fmaxf(s[0][x][0], s[0][x][1]);
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int i = t ? 0 : 2; i < 4; ++i) mx = fmaxf(mx, s[t][x][i]);
+    mx = fmaxf(fmaxf(mx, s[0][x][2]), s[0][x][3]);
+    mx = fmaxf(fmaxf(mx, s[1][x][0]), s[1][x][1]);
+    mx = fmaxf(fmaxf(mx, s[1][x][2]), s[1][x][3]);
     top[x] = quarters_max(mx) * c2;
     over |= top[x] > st.m[x] + kSlack;
   }
@@ -323,96 +499,185 @@ __device__ __forceinline__ void weights(u32x4 (&p)[T][2], f32x4 (&s)[4][T], Stat
 #pragma unroll
   for (int x = 0; x < T; ++x) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 2; ++t) {
       float e[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         e[i] = exp2_fast(fmaf(s[t][x][i], c2, -st.m[x]));
         st.l[x] += e[i];
       }
-      p[x][t >> 1][2 * (t & 1)] = pack_bf16x2(e[0], e[1]);
-      p[x][t >> 1][2 * (t & 1) + 1] = pack_bf16x2(e[2], e[3]);
+      p[x][2 * t] = pack_bf16x2(e[0], e[1]);
+      p[x][2 * t + 1] = pack_bf16x2(e[2], e[3]);
     }
   }
 }
 
 template <int kByte, int T>
-__device__ __forceinline__ void add_pair(State<T>& st, const u32x4 (&p)[T][2], const Vals& v, int h) {
+__device__ __forceinline__ void add_pair(State<T>& st, const u32x4 (&p)[T], const Vals& v) {
   u32x4 even, odd;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint32_t x = fp4_pair<kByte>(v.d[2 * h + t][2 * i], fp4_scale(v.s[2 * h + t][2 * i]));
-      const uint32_t y = fp4_pair<kByte>(v.d[2 * h + t][2 * i + 1], fp4_scale(v.s[2 * h + t][2 * i + 1]));
+      const uint32_t x = fp4_pair<kByte>(v.d[t][2 * i], fp4_scale(v.s[t][2 * i]));
+      const uint32_t y = fp4_pair<kByte>(v.d[t][2 * i + 1], fp4_scale(v.s[t][2 * i + 1]));
       even[2 * t + i] = __builtin_amdgcn_perm(y, x, 0x05040100u);
       odd[2 * t + i] = __builtin_amdgcn_perm(y, x, 0x07060302u);
     }
   }
 #pragma unroll
   for (int x = 0; x < T; ++x) {
-    st.acc[x][2 * kByte] = mfma(even, p[x][h], st.acc[x][2 * kByte]);
-    st.acc[x][2 * kByte + 1] = mfma(odd, p[x][h], st.acc[x][2 * kByte + 1]);
+    st.acc[x][2 * kByte] = mfma(even, p[x], st.acc[x][2 * kByte]);
+    st.acc[x][2 * kByte + 1] = mfma(odd, p[x], st.acc[x][2 * kByte + 1]);
   }
 }
 
 template <int T>
-__device__ __forceinline__ void add_values(State<T>& st, const u32x4 (&p)[T][2], const Vals& v) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    add_pair<0>(st, p, v, h);
-    add_pair<1>(st, p, v, h);
-    add_pair<2>(st, p, v, h);
-    add_pair<3>(st, p, v, h);
-  }
+__device__ __forceinline__ void add_values(State<T>& st, const u32x4 (&p)[T], const Vals& v) {
+  add_pair<0>(st, p, v);
+  add_pair<1>(st, p, v);
+  add_pair<2>(st, p, v);
+  add_pair<3>(st, p, v);
 }
 
-// Whether a value block of the step is NaN (the lanes' scale bytes).
-__device__ __forceinline__ bool any_nan(const Vals& v) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int t = 0; t < 4; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m = max(m, v.s[t][i]);
-  return __builtin_amdgcn_ballot_w64(m == kFp4ScaleNaN) != 0;
-}
-
-// NaN blocks of a step some of whose keys some columns do not see: 0 x NaN would reach those columns through the
+// NaN blocks among keys some of which some columns do not see: 0 x NaN would reach those columns through the
 // matrix product. The blocks are taken as zeros there, and a column that does see such a key gets its NaN here.
 // (Lane l's 32 outputs are the block l / 16 of its column. The scale bytes of one key and all four blocks are lanes
-// 0, 4, 8, 12 of the row of 16 lanes that loaded the key.)
-template <int T>
+// 0, 4, 8, 12 of the row of 16 lanes that has the key.) Rows past the last key hold anything, scales that no cache
+// has among it, whose values are infinite: this is also what keeps them out.
+template <int T, int HEADS>
 __device__ __forceinline__ void nan_values(State<T>& st, Vals& v, const int (&rel)[T], int lane) {
+  uint32_t most = 0;
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = max(most, v.s[t][i]);
+  if (!__builtin_amdgcn_ballot_w64(most > kFp4MaxScale)) return;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int bad = v.s[t][i] == kFp4ScaleNaN;
-#pragma unroll
+      const bool bad = v.s[t][i] > kFp4MaxScale;
+      const uint64_t which = __builtin_amdgcn_ballot_w64(bad);
+      if (!which) continue;
+      if (bad) v.s[t][i] = v.d[t][i] = 0;
       for (int g = 0; g < 4; ++g) {
-        const int here = __shfl(bad, 16 * g + 4 * (lane >> 4));  // key 16 t + 4 g + i, block lane / 16
+        const bool here = which >> (16 * g + 4 * (lane >> 4)) & 1;  // row row_of(4 g + i) of the tile, block lane / 16
 #pragma unroll
         for (int x = 0; x < T; ++x)
-          if (here && 16 * t + 4 * g + i <= rel[x])
+          if (here && 16 * t + row_of<HEADS>(4 * g + i) <= rel[x])
 #pragma unroll
             for (int j = 0; j < 8; ++j) st.acc[x][j] += __builtin_nanf("");
       }
-      if (bad) v.s[t][i] = v.d[t][i] = 0;
     }
 }
 
-// Work-group `index` of the line's. head0: the first kv head of its wavefronts (few rows). Neighbouring runs of
-// MANY, whose tiles read the same keys, go to one XCD (work-groups go to the 8 of them in turn).
-template <bool MANY, int T>
-__device__ __forceinline__ void attend_run(const Fp4AttnArgs& a, const Partials& part, int num_runs, int index, int head0) {
+// 32 keys of a stage, from tile TILE0 of the wavefront's on. rel: the last of them that a column sees, where some
+// column does not see all.
+template <int TILE0, int T, int HEADS, int ROWS>
+__device__ __forceinline__ void take(State<T>& st, const lds_u8* stage, const Lanes<HEADS, ROWS>& at, bool masked,
+                                     const int (&rel)[T], float c2, int lane) {
+  f32x4 s[2][T];
+  scores<TILE0>(s, st, stage, at);
+  if (masked) {
+#pragma unroll
+    for (int x = 0; x < T; ++x)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (16 * t + row_of<HEADS>(4 * (lane >> 4) + i) > rel[x]) s[t][x][i] = -INFINITY;
+  }
+  Vals v;
+  at.template values<TILE0>(v, stage);
+  u32x4 p[T];
+  weights<T>(p, s, st, c2);
+  if (masked) nan_values<T, HEADS>(st, v, rel, lane);
+  add_values<T>(st, p, v);
+}
+
+// ---- results ---------------------------------------------------------------------------------
+
+// COUNT of a lane's 32 output values from value r on (value 8 i + j is dimension 8 i + j of the lane's block): to the
+// output's row, scaled, or to a partial result.
+template <int COUNT>
+__device__ __forceinline__ void put_out(uint16_t* out, const float* x, float inv) {
+  if constexpr (COUNT >= 8) {
+#pragma unroll
+    for (int i = 0; i < COUNT; i += 8) {
+      u32x4 w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(x[i + 2 * j] * inv, x[i + 2 * j + 1] * inv);
+      *reinterpret_cast<u32x4*>(out + i) = w;
+    }
+  } else {
+    *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv)};
+  }
+}
+template <int COUNT>
+__device__ __forceinline__ void put_part(float* out, const float* x) {
+#pragma unroll
+  for (int i = 0; i < COUNT; i += 4) *reinterpret_cast<f32x4*>(out + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+}
+
+// The SLICES wavefronts of a kv head, which took different keys, put their states together in LDS: every one of them
+// ends with the column's m and l and with 32 / SLICES values of each lane, those from (32 / SLICES) slice on.
+template <int SLICES, int HEADS>
+__device__ __forceinline__ void join_slices(float (&x)[32 / SLICES], float* m, float* l, const State<1>& st, lds_u8* lds,
+                                            int wave, int lane) {
+  lds_f32x2* ml = (lds_f32x2*)lds;
+  lds_f32* o = (lds_f32*)(lds + kFewWaves * kWave * 8);
+  const int slot = wave % HEADS, slice = wave / HEADS;
+  const float mine = st.m[0];
+  arrive_all();  // every wavefront is done with the rows in LDS
+  ml[wave * kWave + lane] = f32x2{mine, *l};
+  arrive_all();
+  float top = kLowest, sum = 0.f;
+#pragma unroll
+  for (int s = 0; s < SLICES; ++s) top = fmaxf(top, ml[(s * HEADS + slot) * kWave + lane][0]);
+#pragma unroll
+  for (int s = 0; s < SLICES; ++s) {
+    const f32x2 other = ml[(s * HEADS + slot) * kWave + lane];
+    sum = fmaf(exp2_fast(other[0] - top), other[1], sum);
+  }
+  const float f = exp2_fast(mine - top);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[(wave * 32 + 8 * i + j) * kWave + lane] = st.acc[0][j][i] * f;
+  arrive_all();
+  constexpr int N = 32 / SLICES;
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    x[r] = 0.f;
+#pragma unroll
+    for (int s = 0; s < SLICES; ++s) x[r] += o[((s * HEADS + slot) * 32 + N * slice + r) * kWave + lane];
+  }
+  *m = top;
+  *l = sum;
+}
+
+// ---- the work-groups -------------------------------------------------------------------------
+
+// Work-group `index` of the line's. Few rows: HEADS slots of kv heads from head0 on, of which `heads` are heads, and
+// 8 / HEADS wavefronts to each, which take 32 keys of every step in turn. Neighbouring runs of MANY, whose tiles
+// read the same keys, go to one XCD (work-groups go to the 8 of them in turn).
+template <bool MANY, int T, int HEADS, int ROWS, int WAVES>
+__device__ __forceinline__ void attend_run(const Fp4AttnArgs& a, const Partials& part, int num_runs, int index, int head0,
+                                           int heads, lds_u8* lds) {
   constexpr int D = kHeadDim;
+  constexpr int kSlices = MANY ? 1 : WAVES / HEADS;
+  static_assert(MANY ? ROWS == 2 * kSub : ROWS == kSub * kSlices, "rows of a step");
+  typedef Stage<HEADS, ROWS> S;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = uniform(threadIdx.x / kWave);
   const int n = lane & 15, g = lane >> 4;
-  Line<MANY> line;
+  Line<MANY, ROWS> line;
   line.init(a, lane);
-  if (line.total == 0) return;
   const Cuts cuts = cuts_of(line.total, num_runs);
+  const bool recorder = (MANY || head0 == 0) && threadIdx.x == 0;  // writes what the merge has to know
+  if (index == 0 && recorder) *part.live = (int)cuts.runs;
+  if (line.total == 0) return;
   int run = index;
   if constexpr (MANY) {
     const int per_xcd = ((int)cuts.runs + 7) >> 3;
@@ -421,15 +686,30 @@ __device__ __forceinline__ void attend_run(const Fp4AttnArgs& a, const Partials&
   }
   if (run >= cuts.runs) return;
   const int64_t end = cuts.first(run + 1);
+  int4 split = make_int4(0, 0, 0, 0);
+  const int slot = MANY ? 0 : wave % HEADS, slice = MANY ? 0 : wave / HEADS;
+  const int lds0 = (int)(uintptr_t)lds;
+  Lanes<HEADS, ROWS> at;
+  at.init(slice * kSub, slot, lane);
   for (int64_t p = cuts.first(run); p < end;) {
     const Tile tile = line.at(a, p, lane);
-    const Seq seq = seq_of(a, tile.b);
+    const Seq seq = uniform_seq(a, tile.b);
     const int s0 = (int)(p - tile.start);
     const int s1 = (int)min((int64_t)tile.steps, end - tile.start);
     p = tile.start + s1;
-    const int head = MANY ? tile.head : head0 + wave;
+    const bool live = slot < heads;
+    const int head = MANY ? tile.head : head0 + min(slot, heads - 1);
     const int group = 1 << a.group_shift;
     const int row0 = MANY ? tile.j * (kManyCols >> a.group_shift) : 0;
+
+    // (the last piece's reads of LDS are over)
+    arrive_all();
+    Loader<HEADS, ROWS, WAVES> loader;
+    loader.init(a, a.block_table + (int64_t)tile.b * a.bt_stride, s0 * ROWS, seq.keys, MANY ? tile.head : head0,
+                MANY ? 1 : heads, wave, lane);
+    Cursor mine = loader.at;  // the wavefront's own keys
+    if constexpr (!MANY) mine.init(a, a.block_table + (int64_t)tile.b * a.bt_stride, s0 * ROWS + slice * kSub, seq.keys);
+    loader.issue(a, seq.keys, lds0);
 
     // The columns: their rows, their last keys, q.
     State<T> st;
@@ -440,7 +720,7 @@ __device__ __forceinline__ void attend_run(const Fp4AttnArgs& a, const Partials&
     for (int x = 0; x < T; ++x) {
       col[x] = (MANY ? wave * T * 16 : 0) + 16 * x + n;
       row[x] = row0 + (col[x] >> a.group_shift);
-      const bool real = row[x] < seq.rows;
+      const bool real = row[x] < seq.rows && live;
       last[x] = real ? min(seq.keys - 1, row[x] + seq.shift) : -1;
       if (real) {
         lowest = min(lowest, last[x]);
@@ -462,144 +742,131 @@ __device__ __forceinline__ void attend_run(const Fp4AttnArgs& a, const Partials&
     lowest = uniform(lowest);
     furthest = uniform(furthest);
 
-    Offsets o;
-    o.k = n * a.row_bytes + head * kFp4HeadBytes + 16 * g;
-    o.ks = n * a.row_bytes + a.num_kv_heads * kFp4HeadBytes + head * kFp4HeadScales + g;
+    for (int s = s0; s < s1; ++s) {
+      const int buf = (s - s0) & 1;
+      const lds_u8* stage = lds + buf * S::kBytes;
+      arrive_all();  // step s is there, and step s - 1 done with
+      if (s + 1 < s1) loader.issue(a, seq.keys, lds0 + (buf ^ 1) * S::kBytes);
+      const bool good = mine.good(a);
+      const auto take_half = [&](auto tile0) {
+        constexpr int kTile0 = decltype(tile0)::value;
+        const int t0 = s * ROWS + slice * kSub + 16 * kTile0;
+        if (t0 > furthest || !good) return;  // no column sees these keys
+        int rel[T];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      o.v[i] = (4 * g + i) * a.row_bytes + head * kFp4HeadBytes + 4 * n;
-      o.vs[i] = (4 * g + i) * a.row_bytes + a.num_kv_heads * kFp4HeadBytes + head * kFp4HeadScales + (n >> 2);
-    }
-    const int32_t* table = a.block_table + (int64_t)tile.b * a.bt_stride;
-    // Step s's rows in the caches; a table entry that is no block has none, and its keys are seen by nobody.
-    const uint8_t *kp, *vp;
-    int rows;
-    const auto page = [&](int s) {
-      const int t0 = s * kStep;
-      const int blk = uniform(table[t0 / a.block_size]);
-      const int64_t off = (int64_t)(t0 % a.block_size) * a.row_bytes;
-      const bool good = blk >= 0 && blk < a.num_blocks;
-      kp = a.k + (good ? blk * a.k_block + off : 0);
-      vp = a.v + (good ? blk * a.v_block + off : 0);
-      rows = good ? min(seq.keys - t0, kStep) : 0;
-    };
-
-    // (wavefronts of MANY whose columns see fewer keys than the tile's last end earlier)
-    const int stop = MANY ? min(s1, furthest / kStep + 1) : s1;
-    if (s0 < stop && furthest >= 0) {
-      Keys k;
-      Vals v;
-      page(s0);
-      load_keys(k, kp, rows, a.row_bytes, o);
-      load_vals(v, vp, rows, a.row_bytes, o);
-      for (int s = s0; s < stop; ++s) {
-        const int t0 = s * kStep;
-        const bool bad_page = rows == 0;
-        f32x4 sc[4][T];
-        scores<T>(sc, st, k);
-        if (s + 1 < stop) {
-          page(s + 1);
-          load_keys(k, kp, rows, a.row_bytes, o);
-        }
-        if (t0 + kStep - 1 > lowest || bad_page) {
-          int rel[T];
-#pragma unroll
-          for (int x = 0; x < T; ++x) {
-            rel[x] = bad_page ? -1 : last[x] - t0;
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (16 * t + 4 * g + i > rel[x]) sc[t][x][i] = -INFINITY;
-          }
-          if (any_nan(v)) nan_values<T>(st, v, rel, lane);
-        }
-        u32x4 pw[T][2];
-        weights<T>(pw, sc, st, a.scale_log2);
-        add_values<T>(st, pw, v);
-        if (s + 1 < stop) load_vals(v, vp, rows, a.row_bytes, o);
-      }
+        for (int x = 0; x < T; ++x) rel[x] = last[x] - t0;
+        take<kTile0>(st, stage, at, t0 + kSub - 1 > lowest, rel, a.scale_log2, lane);
+      };
+      take_half(std::integral_constant<int, 0>{});
+      if constexpr (MANY) take_half(std::integral_constant<int, 2>{});
+      mine.next(a, ROWS);
     }
 
     // A whole tile's output, or a partial result of a split one.
     const bool whole = s0 == 0 && s1 == tile.steps;
-    const int64_t slot = 2 * (int64_t)run + (s0 == 0 ? 1 : 0);
+    const int64_t slot_of = 2 * (int64_t)run + (s0 == 0 ? 1 : 0);
+    if (s0 == 0 && !whole)
+      split = make_int4(seq.q0 + row0, min((seq.rows - row0) << a.group_shift, part.cols),
+                        cuts.run_of(tile.start + tile.steps - 1) - run + 1, head);
 #pragma unroll
     for (int x = 0; x < T; ++x) {
-      const float l = quarters_sum(st.l[x]);
-      if (row[x] >= seq.rows) continue;
-      if (whole) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
-        uint16_t* out = a.out + (int64_t)(seq.q0 + row[x]) * a.out_stride + (head * group + (col[x] & (group - 1))) * D + 32 * g;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          u32x4 w;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(st.acc[x][2 * j][i] * inv, st.acc[x][2 * j + 1][i] * inv);
-          *reinterpret_cast<u32x4*>(out + 8 * i) = w;
-        }
+      constexpr int N = 32 / kSlices;
+      float v[N], m = st.m[x], l = quarters_sum(st.l[x]);
+      if constexpr (kSlices > 1) {
+        join_slices<kSlices, HEADS>(v, &m, &l, st, lds, wave, lane);
       } else {
-        const int64_t at = part.at(slot, MANY ? 0 : head, col[x]);
-        float* po = part.o + at * D + 32 * g;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          *reinterpret_cast<f32x4*>(po + 8 * i) = f32x4{st.acc[x][0][i], st.acc[x][1][i], st.acc[x][2][i], st.acc[x][3][i]};
-          *reinterpret_cast<f32x4*>(po + 8 * i + 4) = f32x4{st.acc[x][4][i], st.acc[x][5][i], st.acc[x][6][i], st.acc[x][7][i]};
-        }
-        if (g == 0) part.ml[at] = make_float2(st.m[x], l);
+        for (int r = 0; r < 32; ++r) v[r] = st.acc[x][r & 7][r >> 3];
+      }
+      if (row[x] >= seq.rows || !live) continue;
+      const int dim = 32 * g + N * slice;
+      if (whole) {
+        uint16_t* out = a.out + (int64_t)(seq.q0 + row[x]) * a.out_stride + (head * group + (col[x] & (group - 1))) * D + dim;
+        put_out<N>(out, v, l == 0.f ? 0.f : 1.f / l);  // no key seen: zeros
+      } else {
+        const int64_t at_part = part.at(slot_of, MANY ? 0 : head, col[x]);
+        put_part<N>(part.o + at_part * D + dim, v);
+        if (g == 0 && slice == 0) part.ml[at_part] = make_float2(m, l);
       }
     }
   }
+  if (recorder) part.split[run] = split;
 }
 
-__global__ __launch_bounds__(8 * kWave, 2) void attend_few_kernel(const Fp4AttnArgs a, const Partials part, int runs) {
-  attend_run<false, 1>(a, part, runs, blockIdx.x, blockIdx.y * (blockDim.x / kWave));
+template <int HEADS>
+__global__ __launch_bounds__(kFewWaves* kWave, 4) void attend_few_kernel(const Fp4AttnArgs a, const Partials part, int runs,
+                                                                         int heads) {
+  constexpr int kRows = kSub * kFewWaves / HEADS;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * Stage<HEADS, kRows>::kBytes];
+  attend_run<false, 1, HEADS, kRows, kFewWaves>(a, part, runs, blockIdx.x, blockIdx.y * heads, heads, (lds_u8*)lds);
 }
 
 __global__ __launch_bounds__(kManyWaves* kWave, 2) void attend_many_kernel(const Fp4AttnArgs a, const Partials part, int runs) {
-  attend_run<true, kManyTiles>(a, part, runs, blockIdx.x, 0);
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * Stage<1, kManyStep>::kBytes];
+  attend_run<true, kManyTiles, 1, kManyStep, kManyWaves>(a, part, runs, blockIdx.x, 0, 1, (lds_u8*)lds);
 }
 
-// Work-group i: the tile that the cut between runs i and i + 1 splits, if that is its first cut. Its partial results
-// are run i's second slot and the first ones of the runs after it. 32 threads a column, 4 dimensions each.
+// Work-group (run, y): the tile that begins in the run and goes on, if there is one; its partial results are the
+// run's second slot and the first ones of the runs after it. 32 threads take a column (of a kv head), 4 dimensions
+// each, and `slices` of them share a column's partial results, which meet in LDS.
 constexpr int kMergeThreads = 256;
+constexpr int kMergeTeams = kMergeThreads / 32;
 template <bool MANY>
-__global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Fp4AttnArgs a, const Partials part, int runs) {
+__global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Fp4AttnArgs a, const Partials part, int slices) {
   constexpr int D = kHeadDim;
-  const int lane = threadIdx.x & (kWave - 1);
-  Line<MANY> line;
-  line.init(a, lane);
-  if (line.total == 0) return;
-  const Cuts cuts = cuts_of(line.total, runs);
-  const int i = blockIdx.x;
-  if (i + 1 >= cuts.runs) return;
-  const int64_t cut = cuts.first(i + 1);
-  const Tile tile = line.at(a, cut, lane);
-  if (tile.start == cut || tile.start < cuts.first(i)) return;
-  const Seq seq = seq_of(a, tile.b);
-  const int pieces = cuts.run_of(tile.start + tile.steps - 1) - i + 1;
-  const int head = MANY ? tile.head : (int)blockIdx.y;
+  __shared__ f32x4 acc_of[kMergeTeams][32];
+  __shared__ float2 ml_of[kMergeTeams];
+  const int run = blockIdx.x;
+  const int4 split = part.split[run];
+  if (run >= *part.live || split.z == 0) return;
+  const int cols = split.y, pieces = split.z;
+  const int pairs = MANY ? cols : cols * a.num_kv_heads;
   const int group = 1 << a.group_shift;
-  const int row0 = MANY ? tile.j * (kManyCols >> a.group_shift) : 0;
-  const int cols = min((seq.rows - row0) << a.group_shift, part.cols);
-  const int t = threadIdx.x & 31;
-  for (int col = threadIdx.x >> 5; col < cols; col += kMergeThreads / 32) {
-    const auto at = [&](int j) { return part.at(2 * (int64_t)(i + j) + (j == 0 ? 1 : 0), MANY ? 0 : head, col); };
-    float m = kLowest;
-    for (int j = t; j < pieces; j += 32) m = fmaxf(m, part.ml[at(j)].x);
-#pragma unroll
-    for (int sh = 1; sh < 32; sh *= 2) m = fmaxf(m, __shfl_xor(m, sh, 32));
-    float l = 0.f;
+  const int t = threadIdx.x & 31, team = threadIdx.x >> 5;
+  const int slice = team & (slices - 1);
+  const int per_pass = kMergeTeams / slices;
+  for (int base = blockIdx.y * per_pass; base < pairs; base += gridDim.y * per_pass) {
+    const int pair = base + team / slices;
+    const int head = MANY ? split.w : pair / cols;
+    const int col = MANY ? pair : pair - head * cols;
+    float m = kLowest, l = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int j = 0; j < pieces; ++j) {
-      const float2 ml = part.ml[at(j)];
-      const float w = exp2_fast(ml.x - m);
-      l = fmaf(w, ml.y, l);
-      acc += w * *reinterpret_cast<const f32x4*>(part.o + at(j) * D + 4 * t);
+    if (pair < pairs) {
+      const auto at = [&](int j) { return part.at(2 * (int64_t)(run + j) + (j == 0 ? 1 : 0), MANY ? 0 : head, col); };
+      for (int j = slice + t * slices; j < pieces; j += 32 * slices) m = fmaxf(m, part.ml[at(j)].x);
+#pragma unroll
+      for (int sh = 1; sh < 32; sh *= 2) m = fmaxf(m, __shfl_xor(m, sh, 32));
+#pragma unroll 4
+      for (int j = slice; j < pieces; j += slices) {
+        const float2 ml = part.ml[at(j)];
+        const float w = exp2_fast(ml.x - m);
+        l = fmaf(w, ml.y, l);
+        acc += w * *reinterpret_cast<const f32x4*>(part.o + at(j) * D + 4 * t);
+      }
     }
-    const int row = row0 + (col >> a.group_shift);
+    if (slices > 1) {
+      acc_of[team][t] = acc;
+      if (t == 0) ml_of[team] = make_float2(m, l);
+      __syncthreads();
+      if (slice == 0 && pair < pairs) {
+        float top = m;
+        for (int i = 1; i < slices; ++i) top = fmaxf(top, ml_of[team + i].x);
+        const float f = exp2_fast(m - top);
+        l *= f;
+        acc *= f;
+        for (int i = 1; i < slices; ++i) {
+          const float2 ml = ml_of[team + i];
+          const float w = exp2_fast(ml.x - top);
+          l = fmaf(w, ml.y, l);
+          acc += w * acc_of[team + i][t];
+        }
+      }
+      __syncthreads();
+    }
+    if (slice != 0 || pair >= pairs) continue;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    uint16_t* out = a.out + (int64_t)(seq.q0 + row) * a.out_stride + (head * group + (col & (group - 1))) * D + 4 * t;
+    const int64_t row = split.x + (col >> a.group_shift);
+    uint16_t* out = a.out + row * a.out_stride + (head * group + (col & (group - 1))) * D + 4 * t;
     *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
   }
 }
@@ -607,15 +874,31 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Fp4AttnArgs 
 template <bool MANY>
 Partials partials_of(const Fp4AttnArgs& a, const Fp4AttnPlan& p, char* ws) {
   const size_t rows = partial_rows<MANY>(p, a.num_kv_heads);
+  const int runs = MANY ? p.many_runs : p.few_runs;
   Partials r;
-  r.o = reinterpret_cast<float*>(ws);
-  r.ml = reinterpret_cast<float2*>(ws + rows * kHeadDim * sizeof(float));
+  r.split = reinterpret_cast<int4*>(ws);
+  r.live = reinterpret_cast<int32_t*>(r.split + runs);
+  r.o = reinterpret_cast<float*>(ws + ((size_t)runs + 1) * sizeof(int4));
+  r.ml = reinterpret_cast<float2*>(r.o + rows * kHeadDim);
   r.heads = MANY ? 1 : a.num_kv_heads;
   r.cols = MANY ? kManyCols : p.few_cols;
   return r;
 }
 
-size_t partial_bytes(size_t rows) { return (rows * (kHeadDim * sizeof(float) + sizeof(float2)) + 255) / 256 * 256; }
+size_t partial_bytes(size_t rows, size_t runs) {
+  return ((runs + 1) * sizeof(int4) + rows * (kHeadDim * sizeof(float) + sizeof(float2)) + 255) / 256 * 256;
+}
+
+// Teams of 32 threads for one column of a merge: one for every four of the partial results that a tile has if the
+// call has as many tiles as its bounds say, 8 at most.
+int merge_slices(int runs, int64_t tiles) {
+  int slices = 1;
+  while (slices < kMergeTeams && tiles * slices * 4 < runs) slices *= 2;
+  return slices;
+}
+
+// Work-groups that share a split tile's passes: most runs have no such tile, and empty work-groups cost their launch.
+int merge_groups(int runs, int passes) { return std::max(1, std::min(passes, 8192 / runs)); }
 
 }  // namespace
 
@@ -623,20 +906,23 @@ Fp4AttnPlan fp4_attention_plan(int32_t num_seqs, int32_t num_heads, int32_t num_
                                int32_t max_seqlen_k, int64_t num_rows) {
   Fp4AttnPlan p{};
   const int group = num_heads / num_kv_heads;
-  const int64_t steps = ((int64_t)max_seqlen_k + kStep - 1) / kStep;
-  // a work-group has as many kv heads as divide them evenly, 8 at most
-  p.few_heads = std::min(num_kv_heads, 8);
+  // a work-group has as many kv heads as divide them evenly, 8 at most, in 1, 2, 4 or 8 slots
+  p.few_heads = std::min(num_kv_heads, kFewWaves);
   while (num_kv_heads % p.few_heads) --p.few_heads;
+  p.few_slots = 1;
+  while (p.few_slots < p.few_heads) p.few_slots *= 2;
+  const int64_t few_steps = ((int64_t)max_seqlen_k * p.few_slots + kSub * kFewWaves - 1) / (kSub * kFewWaves);
+  p.too_long = num_seqs * few_steps > INT32_MAX;
   p.few_cols = (int)std::min<int64_t>(16, (int64_t)max_seqlen_q * group);
-  const int64_t waves = 4096;
-  p.few_runs = (int)std::min<int64_t>(waves / p.few_heads, num_seqs * steps);
-  p.too_long = num_seqs * steps > INT32_MAX;
-  p.few_bytes = partial_bytes(partial_rows<false>(p, num_kv_heads));
+  p.few_runs = (int)std::min<int64_t>(512, num_seqs * few_steps);
+  p.few_bytes = partial_bytes(partial_rows<false>(p, num_kv_heads), p.few_runs);
   if ((int64_t)max_seqlen_q * group > 16) {
+    const int64_t steps = ((int64_t)max_seqlen_k + kManyStep - 1) / kManyStep;
     const int64_t tiles = num_rows * group / kManyCols + num_seqs;  // of a kv head
     p.too_long |= tiles * steps > INT32_MAX;
+    p.many_tiles = std::max<int64_t>(1, num_rows * group / kManyCols) * num_kv_heads;
     p.many_runs = 512;
-    p.many_bytes = partial_bytes(partial_rows<true>(p, num_kv_heads));
+    p.many_bytes = partial_bytes(partial_rows<true>(p, num_kv_heads), p.many_runs);
   }
   return p;
 }
@@ -644,21 +930,30 @@ Fp4AttnPlan fp4_attention_plan(int32_t num_seqs, int32_t num_heads, int32_t num_
 hipError_t launch_fp4_attention(const Fp4AttnArgs& a, const Fp4AttnPlan& p, hipStream_t stream) {
   char* ws = static_cast<char*>(a.workspace);
   const Partials few = partials_of<false>(a, p, ws);
-  const int head_groups = a.num_kv_heads / p.few_heads;
-  hipLaunchKernelGGL(attend_few_kernel, dim3((unsigned)p.few_runs, (unsigned)head_groups),
-                     dim3((unsigned)(p.few_heads * kWave)), 0, stream, a, few, p.few_runs);
+  const dim3 grid((unsigned)p.few_runs, (unsigned)(a.num_kv_heads / p.few_heads)), block(kFewWaves * kWave);
+  switch (p.few_slots) {
+    case 1: hipLaunchKernelGGL(attend_few_kernel<1>, grid, block, 0, stream, a, few, p.few_runs, p.few_heads); break;
+    case 2: hipLaunchKernelGGL(attend_few_kernel<2>, grid, block, 0, stream, a, few, p.few_runs, p.few_heads); break;
+    case 4: hipLaunchKernelGGL(attend_few_kernel<4>, grid, block, 0, stream, a, few, p.few_runs, p.few_heads); break;
+    default: hipLaunchKernelGGL(attend_few_kernel<8>, grid, block, 0, stream, a, few, p.few_runs, p.few_heads); break;
+  }
   if (hipError_t err = hipGetLastError()) return err;
-  if (p.few_runs > 1)
-    hipLaunchKernelGGL((merge_kernel<false>), dim3((unsigned)(p.few_runs - 1), (unsigned)a.num_kv_heads),
-                       dim3(kMergeThreads), 0, stream, a, few, p.few_runs);
+  if (p.few_runs > 1) {
+    const int slices = merge_slices(p.few_runs, a.num_seqs), per_pass = kMergeTeams / slices;
+    const int passes = (a.num_kv_heads * p.few_cols + per_pass - 1) / per_pass;
+    hipLaunchKernelGGL((merge_kernel<false>), dim3((unsigned)(p.few_runs - 1), (unsigned)merge_groups(p.few_runs, passes)),
+                       dim3(kMergeThreads), 0, stream, a, few, slices);
+  }
   if (hipError_t err = hipGetLastError()) return err;
   if (p.many_runs) {
     const Partials many = partials_of<true>(a, p, ws + p.few_bytes);
     hipLaunchKernelGGL(attend_many_kernel, dim3((unsigned)p.many_runs), dim3(kManyWaves * kWave), 0, stream, a, many,
                        p.many_runs);
     if (hipError_t err = hipGetLastError()) return err;
-    hipLaunchKernelGGL((merge_kernel<true>), dim3((unsigned)(p.many_runs - 1)), dim3(kMergeThreads), 0, stream, a, many,
-                       p.many_runs);
+    const int slices = merge_slices(p.many_runs, p.many_tiles);
+    const int passes = kManyCols * slices / kMergeTeams;
+    hipLaunchKernelGGL((merge_kernel<true>), dim3((unsigned)(p.many_runs - 1), (unsigned)merge_groups(p.many_runs, passes)),
+                       dim3(kMergeThreads), 0, stream, a, many, slices);
   }
   return hipGetLastError();
 }
