@@ -40,10 +40,12 @@ namespace pk {
 namespace {
 
 constexpr int kFewWaves = 8;          // wavefronts of a work-group over sequences of few rows
-constexpr int kManyWaves = 4;         // ... of more rows
+constexpr int kFewRing = 3;           // steps in LDS
+constexpr int kManyWaves = 8;         // ... of more rows
 constexpr int kManyTiles = 2;         // tiles of 16 columns a wavefront of the latter holds
 constexpr int kManyCols = kManyWaves * kManyTiles * 16;
 constexpr int kManyStep = 64;         // keys of its step
+constexpr int kManyRing = 4;          // steps of 4-bit rows in LDS
 constexpr int kSub = 32;              // keys a wavefront takes at once
 constexpr int kSlots = 8;             // sequences a lane keeps the steps of
 constexpr int kChunk = kSlots * kWave;
@@ -54,6 +56,9 @@ typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 frag;
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 typedef __attribute__((address_space(3))) uint32_t lds_u32;
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
 typedef __attribute__((address_space(3))) float lds_f32;
 typedef __attribute__((address_space(3))) f32x2 lds_f32x2;
 
@@ -289,6 +294,17 @@ __device__ __forceinline__ void arrive_all() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// Waits until at most N of this wavefront's loads are in flight (and arrive_but: for the other wavefronts).
+template <int N>
+__device__ __forceinline__ void arrive_but() {
+  asm volatile("s_waitcnt vmcnt(%c0) lgkmcnt(0)\n\ts_barrier" : : "i"(N) : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void wait_but() {
+  asm volatile("s_waitcnt vmcnt(%c0)" : : "i"(N) : "memory");
+}
+
 // 16 or 4 bytes per active lane from base + off to lds + 16 or 4 lane, in flight until arrive_all.
 __device__ __forceinline__ void stage16(const uint8_t* base, int off, int lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
@@ -342,21 +358,22 @@ struct Cursor {
   }
 };
 
-// One wavefront's share of a step's loads. Few rows (256 slots of a head and row, 8 wavefronts): of each cache two KiB
-// of values, of one cache a quarter of the scales. More rows (64 rows of one head, 4 wavefronts): one KiB of
-// each cache's values, the first two wavefronts a cache's scales.
-template <int HEADS, int ROWS, int WAVES>
+// One wavefront's share of a step's loads: of each cache two KiB of values, of one cache a quarter of the scales
+// (256 slots of a head and row, 8 wavefronts).
+template <int HEADS, int ROWS>
 struct Loader {
   typedef Stage<HEADS, ROWS> S;
-  static constexpr int kJobs = ROWS * HEADS / 16 / WAVES;   // KiB of values of a cache
-  static constexpr int kScaleJobs = ROWS * HEADS / 64;      // 256 bytes of scales of a cache
-  static_assert(kJobs * WAVES * 16 == ROWS * HEADS && 2 * kScaleJobs <= WAVES, "loads divide among the wavefronts");
-  int off[kJobs], row[kJobs];  // the lane's bytes and row after the cursor; no row where its slot is no head
-  int scale_off, scale_row;
+  static constexpr int kJobs = ROWS * HEADS / 16 / kFewWaves;  // KiB of values of a cache
+  static constexpr int kScaleJobs = ROWS * HEADS / 64;         // 256 bytes of scales of a cache
+  static_assert(kJobs * kFewWaves * 16 == ROWS * HEADS && 2 * kScaleJobs == kFewWaves, "loads divide among the wavefronts");
+  static constexpr int kLoads = 2 * kJobs + 1;                 // of a wavefront and step
+  int row[kJobs], col[kJobs];  // the lane's row after the cursor, and its place in the row
+  int scale_row, scale_col;
   int lds, scale_lds;
-  bool has_scales, scales_of_v;
+  bool scales_of_v;
   Cursor at, scale_at;
 
+  // (a slot that is no head reads the last one's bytes, which nobody looks at)
   __device__ __forceinline__ void init(const Fp4AttnArgs& a, const int32_t* table, int t0, int keys, int head0, int heads,
                                        int wave, int lane) {
     const int first = wave * kJobs * 64 / (4 * HEADS);  // the first row
@@ -365,41 +382,37 @@ struct Loader {
       const int slot = (wave * kJobs + j) * 64 + lane;
       const int r = slot / (4 * HEADS), c = (slot % (4 * HEADS)) ^ swizzle<HEADS>(r);
       row[j] = r - (first & ~31);
-      off[j] = row[j] * a.row_bytes + (head0 + (c >> 2)) * kFp4HeadBytes + 16 * (c & 3);
-      if ((c >> 2) >= heads) row[j] = INT32_MAX;
+      col[j] = (head0 + min(c >> 2, heads - 1)) * kFp4HeadBytes + 16 * (c & 3);
     }
     lds = wave * kJobs * 1024;
-    const int part = wave % (WAVES / 2 < kScaleJobs ? WAVES / 2 : kScaleJobs);
-    has_scales = wave < 2 * kScaleJobs;
+    const int part = wave % kScaleJobs;
     scales_of_v = wave >= kScaleJobs;
     const int s = part * 64 + lane, r = s / HEADS, h = s % HEADS;
     const int scale_first = part * 64 / HEADS & ~31;
     scale_row = r - scale_first;
-    scale_off = scale_row * a.row_bytes + a.num_kv_heads * kFp4HeadBytes + (head0 + h) * kFp4HeadScales;
-    if (h >= heads) scale_row = INT32_MAX;
+    scale_col = a.num_kv_heads * kFp4HeadBytes + (head0 + min(h, heads - 1)) * kFp4HeadScales;
     scale_lds = (scales_of_v ? S::kCache : 0) + S::kValues + part * 256;
     at.init(a, table, t0 + (first & ~31), keys);
     scale_at.init(a, table, t0 + scale_first, keys);
   }
 
-  // The next step's rows into a stage of LDS. (A row that is no key is not read: its place keeps what it has.)
+  // The next step's rows into a stage of LDS. A row that is no key reads the last one that is (or, where there is
+  // none, the cache's first row): the count of loads in flight is the same in every step.
   __device__ __forceinline__ void issue(const Fp4AttnArgs& a, int keys, int stage) {
-    const int rows = at.rows(a, keys);
+    const int last = max(at.rows(a, keys), 1) - 1;
     const uint8_t* k = uniform_ptr(at.at(a, a.k, a.k_block));
     const uint8_t* v = uniform_ptr(at.at(a, a.v, a.v_block));
 #pragma unroll
-    for (int j = 0; j < kJobs; ++j)
-      if (row[j] < rows) {
-        stage16(k, off[j], stage + lds + 1024 * j);
-        stage16(v, off[j], stage + S::kCache + lds + 1024 * j);
-      }
-    at.next(a, ROWS);
-    if (has_scales) {
-      const int scale_rows = scale_at.rows(a, keys);
-      const uint8_t* c = uniform_ptr(scales_of_v ? scale_at.at(a, a.v, a.v_block) : scale_at.at(a, a.k, a.k_block));
-      if (scale_row < scale_rows) stage4(c, scale_off, stage + scale_lds);
-      scale_at.next(a, ROWS);
+    for (int j = 0; j < kJobs; ++j) {
+      const int off = min(row[j], last) * a.row_bytes + col[j];
+      stage16(k, off, uniform(stage + lds + 1024 * j));
+      stage16(v, off, uniform(stage + S::kCache + lds + 1024 * j));
     }
+    at.next(a, ROWS);
+    const int scale_last = max(scale_at.rows(a, keys), 1) - 1;
+    const uint8_t* c = uniform_ptr(scales_of_v ? scale_at.at(a, a.v, a.v_block) : scale_at.at(a, a.k, a.k_block));
+    stage4(c, min(scale_row, scale_last) * a.row_bytes + scale_col, uniform(stage + scale_lds));
+    scale_at.next(a, ROWS);
   }
 };
 
@@ -439,27 +452,25 @@ struct Lanes {
     }
     vs = S::kCache + S::kValues + ((first + row_of<HEADS>(4 * g)) * HEADS + slot) * 4 + (n >> 2);
   }
-  // Rows 16 tile0 on of the wavefront's.
-  template <int TILE0>
   __device__ __forceinline__ void values(Vals& x, const lds_u8* stage) const {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x.d[t][i] = *(const lds_u32*)(stage + v[i] + (TILE0 + t) * kTile);
-        x.s[t][i] = *(const lds_u8*)(stage + vs + (TILE0 + t) * kScaleTile + row_of<HEADS>(i) * HEADS * 4);
+        x.d[t][i] = *(const lds_u32*)(stage + v[i] + t * kTile);
+        x.s[t][i] = *(const lds_u8*)(stage + vs + t * kScaleTile + row_of<HEADS>(i) * HEADS * 4);
       }
   }
 };
 
 // S^T of two tiles of 16 keys.
-template <int TILE0, int T, int HEADS, int ROWS>
+template <int T, int HEADS, int ROWS>
 __device__ __forceinline__ void scores(f32x4 (&s)[2][T], const State<T>& st, const lds_u8* stage,
                                        const Lanes<HEADS, ROWS>& at) {
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const u32x4 d = *(const lds_u32x4*)(stage + at.k + (TILE0 + t) * at.kTile);
-    const float scale = fp4_scale(*(const lds_u8*)(stage + at.ks + (TILE0 + t) * at.kScaleTile));
+    const u32x4 d = *(const lds_u32x4*)(stage + at.k + t * at.kTile);
+    const float scale = fp4_scale(*(const lds_u8*)(stage + at.ks + t * at.kScaleTile));
 #pragma unroll
     for (int x = 0; x < T; ++x) s[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -572,13 +583,12 @@ __device__ __forceinline__ void nan_values(State<T>& st, Vals& v, const int (&re
     }
 }
 
-// 32 keys of a stage, from tile TILE0 of the wavefront's on. rel: the last of them that a column sees, where some
-// column does not see all.
-template <int TILE0, int T, int HEADS, int ROWS>
+// 32 keys of a stage. rel: the last of them that a column sees, where some column does not see all.
+template <int T, int HEADS, int ROWS>
 __device__ __forceinline__ void take(State<T>& st, const lds_u8* stage, const Lanes<HEADS, ROWS>& at, bool masked,
                                      const int (&rel)[T], float c2, int lane) {
   f32x4 s[2][T];
-  scores<TILE0>(s, st, stage, at);
+  scores(s, st, stage, at);
   if (masked) {
 #pragma unroll
     for (int x = 0; x < T; ++x)
@@ -589,12 +599,33 @@ __device__ __forceinline__ void take(State<T>& st, const lds_u8* stage, const La
           if (16 * t + row_of<HEADS>(4 * (lane >> 4) + i) > rel[x]) s[t][x][i] = -INFINITY;
   }
   Vals v;
-  at.template values<TILE0>(v, stage);
+  at.values(v, stage);
   u32x4 p[T];
   weights<T>(p, s, st, c2);
   if (masked) nan_values<T, HEADS>(st, v, rel, lane);
   add_values<T>(st, p, v);
 }
+
+// The 16 columns of a wavefront over few rows, through LDS like the keys (4 KiB a wavefront, where the last stage of
+// the ring will be): loads into registers would be waited for together with every row that is in flight. Columns
+// past the last row hold the last row's q; nobody looks at what comes of them.
+struct Queries {
+  __device__ __forceinline__ void issue(const Fp4AttnArgs& a, const Seq& seq, int head, int wave, int lane, int lds) const {
+    const int last = (seq.rows << a.group_shift) - 1, group = 1 << a.group_shift;
+    const uint8_t* q = uniform_ptr(reinterpret_cast<const uint8_t*>(a.q + seq.q0 * a.q_stride + (int64_t)head * group * kHeadDim));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int col = 4 * i + (lane >> 4), real = min(col, last);
+      const int off = (int)((real >> a.group_shift) * a.q_stride + (real & (group - 1)) * kHeadDim) * 2 + 16 * ((lane ^ col) & 15);
+      stage16(q, off, uniform(lds + wave * 4096 + 1024 * i));
+    }
+  }
+  __device__ __forceinline__ void read(u32x4 (&q)[4], const lds_u8* lds, int wave, int lane) const {
+    const int n = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) q[c] = *(const lds_u32x4*)(lds + wave * 4096 + n * 256 + (((4 * g + c) ^ n) * 16));
+  }
+};
 
 // ---- results ---------------------------------------------------------------------------------
 
@@ -659,80 +690,80 @@ __device__ __forceinline__ void join_slices(float (&x)[32 / SLICES], float* m, f
 
 // ---- the work-groups -------------------------------------------------------------------------
 
-// Work-group `index` of the line's. Few rows: HEADS slots of kv heads from head0 on, of which `heads` are heads, and
-// 8 / HEADS wavefronts to each, which take 32 keys of every step in turn. Neighbouring runs of MANY, whose tiles
-// read the same keys, go to one XCD (work-groups go to the 8 of them in turn).
-template <bool MANY, int T, int HEADS, int ROWS, int WAVES>
-__device__ __forceinline__ void attend_run(const Fp4AttnArgs& a, const Partials& part, int num_runs, int index, int head0,
-                                           int heads, lds_u8* lds) {
-  constexpr int D = kHeadDim;
-  constexpr int kSlices = MANY ? 1 : WAVES / HEADS;
-  static_assert(MANY ? ROWS == 2 * kSub : ROWS == kSub * kSlices, "rows of a step");
-  typedef Stage<HEADS, ROWS> S;
-  const int lane = threadIdx.x & (kWave - 1);
-  const int wave = uniform(threadIdx.x / kWave);
-  const int n = lane & 15, g = lane >> 4;
-  Line<MANY, ROWS> line;
-  line.init(a, lane);
-  const Cuts cuts = cuts_of(line.total, num_runs);
-  const bool recorder = (MANY || head0 == 0) && threadIdx.x == 0;  // writes what the merge has to know
-  if (index == 0 && recorder) *part.live = (int)cuts.runs;
-  if (line.total == 0) return;
-  int run = index;
-  if constexpr (MANY) {
-    const int per_xcd = ((int)cuts.runs + 7) >> 3;
-    if ((index >> 3) >= per_xcd) return;
-    run = (index & 7) * per_xcd + (index >> 3);
+// A work-group's part of the line, and what the merge has to know of it.
+template <bool MANY, int STEP>
+struct Run {
+  Line<MANY, STEP> line;
+  Cuts cuts;
+  int run;
+  int64_t p, end;         // the next step, the one after the last
+  int4 split;
+  Tile tile;
+  Seq seq;
+  int s0, s1;             // the steps of the tile that are this run's
+  bool whole;
+  int row0;
+
+  // False if there is nothing to do. Neighbouring runs of MANY, whose tiles read the same keys, go to one XCD
+  // (work-groups go to the 8 of them in turn).
+  __device__ __forceinline__ bool init(const Fp4AttnArgs& a, const Partials& part, int num_runs, int index, bool recorder,
+                                       int lane) {
+    line.init(a, lane);
+    cuts = cuts_of(line.total, num_runs);
+    if (index == 0 && recorder) *part.live = (int)cuts.runs;
+    if (line.total == 0) return false;
+    run = index;
+    if constexpr (MANY) {
+      const int per_xcd = ((int)cuts.runs + 7) >> 3;
+      if ((index >> 3) >= per_xcd) return false;
+      run = (index & 7) * per_xcd + (index >> 3);
+    }
+    if (run >= cuts.runs) return false;
+    p = cuts.first(run);
+    end = cuts.first(run + 1);
+    split = make_int4(0, 0, 0, 0);
+    return true;
   }
-  if (run >= cuts.runs) return;
-  const int64_t end = cuts.first(run + 1);
-  int4 split = make_int4(0, 0, 0, 0);
-  const int slot = MANY ? 0 : wave % HEADS, slice = MANY ? 0 : wave / HEADS;
-  const int lds0 = (int)(uintptr_t)lds;
-  Lanes<HEADS, ROWS> at;
-  at.init(slice * kSub, slot, lane);
-  for (int64_t p = cuts.first(run); p < end;) {
-    const Tile tile = line.at(a, p, lane);
-    const Seq seq = uniform_seq(a, tile.b);
-    const int s0 = (int)(p - tile.start);
-    const int s1 = (int)min((int64_t)tile.steps, end - tile.start);
+  __device__ __forceinline__ bool next(const Fp4AttnArgs& a, const Partials& part, int lane) {
+    if (p >= end) return false;
+    tile = line.at(a, p, lane);
+    seq = uniform_seq(a, tile.b);
+    s0 = (int)(p - tile.start);
+    s1 = (int)min((int64_t)tile.steps, end - tile.start);
     p = tile.start + s1;
-    const bool live = slot < heads;
-    const int head = MANY ? tile.head : head0 + min(slot, heads - 1);
-    const int group = 1 << a.group_shift;
-    const int row0 = MANY ? tile.j * (kManyCols >> a.group_shift) : 0;
+    whole = s0 == 0 && s1 == tile.steps;
+    row0 = MANY ? tile.j * (kManyCols >> a.group_shift) : 0;
+    if (s0 == 0 && !whole)
+      split = make_int4(seq.q0 + row0, min((seq.rows - row0) << a.group_shift, part.cols),
+                        cuts.run_of(tile.start + tile.steps - 1) - run + 1, tile.head);
+    return true;
+  }
+  __device__ __forceinline__ int64_t slot() const { return 2 * (int64_t)run + (s0 == 0 ? 1 : 0); }
+};
 
-    // (the last piece's reads of LDS are over)
-    arrive_all();
-    Loader<HEADS, ROWS, WAVES> loader;
-    loader.init(a, a.block_table + (int64_t)tile.b * a.bt_stride, s0 * ROWS, seq.keys, MANY ? tile.head : head0,
-                MANY ? 1 : heads, wave, lane);
-    Cursor mine = loader.at;  // the wavefront's own keys
-    if constexpr (!MANY) mine.init(a, a.block_table + (int64_t)tile.b * a.bt_stride, s0 * ROWS + slice * kSub, seq.keys);
-    loader.issue(a, seq.keys, lds0);
+// A lane's columns: their rows and the last keys that they see.
+template <int T>
+struct Columns {
+  int row[T], head[T], last[T];  // row of the sequence, query head
+  bool real[T];
+  int lowest;                    // the last key that every column sees
+  int furthest;                  // the last key that some column sees
 
-    // The columns: their rows, their last keys, q.
-    State<T> st;
-    int col[T], row[T], last[T];
-    int lowest = a.max_seqlen_k;  // the last key that every column sees
-    int furthest = -1;            // the last key that some column sees
+  __device__ __forceinline__ void init(const Fp4AttnArgs& a, const Seq& seq, int row0, int kv_head, int first, bool live,
+                                       int n) {
+    lowest = a.max_seqlen_k;
+    furthest = -1;
 #pragma unroll
     for (int x = 0; x < T; ++x) {
-      col[x] = (MANY ? wave * T * 16 : 0) + 16 * x + n;
-      row[x] = row0 + (col[x] >> a.group_shift);
-      const bool real = row[x] < seq.rows && live;
-      last[x] = real ? min(seq.keys - 1, row[x] + seq.shift) : -1;
-      if (real) {
+      const int col = first + 16 * x + n;
+      row[x] = row0 + (col >> a.group_shift);
+      head[x] = (kv_head << a.group_shift) + (col & ((1 << a.group_shift) - 1));
+      real[x] = row[x] < seq.rows && live;
+      last[x] = real[x] ? min(seq.keys - 1, row[x] + seq.shift) : -1;
+      if (real[x]) {
         lowest = min(lowest, last[x]);
         furthest = max(furthest, last[x]);
       }
-      const uint16_t* q = a.q + (int64_t)(seq.q0 + row[x]) * a.q_stride + (head * group + (col[x] & (group - 1))) * D + 32 * g;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) st.q[x][c] = real ? *reinterpret_cast<const u32x4*>(q + 8 * c) : u32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) st.acc[x][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      st.m[x] = kLowest;
-      st.l[x] = 0.f;
     }
 #pragma unroll
     for (int sh = 1; sh < 16; sh *= 2) {
@@ -741,69 +772,336 @@ __device__ __forceinline__ void attend_run(const Fp4AttnArgs& a, const Partials&
     }
     lowest = uniform(lowest);
     furthest = uniform(furthest);
+  }
+};
 
-    for (int s = s0; s < s1; ++s) {
-      const int buf = (s - s0) & 1;
-      const lds_u8* stage = lds + buf * S::kBytes;
-      arrive_all();  // step s is there, and step s - 1 done with
-      if (s + 1 < s1) loader.issue(a, seq.keys, lds0 + (buf ^ 1) * S::kBytes);
-      const bool good = mine.good(a);
-      const auto take_half = [&](auto tile0) {
-        constexpr int kTile0 = decltype(tile0)::value;
-        const int t0 = s * ROWS + slice * kSub + 16 * kTile0;
-        if (t0 > furthest || !good) return;  // no column sees these keys
-        int rel[T];
+// Few rows: HEADS slots of kv heads from head0 on, of which `heads` are heads, and 8 / HEADS wavefronts to each, which
+// take 32 keys of every step in turn.
+template <int HEADS>
+__global__ __launch_bounds__(kFewWaves* kWave, 2) void attend_few_kernel(const Fp4AttnArgs a, const Partials part, int runs,
+                                                                         int heads) {
+  constexpr int D = kHeadDim;
+  constexpr int kSlices = kFewWaves / HEADS, ROWS = kSub * kSlices;
+  typedef Stage<HEADS, ROWS> S;
+  typedef Loader<HEADS, ROWS> L;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kFewRing * S::kBytes];
+  lds_u8* const lds = (lds_u8*)smem;
+  const int lds0 = (int)(uintptr_t)lds;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = uniform(threadIdx.x / kWave);
+  const int n = lane & 15, g = lane >> 4;
+  const int head0 = blockIdx.y * heads;
+  const bool recorder = head0 == 0 && threadIdx.x == 0;
+  Run<false, ROWS> run;
+  if (!run.init(a, part, runs, blockIdx.x, recorder, lane)) return;
+  const int slot = wave % HEADS, slice = wave / HEADS;
+  const bool live = slot < heads;
+  const int head = head0 + min(slot, heads - 1);
+  Queries queries;
+  Lanes<HEADS, ROWS> at;
+  at.init(slice * kSub, slot, lane);
+  while (run.next(a, part, lane)) {
+    const Seq seq = run.seq;
+    const int s0 = run.s0, s1 = run.s1;
+    arrive_all();  // (the last piece's reads of LDS are over)
+    const int32_t* table = a.block_table + (int64_t)run.tile.b * a.bt_stride;
+    L loader;
+    loader.init(a, table, s0 * ROWS, seq.keys, head0, heads, wave, lane);
+    Cursor mine;  // the wavefront's own keys
+    mine.init(a, table, s0 * ROWS + slice * kSub, seq.keys);
+    queries.issue(a, seq, head, wave, lane, lds0 + (kFewRing - 1) * S::kBytes);
 #pragma unroll
-        for (int x = 0; x < T; ++x) rel[x] = last[x] - t0;
-        take<kTile0>(st, stage, at, t0 + kSub - 1 > lowest, rel, a.scale_log2, lane);
-      };
-      take_half(std::integral_constant<int, 0>{});
-      if constexpr (MANY) take_half(std::integral_constant<int, 2>{});
+    for (int i = 0; i < kFewRing - 1; ++i)
+      if (i < s1 - s0) loader.issue(a, seq.keys, lds0 + i * S::kBytes);
+
+    Columns<1> cols;
+    cols.init(a, seq, 0, head, 0, live, n);
+    State<1> st;
+    st.m[0] = kLowest;
+    st.l[0] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) st.acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (s1 - s0 >= kFewRing - 1)
+      wait_but<(kFewRing - 1) * L::kLoads>();
+    else
+      wait_but<0>();
+    queries.read(st.q[0], lds + (kFewRing - 1) * S::kBytes, wave, lane);
+
+    int buf = 0, next_buf = kFewRing - 1;
+    for (int s = s0; s < s1; ++s) {
+      const lds_u8* stage = lds + buf * S::kBytes;
+      // step s is there, and step s - 1 done with
+      if (s + 1 < s1)
+        arrive_but<(kFewRing - 2) * L::kLoads>();
+      else
+        arrive_but<0>();
+      if (s + kFewRing - 1 < s1) loader.issue(a, seq.keys, lds0 + next_buf * S::kBytes);
+      buf = buf + 1 == kFewRing ? 0 : buf + 1;
+      next_buf = next_buf + 1 == kFewRing ? 0 : next_buf + 1;
+      const int t0 = s * ROWS + slice * kSub;
+      if (t0 <= cols.furthest && mine.good(a)) {  // (otherwise no column sees these keys)
+        const int rel[1] = {cols.last[0] - t0};
+        take(st, stage, at, t0 + kSub - 1 > cols.lowest, rel, a.scale_log2, lane);
+      }
       mine.next(a, ROWS);
     }
 
-    // A whole tile's output, or a partial result of a split one.
-    const bool whole = s0 == 0 && s1 == tile.steps;
-    const int64_t slot_of = 2 * (int64_t)run + (s0 == 0 ? 1 : 0);
-    if (s0 == 0 && !whole)
-      split = make_int4(seq.q0 + row0, min((seq.rows - row0) << a.group_shift, part.cols),
-                        cuts.run_of(tile.start + tile.steps - 1) - run + 1, head);
+    constexpr int N = 32 / kSlices;
+    float v[N], m = st.m[0], l = quarters_sum(st.l[0]);
+    if constexpr (kSlices > 1) {
+      join_slices<kSlices, HEADS>(v, &m, &l, st, lds, wave, lane);
+    } else {
 #pragma unroll
-    for (int x = 0; x < T; ++x) {
-      constexpr int N = 32 / kSlices;
-      float v[N], m = st.m[x], l = quarters_sum(st.l[x]);
-      if constexpr (kSlices > 1) {
-        join_slices<kSlices, HEADS>(v, &m, &l, st, lds, wave, lane);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 32; ++r) v[r] = st.acc[x][r & 7][r >> 3];
-      }
-      if (row[x] >= seq.rows || !live) continue;
-      const int dim = 32 * g + N * slice;
-      if (whole) {
-        uint16_t* out = a.out + (int64_t)(seq.q0 + row[x]) * a.out_stride + (head * group + (col[x] & (group - 1))) * D + dim;
-        put_out<N>(out, v, l == 0.f ? 0.f : 1.f / l);  // no key seen: zeros
-      } else {
-        const int64_t at_part = part.at(slot_of, MANY ? 0 : head, col[x]);
-        put_part<N>(part.o + at_part * D + dim, v);
-        if (g == 0 && slice == 0) part.ml[at_part] = make_float2(m, l);
-      }
+      for (int r = 0; r < 32; ++r) v[r] = st.acc[0][r & 7][r >> 3];
+    }
+    if (!cols.real[0]) continue;
+    const int dim = 32 * g + N * slice;
+    if (run.whole) {
+      uint16_t* out = a.out + (int64_t)(seq.q0 + cols.row[0]) * a.out_stride + cols.head[0] * D + dim;
+      put_out<N>(out, v, l == 0.f ? 0.f : 1.f / l);  // no key seen: zeros
+    } else {
+      const int64_t at_part = part.at(run.slot(), head, n);
+      put_part<N>(part.o + at_part * D + dim, v);
+      if (g == 0 && slice == 0) part.ml[at_part] = make_float2(m, l);
     }
   }
-  if (recorder) part.split[run] = split;
+  if (recorder) part.split[run.run] = run.split;
 }
 
-template <int HEADS>
-__global__ __launch_bounds__(kFewWaves* kWave, 4) void attend_few_kernel(const Fp4AttnArgs a, const Partials part, int runs,
-                                                                         int heads) {
-  constexpr int kRows = kSub * kFewWaves / HEADS;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * Stage<HEADS, kRows>::kBytes];
-  attend_run<false, 1, HEADS, kRows, kFewWaves>(a, part, runs, blockIdx.x, blockIdx.y * heads, heads, (lds_u8*)lds);
+// ---- more rows -------------------------------------------------------------------------------
+//
+// 256 columns of one kv head share its keys: a step's 64 rows come to LDS in 4 bits, the work-group's 512 threads
+// convert them to bf16 tiles once (16 values of K and of V each), and its 8 wavefronts read these. (With each
+// wavefront converting the rows for its own 32 columns the kernel was bound by its vector instructions, 282 for 32
+// keys and 32 columns, 106 of them conversions.) Step s + 1 is converted while step s is computed, steps s + 2 and
+// s + 3 are on their way.
+//
+// The tiles have 256-byte rows, 16 chunks of 16 bytes. K: chunk c of row r in slot c ^ (r & 15): the 16 lanes of a
+// quarter wavefront read one chunk of 16 rows. V: slot c ^ (2 r & 15): the transposing read takes four rows and 32
+// bytes a quarter, two quarters at once: 16 different slots. Dimensions are in their own order here: lane l holds
+// dimensions 32 c + 8 (l / 16) .. + 7 of key l % 16 (and of q), and dimension 16 j + l % 16 of V's four keys.
+struct ManyLds {
+  static constexpr int kRow = kHeadDim * 2;
+  static constexpr int kTile = kManyStep * kRow;                   // bf16 rows of a cache
+  static constexpr int kRawValues = kManyStep * kFp4HeadBytes;     // 4-bit rows of a cache
+  static constexpr int kRawScales = kManyStep * kFp4HeadScales;
+  static constexpr int kRawCache = kRawValues + kRawScales;
+  static constexpr int kRaw = 2 * kRawCache;
+  static constexpr int kTiles = kManyRing * kRaw;                  // after the ring: two pairs of tiles
+  static constexpr int kBytes = kTiles + 4 * kTile;
+  // A wavefront's loads of a step: 16 rows of one cache, 16 bytes a lane and four scales by its first 16 lanes.
+  static constexpr int kLoads = 2;
+};
+
+struct ManyLoader {
+  Cursor at;
+  const uint8_t* cache;
+  int64_t block;
+  int row, col, scale_row, scale_col, lds, scale_lds;
+
+  __device__ __forceinline__ void init(const Fp4AttnArgs& a, const int32_t* table, int t0, int keys, int head, int wave,
+                                       int lane) {
+    at.init(a, table, t0, keys);
+    const bool is_v = wave >= kManyWaves / 2;
+    cache = is_v ? a.v : a.k;
+    block = is_v ? a.v_block : a.k_block;
+    const int first = 16 * (wave % (kManyWaves / 2));
+    row = first + (lane >> 2);
+    col = head * kFp4HeadBytes + 16 * (lane & 3);
+    scale_row = first + (lane & 15);
+    scale_col = a.num_kv_heads * kFp4HeadBytes + head * kFp4HeadScales;
+    lds = (is_v ? ManyLds::kRawCache : 0) + first * kFp4HeadBytes;
+    scale_lds = (is_v ? ManyLds::kRawCache : 0) + ManyLds::kRawValues + first * kFp4HeadScales;
+  }
+  // (as Loader's)
+  __device__ __forceinline__ void issue(const Fp4AttnArgs& a, int keys, int stage, int lane) {
+    const int last = max(at.rows(a, keys), 1) - 1;
+    const uint8_t* c = uniform_ptr(at.at(a, cache, block));
+    stage16(c, min(row, last) * a.row_bytes + col, uniform(stage + lds));
+    if (lane < 16) stage4(c, min(scale_row, last) * a.row_bytes + scale_col, uniform(stage + scale_lds));
+    at.next(a, kManyStep);
+  }
+};
+
+// A step's rows from 4 bits to bf16: thread t has dimensions 16 (t % 8) .. of row t / 8. NaN blocks of V (and what
+// lies past the last key) become zeros, which reach no column; columns that see a NaN block get theirs from
+// many_nan. K's make their key's scores NaN.
+__device__ __forceinline__ void convert_rows(const lds_u8* raw, lds_u8* tiles, int thread) {
+  const int r = thread >> 3, part = thread & 7;
+  const lds_u8* rk = raw + r * kFp4HeadBytes + 8 * part;
+  const lds_u8* rs = raw + ManyLds::kRawValues + r * kFp4HeadScales + (part >> 1);
+  const u32x2 k = *(const lds_u32x2*)rk;
+  u32x2 v = *(const lds_u32x2*)(rk + ManyLds::kRawCache);
+  const uint32_t ks = *rs;
+  uint32_t vs = *(rs + ManyLds::kRawCache);
+  if (vs > kFp4MaxScale) {
+    vs = 0;
+    v = u32x2{0, 0};
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int c = 2 * part + i;
+    const uint4 wk = fp4_unpack8(k[i], fp4_scale(ks)), wv = fp4_unpack8(v[i], fp4_scale(vs));
+    *(lds_u32x4*)(tiles + r * ManyLds::kRow + (c ^ (r & 15)) * 16) = u32x4{wk.x, wk.y, wk.z, wk.w};
+    *(lds_u32x4*)(tiles + ManyLds::kTile + r * ManyLds::kRow + (c ^ (2 * r & 15)) * 16) = u32x4{wv.x, wv.y, wv.z, wv.w};
+  }
+}
+
+// acc[x][j][i]: dimension 16 j + 4 (l / 16) + i. A column that sees a row of the step with NaN blocks of V gets NaN in
+// their dimensions. rel: the last row that a column sees.
+template <int T>
+__device__ __forceinline__ void many_nan(State<T>& st, const lds_u8* raw, const int (&rel)[T], int rows, int lane) {
+  const uint32_t s = *(const lds_u32*)(raw + ManyLds::kRawCache + ManyLds::kRawValues + 4 * lane);
+  uint32_t bad = 0;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) bad |= (uint32_t)((s >> 8 * b & 0xff) > kFp4MaxScale) << b;
+  uint64_t which = __builtin_amdgcn_ballot_w64(bad != 0 && lane < rows);
+  while (which) {
+    const int r = __builtin_ctzll(which);
+    which &= which - 1;
+    const uint32_t blocks = (uint32_t)__builtin_amdgcn_readlane((int)bad, r);
+#pragma unroll
+    for (int x = 0; x < T; ++x)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if ((blocks >> (j >> 1) & 1) && r <= rel[x]) st.acc[x][j] += __builtin_nanf("");
+  }
+}
+
+// 32 keys of a pair of tiles. k0, v0: the lane's places in them.
+template <int HALF, int T>
+__device__ __forceinline__ void many_take(State<T>& st, const lds_u8* tiles, int k0, int v0, bool masked,
+                                          const int (&rel)[T], float c2, int lane) {
+  f32x4 s[2][T];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+#pragma unroll
+    for (int x = 0; x < T; ++x) s[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {  // (the chunk 4 c + l / 16: bits that the slot's XOR only flips)
+      const u32x4 w = *(const lds_u32x4*)(tiles + (k0 ^ 64 * c) + (2 * HALF + t) * 16 * ManyLds::kRow);
+#pragma unroll
+      for (int x = 0; x < T; ++x) s[t][x] = mfma(w, st.q[x][c], s[t][x]);
+    }
+  }
+  if (masked) {
+#pragma unroll
+    for (int x = 0; x < T; ++x)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (32 * HALF + 16 * t + 4 * (lane >> 4) + i > rel[x]) s[t][x][i] = -INFINITY;
+  }
+  u32x4 p[T];
+  weights<T>(p, s, st, c2);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    u32x4 w;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      lds_u8* at = const_cast<lds_u8*>(tiles + ManyLds::kTile + (v0 ^ 32 * j) + (2 * HALF + t) * 16 * ManyLds::kRow);
+      const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at));
+      w[2 * t] = x[0];
+      w[2 * t + 1] = x[1];
+    }
+#pragma unroll
+    for (int x = 0; x < T; ++x) st.acc[x][j] = mfma(w, p[x], st.acc[x][j]);
+  }
 }
 
 __global__ __launch_bounds__(kManyWaves* kWave, 2) void attend_many_kernel(const Fp4AttnArgs a, const Partials part, int runs) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * Stage<1, kManyStep>::kBytes];
-  attend_run<true, kManyTiles, 1, kManyStep, kManyWaves>(a, part, runs, blockIdx.x, 0, 1, (lds_u8*)lds);
+  constexpr int D = kHeadDim, T = kManyTiles;
+  typedef ManyLds S;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[S::kBytes];
+  lds_u8* const lds = (lds_u8*)smem;
+  const int lds0 = (int)(uintptr_t)lds;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = uniform(threadIdx.x / kWave);
+  const int n = lane & 15, g = lane >> 4;
+  Run<true, kManyStep> run;
+  if (!run.init(a, part, runs, blockIdx.x, threadIdx.x == 0, lane)) return;
+  const int k0 = n * S::kRow + (g ^ n) * 16;                        // chunk g of row n
+  const int vr = 4 * g + (n >> 2), vc = (n & 3) >> 1;               // rows 4 g .. + 3, 8 bytes of chunks 0 and 1
+  const int v0 = vr * S::kRow + (vc ^ (2 * vr & 15)) * 16 + 8 * (n & 1);
+  while (run.next(a, part, lane)) {
+    const Seq seq = run.seq;
+    const int s0 = run.s0, s1 = run.s1, head = run.tile.head;
+    Columns<T> cols;
+    cols.init(a, seq, run.row0, head, wave * T * 16, true, n);
+    State<T> st;
+#pragma unroll
+    for (int x = 0; x < T; ++x) {
+      const uint16_t* q = a.q + (int64_t)(seq.q0 + cols.row[x]) * a.q_stride + cols.head[x] * D + 8 * g;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) st.q[x][c] = cols.real[x] ? *reinterpret_cast<const u32x4*>(q + 32 * c) : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) st.acc[x][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      st.m[x] = kLowest;
+      st.l[x] = 0.f;
+    }
+    // (q is waited for here: in the loop the wait would be for every row in flight)
+#pragma unroll
+    for (int x = 0; x < T; ++x)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) asm volatile("" : "+v"(st.q[x][c]));
+    arrive_all();  // (the last piece's reads of LDS are over)
+    const int32_t* table = a.block_table + (int64_t)run.tile.b * a.bt_stride;
+    ManyLoader loader;
+    loader.init(a, table, s0 * kManyStep, seq.keys, head, wave, lane);
+    Cursor mine = loader.at;
+#pragma unroll
+    for (int i = 0; i < kManyRing - 1; ++i)
+      if (i < s1 - s0) loader.issue(a, seq.keys, lds0 + i * S::kRaw, lane);
+    if (s0 + 2 < s1)
+      arrive_but<2 * S::kLoads>();
+    else
+      arrive_but<0>();
+    convert_rows(lds, lds + S::kTiles, threadIdx.x);
+
+    for (int s = s0; s < s1; ++s) {
+      const int i = s - s0;
+      // step s + 1's rows and step s's tiles are there, and step s - 1 is done with
+      if (s + 2 < s1)
+        arrive_but<S::kLoads>();
+      else
+        arrive_but<0>();
+      if (s + 3 < s1) loader.issue(a, seq.keys, lds0 + ((i + 3) & 3) * S::kRaw, lane);
+      if (s + 1 < s1) convert_rows(lds + ((i + 1) & 3) * S::kRaw, lds + S::kTiles + ((i + 1) & 1) * 2 * S::kTile, threadIdx.x);
+      const int t0 = s * kManyStep;
+      if (t0 <= cols.furthest && mine.good(a)) {  // (otherwise no column sees these keys)
+        const lds_u8* tiles = lds + S::kTiles + (i & 1) * 2 * S::kTile;
+        int rel[T];
+#pragma unroll
+        for (int x = 0; x < T; ++x) rel[x] = cols.last[x] - t0;
+        many_take<0>(st, tiles, k0, v0, t0 + 31 > cols.lowest, rel, a.scale_log2, lane);
+        if (t0 + 32 <= cols.furthest)
+          many_take<1>(st, tiles, k0, v0, t0 + 63 > cols.lowest, rel, a.scale_log2, lane);
+        many_nan(st, lds + (i & 3) * S::kRaw, rel, seq.keys - t0, lane);
+      }
+      mine.next(a, kManyStep);
+    }
+
+#pragma unroll
+    for (int x = 0; x < T; ++x) {
+      const float l = quarters_sum(st.l[x]);
+      if (!cols.real[x]) continue;
+      if (run.whole) {
+        uint16_t* out = a.out + (int64_t)(seq.q0 + cols.row[x]) * a.out_stride + cols.head[x] * D + 4 * g;
+        const float inv = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<u32x2*>(out + 16 * j) = u32x2{pack_bf16x2(st.acc[x][j][0] * inv, st.acc[x][j][1] * inv),
+                                                          pack_bf16x2(st.acc[x][j][2] * inv, st.acc[x][j][3] * inv)};
+      } else {
+        const int64_t at_part = part.at(run.slot(), 0, wave * T * 16 + 16 * x + n);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) *reinterpret_cast<f32x4*>(part.o + at_part * D + 16 * j + 4 * g) = st.acc[x][j];
+        if (g == 0) part.ml[at_part] = make_float2(st.m[x], l);
+      }
+    }
+  }
+  if (threadIdx.x == 0) part.split[run.run] = run.split;
 }
 
 // Work-group (run, y): the tile that begins in the run and goes on, if there is one; its partial results are the
@@ -914,14 +1212,14 @@ Fp4AttnPlan fp4_attention_plan(int32_t num_seqs, int32_t num_heads, int32_t num_
   const int64_t few_steps = ((int64_t)max_seqlen_k * p.few_slots + kSub * kFewWaves - 1) / (kSub * kFewWaves);
   p.too_long = num_seqs * few_steps > INT32_MAX;
   p.few_cols = (int)std::min<int64_t>(16, (int64_t)max_seqlen_q * group);
-  p.few_runs = (int)std::min<int64_t>(512, num_seqs * few_steps);
+  p.few_runs = (int)std::min<int64_t>(256, num_seqs * few_steps);
   p.few_bytes = partial_bytes(partial_rows<false>(p, num_kv_heads), p.few_runs);
   if ((int64_t)max_seqlen_q * group > 16) {
     const int64_t steps = ((int64_t)max_seqlen_k + kManyStep - 1) / kManyStep;
     const int64_t tiles = num_rows * group / kManyCols + num_seqs;  // of a kv head
     p.too_long |= tiles * steps > INT32_MAX;
     p.many_tiles = std::max<int64_t>(1, num_rows * group / kManyCols) * num_kv_heads;
-    p.many_runs = 512;
+    p.many_runs = 256;
     p.many_bytes = partial_bytes(partial_rows<true>(p, num_kv_heads), p.many_runs);
   }
   return p;
