@@ -38,6 +38,11 @@ __device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t top) {
 
 typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 fp4_bf16x2;
 
+// Two fp32 values to a packed bf16 pair, rounded to nearest even in one instruction.
+__device__ __forceinline__ uint32_t fp4_pack_bf16(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, fp4_bf16x2));
+}
+
 // The scale of a scale byte as v_cvt_scalef32_* take it: they use its exponent alone, and an exponent of all
 // ones gives NaN.
 __device__ __forceinline__ float fp4_scale(uint32_t byte) { return __uint_as_float(byte << 23); }

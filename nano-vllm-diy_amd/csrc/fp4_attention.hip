@@ -339,6 +339,8 @@ struct Cursor {
     last = (keys - 1) / a.block_size;
     blk = scalar_i32(table + min(entry, last));
   }
+  // (the entry is waited for here, ahead of the reads of LDS that would otherwise be waited for together with it)
+  __device__ __forceinline__ void arrive() { asm volatile("" : "+s"(blk)); }
   __device__ __forceinline__ bool good(const Fp4AttnArgs& a) const { return blk >= 0 && blk < a.num_blocks; }
   __device__ __forceinline__ int rows(const Fp4AttnArgs& a, int keys) const { return good(a) ? keys - t : 0; }
   // Rows from here on in a cache (any place of the cache where there are none).
@@ -396,9 +398,11 @@ struct Loader {
     scale_at.init(a, table, t0 + scale_first, keys);
   }
 
-  // The next step's rows into a stage of LDS. A row that is no key reads the last one that is (or, where there is
-  // none, the cache's first row): the count of loads in flight is the same in every step.
-  __device__ __forceinline__ void issue(const Fp4AttnArgs& a, int keys, int stage) {
+  // The next step's rows into a stage of LDS; whether the wavefront's own 32 keys among them are in a block. A row that
+  // is no key reads the last one that is (or, where there is none, the cache's first row): the count of loads in
+  // flight is the same in every step.
+  __device__ __forceinline__ bool issue(const Fp4AttnArgs& a, int keys, int stage) {
+    const bool good = at.good(a);
     const int last = max(at.rows(a, keys), 1) - 1;
     const uint8_t* k = uniform_ptr(at.at(a, a.k, a.k_block));
     const uint8_t* v = uniform_ptr(at.at(a, a.v, a.v_block));
@@ -413,6 +417,7 @@ struct Loader {
     const uint8_t* c = uniform_ptr(scales_of_v ? scale_at.at(a, a.v, a.v_block) : scale_at.at(a, a.k, a.k_block));
     stage4(c, min(scale_row, scale_last) * a.row_bytes + scale_col, uniform(stage + scale_lds));
     scale_at.next(a, ROWS);
+    return good;
   }
 };
 
@@ -463,43 +468,57 @@ struct Lanes {
   }
 };
 
+struct Keys {
+  u32x4 d[2];        // row row_of(l % 16) of a tile: dimensions 32 (l / 16) .. + 31
+  uint32_t s[2];
+};
+
 // S^T of two tiles of 16 keys.
-template <int T, int HEADS, int ROWS>
-__device__ __forceinline__ void scores(f32x4 (&s)[2][T], const State<T>& st, const lds_u8* stage,
-                                       const Lanes<HEADS, ROWS>& at) {
+template <int T>
+__device__ __forceinline__ void scores(f32x4 (&s)[2][T], const State<T>& st, const Keys& k) {
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const u32x4 d = *(const lds_u32x4*)(stage + at.k + t * at.kTile);
-    const float scale = fp4_scale(*(const lds_u8*)(stage + at.ks + t * at.kScaleTile));
-#pragma unroll
-    for (int x = 0; x < T; ++x) s[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float scale = fp4_scale(k.s[t]);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const uint4 w = fp4_unpack8(d[c], scale);
+      const uint4 w = fp4_unpack8(k.d[t][c], scale);
 #pragma unroll
-      for (int x = 0; x < T; ++x) s[t][x] = mfma(u32x4{w.x, w.y, w.z, w.w}, st.q[x][c], s[t][x]);
+      for (int x = 0; x < T; ++x)
+        s[t][x] = mfma(u32x4{w.x, w.y, w.z, w.w}, st.q[x][c], c ? s[t][x] : f32x4{0.f, 0.f, 0.f, 0.f});
     }
   }
 }
 
-// The weights of the columns, in bf16 pairs, as the operand of the product with V: tile by tile, i by i.
-template <int T>
-__device__ __forceinline__ void weights(u32x4 (&p)[T], const f32x4 (&s)[2][T], State<T>& st, float c2) {
+// a.x + a.y + c on a packed bf16 pair.
+__device__ __forceinline__ float add_bf16x2(uint32_t a, float c) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(fp4_bf16x2, a), __builtin_bit_cast(fp4_bf16x2, 0x3f803f80u), c,
+                                         false);
+}
+
+// The weights of the columns over NT tiles of 16 keys, in bf16 pairs, as the operand of the product with V: two
+// tiles an operand, tile by tile, i by i. The sum is of the rounded weights, which is what the product weighs V with.
+// (Whether the reference holds is asked of each lane's own scores; the column's largest is formed only where it
+// does not.)
+template <int T, int NT>
+__device__ __forceinline__ void weights(u32x4 (&p)[T][NT / 2], const f32x4 (&s)[NT][T], State<T>& st, float c2) {
   float top[T];
   bool over = false;
 #pragma unroll
   for (int x = 0; x < T; ++x) {
     float mx = fmaxf(s[0][x][0], s[0][x][1]);
     mx = fmaxf(fmaxf(mx, s[0][x][2]), s[0][x][3]);
-    mx = fmaxf(fmaxf(mx, s[1][x][0]), s[1][x][1]);
-    mx = fmaxf(fmaxf(mx, s[1][x][2]), s[1][x][3]);
-    top[x] = quarters_max(mx) * c2;
-    over |= top[x] > st.m[x] + kSlack;
+#pragma unroll
+    for (int t = 1; t < NT; ++t) {
+      mx = fmaxf(fmaxf(mx, s[t][x][0]), s[t][x][1]);
+      mx = fmaxf(fmaxf(mx, s[t][x][2]), s[t][x][3]);
+    }
+    top[x] = mx;
+    over |= mx * c2 > st.m[x] + kSlack;
   }
   if (__builtin_amdgcn_ballot_w64(over)) {
 #pragma unroll
     for (int x = 0; x < T; ++x) {
-      const float m = fmaxf(st.m[x], top[x]);
+      const float m = fmaxf(st.m[x], quarters_max(top[x]) * c2);
       const float f = exp2_fast(st.m[x] - m);
       st.m[x] = m;
       st.l[x] *= f;
@@ -510,21 +529,20 @@ __device__ __forceinline__ void weights(u32x4 (&p)[T], const f32x4 (&s)[2][T], S
 #pragma unroll
   for (int x = 0; x < T; ++x) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < NT; ++t) {
       float e[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        e[i] = exp2_fast(fmaf(s[t][x][i], c2, -st.m[x]));
-        st.l[x] += e[i];
-      }
-      p[x][2 * t] = pack_bf16x2(e[0], e[1]);
-      p[x][2 * t + 1] = pack_bf16x2(e[2], e[3]);
+      for (int i = 0; i < 4; ++i) e[i] = exp2_fast(fmaf(s[t][x][i], c2, -st.m[x]));
+      const uint32_t lo = fp4_pack_bf16(e[0], e[1]), hi = fp4_pack_bf16(e[2], e[3]);
+      p[x][t >> 1][2 * (t & 1)] = lo;
+      p[x][t >> 1][2 * (t & 1) + 1] = hi;
+      st.l[x] = add_bf16x2(hi, add_bf16x2(lo, st.l[x]));
     }
   }
 }
 
 template <int kByte, int T>
-__device__ __forceinline__ void add_pair(State<T>& st, const u32x4 (&p)[T], const Vals& v) {
+__device__ __forceinline__ void add_pair(State<T>& st, const u32x4 (&p)[T][1], const Vals& v) {
   u32x4 even, odd;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -538,13 +556,13 @@ __device__ __forceinline__ void add_pair(State<T>& st, const u32x4 (&p)[T], cons
   }
 #pragma unroll
   for (int x = 0; x < T; ++x) {
-    st.acc[x][2 * kByte] = mfma(even, p[x], st.acc[x][2 * kByte]);
-    st.acc[x][2 * kByte + 1] = mfma(odd, p[x], st.acc[x][2 * kByte + 1]);
+    st.acc[x][2 * kByte] = mfma(even, p[x][0], st.acc[x][2 * kByte]);
+    st.acc[x][2 * kByte + 1] = mfma(odd, p[x][0], st.acc[x][2 * kByte + 1]);
   }
 }
 
 template <int T>
-__device__ __forceinline__ void add_values(State<T>& st, const u32x4 (&p)[T], const Vals& v) {
+__device__ __forceinline__ void add_values(State<T>& st, const u32x4 (&p)[T][1], const Vals& v) {
   add_pair<0>(st, p, v);
   add_pair<1>(st, p, v);
   add_pair<2>(st, p, v);
@@ -587,8 +605,18 @@ __device__ __forceinline__ void nan_values(State<T>& st, Vals& v, const int (&re
 template <int T, int HEADS, int ROWS>
 __device__ __forceinline__ void take(State<T>& st, const lds_u8* stage, const Lanes<HEADS, ROWS>& at, bool masked,
                                      const int (&rel)[T], float c2, int lane) {
+  // (all reads of LDS at once, ahead of everything that waits for them)
+  Keys k;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    k.d[t] = *(const lds_u32x4*)(stage + at.k + t * at.kTile);
+    k.s[t] = *(const lds_u8*)(stage + at.ks + t * at.kScaleTile);
+  }
+  Vals v;
+  at.values(v, stage);
+  __builtin_amdgcn_sched_barrier(0);
   f32x4 s[2][T];
-  scores(s, st, stage, at);
+  scores(s, st, k);
   if (masked) {
 #pragma unroll
     for (int x = 0; x < T; ++x)
@@ -598,10 +626,8 @@ __device__ __forceinline__ void take(State<T>& st, const lds_u8* stage, const La
         for (int i = 0; i < 4; ++i)
           if (16 * t + row_of<HEADS>(4 * (lane >> 4) + i) > rel[x]) s[t][x][i] = -INFINITY;
   }
-  Vals v;
-  at.values(v, stage);
-  u32x4 p[T];
-  weights<T>(p, s, st, c2);
+  u32x4 p[T][1];
+  weights<T, 2>(p, s, st, c2);
   if (masked) nan_values<T, HEADS>(st, v, rel, lane);
   add_values<T>(st, p, v);
 }
@@ -638,11 +664,11 @@ __device__ __forceinline__ void put_out(uint16_t* out, const float* x, float inv
     for (int i = 0; i < COUNT; i += 8) {
       u32x4 w;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(x[i + 2 * j] * inv, x[i + 2 * j + 1] * inv);
+      for (int j = 0; j < 4; ++j) w[j] = fp4_pack_bf16(x[i + 2 * j] * inv, x[i + 2 * j + 1] * inv);
       *reinterpret_cast<u32x4*>(out + i) = w;
     }
   } else {
-    *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv)};
+    *reinterpret_cast<u32x2*>(out) = u32x2{fp4_pack_bf16(x[0] * inv, x[1] * inv), fp4_pack_bf16(x[2] * inv, x[3] * inv)};
   }
 }
 template <int COUNT>
@@ -807,12 +833,11 @@ __global__ __launch_bounds__(kFewWaves* kWave, 2) void attend_few_kernel(const F
     const int32_t* table = a.block_table + (int64_t)run.tile.b * a.bt_stride;
     L loader;
     loader.init(a, table, s0 * ROWS, seq.keys, head0, heads, wave, lane);
-    Cursor mine;  // the wavefront's own keys
-    mine.init(a, table, s0 * ROWS + slice * kSub, seq.keys);
+    uint32_t good = 0;  // bit i: step s + i's keys are in a block
     queries.issue(a, seq, head, wave, lane, lds0 + (kFewRing - 1) * S::kBytes);
 #pragma unroll
     for (int i = 0; i < kFewRing - 1; ++i)
-      if (i < s1 - s0) loader.issue(a, seq.keys, lds0 + i * S::kBytes);
+      if (i < s1 - s0) good |= (uint32_t)loader.issue(a, seq.keys, lds0 + i * S::kBytes) << i;
 
     Columns<1> cols;
     cols.init(a, seq, 0, head, 0, live, n);
@@ -835,15 +860,18 @@ __global__ __launch_bounds__(kFewWaves* kWave, 2) void attend_few_kernel(const F
         arrive_but<(kFewRing - 2) * L::kLoads>();
       else
         arrive_but<0>();
-      if (s + kFewRing - 1 < s1) loader.issue(a, seq.keys, lds0 + next_buf * S::kBytes);
+      if (s + kFewRing - 1 < s1)
+        good |= (uint32_t)loader.issue(a, seq.keys, lds0 + next_buf * S::kBytes) << (kFewRing - 1);
+      loader.at.arrive();
+      loader.scale_at.arrive();
       buf = buf + 1 == kFewRing ? 0 : buf + 1;
       next_buf = next_buf + 1 == kFewRing ? 0 : next_buf + 1;
       const int t0 = s * ROWS + slice * kSub;
-      if (t0 <= cols.furthest && mine.good(a)) {  // (otherwise no column sees these keys)
+      if (t0 <= cols.furthest && (uniform(good) & 1)) {  // (otherwise no column sees these keys)
         const int rel[1] = {cols.last[0] - t0};
         take(st, stage, at, t0 + kSub - 1 > cols.lowest, rel, a.scale_log2, lane);
       }
-      mine.next(a, ROWS);
+      good >>= 1;
     }
 
     constexpr int N = 32 / kSlices;
@@ -914,12 +942,14 @@ struct ManyLoader {
     scale_lds = (is_v ? ManyLds::kRawCache : 0) + ManyLds::kRawValues + first * kFp4HeadScales;
   }
   // (as Loader's)
-  __device__ __forceinline__ void issue(const Fp4AttnArgs& a, int keys, int stage, int lane) {
+  __device__ __forceinline__ bool issue(const Fp4AttnArgs& a, int keys, int stage, int lane) {
+    const bool good = at.good(a);
     const int last = max(at.rows(a, keys), 1) - 1;
     const uint8_t* c = uniform_ptr(at.at(a, cache, block));
     stage16(c, min(row, last) * a.row_bytes + col, uniform(stage + lds));
     if (lane < 16) stage4(c, min(scale_row, last) * a.row_bytes + scale_col, uniform(stage + scale_lds));
     at.next(a, kManyStep);
+    return good;
   }
 };
 
@@ -968,45 +998,60 @@ __device__ __forceinline__ void many_nan(State<T>& st, const lds_u8* raw, const 
   }
 }
 
-// 32 keys of a pair of tiles. k0, v0: the lane's places in them.
-template <int HALF, int T>
-__device__ __forceinline__ void many_take(State<T>& st, const lds_u8* tiles, int k0, int v0, bool masked,
-                                          const int (&rel)[T], float c2, int lane) {
-  f32x4 s[2][T];
+// The 64 keys of a pair of tiles. k, v: the lane's places in them, for every chunk of K and every 16 dimensions of V.
+// The reads are kept ahead of the products that use them (the compiler's own order reads each operand right before
+// its product and waits for it).
+template <int T>
+__device__ __forceinline__ void many_take(State<T>& st, const lds_u8* tiles, const int (&k)[4], const int (&v)[8],
+                                          bool masked, const int (&rel)[T], float c2, int lane) {
+  constexpr int kTile16 = 16 * ManyLds::kRow;
+  constexpr int kAheadK = 4, kAheadV = 2;
+  f32x4 s[4][T];
+  u32x4 kw[kAheadK];
+  u32x4 vw[kAheadV + 1][2];
+  const auto read_k = [&](int i) { return *(const lds_u32x4*)(tiles + k[i & 3] + (i >> 2) * kTile16); };
+  const auto read_v = [&](u32x4 (&w)[2], int j) {
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-#pragma unroll
-    for (int x = 0; x < T; ++x) s[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {  // (the chunk 4 c + l / 16: bits that the slot's XOR only flips)
-      const u32x4 w = *(const lds_u32x4*)(tiles + (k0 ^ 64 * c) + (2 * HALF + t) * 16 * ManyLds::kRow);
-#pragma unroll
-      for (int x = 0; x < T; ++x) s[t][x] = mfma(w, st.q[x][c], s[t][x]);
+    for (int t = 0; t < 4; ++t) {
+      lds_u8* at = const_cast<lds_u8*>(tiles + ManyLds::kTile + v[j] + t * kTile16);
+      const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at));
+      w[t >> 1][2 * (t & 1)] = x[0];
+      w[t >> 1][2 * (t & 1) + 1] = x[1];
     }
+  };
+#pragma unroll
+  for (int i = 0; i < kAheadK; ++i) kw[i] = read_k(i);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const u32x4 w = kw[i % kAheadK];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int x = 0; x < T; ++x) s[i >> 2][x] = mfma(w, st.q[x][i & 3], i & 3 ? s[i >> 2][x] : f32x4{0.f, 0.f, 0.f, 0.f});
+    if (i + kAheadK < 16) kw[i % kAheadK] = read_k(i + kAheadK);
   }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < kAheadV; ++j) read_v(vw[j], j);
   if (masked) {
 #pragma unroll
     for (int x = 0; x < T; ++x)
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (32 * HALF + 16 * t + 4 * (lane >> 4) + i > rel[x]) s[t][x][i] = -INFINITY;
+          if (16 * t + 4 * (lane >> 4) + i > rel[x]) s[t][x][i] = -INFINITY;
   }
-  u32x4 p[T];
-  weights<T>(p, s, st, c2);
+  u32x4 p[T][2];
+  weights<T, 4>(p, s, st, c2);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    u32x4 w;
+    if (j + kAheadV < 8) read_v(vw[(j + kAheadV) % (kAheadV + 1)], j + kAheadV);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      lds_u8* at = const_cast<lds_u8*>(tiles + ManyLds::kTile + (v0 ^ 32 * j) + (2 * HALF + t) * 16 * ManyLds::kRow);
-      const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at));
-      w[2 * t] = x[0];
-      w[2 * t + 1] = x[1];
-    }
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int x = 0; x < T; ++x) st.acc[x][j] = mfma(w, p[x], st.acc[x][j]);
+      for (int x = 0; x < T; ++x) st.acc[x][j] = mfma(vw[j % (kAheadV + 1)][h], p[x][h], st.acc[x][j]);
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
@@ -1021,9 +1066,12 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void attend_many_kernel(const
   const int n = lane & 15, g = lane >> 4;
   Run<true, kManyStep> run;
   if (!run.init(a, part, runs, blockIdx.x, threadIdx.x == 0, lane)) return;
-  const int k0 = n * S::kRow + (g ^ n) * 16;                        // chunk g of row n
-  const int vr = 4 * g + (n >> 2), vc = (n & 3) >> 1;               // rows 4 g .. + 3, 8 bytes of chunks 0 and 1
-  const int v0 = vr * S::kRow + (vc ^ (2 * vr & 15)) * 16 + 8 * (n & 1);
+  int k_at[4], v_at[8];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) k_at[c] = n * S::kRow + ((4 * c + g) ^ n) * 16;
+  const int vr = 4 * g + (n >> 2);  // rows 4 g .. + 3, 8 bytes each
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v_at[j] = vr * S::kRow + ((2 * j + ((n & 3) >> 1)) ^ (2 * vr & 15)) * 16 + 8 * (n & 1);
   while (run.next(a, part, lane)) {
     const Seq seq = run.seq;
     const int s0 = run.s0, s1 = run.s1, head = run.tile.head;
@@ -1049,10 +1097,10 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void attend_many_kernel(const
     const int32_t* table = a.block_table + (int64_t)run.tile.b * a.bt_stride;
     ManyLoader loader;
     loader.init(a, table, s0 * kManyStep, seq.keys, head, wave, lane);
-    Cursor mine = loader.at;
+    uint32_t good = 0;  // bit i: step s + i's keys are in a block
 #pragma unroll
     for (int i = 0; i < kManyRing - 1; ++i)
-      if (i < s1 - s0) loader.issue(a, seq.keys, lds0 + i * S::kRaw, lane);
+      if (i < s1 - s0) good |= (uint32_t)loader.issue(a, seq.keys, lds0 + i * S::kRaw, lane) << i;
     if (s0 + 2 < s1)
       arrive_but<2 * S::kLoads>();
     else
@@ -1066,20 +1114,19 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void attend_many_kernel(const
         arrive_but<S::kLoads>();
       else
         arrive_but<0>();
-      if (s + 3 < s1) loader.issue(a, seq.keys, lds0 + ((i + 3) & 3) * S::kRaw, lane);
+      if (s + 3 < s1) good |= (uint32_t)loader.issue(a, seq.keys, lds0 + ((i + 3) & 3) * S::kRaw, lane) << 3;
       if (s + 1 < s1) convert_rows(lds + ((i + 1) & 3) * S::kRaw, lds + S::kTiles + ((i + 1) & 1) * 2 * S::kTile, threadIdx.x);
+      loader.at.arrive();
       const int t0 = s * kManyStep;
-      if (t0 <= cols.furthest && mine.good(a)) {  // (otherwise no column sees these keys)
+      if (t0 <= cols.furthest && (uniform(good) & 1)) {  // (otherwise no column sees these keys)
         const lds_u8* tiles = lds + S::kTiles + (i & 1) * 2 * S::kTile;
         int rel[T];
 #pragma unroll
         for (int x = 0; x < T; ++x) rel[x] = cols.last[x] - t0;
-        many_take<0>(st, tiles, k0, v0, t0 + 31 > cols.lowest, rel, a.scale_log2, lane);
-        if (t0 + 32 <= cols.furthest)
-          many_take<1>(st, tiles, k0, v0, t0 + 63 > cols.lowest, rel, a.scale_log2, lane);
+        many_take(st, tiles, k_at, v_at, t0 + kManyStep - 1 > cols.lowest, rel, a.scale_log2, lane);
         many_nan(st, lds + (i & 3) * S::kRaw, rel, seq.keys - t0, lane);
       }
-      mine.next(a, kManyStep);
+      good >>= 1;
     }
 
 #pragma unroll
@@ -1091,8 +1138,8 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void attend_many_kernel(const
         const float inv = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          *reinterpret_cast<u32x2*>(out + 16 * j) = u32x2{pack_bf16x2(st.acc[x][j][0] * inv, st.acc[x][j][1] * inv),
-                                                          pack_bf16x2(st.acc[x][j][2] * inv, st.acc[x][j][3] * inv)};
+          *reinterpret_cast<u32x2*>(out + 16 * j) = u32x2{fp4_pack_bf16(st.acc[x][j][0] * inv, st.acc[x][j][1] * inv),
+                                                          fp4_pack_bf16(st.acc[x][j][2] * inv, st.acc[x][j][3] * inv)};
       } else {
         const int64_t at_part = part.at(run.slot(), 0, wave * T * 16 + 16 * x + n);
 #pragma unroll
@@ -1165,7 +1212,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Fp4AttnArgs 
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int64_t row = split.x + (col >> a.group_shift);
     uint16_t* out = a.out + row * a.out_stride + (head * group + (col & (group - 1))) * D + 4 * t;
-    *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
+    *reinterpret_cast<u32x2*>(out) = u32x2{fp4_pack_bf16(acc[0] * inv, acc[1] * inv), fp4_pack_bf16(acc[2] * inv, acc[3] * inv)};
   }
 }
 
