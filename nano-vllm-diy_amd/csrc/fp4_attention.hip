@@ -9,28 +9,28 @@
 // output are fp32; p is rounded to bf16 for the matrix product, as the 16-bit cache's kernels round it.
 //
 // Columns. A kv head's query heads and a sequence's query rows are the columns of one matrix product: column
-// r G + i is query head i of the group and row r. A wavefront holds T tiles of 16 columns of one kv head and takes
-// 64 keys a step:
-//   S^T = K Q^T  v_mfma_f32_16x16x32_bf16, 16 keys x 16 columns: lane l holds key l % 16 and, of its 128
-//                dimensions, the 32 from 32 (l / 16) -- 16 consecutive bytes of the cache with one scale byte. The
-//                product runs over them 8 at a time; q is laid out in the same order of dimensions.
+// r G + i is query head i of the group and row r. A wavefront holds T tiles of 16 columns of one kv head:
+//   S^T = K Q^T  v_mfma_f32_16x16x32_bf16, 16 keys x 16 columns: lane l holds key l % 16.
 //   O^T += V^T P^T  lane l of S^T has column l % 16 and keys 16 t + 4 (l / 16) + i (tile t, i < 4): as the operand
 //                P^T of the next product these are the 8 keys of its lane for two tiles, so P never changes lanes.
-//                V^T's operand needs, for those 8 keys, dimension n(l % 16): lane l loads 4 bytes of each of them,
-//                the dimensions 8 (l % 16) .. + 7, and dimension 8 (l % 16) + j is row l % 16 of the j-th of 8
-//                products. So the output's rows are a permutation of the dimensions and V needs no transposition
-//                either: two keys' values of one dimension are put side by side by a byte permute.
 // Values convert to bf16 with their scale in one instruction for two. (The matrix instructions that read 4-bit
 // values with their scales keep about 12 bits below the largest product of a sum, measured; scores here are
-// held in 32, so they are not used.)
+// held in 32, so they are not used.) The two kernels differ in who converts:
+//   few rows (rows x group <= 16): T = 1, a tile of work is all of a sequence's rows and up to 8 kv heads, and a
+//       wavefront converts the keys that it takes, 32 of one head at once, straight into the products' operands. Of
+//       K, lane l has of key l % 16 the 32 dimensions from 32 (l / 16): 16 consecutive bytes with one scale byte; the
+//       product runs over them 8 at a time, and q is laid out in the same order of dimensions. Of V, lane l loads 4
+//       bytes of each of its 8 keys, the dimensions 8 (l % 16) .. + 7, and dimension 8 (l % 16) + j is row l % 16 of
+//       the j-th of 8 products: the output's rows are a permutation of the dimensions and V needs no transposition,
+//       two keys' values of one dimension are put side by side by a byte permute.
+//   more rows: T = 2, a tile of work is 256 columns of one kv head, a wavefront 32 of them, and the work-group
+//       converts a step's rows once for its wavefronts.
 //
-// Work. The steps of 64 keys of every tile of query rows lie end to end on a line, which is cut into `runs` equal
-// runs, one work-group each, whatever the lengths: a work-group takes the end of one tile, whole tiles and the
-// beginning of another. A tile that a cut splits leaves fp32 partial results (o, m, sum), which a second kernel
-// merges; a cut splits at most one tile, so there are at most two partial results a run.
-//   few rows (rows x group <= 16): T = 1, a tile is all of a sequence's rows, a wavefront is one kv head and the
-//       work-group reads whole token rows.
-//   more rows: T = 2, a tile is 128 columns of one kv head, a wavefront 32 of them.
+// Work. The steps of every tile lie end to end on a line, which is cut into `runs` equal runs, one work-group each,
+// whatever the lengths: a work-group takes the end of one tile, whole tiles and the beginning of another. A tile that
+// a cut splits leaves fp32 partial results (o, m, sum), which a second kernel merges; a cut splits at most one tile,
+// so there are at most two partial results a run. The lengths are on the GPU only, so both kernels are launched
+// wherever the call's bounds allow sequences of their kind; one without any costs 5 us with its merge.
 #include <algorithm>
 #include <type_traits>
 
@@ -901,13 +901,20 @@ __global__ __launch_bounds__(kFewWaves* kWave, 2) void attend_few_kernel(const F
 // 256 columns of one kv head share its keys: a step's 64 rows come to LDS in 4 bits, the work-group's 512 threads
 // convert them to bf16 tiles once (16 values of K and of V each), and its 8 wavefronts read these. (With each
 // wavefront converting the rows for its own 32 columns the kernel was bound by its vector instructions, 282 for 32
-// keys and 32 columns, 106 of them conversions.) Step s + 1 is converted while step s is computed, steps s + 2 and
-// s + 3 are on their way.
+// keys and 32 columns, 106 of them conversions.) Step s + 1 is converted after step s's products, in their shadow
+// (before them: 712 us in place of 698 for 16 chunks of 1024 rows behind 4096 keys), steps s + 2 and s + 3 are on their way.
+//
+// Bound by the vector instructions and the products together: the matrix cores are busy for 42% of a SIMD's time,
+// the vector units for 48%. Two other forms ran within 3% of this one: step s's exponentials between the products of
+// step s + 1, and that with four wavefronts of 64 columns, half the reads of LDS.
 //
 // The tiles have 256-byte rows, 16 chunks of 16 bytes. K: chunk c of row r in slot c ^ (r & 15): the 16 lanes of a
-// quarter wavefront read one chunk of 16 rows. V: slot c ^ (2 r & 15): the transposing read takes four rows and 32
-// bytes a quarter, two quarters at once: 16 different slots. Dimensions are in their own order here: lane l holds
-// dimensions 32 c + 8 (l / 16) .. + 7 of key l % 16 (and of q), and dimension 16 j + l % 16 of V's four keys.
+// quarter wavefront read one chunk of 16 rows. V: slot c ^ v_swizzle(r): the transposing read takes four rows and 32
+// bytes a quarter, two quarters at once, 16 different slots; and the conversion writes one chunk in two of each
+// of two rows at once, 16 different slots again. Dimensions are in their own order here: lane l holds dimensions
+// 32 c + 8 (l / 16) .. + 7 of key l % 16 (and of q), and dimension 16 j + l % 16 of V's four keys.
+__device__ __forceinline__ int v_swizzle(int r) { return (2 * r & 14) | (r & 1); }
+
 struct ManyLds {
   static constexpr int kRow = kHeadDim * 2;
   static constexpr int kTile = kManyStep * kRow;                   // bf16 rows of a cache
@@ -973,7 +980,7 @@ __device__ __forceinline__ void convert_rows(const lds_u8* raw, lds_u8* tiles, i
     const int c = 2 * part + i;
     const uint4 wk = fp4_unpack8(k[i], fp4_scale(ks)), wv = fp4_unpack8(v[i], fp4_scale(vs));
     *(lds_u32x4*)(tiles + r * ManyLds::kRow + (c ^ (r & 15)) * 16) = u32x4{wk.x, wk.y, wk.z, wk.w};
-    *(lds_u32x4*)(tiles + ManyLds::kTile + r * ManyLds::kRow + (c ^ (2 * r & 15)) * 16) = u32x4{wv.x, wv.y, wv.z, wv.w};
+    *(lds_u32x4*)(tiles + ManyLds::kTile + r * ManyLds::kRow + (c ^ v_swizzle(r)) * 16) = u32x4{wv.x, wv.y, wv.z, wv.w};
   }
 }
 
@@ -1071,7 +1078,7 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void attend_many_kernel(const
   for (int c = 0; c < 4; ++c) k_at[c] = n * S::kRow + ((4 * c + g) ^ n) * 16;
   const int vr = 4 * g + (n >> 2);  // rows 4 g .. + 3, 8 bytes each
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v_at[j] = vr * S::kRow + ((2 * j + ((n & 3) >> 1)) ^ (2 * vr & 15)) * 16 + 8 * (n & 1);
+  for (int j = 0; j < 8; ++j) v_at[j] = vr * S::kRow + ((2 * j + ((n & 3) >> 1)) ^ v_swizzle(vr)) * 16 + 8 * (n & 1);
   while (run.next(a, part, lane)) {
     const Seq seq = run.seq;
     const int s0 = run.s0, s1 = run.s1, head = run.tile.head;
@@ -1115,7 +1122,6 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void attend_many_kernel(const
       else
         arrive_but<0>();
       if (s + 3 < s1) good |= (uint32_t)loader.issue(a, seq.keys, lds0 + ((i + 3) & 3) * S::kRaw, lane) << 3;
-      if (s + 1 < s1) convert_rows(lds + ((i + 1) & 3) * S::kRaw, lds + S::kTiles + ((i + 1) & 1) * 2 * S::kTile, threadIdx.x);
       loader.at.arrive();
       const int t0 = s * kManyStep;
       if (t0 <= cols.furthest && (uniform(good) & 1)) {  // (otherwise no column sees these keys)
@@ -1126,6 +1132,7 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void attend_many_kernel(const
         many_take(st, tiles, k_at, v_at, t0 + kManyStep - 1 > cols.lowest, rel, a.scale_log2, lane);
         many_nan(st, lds + (i & 3) * S::kRaw, rel, seq.keys - t0, lane);
       }
+      if (s + 1 < s1) convert_rows(lds + ((i + 1) & 3) * S::kRaw, lds + S::kTiles + ((i + 1) & 1) * 2 * S::kTile, threadIdx.x);
       good >>= 1;
     }
 
