@@ -1158,17 +1158,15 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void attend_many_kernel(const
   if (threadIdx.x == 0) part.split[run.run] = run.split;
 }
 
-// Work-group (run, y): the tile that begins in the run and goes on, if there is one; its partial results are the
-// run's second slot and the first ones of the runs after it. 32 threads take a column (of a kv head), 4 dimensions
+// The tile that begins in a run and goes on, if there is one; its partial results are the run's second slot and the
+// first ones of the runs after it. `groups` work-groups share a run's columns. 32 threads take a column (of a kv head), 4 dimensions
 // each, and `slices` of them share a column's partial results, which meet in LDS.
 constexpr int kMergeThreads = 256;
 constexpr int kMergeTeams = kMergeThreads / 32;
 template <bool MANY>
-__global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Fp4AttnArgs a, const Partials part, int slices) {
+__device__ __forceinline__ void merge(const Fp4AttnArgs& a, const Partials& part, int run, int first, int groups, int slices,
+                                      f32x4 (&acc_of)[kMergeTeams][32], float2 (&ml_of)[kMergeTeams]) {
   constexpr int D = kHeadDim;
-  __shared__ f32x4 acc_of[kMergeTeams][32];
-  __shared__ float2 ml_of[kMergeTeams];
-  const int run = blockIdx.x;
   const int4 split = part.split[run];
   if (run >= *part.live || split.z == 0) return;
   const int cols = split.y, pieces = split.z;
@@ -1177,7 +1175,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Fp4AttnArgs 
   const int t = threadIdx.x & 31, team = threadIdx.x >> 5;
   const int slice = team & (slices - 1);
   const int per_pass = kMergeTeams / slices;
-  for (int base = blockIdx.y * per_pass; base < pairs; base += gridDim.y * per_pass) {
+  for (int base = first * per_pass; base < pairs; base += groups * per_pass) {
     const int pair = base + team / slices;
     const int head = MANY ? split.w : pair / cols;
     const int col = MANY ? pair : pair - head * cols;
@@ -1221,6 +1219,23 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Fp4AttnArgs 
     uint16_t* out = a.out + row * a.out_stride + (head * group + (col & (group - 1))) * D + 4 * t;
     *reinterpret_cast<u32x2*>(out) = u32x2{fp4_pack_bf16(acc[0] * inv, acc[1] * inv), fp4_pack_bf16(acc[2] * inv, acc[3] * inv)};
   }
+}
+
+// One of the two kernels' merges.
+struct Merge {
+  Partials part;
+  int runs, groups, slices;  // runs that may begin a split tile
+};
+
+// Work-groups of both merges: few's runs x groups, then many's.
+__global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Fp4AttnArgs a, const Merge few, const Merge many) {
+  __shared__ f32x4 acc_of[kMergeTeams][32];
+  __shared__ float2 ml_of[kMergeTeams];
+  const int i = blockIdx.x, j = i - few.runs * few.groups;
+  if (j < 0)
+    merge<false>(a, few.part, i / few.groups, i % few.groups, few.groups, few.slices, acc_of, ml_of);
+  else
+    merge<true>(a, many.part, j / many.groups, j % many.groups, many.groups, many.slices, acc_of, ml_of);
 }
 
 template <bool MANY>
@@ -1290,23 +1305,22 @@ hipError_t launch_fp4_attention(const Fp4AttnArgs& a, const Fp4AttnPlan& p, hipS
     default: hipLaunchKernelGGL(attend_few_kernel<8>, grid, block, 0, stream, a, few, p.few_runs, p.few_heads); break;
   }
   if (hipError_t err = hipGetLastError()) return err;
-  if (p.few_runs > 1) {
-    const int slices = merge_slices(p.few_runs, a.num_seqs), per_pass = kMergeTeams / slices;
-    const int passes = (a.num_kv_heads * p.few_cols + per_pass - 1) / per_pass;
-    hipLaunchKernelGGL((merge_kernel<false>), dim3((unsigned)(p.few_runs - 1), (unsigned)merge_groups(p.few_runs, passes)),
-                       dim3(kMergeThreads), 0, stream, a, few, slices);
+  Merge merge_few{few, p.few_runs - 1, 1, 1}, merge_many{few, 0, 1, 1};
+  if (merge_few.runs > 0) {
+    merge_few.slices = merge_slices(p.few_runs, a.num_seqs);
+    const int per_pass = kMergeTeams / merge_few.slices;
+    merge_few.groups = merge_groups(p.few_runs, (a.num_kv_heads * p.few_cols + per_pass - 1) / per_pass);
   }
-  if (hipError_t err = hipGetLastError()) return err;
   if (p.many_runs) {
     const Partials many = partials_of<true>(a, p, ws + p.few_bytes);
     hipLaunchKernelGGL(attend_many_kernel, dim3((unsigned)p.many_runs), dim3(kManyWaves * kWave), 0, stream, a, many,
                        p.many_runs);
     if (hipError_t err = hipGetLastError()) return err;
     const int slices = merge_slices(p.many_runs, p.many_tiles);
-    const int passes = kManyCols * slices / kMergeTeams;
-    hipLaunchKernelGGL((merge_kernel<true>), dim3((unsigned)(p.many_runs - 1), (unsigned)merge_groups(p.many_runs, passes)),
-                       dim3(kMergeThreads), 0, stream, a, many, slices);
+    merge_many = Merge{many, p.many_runs - 1, merge_groups(p.many_runs, kManyCols * slices / kMergeTeams), slices};
   }
+  const int groups = merge_few.runs * merge_few.groups + merge_many.runs * merge_many.groups;
+  if (groups) hipLaunchKernelGGL(merge_kernel, dim3((unsigned)groups), dim3(kMergeThreads), 0, stream, a, merge_few, merge_many);
   return hipGetLastError();
 }
 
