@@ -583,7 +583,8 @@ int pk_compact_blocks(void* k_caches, void* v_caches, int64_t k_layer_stride, in
  * Four bits are a sign, two of exponent and one of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6; the value is that
  * times 2^(scale byte - 127). Of 32 values with the largest magnitude a the scale is the smallest power
  * of two s with a <= 7 s, within 2^-126 .. 2^125; values are divided by it and rounded to nearest, ties to
- * even, at most 6. An infinity or NaN among the 32 makes all of them NaN (scale byte 255). Every value is
+ * even, at most 6. An infinity or NaN among the 32 makes all of them NaN (scale byte 255; 0, 253 and 254 are
+ * not written, and a cache of other origin must not hold them). Every value is
  * exact in bf16. A finite value is off by at most a / 5.
  * To the page operators (pk_copy_blocks and those after it) such a cache is one of row_elems =
  * pk_fp4_row_bytes / 2 16-bit elements where that is a multiple of 8, which it always is.
@@ -598,19 +599,22 @@ int pk_compact_blocks(void* k_caches, void* v_caches, int64_t k_layer_stride, in
  *   sees what later steps read. The norm's root is taken in 64 bits and no products are fused, so a key's
  *   4-bit values follow from the formula alone. A row whose squares sum to no finite number is NaN.
  * pk_gather_kv_fp4 -- pk_gather_kv of such a cache: the values of every sequence's rows in bf16, (sum Lk,
- *   num_kv_heads, head_dim). Sequence b's rows begin at cu_seqlens_k[b]; rows at and past max_seqlen_k are not
- *   written. Rows of table entries that are no block are 0.
+ *   num_kv_heads, head_dim). Sequence b's rows begin at cu_seqlens_k[b]; its rows at and past max_seqlen_k, and
+ *   rows past dst's num_rows, are not written. Rows of table entries that are no block are 0.
  * pk_varlen_attention_fp4 -- pk_varlen_attention in paged mode over such caches, in q's and out's layout, mask
  *   and GQA groups: sequences with any number of query rows in one call (one, a few, chunks). The keys
  *   of a table entry that is no block are seen by no row. Sequences without rows or keys are passed over, rows
  *   past max_seqlen_q not written, keys past max_seqlen_k ignored; a row that sees no key (or none with a
  *   score above -infinity) is written as 0.
- *   num_rows: the rows of q, cu_seqlens_q[num_seqs] or more. Softmax, sums and partial results are fp32, the
+ *   num_rows: the rows of q, cu_seqlens_q[num_seqs] or more; q's row stride below 2^25. block_size a multiple
+ *   of 64, GQA groups of 1, 2, 4 or 8. Softmax, sums and partial results are fp32, the
  *   weights rounded to bf16 for the product with V. NaN blocks reach the rows that see them and no
  *   others. A row's result depends on the call's other sequences by the rounding of its partial sums; equal
  *   calls give equal bits. At most 2^31 steps of 64 keys over the call's bounds.
- *   workspace: pk_varlen_attention_fp4_workspace_bytes, 256-byte aligned (at most about 350 MB, 34 MB when
- *   max_seqlen_q is 1); calls that may overlap must not share one.
+ *   workspace: pk_varlen_attention_fp4_workspace_bytes, 256-byte aligned (at most 520 bytes for 512
+ *   num_kv_heads min(16, max_seqlen_q num_heads / num_kv_heads) partial results, 4.3 MB for single rows of 16
+ *   heads on 8, and 68 MB more where a sequence may have more columns than 16); calls that may overlap
+ *   must not share one.
  */
 size_t pk_fp4_row_bytes(int32_t num_kv_heads);
 int pk_store_kvcache_fp4(const void* key, int64_t key_row_stride, const void* value, int64_t value_row_stride,
@@ -624,7 +628,7 @@ int pk_qk_norm_rope_store_fp4(const void* qkv, int64_t qkv_row_stride, const int
                               const int32_t* slot_mapping, int64_t num_slots, pk_stream_t stream);
 int pk_gather_kv_fp4(const void* cache, int64_t block_stride, int32_t num_blocks, int32_t block_size,
                      int32_t num_kv_heads, int32_t head_dim, const int32_t* block_table, int32_t block_table_stride,
-                     const int32_t* cu_seqlens_k, int32_t num_seqs, int32_t max_seqlen_k, void* dst,
+                     const int32_t* cu_seqlens_k, int32_t num_seqs, int32_t max_seqlen_k, int64_t num_rows, void* dst,
                      pk_stream_t stream);
 size_t pk_varlen_attention_fp4_workspace_bytes(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
                                                int32_t max_seqlen_q, int32_t max_seqlen_k);

@@ -1154,14 +1154,16 @@ int pk_qk_norm_rope_store_fp4(const void* qkv, int64_t qkv_row_stride, const int
 
 int pk_gather_kv_fp4(const void* cache, int64_t block_stride, int32_t num_blocks, int32_t block_size,
                      int32_t num_kv_heads, int32_t head_dim, const int32_t* block_table, int32_t block_table_stride,
-                     const int32_t* cu_seqlens_k, int32_t num_seqs, int32_t max_seqlen_k, void* dst, pk_stream_t stream) {
+                     const int32_t* cu_seqlens_k, int32_t num_seqs, int32_t max_seqlen_k, int64_t num_rows, void* dst,
+                     pk_stream_t stream) {
   g_last_error.clear();
   const char* what = "gather_kv_fp4";
   if (int rc = fp4_heads(what, num_kv_heads, head_dim)) return rc;
+  if (num_rows < 0) return fail(PK_ERR_INVALID_ARG, "%s: num_rows=%lld", what, (long long)num_rows);
   if (num_seqs < 0 || num_seqs > kMaxSeqs || max_seqlen_k < 0 || max_seqlen_k > kMaxSeqlen)
     return fail(PK_ERR_INVALID_ARG, "%s: num_seqs=%d (at most %d), max_seqlen_k=%d (at most %d)", what, num_seqs,
                 kMaxSeqs, max_seqlen_k, kMaxSeqlen);
-  if (num_seqs == 0 || max_seqlen_k == 0) return PK_OK;
+  if (num_seqs == 0 || max_seqlen_k == 0 || num_rows == 0) return PK_OK;
   if (int rc = fp4_blocks(what, block_stride, num_blocks, block_size, pk::fp4_row_bytes(num_kv_heads))) return rc;
   if (!cache || !block_table || !cu_seqlens_k || !dst) return fail(PK_ERR_INVALID_ARG, "%s: null pointer argument", what);
   if (!aligned16(cache) || !aligned16(dst))
@@ -1181,6 +1183,7 @@ int pk_gather_kv_fp4(const void* cache, int64_t block_stride, int32_t num_blocks
   a.cu_k = cu_seqlens_k;
   a.num_seqs = num_seqs;
   a.max_seqlen_k = max_seqlen_k;
+  a.num_rows = num_rows;
   a.dst = static_cast<uint16_t*>(dst);
   return hip_status(pk::launch_gather_fp4(a, reinterpret_cast<hipStream_t>(stream)), "gather_kv_fp4 launch");
 }
@@ -1217,6 +1220,8 @@ int pk_varlen_attention_fp4(const void* q, int64_t q_row_stride, const void* k_c
     return fail(PK_ERR_UNSUPPORTED, "%s: max_seqlen_q=%d / max_seqlen_k=%d above %d", what, max_seqlen_q, max_seqlen_k,
                 kMaxSeqlen);
   if (int rc = fp4_rows(what, "q", q, q_row_stride, num_heads)) return rc;
+  if (q_row_stride >= (1ll << 25))  // (16 rows' offsets in bytes are 32 bits)
+    return fail(PK_ERR_UNSUPPORTED, "%s: q row stride of %lld elements (below 2^25)", what, (long long)q_row_stride);
   if (int rc = fp4_rows(what, "out", out, out_row_stride, num_heads)) return rc;
   if (int rc = fp4_caches(what, k_cache, v_cache)) return rc;
   if (!block_table || !cu_seqlens_q || !cu_seqlens_k)

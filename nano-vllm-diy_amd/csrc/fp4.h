@@ -6,8 +6,8 @@
 //     num_kv_heads x 4 scale bytes, one per 32 dimensions;
 //     0 to 15 bytes up to a multiple of 16, never read or written.
 // A value is a sign, two bits of exponent and one of mantissa -- 0, 0.5, 1, 1.5, 2, 3, 4 or 6 -- times
-// 2^(scale byte - 127); scale byte 255 makes its 32 values NaN, 0, 253 and 254 do not occur. Two such products add up in bf16 without rounding,
-// so a value converts to bf16 exactly (v_cvt_scalef32_pk_bf16_fp4, which applies the scale's exponent as well).
+// 2^(scale byte - 127); scale byte 255 makes its 32 values NaN, 0, 253 and 254 do not occur. Every value is exact in
+// bf16 (v_cvt_scalef32_pk_bf16_fp4 applies the scale's exponent as it converts).
 // Token-major rows keep a page one run of bytes whose first n tokens are its first n rows, which is what the page
 // operators (kv_pages.hip) copy.
 #pragma once
@@ -110,7 +110,8 @@ struct Fp4GatherArgs {
   int32_t bt_stride;
   const int32_t* cu_k;
   int32_t num_seqs, max_seqlen_k;
-  uint16_t* dst;                 // (sum Lk, Hkv, D) bf16
+  int64_t num_rows;              // of dst
+  uint16_t* dst;                 // (num_rows, Hkv, D) bf16
 };
 hipError_t launch_store_fp4(const Fp4StoreArgs& a, hipStream_t stream);
 hipError_t launch_append_fp4(const Fp4AppendArgs& a, hipStream_t stream);

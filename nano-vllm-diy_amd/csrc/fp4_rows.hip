@@ -196,7 +196,8 @@ __global__ __launch_bounds__(kRowThreads) void gather_fp4_kernel(const Fp4Gather
   const int b = blockIdx.y;
   const int c = threadIdx.x & 15;
   const int k0 = a.cu_k[b];
-  const int len = min(a.cu_k[b + 1] - k0, a.max_seqlen_k);
+  if (k0 < 0) return;
+  const int64_t len = min((int64_t)min(a.cu_k[b + 1] - k0, a.max_seqlen_k), a.num_rows - k0);
   const int32_t* table = a.block_table + (int64_t)b * a.bt_stride;
   for (int64_t first = (int64_t)blockIdx.x * tokens; first < len; first += (int64_t)gridDim.x * tokens) {
     const int rows = (int)min((int64_t)tokens, len - first) * a.num_kv_heads;

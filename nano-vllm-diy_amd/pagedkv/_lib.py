@@ -179,7 +179,8 @@ SIGNATURES = {
     "pk_gather_kv_fp4": (ctypes.c_int, [
         _c_void_p, _i64, _i32, _i32,        # cache, block_stride, num_blocks, block_size
         _i32, _i32, _c_void_p, _i32,        # num_kv_heads, head_dim, block_table, its row stride
-        _c_void_p, _i32, _i32, _c_void_p, _c_void_p]),  # cu_seqlens_k, num_seqs, max_seqlen_k, dst, stream
+        _c_void_p, _i32, _i32, _i64,        # cu_seqlens_k, num_seqs, max_seqlen_k, num_rows
+        _c_void_p, _c_void_p]),             # dst, stream
     "pk_varlen_attention_fp4_workspace_bytes": (_size_t, [_i32, _i32, _i32, _i32, _i32]),
     "pk_varlen_attention_fp4": (ctypes.c_int, [
         _c_void_p, _i64, _c_void_p, _c_void_p,  # q, q_row_stride, k_cache, v_cache

@@ -23,6 +23,8 @@ every device operation is a hand-written gfx950 HIP kernel from libpagedkv.so:
 * a Context stating a shared prefix (ctx.cached_prefix_keys > 0) also selects the
   shared-prefix decode path: the decode rows' keys below it are computed once per shared
   block for all sequences that hold it (pk_varlen_attention_shared_prefix).
+* caches held in 4 bits (uint8, fp4.py) take the 4-bit store and attention; a stated prefix is a
+  hint of where to read from and changes nothing there.
 
 The runner rebinds k_cache / v_cache to per-layer views of its KV tensor
 (model_runner.py:159-165), exactly as with the reference layer.
@@ -32,6 +34,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from . import fp4
 from .context import Context
 from .ops import store_kvcache as _store_kvcache
 from .ops import store_decode_attention, varlen_attention
@@ -63,6 +66,8 @@ class Attention(nn.Module):
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ctx: Context) -> torch.Tensor:
         k_cache, v_cache = self.k_cache, self.v_cache
         bound = k_cache.numel() and v_cache.numel()
+        if bound and fp4.is_fp4_cache(k_cache):
+            return self._forward_fp4(q, k, v, ctx)
         hint = getattr(ctx, "cached_prefix_keys", None)  # absent on the reference Context
         if bound and ctx.block_tables is not None and ctx.max_seqlen_q == 1 and hint == 0 and \
                 q.shape[0] == k.shape[0] == ctx.cu_seqlens_q.numel() - 1 and _contiguous_blocks(k_cache) and \
@@ -90,3 +95,12 @@ class Attention(nn.Module):
             cached_prefix_keys=hint,
             shared_prefix_keys=shared,
         )
+
+    def _forward_fp4(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ctx: Context) -> torch.Tensor:
+        """forward over caches held in 4 bits. Without block tables the fresh keys and values are attended over as
+        they are given, as with 16-bit caches; through them, as they were rounded."""
+        fp4.store_kvcache_fp4(k, v, self.k_cache, self.v_cache, ctx.slot_mapping)
+        lens = (ctx.cu_seqlens_q, ctx.cu_seqlens_k, ctx.max_seqlen_q, ctx.max_seqlen_k)
+        if ctx.block_tables is None:
+            return varlen_attention(q, k, v, *lens, softmax_scale=self.scale, causal=True)
+        return fp4.varlen_attention_fp4(q, self.k_cache, self.v_cache, *lens, ctx.block_tables, self.scale)

@@ -9,7 +9,8 @@ lowest number first, in the order of the call's list, so every result is reprodu
 read back to the host, so all of it can run under torch.cuda.graph capture; calls on one pool have
 to be ordered (one stream, or events between streams).
 
-Caches are (L, NB, BS, Hkv, D) tensors as the runner keeps them, or one layer's (NB, BS, Hkv, D).
+Caches are (L, NB, BS, Hkv, D) tensors as the runner keeps them, or one layer's (NB, BS, Hkv, D); held in
+4 bits they are (L, NB, BS, row) or (NB, BS, row), uint8 (fp4.py).
 """
 from __future__ import annotations
 
@@ -17,6 +18,7 @@ import torch
 
 from ._call import call, scratch
 from ._lib import lib
+from .fp4 import _cache as check_fp4_cache
 from .ops import _req_i32
 
 
@@ -32,8 +34,19 @@ def _list_i32(name: str, t: torch.Tensor, device: torch.device) -> int:
     return shape[0]
 
 
+def _fp4_as_16bit(name: str, c: torch.Tensor) -> torch.Tensor:
+    """A cache held in 4 bits as one of 16-bit elements, with a head dimension: pages are copied as bytes."""
+    if c.dim() not in (3, 4):
+        raise ValueError(f"{name} cache of 4 bits must be (L, NB, BS, row) or (NB, BS, row), got {tuple(c.shape)}")
+    one_layer = c if c.dim() == 3 else c[0] if c.shape[0] else c.new_empty(c.shape[1:])
+    check_fp4_cache(f"{name} cache", one_layer, c.device)
+    return c.view(torch.int16).unsqueeze(-2)
+
+
 def _cache_args(k: torch.Tensor, v: torch.Tensor):
     """(pointers, strides, sizes) of the C-ABI for a pair of caches, and their device."""
+    if k.dtype is torch.uint8 and v.dtype is torch.uint8:
+        k, v = _fp4_as_16bit("k", k), _fp4_as_16bit("v", v)
     shape, ks, vs = k.shape, k.stride(), v.stride()
     if v.shape != shape or len(shape) not in (4, 5):
         raise ValueError("caches must be two (L, NB, BS, Hkv, D) or (NB, BS, Hkv, D) tensors of one shape")

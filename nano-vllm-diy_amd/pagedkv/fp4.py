@@ -165,7 +165,7 @@ def gather_kv_fp4(cache: torch.Tensor, block_table: torch.Tensor, cu_seqlens_k: 
     of entries that are no block are 0).
 
     total_k (= cu_seqlens_k[-1]) sizes the output; pass it to avoid a device read. max_seqlen_k must bound every
-    length (rows past it are not written)."""
+    length (rows past it, or past total_k, are not written)."""
     dev = cache.device
     heads = _cache("cache", cache, dev)
     num_seqs = cu_seqlens_k.numel() - 1
@@ -178,7 +178,7 @@ def gather_kv_fp4(cache: torch.Tensor, block_table: torch.Tensor, cu_seqlens_k: 
     dst = torch.empty(total_k, heads, HEAD_DIM, dtype=_BF16, device=dev)
     if total_k and num_seqs:
         call(lib().pk_gather_kv_fp4, "pk_gather_kv_fp4", dev, cache.data_ptr(), cache.stride(0), cache.shape[0],
-             cache.shape[1], heads, HEAD_DIM, bt_ptr, bt_stride, cu_ptr, num_seqs, int(max_seqlen_k), dst.data_ptr())
+             cache.shape[1], heads, HEAD_DIM, bt_ptr, bt_stride, cu_ptr, num_seqs, int(max_seqlen_k), total_k, dst.data_ptr())
     return dst
 
 

@@ -21,7 +21,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
-from . import lora, ops
+from . import fp4, lora, ops
 from .context import Context
 
 
@@ -85,7 +85,8 @@ class Qwen3Adapters:
 
 
 class Qwen3Model:
-    """Forward over one step's tokens; K/V caches are (L, NB, BS, Hkv, D) per operand."""
+    """Forward over one step's tokens; K/V caches are (L, NB, BS, Hkv, D) per operand, or held in
+    4 bits (L, NB, BS, fp4_row_bytes(Hkv)) uint8."""
 
     def __init__(self, cfg: Qwen3Config, weights: Qwen3Weights, k_caches: torch.Tensor | None,
                  v_caches: torch.Tensor | None, max_position: int):
@@ -106,9 +107,19 @@ class Qwen3Model:
         self.adapters = adapters
 
     def bind_caches(self, k_caches: torch.Tensor | None, v_caches: torch.Tensor | None) -> None:
-        """Per-layer K/V cache views, (L, NB, BS, Hkv, D) per operand (model_runner.py:161-165)."""
+        """Per-layer K/V cache views, (L, NB, BS, Hkv, D) per operand (model_runner.py:161-165), or
+        (L, NB, BS, row) uint8 of a cache held in 4 bits."""
         if (k_caches is None) != (v_caches is None):
             raise ValueError("bind both caches or neither")
+        if k_caches is not None and (fp4.is_fp4_cache(k_caches) or fp4.is_fp4_cache(v_caches)):
+            cfg = self.cfg
+            row = fp4.fp4_row_bytes(cfg.num_key_value_heads)
+            for c in (k_caches, v_caches):
+                if not fp4.is_fp4_cache(c) or cfg.head_dim != fp4.HEAD_DIM or c.dim() != 4 or \
+                        c.shape[0] != cfg.num_hidden_layers or c.shape[3] != row:
+                    raise ValueError(f"caches held in 4 bits must both be ({cfg.num_hidden_layers}, NB, BS, {row}) uint8 "
+                                     f"for {cfg.num_key_value_heads} kv heads of {fp4.HEAD_DIM}, got "
+                                     f"{tuple(c.shape)} {c.dtype} for heads of {cfg.head_dim}")
         self.k_caches = k_caches
         self.v_caches = v_caches
 
@@ -137,7 +148,10 @@ class Qwen3Model:
         ctx.cached_prefix_keys has Attention.forward's meaning, and None states, as 0 does, that no
         block is shared (the engine has no prefix cache): decode reads stream, and a decode step
         stores inside the attention launch. Forks share full blocks, which the one launch may read
-        too; with the bound stated (above 0) they are computed once, after a store of its own."""
+        too; with the bound stated (above 0) they are computed once, after a store of its own.
+        Caches held in 4 bits: every step is the 4-bit append and attention, whatever the bound; a fresh
+        prompt attends over the values that its stored rows hold, so what is computed does not hang on how
+        a prompt is cut into steps."""
         cfg, W = self.cfg, self.w
         Hq, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         eps = cfg.rms_norm_eps
@@ -173,7 +187,15 @@ class Qwen3Model:
                 x, residual = ops.add_rmsnorm(h, L["input_norm"], eps, residual=residual)
             qkv = project(x, L, li, "qkv")
             kc, vc = (None, None) if self.k_caches is None else (self.k_caches[li], self.v_caches[li])
-            if decode:
+            if kc is not None and fp4.is_fp4_cache(kc):
+                q, k, v = fp4.qk_norm_rope_store_fp4(qkv, positions, self.cos_sin, Hq, Hkv, D, L["q_norm"], L["k_norm"],
+                                                     eps, kc, vc, ctx.slot_mapping, return_kv=flat)
+                lens = (ctx.cu_seqlens_q, ctx.cu_seqlens_k, ctx.max_seqlen_q, ctx.max_seqlen_k)
+                if flat:
+                    o = ops.varlen_attention(q, k, v, *lens, self.scale, True)
+                else:
+                    o = fp4.varlen_attention_fp4(q, kc, vc, *lens, ctx.block_tables, self.scale)
+            elif decode:
                 # one launch: q/k norm + RoPE, the K/V store and paged decode attention; no
                 # block is stated to be shared, so every decode read streams
                 o = ops.qkv_decode_attention(qkv, positions, self.cos_sin, Hq, Hkv, D, L["q_norm"], L["k_norm"],

@@ -24,6 +24,8 @@ import torch
 from . import ops
 from ._host import Step
 from .context import Context
+from .fp4 import HEAD_DIM as FP4_HEAD_DIM
+from .fp4 import fp4_row_bytes
 from .qwen3 import Qwen3Config, Qwen3Model, Qwen3Weights
 
 
@@ -43,19 +45,24 @@ def context_buckets(max_seq_len: int, smallest: int = 512) -> list[int]:
 
 def kv_cache_num_blocks(num_layers: int, block_size: int, num_kv_heads: int, head_dim: int,
                         gpu_memory_utilization: float = 0.9, requested: int | None = None,
-                        itemsize: int = 2, device: torch.device | str | None = None) -> int:
+                        itemsize: int = 2, device: torch.device | str | None = None,
+                        row_bytes: int | None = None) -> int:
     """KV-cache blocks that fit in gpu_memory_utilization of the device, as the reference
     sizes its cache (model_runner.py:149-157): total x utilization, minus what is in use,
     minus the allocator's peak beyond its current allocation (the activations a forward pass
     needs on top of the weights), divided by one block's K and V over all layers. A request
     above that raises, as the reference's assert does; requested None or <= 0 takes them all.
+    row_bytes: the bytes of a token's row of K or of V where they are not heads x head_dim elements
+    (fp4_row_bytes(num_kv_heads) of a cache held in 4 bits).
     """
     free, total = torch.cuda.mem_get_info(device)
     used = total - free
     stats = torch.cuda.memory_stats(device)
     peak = stats["allocated_bytes.all.peak"]
     current = stats["allocated_bytes.all.current"]
-    block_bytes = 2 * num_layers * block_size * num_kv_heads * head_dim * itemsize
+    if row_bytes is None:
+        row_bytes = num_kv_heads * head_dim * itemsize
+    block_bytes = 2 * num_layers * block_size * row_bytes
     max_blocks = int(total * gpu_memory_utilization - used - peak + current) // block_bytes
     if requested is None or requested <= 0:
         requested = max_blocks
@@ -70,11 +77,18 @@ class ModelRunner:
     def __init__(self, cfg: Qwen3Config, device: torch.device | str, num_blocks: int | None,
                  block_size: int = 256, max_seq_len: int = 8192, max_graph_bs: int = 128,
                  enforce_eager: bool = False, seed: int = 5, gpu_memory_utilization: float = 0.9,
-                 max_num_batched_tokens: int = 16384, max_num_seqs: int = 512):
+                 max_num_batched_tokens: int = 16384, max_num_seqs: int = 512, kv_cache_dtype: str = "bf16"):
         """As the reference's runner (model_runner.py:35-56): the weights, a warmup forward at
         the largest step (warmup_model), then the KV cache -- num_blocks None: as many blocks
         as fit in gpu_memory_utilization of the device beside the weights and the warmup's
-        activation peak (kv_cache_num_blocks) -- then the decode graphs."""
+        activation peak (kv_cache_num_blocks) -- then the decode graphs.
+        kv_cache_dtype (an addition): "bf16", or "fp4" for a cache held in 4 bits (fp4.py), 3.76 times
+        the blocks in the same memory."""
+        if kv_cache_dtype not in ("bf16", "fp4"):
+            raise ValueError(f'kv_cache_dtype must be "bf16" or "fp4", got {kv_cache_dtype!r}')
+        if kv_cache_dtype == "fp4" and (cfg.head_dim != FP4_HEAD_DIM or block_size % 64):
+            raise ValueError(f"a cache held in 4 bits takes heads of {FP4_HEAD_DIM} and blocks of a multiple of 64 tokens, "
+                             f"got {cfg.head_dim} and {block_size}")
         self.cfg = cfg
         self.dev = torch.device(device)
         self.block_size = block_size
@@ -86,11 +100,16 @@ class ModelRunner:
         stats = torch.cuda.memory_stats(self.dev)
         # what the sizing keeps free for activations: the warmup's peak above the weights
         self.activation_headroom = stats["allocated_bytes.all.peak"] - stats["allocated_bytes.all.current"]
+        row_bytes = fp4_row_bytes(Hkv) if kv_cache_dtype == "fp4" else None
         if num_blocks is None:
-            num_blocks = kv_cache_num_blocks(L, block_size, Hkv, D, gpu_memory_utilization, device=self.dev)
+            num_blocks = kv_cache_num_blocks(L, block_size, Hkv, D, gpu_memory_utilization, device=self.dev,
+                                             row_bytes=row_bytes)
         self.num_blocks = num_blocks
-        self.kv_cache = torch.empty(2, L, num_blocks, block_size, Hkv, D, dtype=torch.bfloat16,
-                                    device=self.dev)
+        if kv_cache_dtype == "fp4":
+            self.kv_cache = torch.empty(2, L, num_blocks, block_size, row_bytes, dtype=torch.uint8, device=self.dev)
+        else:
+            self.kv_cache = torch.empty(2, L, num_blocks, block_size, Hkv, D, dtype=torch.bfloat16,
+                                        device=self.dev)
         self.model.bind_caches(self.kv_cache[0], self.kv_cache[1])
         self.graphs: dict[tuple[int, int], torch.cuda.CUDAGraph] = {}
         self.graph_bs: list[int] = []

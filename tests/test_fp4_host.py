@@ -21,7 +21,7 @@ CALLS = {
                                       k_out=None, k_out_stride=0, v_out=None, v_out_stride=0, k=PTR, v=PTR, slots=PTR,
                                       num_slots=64, stream=None),
     "pk_gather_kv_fp4": dict(cache=PTR, block_stride=64 * 544, nb=4, bs=64, kv=8, d=128, table=PTR, table_stride=4,
-                             cu_k=PTR, num_seqs=2, max_k=200, dst=PTR, stream=None),
+                             cu_k=PTR, num_seqs=2, max_k=200, rows=300, dst=PTR, stream=None),
     "pk_varlen_attention_fp4": dict(q=PTR, q_stride=2048, k=PTR, v=PTR, k_block=64 * 544, v_block=64 * 544, nb=4, bs=64,
                                     table=PTR, table_stride=4, cu_q=PTR, cu_k=PTR, num_seqs=2, rows=2, max_q=1,
                                     max_k=200, heads=16, kv=8, d=128, scale=0.1, causal=1, out=PTR, out_stride=2048,
@@ -55,12 +55,13 @@ def _call(name, **kw):
     ("pk_gather_kv_fp4", dict(block_stride=64 * 544 - 16), ARG), ("pk_gather_kv_fp4", dict(block_stride=64 * 544 + 8), ARG),
     ("pk_gather_kv_fp4", dict(nb=0), ARG), ("pk_gather_kv_fp4", dict(bs=0), ARG), ("pk_gather_kv_fp4", dict(max_k=257), ARG),
     ("pk_gather_kv_fp4", dict(max_k=-1), ARG), ("pk_gather_kv_fp4", dict(dst=None), ARG),
-    ("pk_gather_kv_fp4", dict(cache=PTR + 8), ARG),
+    ("pk_gather_kv_fp4", dict(cache=PTR + 8), ARG), ("pk_gather_kv_fp4", dict(rows=-1), ARG),
     ("pk_varlen_attention_fp4", dict(d=64), UNSUPPORTED), ("pk_varlen_attention_fp4", dict(heads=20), ARG),
     ("pk_varlen_attention_fp4", dict(heads=24), UNSUPPORTED), ("pk_varlen_attention_fp4", dict(num_seqs=-1), ARG),
     ("pk_varlen_attention_fp4", dict(num_seqs=70000), ARG), ("pk_varlen_attention_fp4", dict(rows=-1), ARG),
     ("pk_varlen_attention_fp4", dict(max_q=-1), ARG), ("pk_varlen_attention_fp4", dict(max_k=1 << 23), UNSUPPORTED),
     ("pk_varlen_attention_fp4", dict(q=None), ARG), ("pk_varlen_attention_fp4", dict(q_stride=2040), ARG),
+    ("pk_varlen_attention_fp4", dict(q_stride=1 << 25), UNSUPPORTED),
     ("pk_varlen_attention_fp4", dict(out=PTR + 8), ARG), ("pk_varlen_attention_fp4", dict(out_stride=2050), ARG),
     ("pk_varlen_attention_fp4", dict(bs=96, k_block=96 * 544, v_block=96 * 544), ARG),
     ("pk_varlen_attention_fp4", dict(k_block=64 * 543), ARG), ("pk_varlen_attention_fp4", dict(v_block=8), ARG),
@@ -79,6 +80,7 @@ def test_nothing_to_do_touches_no_pointer():
     assert _call("pk_store_kvcache_fp4", n=0, key=None, k=None) == 0
     assert _call("pk_qk_norm_rope_store_fp4", n=0, qkv=None) == 0
     assert _call("pk_gather_kv_fp4", num_seqs=0, cache=None) == 0
+    assert _call("pk_gather_kv_fp4", rows=0, cache=None) == 0
     for kw in (dict(num_seqs=0), dict(rows=0), dict(max_q=0), dict(max_k=0)):
         assert _call("pk_varlen_attention_fp4", q=None, out=None, **kw) == 0
 
@@ -95,8 +97,8 @@ def test_row_bytes():
 
 def test_workspace_bytes():
     one = pagedkv.fp4_workspace_bytes(256, 16, 8, 1, 8192)
-    assert 0 < one <= 40 << 20
-    assert one < pagedkv.fp4_workspace_bytes(256, 16, 8, 512, 8192) <= 350 << 20
+    assert 0 < one <= 5 << 20
+    assert one < pagedkv.fp4_workspace_bytes(256, 16, 8, 512, 8192) <= 105 << 20
     for bad in ((0, 16, 8, 1, 64), (1, 16, 0, 1, 64), (1, 15, 8, 1, 64), (1, 16, 8, 0, 64), (1, 16, 8, 1, 0)):
         assert pagedkv.fp4_workspace_bytes(*bad) == 0
 
