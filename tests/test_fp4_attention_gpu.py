@@ -307,3 +307,10 @@ def test_append_then_attend_as_a_step_does(gpu):
         _check(c, _run(c))
     cu = _cu(have, gpu)
     assert torch.equal(pagedkv.gather_kv_fp4(kc, tables.to(gpu), cu, max(have), sum(have)), torch.cat(keys))
+
+
+@pytest.mark.parametrize("heads,kv", [(22, 11), (24, 12), (40, 40), (112, 14)])
+def test_head_counts_that_no_slot_count_divides(gpu, heads, kv):
+    """Work-groups of 1, 6, 8 and 7 kv heads, more than one of them side by side."""
+    c = _case(gpu, heads, kv, [(1, 200), (2, 90), (1, 1), (40, 130), (3, 64), (1, 700)], seed=heads)
+    _check(c, _run(c))

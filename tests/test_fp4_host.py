@@ -187,3 +187,56 @@ def test_attention_and_gather_wrapper_refusals():
             pagedkv.gather_kv_fp4(**{**dict(cache=kc, block_table=table, cu_seqlens_k=cu, max_seqlen_k=100, total_k=4), **kw})
     with pytest.raises(ValueError, match="GPU"):
         pagedkv.varlen_attention_fp4(**ok)
+
+
+def test_page_operators_refuse_what_is_no_fp4_cache():
+    one = torch.zeros(1, dtype=torch.int32)
+    k = torch.zeros(2, 4, 64, 544, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="one GPU"):  # (the shapes are taken)
+        pagedkv.copy_blocks(k, k.clone(), one, one)
+    with pytest.raises(ValueError, match="one GPU"):
+        pagedkv.copy_blocks(k[0], k[1], one, one)
+    for bad in (k[..., :540], k[..., :528].contiguous(), k[0, 0], k.unsqueeze(0)):
+        with pytest.raises(ValueError, match="4 bits|4-bit rows|contiguous"):
+            pagedkv.copy_blocks(bad, bad.clone(), one, one)
+    with pytest.raises(ValueError, match="one shape"):
+        pagedkv.copy_blocks(k, k[:1].clone(), one, one)
+    with pytest.raises((TypeError, ValueError)):
+        pagedkv.copy_blocks(k, torch.zeros(2, 4, 64, 2, 128, dtype=torch.bfloat16), one, one)
+
+
+def test_model_and_runner_refusals():
+    from pagedkv.qwen3 import Qwen3Config, Qwen3Model, Qwen3Weights
+    from pagedkv.runner import ModelRunner
+    cfg = Qwen3Config(vocab_size=32, hidden_size=64, num_hidden_layers=2, num_attention_heads=2, num_key_value_heads=1,
+                      intermediate_size=96, max_position_embeddings=64)
+    model = Qwen3Model(cfg, Qwen3Weights(cfg, torch.device("cpu")), None, None, 64)
+    good = torch.zeros(2, 4, 64, 80, dtype=torch.uint8)
+    model.bind_caches(good, good.clone())
+    wide = torch.zeros(2, 4, 64, 1, 128, dtype=torch.bfloat16)
+    model.bind_caches(wide, wide.clone())
+    for k, v in ((good, wide), (wide, good), (good[:1], good[:1]), (good[..., :64], good[..., :64]),
+                 (torch.zeros(2, 4, 64, 144, dtype=torch.uint8),) * 2, (good[0], good[0])):
+        with pytest.raises(ValueError, match="4 bits"):
+            model.bind_caches(k, v)
+    with pytest.raises(ValueError, match="kv_cache_dtype"):
+        ModelRunner(cfg, "cpu", 4, kv_cache_dtype="fp8")
+    with pytest.raises(ValueError, match="64 tokens"):
+        ModelRunner(cfg, "cpu", 4, block_size=32, kv_cache_dtype="fp4")
+
+
+@pytest.mark.parametrize("flat", [True, False])
+@pytest.mark.parametrize("hint", [None, 0, 64])
+def test_attention_layer_takes_the_4_bit_operators(monkeypatch, flat, hint):
+    from pagedkv import attention
+    calls = []
+    monkeypatch.setattr(attention.fp4, "store_kvcache_fp4", lambda k, v, kc, vc, slots: calls.append("store"))
+    monkeypatch.setattr(attention.fp4, "varlen_attention_fp4", lambda q, *a: calls.append("paged") or q)
+    monkeypatch.setattr(attention, "varlen_attention", lambda q, *a, **kw: calls.append("flat") or q)
+    layer = pagedkv.Attention(128, 2, 1, 0.1)
+    layer.k_cache = layer.v_cache = torch.zeros(4, 64, 80, dtype=torch.uint8)
+    q, k = torch.zeros(3, 2, 128, dtype=torch.bfloat16), torch.zeros(3, 1, 128, dtype=torch.bfloat16)
+    cu = torch.arange(4, dtype=torch.int32)
+    layer(q, k, k, pagedkv.Context(cu_seqlens_q=cu, cu_seqlens_k=cu, max_seqlen_q=1, max_seqlen_k=1, slot_mapping=cu[:3],
+                                   block_tables=None if flat else cu[:3, None], cached_prefix_keys=hint))
+    assert calls == ["store", "flat" if flat else "paged"]

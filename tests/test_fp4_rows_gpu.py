@@ -222,3 +222,40 @@ def test_captured_append_store_and_gather(gpu):
         want = step()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         assert torch.equal(kc, bytes_[0]) and torch.equal(vc, bytes_[1])
+
+
+@pytest.mark.parametrize("kv", [33, 70, 255])
+def test_more_head_rows_than_a_work_group_takes_at_once(gpu, kv):
+    """Store and read back of tokens of more than 64 head rows."""
+    g = _gen(kv)
+    n, nb, bs = 5, 2, 64
+    kc, vc = (_bytes(g, nb, bs, ref.row_bytes(kv), device=gpu) for _ in range(2))
+    key, value = _randn(g, n, kv, D, device=gpu), _randn(g, n, kv, D, device=gpu, scale=1e-3)
+    slots = [70, -1, 3, 64, 127]
+    want = _expect(kc, slots, key), _expect(vc, slots, value)
+    pagedkv.store_kvcache_fp4(key, value, kc, vc, torch.tensor(slots, dtype=torch.int32, device=gpu))
+    assert torch.equal(kc.cpu(), want[0]) and torch.equal(vc.cpu(), want[1])
+    kc[..., 64 * kv:68 * kv] = kc[..., 64 * kv:68 * kv].clamp(100, 150)
+    table = torch.tensor([[1], [0]], dtype=torch.int32, device=gpu)
+    cu = torch.tensor([0, 64, 68], dtype=torch.int32, device=gpu)
+    got = pagedkv.gather_kv_fp4(kc, table, cu, 64, 68)
+    assert torch.equal(got.cpu().double(), ref.values(torch.cat((kc[1], kc[0, :4])).cpu(), kv))
+
+
+def test_read_back_stops_at_its_output(gpu):
+    """Lengths that end past the output's rows, and past max_seqlen_k: nothing is written there."""
+    kv, bs = 2, 64
+    kc, _ = ref.make_cache(kv, 4, bs, _gen(2), gpu)
+    table = torch.tensor([[2, 0], [1, 3]], dtype=torch.int32, device=gpu)
+    cu = torch.tensor([0, 100, 228], dtype=torch.int32, device=gpu)
+    room = torch.full((256, kv, D), 7.0, dtype=torch.bfloat16, device=gpu)
+    rows = torch.cat((kc[2], kc[0, :36], kc[1], kc[3]))
+    from pagedkv._call import call
+    from pagedkv._lib import lib
+    call(lib().pk_gather_kv_fp4, "pk_gather_kv_fp4", gpu, kc.data_ptr(), kc.stride(0), 4, bs, kv, D, table.data_ptr(), 2,
+         cu.data_ptr(), 2, 120, 190, room.data_ptr())
+    assert torch.equal(room[:190].double(), ref.values(rows, kv)[:190]) and (room[190:] == 7).all()
+    room.fill_(7.0)
+    call(lib().pk_gather_kv_fp4, "pk_gather_kv_fp4", gpu, kc.data_ptr(), kc.stride(0), 4, bs, kv, D, table.data_ptr(), 2,
+         cu.data_ptr(), 2, 120, 256, room.data_ptr())
+    assert torch.equal(room[:220].double(), ref.values(rows, kv)[:220]) and (room[220:] == 7).all()
