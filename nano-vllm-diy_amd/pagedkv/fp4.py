@@ -58,6 +58,14 @@ def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, device: torch.device) 
 
 def _slot_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, device: torch.device) -> tuple[int, int]:
     """(kv heads, slots) of caches whose slot s is row s: contiguous blocks."""
+    shape = k_cache.shape
+    if len(shape) == 3 and v_cache.shape == shape and k_cache.dtype is v_cache.dtype is _U8 and \
+            k_cache.is_contiguous() and v_cache.is_contiguous() and k_cache.device == v_cache.device == device:
+        blocks, block_size, row = shape
+        heads = row // _HEAD_BYTES
+        if 0 < heads <= 255 and (_HEAD_BYTES * heads + 15) // 16 * 16 == row:
+            return heads, blocks * block_size
+    # (which of them it was)
     heads = _caches(k_cache, v_cache, device)
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("rows are stored into caches with contiguous blocks")
@@ -126,15 +134,17 @@ def qk_norm_rope_store_fp4(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: 
     width = (num_heads + 2 * num_kv_heads) * head_dim
     if heads != num_kv_heads or head_dim != HEAD_DIM:
         raise ValueError(f"caches hold {heads} kv heads of {HEAD_DIM}, got {num_kv_heads} of {head_dim}")
-    if qkv.dim() != 2 or qkv.dtype is not _BF16 or qkv.shape[1] != width or qkv.stride(1) != 1:
+    shape, stride = qkv.shape, qkv.stride()
+    if len(shape) != 2 or qkv.dtype is not _BF16 or shape[1] != width or stride[1] != 1:
         raise ValueError(f"qkv must be (N, {width}) bf16 with contiguous rows")
-    n = qkv.shape[0]
+    n = shape[0]
     if positions.dtype is not torch.int64 or positions.device != dev or positions.shape != (n,) or \
             not positions.is_contiguous():
         raise ValueError("positions must be a contiguous (N,) int64 tensor on the qkv device")
     if cos_sin.dim() == 3:
         cos_sin = cos_sin.squeeze(1)
-    if cos_sin.dtype is not torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[1] != HEAD_DIM or \
+    table = cos_sin.shape
+    if cos_sin.dtype is not torch.float32 or len(table) != 2 or table[1] != HEAD_DIM or \
             not cos_sin.is_contiguous() or cos_sin.device != dev:
         raise ValueError("cos_sin must be a contiguous (P, 128) float32 table on the qkv device")
     for name, w in (("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight)):
@@ -142,16 +152,18 @@ def qk_norm_rope_store_fp4(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: 
                               w.device != dev):
             raise ValueError(f"{name} must be a contiguous ({HEAD_DIM},) bf16 tensor on the qkv device")
     slot_ptr = _i32("slot_mapping", slot_mapping, n, dev)
+    q_stride, row = num_heads * HEAD_DIM, heads * HEAD_DIM
     if q_out is None:
         q_out = torch.empty(n, num_heads, HEAD_DIM, dtype=_BF16, device=dev)
-    q_stride = _rows("q_out", q_out, n, num_heads, dev)
+    else:
+        q_stride = _rows("q_out", q_out, n, num_heads, dev)
     k = v = None
     if return_kv:
-        k, v = (torch.empty(n, heads, HEAD_DIM, dtype=_BF16, device=dev) for _ in range(2))
-    row = heads * HEAD_DIM
+        k = torch.empty(n, heads, HEAD_DIM, dtype=_BF16, device=dev)
+        v = torch.empty_like(k)
     if n:
         call(lib().pk_qk_norm_rope_store_fp4, "pk_qk_norm_rope_store_fp4", dev, qkv.data_ptr(),
-             qkv.stride(0) if n > 1 else width, positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0],
+             stride[0] if n > 1 else width, positions.data_ptr(), cos_sin.data_ptr(), table[0],
              0 if q_norm_weight is None else q_norm_weight.data_ptr(),
              0 if k_norm_weight is None else k_norm_weight.data_ptr(), float(eps), n, num_heads, heads, HEAD_DIM,
              q_out.data_ptr(), q_stride, 0 if k is None else k.data_ptr(), row, 0 if v is None else v.data_ptr(), row,
@@ -210,9 +222,11 @@ def varlen_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         raise ValueError("cu_seqlens_q must have one more entry than there are sequences")
     cu_q, cu_k = _i32("cu_seqlens_q", cu_seqlens_q, num_seqs + 1, dev), _i32("cu_seqlens_k", cu_seqlens_k, num_seqs + 1, dev)
     bt_ptr, bt_stride = _table(block_table, num_seqs, max_seqlen_k, k_cache.shape[1], dev)
+    out_stride = num_heads * HEAD_DIM
     if out is None:
         out = torch.empty(n, num_heads, HEAD_DIM, dtype=_BF16, device=dev)
-    out_stride = _rows("out", out, n, num_heads, dev)
+    else:
+        out_stride = _rows("out", out, n, num_heads, dev)
     if not n or not num_seqs:
         return out
     nbytes = fp4_workspace_bytes(num_seqs, num_heads, heads, max_seqlen_q, max_seqlen_k)
