@@ -47,8 +47,7 @@ constexpr int kManyCols = kManyWaves * kManyTiles * 16;
 constexpr int kManyStep = 64;         // keys of its step
 constexpr int kManyRing = 4;          // steps of 4-bit rows in LDS
 constexpr int kSub = 32;              // keys a wavefront takes at once
-constexpr int kSlots = 8;             // sequences a lane keeps the steps of
-constexpr int kChunk = kSlots * kWave;
+constexpr int kChunk = 64 * kWave;    // sequences whose steps are in LDS at a time
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kSlack = 8.f;         // the scores may exceed their reference by this (exp2 domain)
 
@@ -59,6 +58,7 @@ typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+typedef __attribute__((address_space(3))) int lds_i32;
 typedef __attribute__((address_space(3))) float lds_f32;
 typedef __attribute__((address_space(3))) f32x2 lds_f32x2;
 
@@ -150,60 +150,76 @@ struct Tile {
   int steps;
 };
 
+// Waits until the wavefronts' reads and writes of LDS are over.
+__device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// n / d rounded down, of whole numbers below 2^53, the same for the wavefront: a quotient that is not whole is at least
+// 1 / d below the next one, more than 2^-53 of it, so the rounding of 64-bit floating point does not reach it. (An
+// eighth of the instructions of the division of 64-bit integers.)
+__device__ __forceinline__ int64_t div_floor(int64_t n, int64_t d) {
+  const int64_t q = (int64_t)((double)n / (double)d);
+  return (int64_t)((uint64_t)(uint32_t)uniform((int)(q >> 32)) << 32 | (uint32_t)uniform((int)q));
+}
+
 // The line of steps: MANY: kv head by kv head, sequence by sequence, tile by tile; otherwise the sequences' steps,
-// which the wavefronts take for a kv head each.
+// which the wavefronts take for a kv head each. A chunk's steps are summed up in LDS, a thread to a sequence, and looked
+// up from there. (With every wavefront keeping the steps of 512 sequences in registers, and beginning with the first
+// of all sequences for every piece: 106 us in place of 77 for 1024 sequences of 100-400 keys, 5165 in place of 360
+// for 16384 of 16-64, 36.8 in place of 35.8 for 128 of 100-2048.)
 template <bool MANY, int STEP>
 struct Line {
-  int n[kSlots];     // steps of sequence `base` + 64 s + lane
-  int base;
+  static constexpr int kBytes = (kChunk + kWave) * 4;
+  lds_i32* sums;     // [kChunk] steps of a group of 64 sequences up to and with each of them, [64] of whole groups
+  int base, before;  // the chunk's first sequence, the steps before it
   int per_head;      // steps of all sequences
   int64_t total;
 
-  __device__ __forceinline__ void load(const Fp4AttnArgs& a, int first, int lane) {
+  // (every wavefront of the work-group comes here)
+  __device__ __forceinline__ void load(const Fp4AttnArgs& a, int first, int steps_before, int wave, int lane) {
     base = first;
-#pragma unroll
-    for (int s = 0; s < kSlots; ++s) {
-      n[s] = 0;
-      const int b = first + 64 * s + lane;
-      if (first + 64 * s < a.num_seqs && b < a.num_seqs) n[s] = seq_steps<MANY, STEP>(a, seq_of(a, b));
+    before = steps_before;
+    meet();  // the last chunk has been read
+#pragma unroll 1
+    for (int group = wave; group < kWave; group += 8) {
+      int sum = 0;
+      if (first + 64 * group < a.num_seqs) {
+        const int b = first + 64 * group + lane;
+        sum = scan64(b < a.num_seqs ? seq_steps<MANY, STEP>(a, seq_of(a, b)) : 0, lane);
+        sums[64 * group + lane] = sum;
+      }
+      if (lane == kWave - 1) sums[kChunk + group] = sum;
     }
+    meet();
   }
-  __device__ __forceinline__ void init(const Fp4AttnArgs& a, int lane) {
+  __device__ __forceinline__ void init(const Fp4AttnArgs& a, lds_u8* lds, int wave, int lane) {
+    sums = (lds_i32*)lds;
     per_head = 0;
     for (int first = 0; first < a.num_seqs; first += kChunk) {
-      load(a, first, lane);
-#pragma unroll
-      for (int s = 0; s < kSlots; ++s)
-        if (first + 64 * s < a.num_seqs) per_head += __builtin_amdgcn_readlane(scan64(n[s], lane), kWave - 1);
+      load(a, first, per_head, wave, lane);
+      per_head += __builtin_amdgcn_readlane(scan64(sums[kChunk + lane], lane), kWave - 1);
     }
     total = MANY ? (int64_t)per_head * a.num_kv_heads : per_head;
   }
-  // The tile at position p < total.
-  __device__ __forceinline__ Tile at(const Fp4AttnArgs& a, int64_t p, int lane) {
+  // The tile at position p < total. (Positions that grow walk the chunks once.)
+  __device__ __forceinline__ Tile at(const Fp4AttnArgs& a, int64_t p, int wave, int lane) {
     Tile t;
-    t.head = MANY ? (int)(p / per_head) : 0;
+    t.head = MANY ? (int)div_floor(p, per_head) : 0;
     t.j = 0;
     const int64_t head_start = (int64_t)t.head * per_head;
     const int want = (int)(p - head_start);
-    int before = 0, b = 0, seq_start = 0;
-    bool found = false;
-    for (int first = 0; first < a.num_seqs && !found; first += kChunk) {
-      if (base != first) load(a, first, lane);
-#pragma unroll
-      for (int s = 0; s < kSlots; ++s) {
-        if (!found && first + 64 * s < a.num_seqs) {
-          const int incl = before + scan64(n[s], lane);
-          const uint64_t m = __builtin_amdgcn_ballot_w64(want < incl);
-          if (m) {
-            const int j = __builtin_ctzll(m);
-            b = first + 64 * s + j;
-            seq_start = __builtin_amdgcn_readlane(incl - n[s], j);
-            found = true;
-          }
-          before = __builtin_amdgcn_readlane(incl, kWave - 1);
-        }
-      }
+    if (want < before) load(a, 0, 0, wave, lane);
+    int group_steps = sums[kChunk + lane], group_end = before + scan64(group_steps, lane);
+    while (want >= __builtin_amdgcn_readlane(group_end, kWave - 1)) {
+      load(a, base + kChunk, __builtin_amdgcn_readlane(group_end, kWave - 1), wave, lane);
+      group_steps = sums[kChunk + lane];
+      group_end = before + scan64(group_steps, lane);
     }
+    const int group = __builtin_ctzll(__builtin_amdgcn_ballot_w64(want < group_end));
+    const int group_start = __builtin_amdgcn_readlane(group_end - group_steps, group);
+    const int end = group_start + sums[64 * group + lane];
+    const int in_group = __builtin_ctzll(__builtin_amdgcn_ballot_w64(want < end));
+    const int seq_start = in_group ? __builtin_amdgcn_readlane(end, in_group - 1) : group_start;
+    const int b = base + 64 * group + in_group;
     const Seq s = uniform_seq(a, b);
     int start = seq_start, steps = tile_steps<MANY, STEP>(a, s, 0);
     if constexpr (MANY) {
@@ -236,11 +252,11 @@ struct Line {
 // (rounded down) on, so the runs differ by one step at most.
 struct Cuts {
   int64_t total;
-  int64_t runs;
-  __device__ __forceinline__ int64_t first(int64_t w) const { return w * total / runs; }
-  __device__ __forceinline__ int run_of(int64_t p) const { return (int)(((p + 1) * runs - 1) / total); }
+  int runs;
+  __device__ __forceinline__ int64_t first(int w) const { return div_floor(w * total, runs); }
+  __device__ __forceinline__ int run_of(int64_t p) const { return (int)div_floor((p + 1) * runs - 1, total); }
 };
-__device__ __forceinline__ Cuts cuts_of(int64_t total, int runs) { return {total, total < runs ? total : runs}; }
+__device__ __forceinline__ Cuts cuts_of(int64_t total, int runs) { return {total, (int)(total < runs ? total : runs)}; }
 
 // Partial result `slot` (2 run: a tile that began in an earlier run; 2 run + 1: one that goes on in the next),
 // of a kv head (few rows) or of the tile's only one.
@@ -331,12 +347,17 @@ struct Cursor {
   const int32_t* table;
   int t, entry, off, last, blk;
 
-  __device__ __forceinline__ void init(const Fp4AttnArgs& a, const int32_t* row, int first, int keys) {
+  // From `ahead` keys (fewer than 256) behind key t0 on, which is in the page `page`; the last key is in `last_page`.
+  __device__ __forceinline__ void init(const Fp4AttnArgs& a, const int32_t* row, int t0, int page, int last_page, int ahead) {
     table = row;
-    t = first;
-    entry = first / a.block_size;
-    off = first - entry * a.block_size;
-    last = (keys - 1) / a.block_size;
+    t = t0 + ahead;
+    entry = page;
+    off = t - page * a.block_size;
+    last = last_page;
+    while (off >= a.block_size) {
+      off -= a.block_size;
+      ++entry;
+    }
     blk = scalar_i32(table + min(entry, last));
   }
   // (the entry is waited for here, ahead of the reads of LDS that would otherwise be waited for together with it)
@@ -394,8 +415,9 @@ struct Loader {
     scale_row = r - scale_first;
     scale_col = a.num_kv_heads * kFp4HeadBytes + (head0 + min(h, heads - 1)) * kFp4HeadScales;
     scale_lds = (scales_of_v ? S::kCache : 0) + S::kValues + part * 256;
-    at.init(a, table, t0 + (first & ~31), keys);
-    scale_at.init(a, table, t0 + scale_first, keys);
+    const int page = t0 / a.block_size, last_page = (keys - 1) / a.block_size;
+    at.init(a, table, t0, page, last_page, first & ~31);
+    scale_at.init(a, table, t0, page, last_page, scale_first);
   }
 
   // The next step's rows into a stage of LDS; whether the wavefront's own 32 keys among them are in a block. A row that
@@ -733,14 +755,14 @@ struct Run {
   // False if there is nothing to do. Neighbouring runs of MANY, whose tiles read the same keys, go to one XCD
   // (work-groups go to the 8 of them in turn).
   __device__ __forceinline__ bool init(const Fp4AttnArgs& a, const Partials& part, int num_runs, int index, bool recorder,
-                                       int lane) {
-    line.init(a, lane);
+                                       lds_u8* lds, int wave, int lane) {
+    line.init(a, lds, wave, lane);
     cuts = cuts_of(line.total, num_runs);
-    if (index == 0 && recorder) *part.live = (int)cuts.runs;
+    if (index == 0 && recorder) *part.live = cuts.runs;
     if (line.total == 0) return false;
     run = index;
     if constexpr (MANY) {
-      const int per_xcd = ((int)cuts.runs + 7) >> 3;
+      const int per_xcd = (cuts.runs + 7) >> 3;
       if ((index >> 3) >= per_xcd) return false;
       run = (index & 7) * per_xcd + (index >> 3);
     }
@@ -750,9 +772,9 @@ struct Run {
     split = make_int4(0, 0, 0, 0);
     return true;
   }
-  __device__ __forceinline__ bool next(const Fp4AttnArgs& a, const Partials& part, int lane) {
+  __device__ __forceinline__ bool next(const Fp4AttnArgs& a, const Partials& part, int wave, int lane) {
     if (p >= end) return false;
-    tile = line.at(a, p, lane);
+    tile = line.at(a, p, wave, lane);
     seq = uniform_seq(a, tile.b);
     s0 = (int)(p - tile.start);
     s1 = (int)min((int64_t)tile.steps, end - tile.start);
@@ -810,7 +832,7 @@ __global__ __launch_bounds__(kFewWaves* kWave, 2) void attend_few_kernel(const F
   constexpr int kSlices = kFewWaves / HEADS, ROWS = kSub * kSlices;
   typedef Stage<HEADS, ROWS> S;
   typedef Loader<HEADS, ROWS> L;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[kFewRing * S::kBytes];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kFewRing * S::kBytes + Line<false, ROWS>::kBytes];
   lds_u8* const lds = (lds_u8*)smem;
   const int lds0 = (int)(uintptr_t)lds;
   const int lane = threadIdx.x & (kWave - 1);
@@ -819,17 +841,17 @@ __global__ __launch_bounds__(kFewWaves* kWave, 2) void attend_few_kernel(const F
   const int head0 = blockIdx.y * heads;
   const bool recorder = head0 == 0 && threadIdx.x == 0;
   Run<false, ROWS> run;
-  if (!run.init(a, part, runs, blockIdx.x, recorder, lane)) return;
+  if (!run.init(a, part, runs, blockIdx.x, recorder, lds + kFewRing * S::kBytes, wave, lane)) return;
   const int slot = wave % HEADS, slice = wave / HEADS;
   const bool live = slot < heads;
   const int head = head0 + min(slot, heads - 1);
   Queries queries;
   Lanes<HEADS, ROWS> at;
   at.init(slice * kSub, slot, lane);
-  while (run.next(a, part, lane)) {
+  while (run.next(a, part, wave, lane)) {
     const Seq seq = run.seq;
     const int s0 = run.s0, s1 = run.s1;
-    arrive_all();  // (the last piece's reads of LDS are over)
+    meet();  // the last piece has been read
     const int32_t* table = a.block_table + (int64_t)run.tile.b * a.bt_stride;
     L loader;
     loader.init(a, table, s0 * ROWS, seq.keys, head0, heads, wave, lane);
@@ -936,7 +958,7 @@ struct ManyLoader {
 
   __device__ __forceinline__ void init(const Fp4AttnArgs& a, const int32_t* table, int t0, int keys, int head, int wave,
                                        int lane) {
-    at.init(a, table, t0, keys);
+    at.init(a, table, t0, t0 / a.block_size, (keys - 1) / a.block_size, 0);
     const bool is_v = wave >= kManyWaves / 2;
     cache = is_v ? a.v : a.k;
     block = is_v ? a.v_block : a.k_block;
@@ -1012,7 +1034,7 @@ template <int T>
 __device__ __forceinline__ void many_take(State<T>& st, const lds_u8* tiles, const int (&k)[4], const int (&v)[8],
                                           bool masked, const int (&rel)[T], float c2, int lane) {
   constexpr int kTile16 = 16 * ManyLds::kRow;
-  constexpr int kAheadK = 4, kAheadV = 2;
+  constexpr int kAheadK = 4, kAheadV = 1;
   f32x4 s[4][T];
   u32x4 kw[kAheadK];
   u32x4 vw[kAheadV + 1][2];
@@ -1065,21 +1087,21 @@ __device__ __forceinline__ void many_take(State<T>& st, const lds_u8* tiles, con
 __global__ __launch_bounds__(kManyWaves* kWave, 2) void attend_many_kernel(const Fp4AttnArgs a, const Partials part, int runs) {
   constexpr int D = kHeadDim, T = kManyTiles;
   typedef ManyLds S;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[S::kBytes];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[S::kBytes + Line<true, kManyStep>::kBytes];
   lds_u8* const lds = (lds_u8*)smem;
   const int lds0 = (int)(uintptr_t)lds;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = uniform(threadIdx.x / kWave);
   const int n = lane & 15, g = lane >> 4;
   Run<true, kManyStep> run;
-  if (!run.init(a, part, runs, blockIdx.x, threadIdx.x == 0, lane)) return;
+  if (!run.init(a, part, runs, blockIdx.x, threadIdx.x == 0, lds + S::kBytes, wave, lane)) return;
   int k_at[4], v_at[8];
 #pragma unroll
   for (int c = 0; c < 4; ++c) k_at[c] = n * S::kRow + ((4 * c + g) ^ n) * 16;
   const int vr = 4 * g + (n >> 2);  // rows 4 g .. + 3, 8 bytes each
 #pragma unroll
   for (int j = 0; j < 8; ++j) v_at[j] = vr * S::kRow + ((2 * j + ((n & 3) >> 1)) ^ v_swizzle(vr)) * 16 + 8 * (n & 1);
-  while (run.next(a, part, lane)) {
+  while (run.next(a, part, wave, lane)) {
     const Seq seq = run.seq;
     const int s0 = run.s0, s1 = run.s1, head = run.tile.head;
     Columns<T> cols;

@@ -314,3 +314,16 @@ def test_head_counts_that_no_slot_count_divides(gpu, heads, kv):
     """Work-groups of 1, 6, 8 and 7 kv heads, more than one of them side by side."""
     c = _case(gpu, heads, kv, [(1, 200), (2, 90), (1, 1), (40, 130), (3, 64), (1, 700)], seed=heads)
     _check(c, _run(c))
+
+
+def test_more_sequences_than_are_in_lds(gpu):
+    """More than 4096 sequences: short ones, empty ones, chunks on both sides of the border, for several kv heads."""
+    g = torch.Generator().manual_seed(41)
+    lens = [(1, int(k)) for k in torch.randint(0, 90, (8500,), generator=g)]
+    for i, x in ((0, (70, 90)), (4094, (3, 200)), (4095, (150, 300)), (4096, (33, 33)), (4500, (0, 40)), (8191, (1, 700)),
+                 (8192, (20, 500)), (8499, (90, 90))):
+        lens[i] = x
+    c = _case(gpu, 4, 2, lens, seed=42)
+    out = torch.zeros_like(c["q"])
+    _run(c, out=out)
+    _check(c, out)
