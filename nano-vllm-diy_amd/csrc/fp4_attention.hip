@@ -47,7 +47,8 @@ constexpr int kManyCols = kManyWaves * kManyTiles * 16;
 constexpr int kManyStep = 64;         // keys of its step
 constexpr int kManyRing = 4;          // steps of 4-bit rows in LDS
 constexpr int kSub = 32;              // keys a wavefront takes at once
-constexpr int kChunk = 64 * kWave;    // sequences whose steps are in LDS at a time
+constexpr int kGroups = 16;           // groups of 64 sequences that are in LDS at a time
+constexpr int kChunk = kGroups * kWave;
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kSlack = 8.f;         // the scores may exceed their reference by this (exp2 domain)
 
@@ -59,6 +60,8 @@ typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
 typedef __attribute__((address_space(3))) int lds_i32;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i32x4 lds_i32x4;
 typedef __attribute__((address_space(3))) float lds_f32;
 typedef __attribute__((address_space(3))) f32x2 lds_f32x2;
 
@@ -117,12 +120,6 @@ __device__ __forceinline__ Seq make_seq(const Fp4AttnArgs& a, int q0, int q1, in
 __device__ __forceinline__ Seq seq_of(const Fp4AttnArgs& a, int b) {
   return make_seq(a, a.cu_q[b], a.cu_q[b + 1], a.cu_k[b], a.cu_k[b + 1]);
 }
-__device__ __forceinline__ Seq uniform_seq(const Fp4AttnArgs& a, int b) {
-  const Seq s = make_seq(a, scalar_i32(a.cu_q + b), scalar_i32(a.cu_q + b + 1), scalar_i32(a.cu_k + b),
-                         scalar_i32(a.cu_k + b + 1));
-  return {uniform(s.q0), uniform(s.rows), uniform(s.shift), uniform(s.keys)};
-}
-
 // Steps of STEP keys of tile j of a sequence: up to the last key its last row sees, at least one.
 template <bool MANY, int STEP>
 __device__ __forceinline__ int tile_steps(const Fp4AttnArgs& a, const Seq& s, int j) {
@@ -145,6 +142,7 @@ __device__ __forceinline__ int seq_steps(const Fp4AttnArgs& a, const Seq& s) {
 
 // A tile of query rows on the line: steps [start, start + steps) of it.
 struct Tile {
+  Seq seq;
   int b, head, j;    // sequence, kv head (MANY), tile of it
   int64_t start;
   int steps;
@@ -163,13 +161,14 @@ __device__ __forceinline__ int64_t div_floor(int64_t n, int64_t d) {
 
 // The line of steps: MANY: kv head by kv head, sequence by sequence, tile by tile; otherwise the sequences' steps,
 // which the wavefronts take for a kv head each. A chunk's steps are summed up in LDS, a thread to a sequence, and looked
-// up from there. (With every wavefront keeping the steps of 512 sequences in registers, and beginning with the first
-// of all sequences for every piece: 106 us in place of 77 for 1024 sequences of 100-400 keys, 5165 in place of 360
-// for 16384 of 16-64, 36.8 in place of 35.8 for 128 of 100-2048.)
+// up from there, the sequence's lengths with them. (With every wavefront keeping the steps of 512 sequences in
+// registers, and beginning with the first of all sequences for every piece: 106 us in place of 74 for 1024 sequences of
+// 100-400 keys, 5165 in place of 357 for 16384 of 16-64, 36.8 in place of 34.4 for 128 of 100-2048.)
 template <bool MANY, int STEP>
 struct Line {
-  static constexpr int kBytes = (kChunk + kWave) * 4;
-  lds_i32* sums;     // [kChunk] steps of a group of 64 sequences up to and with each of them, [64] of whole groups
+  static constexpr int kBytes = kChunk * 20 + kGroups * 4;
+  lds_i32x4* seqs;   // [kChunk] Seq
+  lds_i32* sums;     // [kChunk] steps of a group of 64 sequences up to and with each of them, [kGroups] of whole groups
   int base, before;  // the chunk's first sequence, the steps before it
   int per_head;      // steps of all sequences
   int64_t total;
@@ -180,23 +179,31 @@ struct Line {
     before = steps_before;
     meet();  // the last chunk has been read
 #pragma unroll 1
-    for (int group = wave; group < kWave; group += 8) {
+    for (int group = wave; group < kGroups; group += 8) {
       int sum = 0;
       if (first + 64 * group < a.num_seqs) {
         const int b = first + 64 * group + lane;
-        sum = scan64(b < a.num_seqs ? seq_steps<MANY, STEP>(a, seq_of(a, b)) : 0, lane);
+        if (b < a.num_seqs) {
+          const Seq s = seq_of(a, b);
+          seqs[64 * group + lane] = i32x4{s.q0, s.rows, s.shift, s.keys};
+          sum = seq_steps<MANY, STEP>(a, s);
+        }
+        sum = scan64(sum, lane);
         sums[64 * group + lane] = sum;
       }
       if (lane == kWave - 1) sums[kChunk + group] = sum;
     }
     meet();
   }
+  // Steps of the chunk's groups up to and with each, a lane a group (the same in all lanes past the last).
+  __device__ __forceinline__ int group_ends(int lane) const { return scan64(lane < kGroups ? sums[kChunk + lane] : 0, lane); }
   __device__ __forceinline__ void init(const Fp4AttnArgs& a, lds_u8* lds, int wave, int lane) {
-    sums = (lds_i32*)lds;
+    seqs = (lds_i32x4*)lds;
+    sums = (lds_i32*)(lds + kChunk * 16);
     per_head = 0;
     for (int first = 0; first < a.num_seqs; first += kChunk) {
       load(a, first, per_head, wave, lane);
-      per_head += __builtin_amdgcn_readlane(scan64(sums[kChunk + lane], lane), kWave - 1);
+      per_head += __builtin_amdgcn_readlane(group_ends(lane), kWave - 1);
     }
     total = MANY ? (int64_t)per_head * a.num_kv_heads : per_head;
   }
@@ -208,19 +215,20 @@ struct Line {
     const int64_t head_start = (int64_t)t.head * per_head;
     const int want = (int)(p - head_start);
     if (want < before) load(a, 0, 0, wave, lane);
-    int group_steps = sums[kChunk + lane], group_end = before + scan64(group_steps, lane);
+    int group_end = before + group_ends(lane);
     while (want >= __builtin_amdgcn_readlane(group_end, kWave - 1)) {
       load(a, base + kChunk, __builtin_amdgcn_readlane(group_end, kWave - 1), wave, lane);
-      group_steps = sums[kChunk + lane];
-      group_end = before + scan64(group_steps, lane);
+      group_end = before + group_ends(lane);
     }
     const int group = __builtin_ctzll(__builtin_amdgcn_ballot_w64(want < group_end));
-    const int group_start = __builtin_amdgcn_readlane(group_end - group_steps, group);
+    const int group_start = group ? __builtin_amdgcn_readlane(group_end, group - 1) : before;
     const int end = group_start + sums[64 * group + lane];
     const int in_group = __builtin_ctzll(__builtin_amdgcn_ballot_w64(want < end));
     const int seq_start = in_group ? __builtin_amdgcn_readlane(end, in_group - 1) : group_start;
     const int b = base + 64 * group + in_group;
-    const Seq s = uniform_seq(a, b);
+    const i32x4 of = seqs[64 * group + in_group];
+    const Seq s = {uniform(of[0]), uniform(of[1]), uniform(of[2]), uniform(of[3])};
+    t.seq = s;
     int start = seq_start, steps = tile_steps<MANY, STEP>(a, s, 0);
     if constexpr (MANY) {
       const int tiles = ((s.rows << a.group_shift) + kManyCols - 1) / kManyCols;
@@ -394,7 +402,10 @@ struct Loader {
   int scale_row, scale_col;
   int lds, scale_lds;
   bool scales_of_v;
-  Cursor at, scale_at;
+  Cursor at, own_scale_at;
+  // (all of a step of 32 rows is in one page)
+  static constexpr bool kOnePage = ROWS == kSub;
+  __device__ __forceinline__ Cursor& scale_at() { return kOnePage ? at : own_scale_at; }
 
   // (a slot that is no head reads the last one's bytes, which nobody looks at)
   __device__ __forceinline__ void init(const Fp4AttnArgs& a, const int32_t* table, int t0, int keys, int head0, int heads,
@@ -417,7 +428,7 @@ struct Loader {
     scale_lds = (scales_of_v ? S::kCache : 0) + S::kValues + part * 256;
     const int page = t0 / a.block_size, last_page = (keys - 1) / a.block_size;
     at.init(a, table, t0, page, last_page, first & ~31);
-    scale_at.init(a, table, t0, page, last_page, scale_first);
+    if constexpr (!kOnePage) own_scale_at.init(a, table, t0, page, last_page, scale_first);
   }
 
   // The next step's rows into a stage of LDS; whether the wavefront's own 32 keys among them are in a block. A row that
@@ -434,11 +445,12 @@ struct Loader {
       stage16(k, off, uniform(stage + lds + 1024 * j));
       stage16(v, off, uniform(stage + S::kCache + lds + 1024 * j));
     }
-    at.next(a, ROWS);
-    const int scale_last = max(scale_at.rows(a, keys), 1) - 1;
-    const uint8_t* c = uniform_ptr(scales_of_v ? scale_at.at(a, a.v, a.v_block) : scale_at.at(a, a.k, a.k_block));
+    const int scale_last = max(scale_at().rows(a, keys), 1) - 1;
+    const uint8_t* c = kOnePage ? (scales_of_v ? v : k)
+                                : uniform_ptr(scales_of_v ? scale_at().at(a, a.v, a.v_block) : scale_at().at(a, a.k, a.k_block));
     stage4(c, min(scale_row, scale_last) * a.row_bytes + scale_col, uniform(stage + scale_lds));
-    scale_at.next(a, ROWS);
+    at.next(a, ROWS);
+    if constexpr (!kOnePage) own_scale_at.next(a, ROWS);
     return good;
   }
 };
@@ -775,7 +787,7 @@ struct Run {
   __device__ __forceinline__ bool next(const Fp4AttnArgs& a, const Partials& part, int wave, int lane) {
     if (p >= end) return false;
     tile = line.at(a, p, wave, lane);
-    seq = uniform_seq(a, tile.b);
+    seq = tile.seq;
     s0 = (int)(p - tile.start);
     s1 = (int)min((int64_t)tile.steps, end - tile.start);
     p = tile.start + s1;
@@ -885,7 +897,7 @@ __global__ __launch_bounds__(kFewWaves* kWave, 2) void attend_few_kernel(const F
       if (s + kFewRing - 1 < s1)
         good |= (uint32_t)loader.issue(a, seq.keys, lds0 + next_buf * S::kBytes) << (kFewRing - 1);
       loader.at.arrive();
-      loader.scale_at.arrive();
+      loader.scale_at().arrive();
       buf = buf + 1 == kFewRing ? 0 : buf + 1;
       next_buf = next_buf + 1 == kFewRing ? 0 : next_buf + 1;
       const int t0 = s * ROWS + slice * kSub;
@@ -1034,7 +1046,7 @@ template <int T>
 __device__ __forceinline__ void many_take(State<T>& st, const lds_u8* tiles, const int (&k)[4], const int (&v)[8],
                                           bool masked, const int (&rel)[T], float c2, int lane) {
   constexpr int kTile16 = 16 * ManyLds::kRow;
-  constexpr int kAheadK = 4, kAheadV = 1;
+  constexpr int kAheadK = 3, kAheadV = 1;
   f32x4 s[4][T];
   u32x4 kw[kAheadK];
   u32x4 vw[kAheadV + 1][2];
@@ -1205,15 +1217,31 @@ __device__ __forceinline__ void merge(const Fp4AttnArgs& a, const Partials& part
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     if (pair < pairs) {
       const auto at = [&](int j) { return part.at(2 * (int64_t)(run + j) + (j == 0 ? 1 : 0), MANY ? 0 : head, col); };
-      for (int j = slice + t * slices; j < pieces; j += 32 * slices) m = fmaxf(m, part.ml[at(j)].x);
+      // four at a time, all of their loads at once: a round trip less than with the maximum found ahead (a mixed step's
+      // 68 MB 14.1 us in place of 17.3, 8 sequences 5.0 in place of 6.0)
+      for (int j0 = slice; j0 < pieces; j0 += 4 * slices) {
+        float2 ml[4];
+        f32x4 o[4];
+        float top = m;
 #pragma unroll
-      for (int sh = 1; sh < 32; sh *= 2) m = fmaxf(m, __shfl_xor(m, sh, 32));
-#pragma unroll 4
-      for (int j = slice; j < pieces; j += slices) {
-        const float2 ml = part.ml[at(j)];
-        const float w = exp2_fast(ml.x - m);
-        l = fmaf(w, ml.y, l);
-        acc += w * *reinterpret_cast<const f32x4*>(part.o + at(j) * D + 4 * t);
+        for (int i = 0; i < 4; ++i) {
+          const int64_t p = at(min(j0 + i * slices, pieces - 1));
+          ml[i] = part.ml[p];
+          o[i] = *reinterpret_cast<const f32x4*>(part.o + p * D + 4 * t);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[i].x);  // (some of another team: it only moves the reference)
+        const float f = exp2_fast(m - top);
+        m = top;
+        l *= f;
+        acc *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool real = j0 + i * slices < pieces;
+          const float w = real ? exp2_fast(ml[i].x - m) : 0.f;
+          l = fmaf(w, real ? ml[i].y : 0.f, l);
+          acc += w * (real ? o[i] : f32x4{0.f, 0.f, 0.f, 0.f});
+        }
       }
     }
     if (slices > 1) {
