@@ -288,7 +288,7 @@ __host__ __device__ __forceinline__ size_t partial_rows(const Fp4AttnPlan& p, in
 //
 // A step's rows of the work-group's kv heads, HEADS slots a row: [K values | K scales | V values | V scales], a row's
 // values HEADS x 4 chunks of 16 bytes, its scales HEADS dwords. They come straight from memory (global_load_lds, 1
-// KiB an instruction for the values), two steps in turn. (With every wavefront reading its own head's bytes into
+// KiB an instruction for the values), a ring of three steps. (With every wavefront reading its own head's bytes into
 // registers the kernel was bound by its load instructions: 40 a step of 64 keys and head, most of them of 16 to 256
 // bytes, 355 us for 256 sequences of 1k-8k keys.)
 //
@@ -836,7 +836,11 @@ struct Columns {
 };
 
 // Few rows: HEADS slots of kv heads from head0 on, of which `heads` are heads, and 8 / HEADS wavefronts to each, which
-// take 32 keys of every step in turn.
+// take 32 keys of every step in turn. Bound by HBM where there is enough to read: 208 to 220 us for 256 sequences of
+// 1k-8k keys of 8 kv heads, 5.6 to 5.9 TB/s; 35 us for 128 of 100-2048 (4 TB/s), 5 of them before the first step is
+// there. Sequences of at most 16 columns, what one tile holds, come here: 48 of 4 to 16 columns and 300-4000 keys of 4 kv
+// heads took 22 us and 6 for the merge; with those of more than 8 columns in the other kernel 15 + 36 + 11, of more
+// than 4 columns 8 + 50 + 12.
 template <int HEADS>
 __global__ __launch_bounds__(kFewWaves* kWave, 2) void attend_few_kernel(const Fp4AttnArgs a, const Partials part, int runs,
                                                                          int heads) {
@@ -1193,8 +1197,9 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void attend_many_kernel(const
 }
 
 // The tile that begins in a run and goes on, if there is one; its partial results are the run's second slot and the
-// first ones of the runs after it. `groups` work-groups share a run's columns. 32 threads take a column (of a kv head), 4 dimensions
-// each, and `slices` of them share a column's partial results, which meet in LDS.
+// first ones of the runs after it. `groups` work-groups share a run's columns. 32 threads take a column (of a kv head),
+// 4 dimensions each, and `slices` of them share a column's partial results, which meet in LDS. Work-groups of 512 and
+// 1024 threads took 30 and 32 us behind 16 chunks in place of 17.
 constexpr int kMergeThreads = 256;
 constexpr int kMergeTeams = kMergeThreads / 32;
 template <bool MANY>
@@ -1331,6 +1336,8 @@ Fp4AttnPlan fp4_attention_plan(int32_t num_seqs, int32_t num_heads, int32_t num_
   const int64_t few_steps = ((int64_t)max_seqlen_k * p.few_slots + kSub * kFewWaves - 1) / (kSub * kFewWaves);
   p.too_long = num_seqs * few_steps > INT32_MAX;
   p.few_cols = (int)std::min<int64_t>(16, (int64_t)max_seqlen_q * group);
+  // a run to a compute unit, whose LDS a work-group fills (64, 128 and 512 runs: 708, 370 and 224 us in place of 215 for
+  // 256 sequences of 1k-8k keys, 16, 14 and 15 in place of 11 for 8 of 256-2048)
   p.few_runs = (int)std::min<int64_t>(256, num_seqs * few_steps);
   p.few_bytes = partial_bytes(partial_rows<false>(p, num_kv_heads), p.few_runs);
   if ((int64_t)max_seqlen_q * group > 16) {

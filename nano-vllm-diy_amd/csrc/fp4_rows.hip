@@ -239,7 +239,13 @@ hipError_t launch_store_fp4(const Fp4StoreArgs& a, hipStream_t stream) {
 
 hipError_t launch_append_fp4(const Fp4AppendArgs& a, hipStream_t stream) {
   const int quads = (a.num_heads + 2 * a.num_kv_heads + 3) / 4;  // 4 head rows per wavefront step
-  const int parts = a.num_tokens < 1024 ? (quads < 4 ? quads : 4) : 1;
+  // A token's head rows are shared by up to 8 wavefronts while that fills an idle card and not after: with 1, 2, 4
+  // and 8 of them, 16 + 8 + 8 head rows took, us
+  //     1 token 5.4 3.8 3.2 2.8    256  6.2  4.4  3.7  3.7    2048 12.7 11.8 11.6 14.8    16384 67 69 86 120
+  //     97      6.0 4.2 3.5 3.1    512  6.5  4.9  4.6  5.1    4096 19.1 18.6 20.1 26.3
+  int parts = 1;
+  while (parts < 8 && (int64_t)a.num_tokens * parts * 2 <= (parts < 4 ? 8192 : 2048)) parts *= 2;
+  parts = parts < quads ? parts : quads;
   const int64_t items = (int64_t)a.num_tokens * parts;
   constexpr int kWaves = kRowThreads / kWave;
   hipLaunchKernelGGL(append_fp4_kernel, dim3((unsigned)((items + kWaves - 1) / kWaves)), dim3(kRowThreads), 0, stream,

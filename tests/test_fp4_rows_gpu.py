@@ -259,3 +259,25 @@ def test_read_back_stops_at_its_output(gpu):
     call(lib().pk_gather_kv_fp4, "pk_gather_kv_fp4", gpu, kc.data_ptr(), kc.stride(0), 4, bs, kv, D, table.data_ptr(), 2,
          cu.data_ptr(), 2, 120, 256, room.data_ptr())
     assert torch.equal(room[:220].double(), ref.values(rows, kv)[:220]) and (room[220:] == 7).all()
+
+
+@pytest.mark.parametrize("n", [300, 2100, 5000])
+def test_append_does_not_hang_on_the_number_of_tokens(gpu, n):
+    """A token's q, rows and values are the same bits alone among few tokens, which 8 wavefronts share, and among many."""
+    heads, kv, bs = 16, 8, 64
+    g = _gen(n)
+    qkv = _randn(g, n, (heads + 2 * kv) * D, device=gpu)
+    pos = torch.randint(0, 512, (n,), generator=g).to(gpu)
+    table = pagedkv.rope_cos_sin(512, D, device=gpu)
+    qw, kw = _randn(g, D, device=gpu), _randn(g, D, device=gpu)
+    slots = torch.randperm(80 * bs, generator=g)[:n].to(torch.int32).to(gpu)
+    caches = [torch.zeros(80, bs, 544, dtype=torch.uint8, device=gpu) for _ in range(4)]
+
+    def append(a, b, kc, vc):
+        return pagedkv.qk_norm_rope_store_fp4(qkv[a:b], pos[a:b], table, heads, kv, D, qw, kw, 1e-6, kc, vc, slots[a:b], True)
+
+    whole = append(0, n, *caches[:2])
+    for a in range(0, n, 100):
+        for x, y in zip(append(a, min(n, a + 100), *caches[2:]), whole):
+            assert torch.equal(x.view(torch.int16), y[a:a + 100].view(torch.int16))
+    assert torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
