@@ -15,7 +15,7 @@
 //                P^T of the next product these are the 8 keys of its lane for two tiles, so P never changes lanes.
 // Values convert to bf16 with their scale in one instruction for two. (The matrix instructions that read 4-bit
 // values with their scales keep about 12 bits below the largest product of a sum, measured; scores here are
-// held in 32, so they are not used.) The two kernels differ in who converts:
+// held in 32, so they are not used.) The two kinds of work-groups differ in who converts:
 //   few rows (rows x group <= 16): T = 1, a tile of work is all of a sequence's rows and up to 8 kv heads, and a
 //       wavefront converts the keys that it takes, 32 of one head at once, straight into the products' operands. Of
 //       K, lane l has of key l % 16 the 32 dimensions from 32 (l / 16): 16 consecutive bytes with one scale byte; the
@@ -29,8 +29,8 @@
 // Work. The steps of every tile lie end to end on a line, which is cut into `runs` equal runs, one work-group each,
 // whatever the lengths: a work-group takes the end of one tile, whole tiles and the beginning of another. A tile that
 // a cut splits leaves fp32 partial results (o, m, sum), which a second kernel merges; a cut splits at most one tile,
-// so there are at most two partial results a run. The lengths are on the GPU only, so both kernels are launched
-// wherever the call's bounds allow sequences of their kind; one without any costs 5 us with its merge.
+// so there are at most two partial results a run. The lengths are on the GPU only, so a launch has work-groups of both
+// kinds wherever the call's bounds allow sequences of more than 16 columns; those without any end at once.
 #include <algorithm>
 #include <type_traits>
 
@@ -842,22 +842,26 @@ struct Columns {
 // heads took 22 us and 6 for the merge; with those of more than 8 columns in the other kernel 15 + 36 + 11, of more
 // than 4 columns 8 + 50 + 12.
 template <int HEADS>
-__global__ __launch_bounds__(kFewWaves* kWave, 2) void attend_few_kernel(const Fp4AttnArgs a, const Partials part, int runs,
-                                                                         int heads) {
+struct FewLds {
+  static constexpr int kRows = kSub * kFewWaves / HEADS;  // of a step
+  static constexpr int kLine = kFewRing * Stage<HEADS, kRows>::kBytes;
+  static constexpr int kBytes = kLine + Line<false, kRows>::kBytes;
+};
+// run: of `runs`, of the kv heads from head0 on.
+template <int HEADS>
+__device__ __forceinline__ void attend_few(const Fp4AttnArgs& a, const Partials& part, int runs, int heads, int index,
+                                           int head0, lds_u8* lds) {
   constexpr int D = kHeadDim;
   constexpr int kSlices = kFewWaves / HEADS, ROWS = kSub * kSlices;
   typedef Stage<HEADS, ROWS> S;
   typedef Loader<HEADS, ROWS> L;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[kFewRing * S::kBytes + Line<false, ROWS>::kBytes];
-  lds_u8* const lds = (lds_u8*)smem;
   const int lds0 = (int)(uintptr_t)lds;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = uniform(threadIdx.x / kWave);
   const int n = lane & 15, g = lane >> 4;
-  const int head0 = blockIdx.y * heads;
   const bool recorder = head0 == 0 && threadIdx.x == 0;
   Run<false, ROWS> run;
-  if (!run.init(a, part, runs, blockIdx.x, recorder, lds + kFewRing * S::kBytes, wave, lane)) return;
+  if (!run.init(a, part, runs, index, recorder, lds + FewLds<HEADS>::kLine, wave, lane)) return;
   const int slot = wave % HEADS, slice = wave / HEADS;
   const bool live = slot < heads;
   const int head = head0 + min(slot, heads - 1);
@@ -1045,12 +1049,14 @@ __device__ __forceinline__ void many_nan(State<T>& st, const lds_u8* raw, const 
 
 // The 64 keys of a pair of tiles. k, v: the lane's places in them, for every chunk of K and every 16 dimensions of V.
 // The reads are kept ahead of the products that use them (the compiler's own order reads each operand right before
-// its product and waits for it).
+// its product and waits for it; 3, 4, 5, 6, 7 and 8 of K: 766, 780, 760, 757, 783 and 757 us for the 16 chunks, and with
+// two of V in place of one 777, 788 and 763 with 3, 4 and 5 -- where the registers come to lie decides more than the
+// distance).
 template <int T>
 __device__ __forceinline__ void many_take(State<T>& st, const lds_u8* tiles, const int (&k)[4], const int (&v)[8],
                                           bool masked, const int (&rel)[T], float c2, int lane) {
   constexpr int kTile16 = 16 * ManyLds::kRow;
-  constexpr int kAheadK = 3, kAheadV = 1;
+  constexpr int kAheadK = 6, kAheadV = 1;
   f32x4 s[4][T];
   u32x4 kw[kAheadK];
   u32x4 vw[kAheadV + 1][2];
@@ -1100,17 +1106,15 @@ __device__ __forceinline__ void many_take(State<T>& st, const lds_u8* tiles, con
   }
 }
 
-__global__ __launch_bounds__(kManyWaves* kWave, 2) void attend_many_kernel(const Fp4AttnArgs a, const Partials part, int runs) {
+__device__ __forceinline__ void attend_many(const Fp4AttnArgs& a, const Partials& part, int runs, int index, lds_u8* lds) {
   constexpr int D = kHeadDim, T = kManyTiles;
   typedef ManyLds S;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[S::kBytes + Line<true, kManyStep>::kBytes];
-  lds_u8* const lds = (lds_u8*)smem;
   const int lds0 = (int)(uintptr_t)lds;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = uniform(threadIdx.x / kWave);
   const int n = lane & 15, g = lane >> 4;
   Run<true, kManyStep> run;
-  if (!run.init(a, part, runs, blockIdx.x, threadIdx.x == 0, lds + S::kBytes, wave, lane)) return;
+  if (!run.init(a, part, runs, index, threadIdx.x == 0, lds + S::kBytes, wave, lane)) return;
   int k_at[4], v_at[8];
 #pragma unroll
   for (int c = 0; c < 4; ++c) k_at[c] = n * S::kRow + ((4 * c + g) ^ n) * 16;
@@ -1194,6 +1198,31 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void attend_many_kernel(const
     }
   }
   if (threadIdx.x == 0) part.split[run.run] = run.split;
+}
+
+constexpr int kManyBytes = ManyLds::kBytes + Line<true, kManyStep>::kBytes;
+static_assert(kFewWaves == kManyWaves, "one launch has work-groups of both");
+
+template <int HEADS>
+__global__ __launch_bounds__(kFewWaves* kWave, 2) void attend_few_kernel(const Fp4AttnArgs a, const Partials few, int few_runs,
+                                                                         int heads) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[FewLds<HEADS>::kBytes];
+  attend_few<HEADS>(a, few, few_runs, heads, blockIdx.x % few_runs, blockIdx.x / few_runs * heads, (lds_u8*)smem);
+}
+
+// Both kinds of sequences: the work-groups of one kind begin where those of the other end. (In two launches a mixed step's
+// kernels took 38.3 and 37.4 us in place of 70.4; 16 chunks alone 745 and 4.8 in place of 757.)
+template <int HEADS>
+__global__ __launch_bounds__(kFewWaves* kWave, 2) void attend_mixed_kernel(const Fp4AttnArgs a, const Partials few,
+                                                                           const Partials many, int few_runs, int many_runs,
+                                                                           int heads) {
+  constexpr int kBytes = FewLds<HEADS>::kBytes > kManyBytes ? FewLds<HEADS>::kBytes : kManyBytes;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kBytes];
+  const int i = (int)blockIdx.x - many_runs;
+  if (i < 0)
+    attend_many(a, many, many_runs, blockIdx.x, (lds_u8*)smem);
+  else
+    attend_few<HEADS>(a, few, few_runs, heads, i % few_runs, i / few_runs * heads, (lds_u8*)smem);
 }
 
 // The tile that begins in a run and goes on, if there is one; its partial results are the run's second slot and the
@@ -1351,15 +1380,28 @@ Fp4AttnPlan fp4_attention_plan(int32_t num_seqs, int32_t num_heads, int32_t num_
   return p;
 }
 
+namespace {
+template <int HEADS>
+void launch_attend(const Fp4AttnArgs& a, const Fp4AttnPlan& p, const Partials& few, const Partials& many, hipStream_t stream) {
+  const unsigned few_groups = (unsigned)p.few_runs * (unsigned)(a.num_kv_heads / p.few_heads);
+  if (p.many_runs)
+    hipLaunchKernelGGL(attend_mixed_kernel<HEADS>, dim3(p.many_runs + few_groups), dim3(kFewWaves * kWave), 0, stream, a, few,
+                       many, p.few_runs, p.many_runs, p.few_heads);
+  else
+    hipLaunchKernelGGL(attend_few_kernel<HEADS>, dim3(few_groups), dim3(kFewWaves * kWave), 0, stream, a, few, p.few_runs,
+                       p.few_heads);
+}
+}  // namespace
+
 hipError_t launch_fp4_attention(const Fp4AttnArgs& a, const Fp4AttnPlan& p, hipStream_t stream) {
   char* ws = static_cast<char*>(a.workspace);
   const Partials few = partials_of<false>(a, p, ws);
-  const dim3 grid((unsigned)p.few_runs, (unsigned)(a.num_kv_heads / p.few_heads)), block(kFewWaves * kWave);
+  const Partials many = p.many_runs ? partials_of<true>(a, p, ws + p.few_bytes) : few;
   switch (p.few_slots) {
-    case 1: hipLaunchKernelGGL(attend_few_kernel<1>, grid, block, 0, stream, a, few, p.few_runs, p.few_heads); break;
-    case 2: hipLaunchKernelGGL(attend_few_kernel<2>, grid, block, 0, stream, a, few, p.few_runs, p.few_heads); break;
-    case 4: hipLaunchKernelGGL(attend_few_kernel<4>, grid, block, 0, stream, a, few, p.few_runs, p.few_heads); break;
-    default: hipLaunchKernelGGL(attend_few_kernel<8>, grid, block, 0, stream, a, few, p.few_runs, p.few_heads); break;
+    case 1: launch_attend<1>(a, p, few, many, stream); break;
+    case 2: launch_attend<2>(a, p, few, many, stream); break;
+    case 4: launch_attend<4>(a, p, few, many, stream); break;
+    default: launch_attend<8>(a, p, few, many, stream); break;
   }
   if (hipError_t err = hipGetLastError()) return err;
   Merge merge_few{few, p.few_runs - 1, 1, 1}, merge_many{few, 0, 1, 1};
@@ -1369,10 +1411,6 @@ hipError_t launch_fp4_attention(const Fp4AttnArgs& a, const Fp4AttnPlan& p, hipS
     merge_few.groups = merge_groups(p.few_runs, (a.num_kv_heads * p.few_cols + per_pass - 1) / per_pass);
   }
   if (p.many_runs) {
-    const Partials many = partials_of<true>(a, p, ws + p.few_bytes);
-    hipLaunchKernelGGL(attend_many_kernel, dim3((unsigned)p.many_runs), dim3(kManyWaves * kWave), 0, stream, a, many,
-                       p.many_runs);
-    if (hipError_t err = hipGetLastError()) return err;
     const int slices = merge_slices(p.many_runs, p.many_tiles);
     merge_many = Merge{many, p.many_runs - 1, merge_groups(p.many_runs, kManyCols * slices / kMergeTeams), slices};
   }
