@@ -1263,6 +1263,7 @@ int pk_varlen_attention_fp4(const void* q, int64_t q_row_stride, const void* k_c
   a.num_seqs = num_seqs;
   a.max_seqlen_q = max_seqlen_q;
   a.max_seqlen_k = max_seqlen_k;
+  a.num_rows = num_rows;
   a.num_heads = num_heads;
   a.num_kv_heads = num_kv_heads;
   a.group_shift = __builtin_ctz((unsigned)group);

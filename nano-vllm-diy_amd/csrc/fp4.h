@@ -130,6 +130,7 @@ struct Fp4AttnArgs {
   const int32_t* cu_q;
   const int32_t* cu_k;
   int32_t num_seqs, max_seqlen_q, max_seqlen_k;
+  int64_t num_rows;              // of q and out: rows past them are not computed
   int32_t num_heads, num_kv_heads;
   int32_t group_shift;           // log2(num_heads / num_kv_heads)
   float scale_log2;              // softmax_scale * log2(e)

@@ -113,7 +113,7 @@ __device__ __forceinline__ Seq make_seq(const Fp4AttnArgs& a, int q0, int q1, in
   Seq s;
   s.q0 = q0;
   s.keys = min(k1 - k0, a.max_seqlen_k);
-  s.rows = s.keys > 0 ? min(q1 - q0, a.max_seqlen_q) : 0;
+  s.rows = s.keys > 0 && q0 >= 0 ? (int)min((int64_t)min(q1 - q0, a.max_seqlen_q), a.num_rows - q0) : 0;
   s.shift = a.causal ? s.keys - (q1 - q0) : s.keys;
   return s;
 }
@@ -1049,14 +1049,14 @@ __device__ __forceinline__ void many_nan(State<T>& st, const lds_u8* raw, const 
 
 // The 64 keys of a pair of tiles. k, v: the lane's places in them, for every chunk of K and every 16 dimensions of V.
 // The reads are kept ahead of the products that use them (the compiler's own order reads each operand right before
-// its product and waits for it; 3, 4, 5, 6, 7 and 8 of K: 766, 780, 760, 757, 783 and 757 us for the 16 chunks, and with
-// two of V in place of one 777, 788 and 763 with 3, 4 and 5 -- where the registers come to lie decides more than the
-// distance).
+// its product and waits for it.) A wavefront goes first while it has products: otherwise the two on a SIMD fall into step
+// in some builds, and wait for the same units (16 chunks: 770 to 785 us in place of 748, with 3, 4, 5, 6 or 8 reads
+// of K ahead, whichever way the registers came to lie; with the priorities 751 and 746 for 3 and 4).
 template <int T>
 __device__ __forceinline__ void many_take(State<T>& st, const lds_u8* tiles, const int (&k)[4], const int (&v)[8],
                                           bool masked, const int (&rel)[T], float c2, int lane) {
   constexpr int kTile16 = 16 * ManyLds::kRow;
-  constexpr int kAheadK = 6, kAheadV = 1;
+  constexpr int kAheadK = 4, kAheadV = 1;
   f32x4 s[4][T];
   u32x4 kw[kAheadK];
   u32x4 vw[kAheadV + 1][2];
@@ -1072,6 +1072,7 @@ __device__ __forceinline__ void many_take(State<T>& st, const lds_u8* tiles, con
   };
 #pragma unroll
   for (int i = 0; i < kAheadK; ++i) kw[i] = read_k(i);
+  __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const u32x4 w = kw[i % kAheadK];
@@ -1092,8 +1093,10 @@ __device__ __forceinline__ void many_take(State<T>& st, const lds_u8* tiles, con
         for (int i = 0; i < 4; ++i)
           if (16 * t + 4 * (lane >> 4) + i > rel[x]) s[t][x][i] = -INFINITY;
   }
+  __builtin_amdgcn_s_setprio(0);
   u32x4 p[T][2];
   weights<T, 4>(p, s, st, c2);
+  __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     if (j + kAheadV < 8) read_v(vw[(j + kAheadV) % (kAheadV + 1)], j + kAheadV);
@@ -1104,6 +1107,7 @@ __device__ __forceinline__ void many_take(State<T>& st, const lds_u8* tiles, con
       for (int x = 0; x < T; ++x) st.acc[x][j] = mfma(vw[j % (kAheadV + 1)][h], p[x][h], st.acc[x][j]);
     __builtin_amdgcn_sched_barrier(0);
   }
+  __builtin_amdgcn_s_setprio(0);
 }
 
 __device__ __forceinline__ void attend_many(const Fp4AttnArgs& a, const Partials& part, int runs, int index, lds_u8* lds) {

@@ -207,7 +207,8 @@ def varlen_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     """varlen_attention over 4-bit paged caches: q (N, Hq, 128) bf16, caches (NB, BS, row) uint8 read through
     block_table (S, W) int32, lengths from cu_seqlens_q / cu_seqlens_k (S + 1,) int32; bottom-right-aligned causal
     mask, GQA h -> h // (Hq / Hkv). One call takes any mixture of sequences with one query row, a few or many.
-    Returns out (N, Hq, 128) bf16; rows of no sequence are left as they are in a given out.
+    Returns out (N, Hq, 128) bf16. A row that sees no key is 0; rows of no sequence, and of sequences without keys
+    (graph padding, as varlen_attention takes it), are left as they are in a given out and hold anything in a new one.
 
     workspace: optional caller-owned uint8 scratch of fp4_workspace_bytes(...) bytes; calls that may overlap must not
     share one. Without it every call, captured ones too, takes its own."""

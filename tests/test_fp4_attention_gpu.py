@@ -327,3 +327,16 @@ def test_more_sequences_than_are_in_lds(gpu):
     out = torch.zeros_like(c["q"])
     _run(c, out=out)
     _check(c, out)
+
+
+def test_rows_past_the_tensors_are_not_touched(gpu):
+    """Cumulative lengths that go on past q's rows: what is there is computed, in its place in the mask."""
+    lens = [(1, 90), (7, 100), (60, 130), (1, 70), (40, 64)]
+    c = _case(gpu, 8, 4, lens, seed=51)
+    want, bound = ref.attention(c["q"], c["kc"], c["vc"], c["tables"], c["q_lens"], c["k_lens"], D ** -0.5)
+    for n in (0, 1, 3, 30, 68, 69, 80):
+        room = torch.full((n + 40, 8, D), 7.0, dtype=torch.bfloat16, device=gpu)
+        out = pagedkv.varlen_attention_fp4(c["q"][:n], c["kc"], c["vc"], _cu(c["q_lens"], gpu), _cu(c["k_lens"], gpu), 60, 130,
+                                           c["tables"], out=room[:n])
+        assert (room[n:] == 7).all()
+        assert ((out.double() - want[:n]).abs() <= bound[:n]).all()
