@@ -249,3 +249,19 @@ def test_blocks_that_fit(gpu):
     fp4 = kv_cache_num_blocks(2, 256, 8, D, util, device=gpu, row_bytes=pagedkv.fp4_row_bytes(8))
     # (the bytes in use are read twice; the cache's rows are 544 bytes in place of 2048)
     assert fp4 * 544 <= (wide + 1) * 2048 and (fp4 + 1) * 544 >= wide * 2048
+
+
+def test_engine_sizes_its_cache(gpu):
+    """num_blocks None with gpu_memory_utilization: as many 4-bit blocks as fit, and the engine serves from them."""
+    cfg = Qwen3Config(num_hidden_layers=2)
+    torch.cuda.empty_cache()
+    free, total = torch.cuda.mem_get_info(gpu)
+    util = (total - free) / total + 0.03
+    eng = E.LLMEngine(cfg, device=gpu, max_live_seqs=8, max_seq_len=1024, enforce_eager=True, gpu_memory_utilization=util,
+                      kv_cache_dtype="fp4")
+    nb = eng.runner.num_blocks
+    assert eng.runner.kv_cache.shape == (2, 2, nb, 256, 544) and nb * 2 * 2 * 256 * 544 <= total * util
+    rng = random.Random(4)
+    prompts = [[rng.randrange(cfg.vocab_size) for _ in range(n)] for n in (40, 700)]
+    outs, _ = eng.generate(prompts, [4, 6], ignore_eos=True)
+    assert [len(o) for o in outs] == [4, 6] and eng.scheduler.num_free_blocks() == nb
