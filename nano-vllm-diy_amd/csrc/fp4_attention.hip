@@ -636,6 +636,7 @@ __device__ __forceinline__ void nan_values(State<T>& st, Vals& v, const int (&re
 }
 
 // 32 keys of a stage. rel: the last of them that a column sees, where some column does not see all.
+// (Products go before the other wavefront's exponentials: 128 sequences 33.8 us in place of 34.7.)
 template <int T, int HEADS, int ROWS>
 __device__ __forceinline__ void take(State<T>& st, const lds_u8* stage, const Lanes<HEADS, ROWS>& at, bool masked,
                                      const int (&rel)[T], float c2, int lane) {
@@ -650,7 +651,9 @@ __device__ __forceinline__ void take(State<T>& st, const lds_u8* stage, const La
   at.values(v, stage);
   __builtin_amdgcn_sched_barrier(0);
   f32x4 s[2][T];
+  __builtin_amdgcn_s_setprio(1);
   scores(s, st, k);
+  __builtin_amdgcn_s_setprio(0);
   if (masked) {
 #pragma unroll
     for (int x = 0; x < T; ++x)
@@ -663,7 +666,9 @@ __device__ __forceinline__ void take(State<T>& st, const lds_u8* stage, const La
   u32x4 p[T][1];
   weights<T, 2>(p, s, st, c2);
   if (masked) nan_values<T, HEADS>(st, v, rel, lane);
+  __builtin_amdgcn_s_setprio(1);
   add_values<T>(st, p, v);
+  __builtin_amdgcn_s_setprio(0);
 }
 
 // The 16 columns of a wavefront over few rows, through LDS like the keys (4 KiB a wavefront, where the last stage of
