@@ -100,7 +100,11 @@ def _table(block_table: torch.Tensor, num_seqs: int, max_seqlen_k: int, block_si
         raise ValueError("block_table must be (S, W) with contiguous rows, one per sequence")
     if shape[1] * block_size < max_seqlen_k:
         raise ValueError(f"block_table of {shape[1]} blocks of {block_size} does not cover max_seqlen_k={max_seqlen_k}")
-    return block_table.data_ptr(), max(stride[0], shape[1])
+    # (the kernels step from row to row by the stride that is given to them: an expanded table has none)
+    if num_seqs > 1 and stride[0] * block_size < max_seqlen_k:
+        raise ValueError(f"block_table rows are {stride[0]} entries apart, which does not cover max_seqlen_k={max_seqlen_k} "
+                         f"in blocks of {block_size} (every sequence needs a row of its own)")
+    return block_table.data_ptr(), stride[0] if num_seqs > 1 else max(stride[0], shape[1])
 
 
 def store_kvcache_fp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
