@@ -608,8 +608,10 @@ int pk_compact_blocks(void* k_caches, void* v_caches, int64_t k_layer_stride, in
  *   score above -infinity) is written as 0.
  *   num_rows: the rows of q and out; a sequence's rows past them are neither read nor written. q's row stride below 2^25. block_size a multiple
  *   of 64, GQA groups of 1, 2, 4 or 8. Softmax, sums and partial results are fp32, the
- *   weights rounded to bf16 for the product with V. NaN blocks reach the rows that see them and no
- *   others. A row's result depends on the call's other sequences by the rounding of its partial sums; equal
+ *   weights rounded to bf16 for the product with V. V may have any values of the format; weights below 2^-126 of
+ *   a row's largest are lost, below 2^-94 where the sequence has scale bytes of V from 192 (2^65) on. Scores are
+ *   fp32: a row with one past its range is NaN, unless that is -infinity, which weighs nothing. NaN blocks reach the
+ *   rows that see them and no others. A row's result depends on the call's other sequences by the rounding of its partial sums; equal
  *   calls give equal bits. At most 2^31 steps of 64 keys over the call's bounds.
  *   workspace: pk_varlen_attention_fp4_workspace_bytes, 256-byte aligned (at most 520 bytes for 512
  *   num_kv_heads min(16, max_seqlen_q num_heads / num_kv_heads) partial results, 4.3 MB for single rows of 16

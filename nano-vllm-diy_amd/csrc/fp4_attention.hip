@@ -7,6 +7,9 @@
 // with K[t], V[t] the rows' values. One pass over the keys: m is a reference at most 8 below the largest score so
 // far (in the exp2 domain); while it holds, nothing is rescaled, and p stays below 2^8. Scores, p's sum and the
 // output are fp32; p is rounded to bf16 for the matrix product, as the 16-bit cache's kernels round it.
+// Sums p V must stay in fp32's range where their mean does: below 6 x 2^64 (scale bytes below kLargeScale) 2^22 keys
+// and weights of 2^8 do; a wavefront that meets a larger scale of V raises its reference by kRaise, and weights of at most
+// 2^-24, over 2^22 keys of at most 6 x 2^125, stay below 2^126. Weights below 2^-94 of the largest then vanish, in place of 2^-126.
 //
 // Columns. A kv head's query heads and a sequence's query rows are the columns of one matrix product: column
 // r G + i is query head i of the group and row r. A wavefront holds T tiles of 16 columns of one kv head:
@@ -51,6 +54,8 @@ constexpr int kGroups = 16;           // groups of 64 sequences that are in LDS 
 constexpr int kChunk = kGroups * kWave;
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kSlack = 8.f;         // the scores may exceed their reference by this (exp2 domain)
+constexpr float kRaise = 32.f;        // what the reference is raised by for large rows of V
+constexpr uint32_t kLargeScale = 192; // their scale bytes: the two highest bits set
 
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 frag;
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
@@ -464,7 +469,23 @@ struct State {
   f32x4 acc[T][8];   // [j][i]: dimension 32 (l / 16) + 8 i + j
   float m[T];        // reference, the same in the column's four lanes
   float l[T];        // this lane's keys' share of the sum
+  float slack;       // by how much scores may exceed m: kSlack, or kSlack - kRaise (the same for the wavefront)
 };
+
+// Raises the reference of all columns, before the weights of the first large rows of V.
+template <int T>
+__device__ __forceinline__ void raise_reference(State<T>& st) {
+  if (st.slack != kSlack) return;
+  st.slack = kSlack - kRaise;
+#pragma unroll
+  for (int x = 0; x < T; ++x) {
+    st.m[x] += kRaise;  // (kLowest stays what it is)
+    st.l[x] *= 0x1p-32f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) st.acc[x][j] *= 0x1p-32f;
+  }
+}
+static_assert(kRaise == 32.f, "raise_reference's factor");
 
 struct Vals {
   uint32_t d[2][4];  // tile t, row row_of(4 (l / 16) + i): dimensions 8 (l % 16) .. + 7
@@ -532,11 +553,11 @@ __device__ __forceinline__ float add_bf16x2(uint32_t a, float c) {
 // The weights of the columns over NT tiles of 16 keys, in bf16 pairs, as the operand of the product with V: two
 // tiles an operand, tile by tile, i by i. The sum is of the rounded weights, which is what the product weighs V with.
 // (Whether the reference holds is asked of each lane's own scores; the column's largest is formed only where it
-// does not.)
+// does not.) large: the lane has met a scale byte of V from kLargeScale on.
 template <int T, int NT>
-__device__ __forceinline__ void weights(u32x4 (&p)[T][NT / 2], const f32x4 (&s)[NT][T], State<T>& st, float c2) {
+__device__ __forceinline__ void weights(u32x4 (&p)[T][NT / 2], const f32x4 (&s)[NT][T], State<T>& st, bool large, float c2) {
   float top[T];
-  bool over = false;
+  bool over = large;
 #pragma unroll
   for (int x = 0; x < T; ++x) {
     float mx = fmaxf(s[0][x][0], s[0][x][1]);
@@ -547,12 +568,13 @@ __device__ __forceinline__ void weights(u32x4 (&p)[T][NT / 2], const f32x4 (&s)[
       mx = fmaxf(fmaxf(mx, s[t][x][2]), s[t][x][3]);
     }
     top[x] = mx;
-    over |= mx * c2 > st.m[x] + kSlack;
+    over |= mx * c2 > st.m[x] + st.slack;
   }
   if (__builtin_amdgcn_ballot_w64(over)) {
+    if (__builtin_amdgcn_ballot_w64(large)) raise_reference(st);
 #pragma unroll
     for (int x = 0; x < T; ++x) {
-      const float m = fmaxf(st.m[x], quarters_max(top[x]) * c2);
+      const float m = fmaxf(st.m[x], quarters_max(top[x]) * c2 + (kSlack - st.slack));
       const float f = exp2_fast(st.m[x] - m);
       st.m[x] = m;
       st.l[x] *= f;
@@ -609,12 +631,7 @@ __device__ __forceinline__ void add_values(State<T>& st, const u32x4 (&p)[T][1],
 // 0, 4, 8, 12 of the row of 16 lanes that has the key.) Rows past the last key hold anything, scales that no cache
 // has among it, whose values are infinite: this is also what keeps them out.
 template <int T, int HEADS>
-__device__ __forceinline__ void nan_values(State<T>& st, Vals& v, const int (&rel)[T], int lane) {
-  uint32_t most = 0;
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) most = max(most, v.s[t][i]);
+__device__ __forceinline__ void nan_values(State<T>& st, Vals& v, uint32_t most, const int (&rel)[T], int lane) {
   if (!__builtin_amdgcn_ballot_w64(most > kFp4MaxScale)) return;
 #pragma unroll
   for (int t = 0; t < 2; ++t)
@@ -663,9 +680,14 @@ __device__ __forceinline__ void take(State<T>& st, const lds_u8* stage, const La
         for (int i = 0; i < 4; ++i)
           if (16 * t + row_of<HEADS>(4 * (lane >> 4) + i) > rel[x]) s[t][x][i] = -INFINITY;
   }
+  uint32_t most = 0;  // the largest scale byte of V's
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = max(most, v.s[t][i]);
   u32x4 p[T][1];
-  weights<T, 2>(p, s, st, c2);
-  if (masked) nan_values<T, HEADS>(st, v, rel, lane);
+  weights<T, 2>(p, s, st, most >= kLargeScale, c2);
+  if (masked) nan_values<T, HEADS>(st, v, most, rel, lane);
   __builtin_amdgcn_s_setprio(1);
   add_values<T>(st, p, v);
   __builtin_amdgcn_s_setprio(0);
@@ -891,6 +913,7 @@ __device__ __forceinline__ void attend_few(const Fp4AttnArgs& a, const Partials&
     State<1> st;
     st.m[0] = kLowest;
     st.l[0] = 0.f;
+    st.slack = kSlack;
 #pragma unroll
     for (int j = 0; j < 8; ++j) st.acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (s1 - s0 >= kFewRing - 1)
@@ -1032,10 +1055,9 @@ __device__ __forceinline__ void convert_rows(const lds_u8* raw, lds_u8* tiles, i
 }
 
 // acc[x][j][i]: dimension 16 j + 4 (l / 16) + i. A column that sees a row of the step with NaN blocks of V gets NaN in
-// their dimensions. rel: the last row that a column sees.
+// their dimensions. s: the lane's row's scale bytes of V, rel: the last row that a column sees.
 template <int T>
-__device__ __forceinline__ void many_nan(State<T>& st, const lds_u8* raw, const int (&rel)[T], int rows, int lane) {
-  const uint32_t s = *(const lds_u32*)(raw + ManyLds::kRawCache + ManyLds::kRawValues + 4 * lane);
+__device__ __forceinline__ void many_nan(State<T>& st, uint32_t s, const int (&rel)[T], int rows, int lane) {
   uint32_t bad = 0;
 #pragma unroll
   for (int b = 0; b < 4; ++b) bad |= (uint32_t)((s >> 8 * b & 0xff) > kFp4MaxScale) << b;
@@ -1053,13 +1075,14 @@ __device__ __forceinline__ void many_nan(State<T>& st, const lds_u8* raw, const 
 }
 
 // The 64 keys of a pair of tiles. k, v: the lane's places in them, for every chunk of K and every 16 dimensions of V.
+// large: the lane's row has a scale byte of V from kLargeScale on.
 // The reads are kept ahead of the products that use them (the compiler's own order reads each operand right before
 // its product and waits for it.) A wavefront goes first while it has products: otherwise the two on a SIMD fall into step
 // in some builds, and wait for the same units (16 chunks: 770 to 785 us in place of 748, with 3, 4, 5, 6 or 8 reads
 // of K ahead, whichever way the registers came to lie; with the priorities 751 and 746 for 3 and 4).
 template <int T>
 __device__ __forceinline__ void many_take(State<T>& st, const lds_u8* tiles, const int (&k)[4], const int (&v)[8],
-                                          bool masked, const int (&rel)[T], float c2, int lane) {
+                                          bool large, bool masked, const int (&rel)[T], float c2, int lane) {
   constexpr int kTile16 = 16 * ManyLds::kRow;
   constexpr int kAheadK = 4, kAheadV = 1;
   f32x4 s[4][T];
@@ -1100,7 +1123,7 @@ __device__ __forceinline__ void many_take(State<T>& st, const lds_u8* tiles, con
   }
   __builtin_amdgcn_s_setprio(0);
   u32x4 p[T][2];
-  weights<T, 4>(p, s, st, c2);
+  weights<T, 4>(p, s, st, large, c2);
   __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -1136,6 +1159,7 @@ __device__ __forceinline__ void attend_many(const Fp4AttnArgs& a, const Partials
     Columns<T> cols;
     cols.init(a, seq, run.row0, head, wave * T * 16, true, n);
     State<T> st;
+    st.slack = kSlack;
 #pragma unroll
     for (int x = 0; x < T; ++x) {
       const uint16_t* q = a.q + (int64_t)(seq.q0 + cols.row[x]) * a.q_stride + cols.head[x] * D + 8 * g;
@@ -1180,8 +1204,10 @@ __device__ __forceinline__ void attend_many(const Fp4AttnArgs& a, const Partials
         int rel[T];
 #pragma unroll
         for (int x = 0; x < T; ++x) rel[x] = cols.last[x] - t0;
-        many_take(st, tiles, k_at, v_at, t0 + kManyStep - 1 > cols.lowest, rel, a.scale_log2, lane);
-        many_nan(st, lds + (i & 3) * S::kRaw, rel, seq.keys - t0, lane);
+        const uint32_t scales = *(const lds_u32*)(lds + (i & 3) * S::kRaw + S::kRawCache + S::kRawValues + 4 * lane);
+        const bool large = (scales & scales << 1 & 0x80808080u) != 0;  // (kLargeScale; NaN blocks are among them)
+        many_take(st, tiles, k_at, v_at, large, t0 + kManyStep - 1 > cols.lowest, rel, a.scale_log2, lane);
+        if (__builtin_amdgcn_ballot_w64(large)) many_nan(st, scales, rel, seq.keys - t0, lane);
       }
       if (s + 1 < s1) convert_rows(lds + ((i + 1) & 3) * S::kRaw, lds + S::kTiles + ((i + 1) & 1) * 2 * S::kTile, threadIdx.x);
       good >>= 1;
