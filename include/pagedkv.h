@@ -612,7 +612,10 @@ int pk_compact_blocks(void* k_caches, void* v_caches, int64_t k_layer_stride, in
  *   a row's largest are lost, below 2^-94 where the sequence has scale bytes of V from 192 (2^65) on. Scores are
  *   fp32: a row with one past its range is NaN, unless that is -infinity, which weighs nothing. NaN blocks reach the
  *   rows that see them and no others. A row's result depends on the call's other sequences by the rounding of its partial sums; equal
- *   calls give equal bits. At most 2^31 steps of 64 keys over the call's bounds.
+ *   calls give equal bits. By the call's bounds there have to be fewer than 2^31 steps: num_seqs
+ *   ceil(max_seqlen_k / keys), keys = 256 / the kv heads that a work-group takes (the largest divisor of
+ *   num_kv_heads up to 8, rounded up to 1, 2, 4 or 8); and where a sequence may have more than 16 columns, rows x
+ *   num_heads / num_kv_heads, (num_rows num_heads / num_kv_heads / 256 + num_seqs) ceil(max_seqlen_k / 64).
  *   workspace: pk_varlen_attention_fp4_workspace_bytes, 256-byte aligned (at most 520 bytes for 512
  *   num_kv_heads min(16, max_seqlen_q num_heads / num_kv_heads) partial results, 4.3 MB for single rows of 16
  *   heads on 8, and 68 MB more where a sequence may have more columns than 16); calls that may overlap

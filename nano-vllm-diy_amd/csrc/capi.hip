@@ -1032,7 +1032,7 @@ int fp4_heads(const char* what, int32_t num_kv_heads, int32_t head_dim) {
   return PK_OK;
 }
 
-// Head rows are counted 16 to a work-group of 256 threads, in 32 bits.
+// Tokens and head rows of a call are counted in 32 bits, up to 8 wavefronts to a token.
 int fp4_tokens(const char* what, int64_t tokens, int64_t head_rows) {
   if (tokens < 0) return fail(PK_ERR_INVALID_ARG, "%s: %lld tokens", what, (long long)tokens);
   if (tokens * head_rows >= (1ll << 27))
@@ -1237,9 +1237,9 @@ int pk_varlen_attention_fp4(const void* q, int64_t q_row_stride, const void* k_c
     return fail(PK_ERR_INVALID_ARG, "%s: softmax_scale must be positive and finite", what);
   const pk::Fp4AttnPlan p =
       pk::fp4_attention_plan(num_seqs, num_heads, num_kv_heads, max_seqlen_q, max_seqlen_k, num_rows);
-  if (p.too_long)
-    return fail(PK_ERR_UNSUPPORTED, "%s: %d sequences of up to %d keys, %lld rows: more than 2^31 steps of 64 keys", what,
-                num_seqs, max_seqlen_k, (long long)num_rows);
+  if (p.steps > INT32_MAX)  // (a line of them is counted in 32 bits)
+    return fail(PK_ERR_UNSUPPORTED, "%s: %d sequences of up to %d keys, %lld rows: up to %lld steps of %d keys (below 2^31)",
+                what, num_seqs, max_seqlen_k, (long long)num_rows, (long long)p.steps, p.step_keys);
   const size_t need = p.few_bytes + p.many_bytes;
   if (!workspace || workspace_bytes < need)
     return fail(PK_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, need,

@@ -148,7 +148,8 @@ struct Fp4AttnPlan {
   int32_t many_runs;             // work-groups over the sequences of more rows, 0: there can be none
   int64_t many_tiles;            // about as many tiles of rows (of all kv heads) as they have
   size_t few_bytes, many_bytes;  // partial results
-  bool too_long;                 // the steps of a kv head may not fit 31 bits
+  int64_t steps;                 // of a line at most, by the call's bounds: those of the sequences of few rows, or of
+  int32_t step_keys;             // more rows on one kv head, whichever are more; keys of one of them
 };
 Fp4AttnPlan fp4_attention_plan(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t max_seqlen_q,
                                int32_t max_seqlen_k, int64_t num_rows);

@@ -1398,7 +1398,8 @@ Fp4AttnPlan fp4_attention_plan(int32_t num_seqs, int32_t num_heads, int32_t num_
   p.few_slots = 1;
   while (p.few_slots < p.few_heads) p.few_slots *= 2;
   const int64_t few_steps = ((int64_t)max_seqlen_k * p.few_slots + kSub * kFewWaves - 1) / (kSub * kFewWaves);
-  p.too_long = num_seqs * few_steps > INT32_MAX;
+  p.steps = num_seqs * few_steps;
+  p.step_keys = kSub * kFewWaves / p.few_slots;
   p.few_cols = (int)std::min<int64_t>(16, (int64_t)max_seqlen_q * group);
   // a run to a compute unit, whose LDS a work-group fills (64, 128 and 512 runs: 708, 370 and 224 us in place of 215 for
   // 256 sequences of 1k-8k keys, 16, 14 and 15 in place of 11 for 8 of 256-2048)
@@ -1407,7 +1408,10 @@ Fp4AttnPlan fp4_attention_plan(int32_t num_seqs, int32_t num_heads, int32_t num_
   if ((int64_t)max_seqlen_q * group > 16) {
     const int64_t steps = ((int64_t)max_seqlen_k + kManyStep - 1) / kManyStep;
     const int64_t tiles = num_rows * group / kManyCols + num_seqs;  // of a kv head
-    p.too_long |= tiles * steps > INT32_MAX;
+    if (tiles * steps > p.steps) {
+      p.steps = tiles * steps;
+      p.step_keys = kManyStep;
+    }
     p.many_tiles = std::max<int64_t>(1, num_rows * group / kManyCols) * num_kv_heads;
     p.many_runs = 256;
     p.many_bytes = partial_bytes(partial_rows<true>(p, num_kv_heads), p.many_runs);

@@ -4,7 +4,8 @@ import torch
 
 import fp4_oracle as ref
 import pagedkv
-from pagedkv import fp4
+from pagedkv import _lib, fp4
+from test_fp4_host import SPACE, UNSUPPORTED, _call
 
 KV, HEADS, BS, NB = 8, 16, 64, 4
 
@@ -48,3 +49,31 @@ def test_row_strides_of_tables(handed, op, what, at):
         assert handed[what][at - 1] == table.data_ptr() and handed[what][at] == stride
     op(torch.zeros(1, 3, dtype=torch.int32).expand(4, 3), num_seqs=1)  # one sequence steps nowhere
     assert handed[what][at] == 3
+
+
+@pytest.mark.parametrize("heads,kv,slots", [(16, 8, 8), (8, 4, 4), (3, 3, 4), (2, 2, 2), (4, 1, 1), (22, 11, 1), (24, 12, 8)])
+def test_most_steps_of_single_rows(heads, kv, slots):
+    """The largest max_seqlen_k for 65535 sequences passes the check of the steps, one step more does not, and the
+    message has the numbers."""
+    step = 256 // slots
+    most = min((2 ** 31 - 1) // 65535 * step, 65535 * 64)
+    row = ref.row_bytes(kv)
+    kw = dict(num_seqs=65535, rows=65535, heads=heads, kv=kv, q_stride=128 * heads, out_stride=128 * heads, k_block=64 * row,
+              v_block=64 * row, table_stride=65535, ws_bytes=0)
+    assert _call("pk_varlen_attention_fp4", **kw, max_k=most) == SPACE, _lib.lib().pk_last_error()
+    if most < 65535 * 64:
+        assert _call("pk_varlen_attention_fp4", **kw, max_k=most + 1) == UNSUPPORTED
+        count = 65535 * (most // step + 1)
+        assert count >= 2 ** 31 and f"{count} steps of {step} keys".encode() in _lib.lib().pk_last_error()
+
+
+@pytest.mark.parametrize("group", [2, 8])
+def test_most_steps_of_more_rows(group):
+    """Steps of 64 keys of one kv head: tiles of 256 columns, and one more for every sequence."""
+    kw = dict(num_seqs=100, max_q=1 << 21, heads=group, kv=1, q_stride=128 * group, out_stride=128 * group, k_block=64 * 80,
+              v_block=64 * 80, table_stride=65535, max_k=65535 * 64, ws_bytes=0)
+    tiles = (2 ** 31 - 1) // 65535
+    rows = (tiles - 100 + 1) * 256 // group - 1
+    assert _call("pk_varlen_attention_fp4", **kw, rows=rows) == SPACE, _lib.lib().pk_last_error()
+    assert _call("pk_varlen_attention_fp4", **kw, rows=rows + 1) == UNSUPPORTED
+    assert f"{(tiles + 1) * 65535} steps of 64 keys".encode() in _lib.lib().pk_last_error()
