@@ -606,7 +606,8 @@ int pk_compact_blocks(void* k_caches, void* v_caches, int64_t k_layer_stride, in
  *   of a table entry that is no block are seen by no row. Sequences without rows or keys are passed over, rows
  *   past max_seqlen_q not written, keys past max_seqlen_k ignored; a row that sees no key (or none with a
  *   score above -infinity) is written as 0.
- *   num_rows: the rows of q and out; a sequence's rows past them are neither read nor written. q's row stride below 2^25. block_size a multiple
+ *   num_rows: the rows of q and out; a sequence's rows past them are neither read nor written, and if the
+ *   lengths overlap and add up to 2^31 steps (below) or more, no row is. q's row stride below 2^25. block_size a multiple
  *   of 64, GQA groups of 1, 2, 4 or 8. Softmax, sums and partial results are fp32, the
  *   weights rounded to bf16 for the product with V. V may have any values of the format; weights below 2^-126 of
  *   a row's largest are lost, below 2^-94 where the sequence has scale bytes of V from 192 (2^65) on. Scores are

@@ -97,16 +97,20 @@ __device__ __forceinline__ int scalar_i32(const int32_t* p) {
   return uniform(*(constant)reinterpret_cast<uintptr_t>(p));
 }
 
+// a + b of counts, at most INT32_MAX: lengths that are no cumulative ones may add up to more steps than a call can
+// have, which must not come back as few.
+__device__ __forceinline__ int add_sat(int a, int b) { return __builtin_elementwise_add_sat(a, b); }
+
 // Inclusive sum over the wavefront.
 __device__ __forceinline__ int scan64(int v, int lane) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1, :2, :4, :8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v = add_sat(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));  // row_shr:1, :2, :4, :8
+  v = add_sat(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+  v = add_sat(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+  v = add_sat(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
   const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = __builtin_amdgcn_readlane(v, 31),
             r2 = __builtin_amdgcn_readlane(v, 47);
   const int row = lane >> 4;
-  return v + (row >= 1 ? r0 : 0) + (row >= 2 ? r1 : 0) + (row >= 3 ? r2 : 0);
+  return add_sat(add_sat(add_sat(v, row >= 1 ? r0 : 0), row >= 2 ? r1 : 0), row >= 3 ? r2 : 0);
 }
 
 // A sequence of the call: its first query row, the rows that are computed, and the keys. causal rows are aligned by
@@ -205,11 +209,12 @@ struct Line {
   __device__ __forceinline__ void init(const Fp4AttnArgs& a, lds_u8* lds, int wave, int lane) {
     seqs = (lds_i32x4*)lds;
     sums = (lds_i32*)(lds + kChunk * 16);
-    per_head = 0;
+    int64_t sum = 0;
     for (int first = 0; first < a.num_seqs; first += kChunk) {
-      load(a, first, per_head, wave, lane);
-      per_head += __builtin_amdgcn_readlane(group_ends(lane), kWave - 1);
+      load(a, first, (int)sum, wave, lane);
+      sum = min(sum + __builtin_amdgcn_readlane(group_ends(lane), kWave - 1), (int64_t)INT32_MAX);
     }
+    per_head = sum < INT32_MAX ? (int)sum : 0;  // (the call's bounds allow fewer steps: there is no work in such lengths)
     total = MANY ? (int64_t)per_head * a.num_kv_heads : per_head;
   }
   // The tile at position p < total. (Positions that grow walk the chunks once.)

@@ -84,3 +84,23 @@ def test_what_is_not_large_keeps_its_bits(gpu):
     same = torch.ones(c["q"].shape[:2], dtype=torch.bool, device=gpu)
     same[0, 2:4] = same[2:62, 2:4] = False
     assert torch.equal(got[same], want[same])
+
+
+def test_lengths_that_overlap_have_no_more_steps_than_a_call(gpu):
+    """Lengths that fall and rise again, so that 656 sequences have the same 6400 rows: their 2^32 + 4194304 steps
+    are no small number of steps (2^32 is 0 in 32 bits), and nothing is computed. Without a block no key is read."""
+    n, heads, pairs, keys = 6400, 8, 656, 1 << 21
+    assert pairs * (n * heads // 256) * (keys // 64) == 2 ** 32 + 4194304
+    cache = torch.zeros(1, keys, 80, dtype=torch.uint8, device=gpu)  # one page holds all keys
+    q = torch.zeros(n, heads, D, dtype=torch.bfloat16, device=gpu)
+    out = torch.full_like(q, 7.0)
+    cu_q = torch.tensor([0, n] * pairs + [0], dtype=torch.int32, device=gpu)
+    cu_k = torch.tensor([0, keys] * pairs + [0], dtype=torch.int32, device=gpu)
+    table = torch.full((2 * pairs, 1), -1, dtype=torch.int32, device=gpu)
+    pagedkv.varlen_attention_fp4(q, cache, cache, cu_q, cu_k, n, keys, table, causal=False, out=out)
+    torch.cuda.synchronize()
+    assert (out == 7).all()
+    # one of them alone: its rows see no key
+    pagedkv.varlen_attention_fp4(q[:64], cache, cache, cu_q[:2].clamp(max=64), cu_k[:2].clamp(max=640), 64, keys, table[:1],
+                                 causal=False, out=out[:64])
+    assert (out[:64] == 0).all() and (out[64:] == 7).all()
