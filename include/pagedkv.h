@@ -585,7 +585,8 @@ int pk_compact_blocks(void* k_caches, void* v_caches, int64_t k_layer_stride, in
  * of two s with a <= 7 s, within 2^-126 .. 2^125; values are divided by it and rounded to nearest, ties to
  * even, at most 6. An infinity or NaN among the 32 makes all of them NaN (scale byte 255; 0, 253 and 254 are
  * not written, and a cache of other origin must not hold them). Every value is
- * exact in bf16. A finite value is off by at most a / 5.
+ * exact in bf16. A finite value is off by at most a / 5, or by 2^-128 where that is more (below 2^-128 nothing is
+ * left); where a is above 7 x 2^125 the largest value, 6 x 2^125, is off by up to a / 4.
  * To the page operators (pk_copy_blocks and those after it) such a cache is one of row_elems =
  * pk_fp4_row_bytes / 2 16-bit elements where that is a multiple of 8, which it always is.
  *

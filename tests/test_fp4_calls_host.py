@@ -77,3 +77,18 @@ def test_most_steps_of_more_rows(group):
     assert _call("pk_varlen_attention_fp4", **kw, rows=rows) == SPACE, _lib.lib().pk_last_error()
     assert _call("pk_varlen_attention_fp4", **kw, rows=rows + 1) == UNSUPPORTED
     assert f"{(tiles + 1) * 65535} steps of 64 keys".encode() in _lib.lib().pk_last_error()
+
+
+def test_how_far_a_stored_value_is_off():
+    """Every finite bf16 value as the largest of its 32, beside values between it and 0: at most a fifth of it, or 2^-128
+    where the scale can get no smaller; a quarter where the scale can get no larger. Both ends reach beyond a fifth."""
+    every = torch.arange(1, 0x7f80, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    x = (every.double().unsqueeze(1) * torch.linspace(1, -1, 128, dtype=torch.float64)).to(torch.bfloat16)
+    # (the four blocks of a row have different largest values)
+    off = (ref.values(ref.pack(x.unsqueeze(1)), 1).squeeze(1) - x.double()).abs().view(-1, 4, 32)
+    top = x.double().abs().view(-1, 4, 32).amax(-1, keepdim=True)
+    end = top > 7 * 2.0 ** 125
+    assert (off <= torch.where(end, top / 4, torch.maximum(top / 5, torch.tensor(2.0 ** -128, dtype=torch.float64)))).all()
+    assert (off[end.expand_as(off)] > 0.24 * top.expand_as(off)[end.expand_as(off)]).any()
+    small = top < 2.0 ** -128
+    assert (off == x.double().abs().view(-1, 4, 32))[small.expand_as(off)].all() and small.any()
