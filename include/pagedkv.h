@@ -598,7 +598,9 @@ int pk_compact_blocks(void* k_caches, void* v_caches, int64_t k_layer_stride, in
  *   rounded to bf16 and stored, v stored as it is. k_out, v_out (num_tokens, num_kv_heads, head_dim), NULL:
  *   none: the values that the stored rows hold, of every token (slot or none), so a fresh prompt's attention
  *   sees what later steps read. The norm's root is taken in 64 bits and no products are fused, so a key's
- *   4-bit values follow from the formula alone. A row whose squares sum to no finite number is NaN.
+ *   4-bit values follow from the formula alone. A normalised row with a NaN is NaN; one with an infinity, whose
+ *   root is infinite, is NaN in the dimensions of its infinities and those that they are rotated with, and 0 in
+ *   the others. (An infinity is none of the numbers that a 4-bit value may be: its 32 are NaN, above.)
  * pk_gather_kv_fp4 -- pk_gather_kv of such a cache: the values of every sequence's rows in bf16, (sum Lk,
  *   num_kv_heads, head_dim). Sequence b's rows begin at cu_seqlens_k[b]; its rows at and past max_seqlen_k, and
  *   rows past dst's num_rows, are not written. Rows of table entries that are no block are 0.
