@@ -75,13 +75,13 @@ def _slot_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, device: torch.dev
 def _rows(name: str, t: torch.Tensor, n: int, heads: int, device: torch.device) -> int:
     """Row stride of a (n, heads, 128) bf16 tensor with contiguous heads."""
     stride = t.stride()
-    if t.dtype is not _BF16 or t.shape != (n, heads, HEAD_DIM) or stride[2] != 1 or stride[1] != HEAD_DIM:
+    if t.dtype is not _BF16 or t.shape != (n, heads, HEAD_DIM) or stride[2] != 1 or (heads > 1 and stride[1] != HEAD_DIM):
         raise ValueError(f"{name} must be a ({n}, {heads}, {HEAD_DIM}) bf16 tensor with contiguous heads, got "
                          f"{tuple(t.shape)} {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
-    # (a single row has no stride of its own)
-    return stride[0] if n > 1 else max(stride[0], heads * HEAD_DIM)
+    # (neither a single row nor a single head has a stride of its own)
+    return stride[0] if n > 1 else heads * HEAD_DIM
 
 
 def _i32(name: str, t: torch.Tensor, n: int, device: torch.device) -> int:

@@ -92,3 +92,23 @@ def test_how_far_a_stored_value_is_off():
     assert (off[end.expand_as(off)] > 0.24 * top.expand_as(off)[end.expand_as(off)]).any()
     small = top < 2.0 ** -128
     assert (off == x.double().abs().view(-1, 4, 32))[small.expand_as(off)].all() and small.any()
+
+
+@pytest.mark.parametrize("n,kv", [(1, 2), (3, 1), (1, 1)])
+def test_strides_of_single_rows_and_heads_do_not_count(handed, n, kv):
+    """A dimension of size one may have any stride: rows are taken that only differ in it."""
+    row = kv * 128
+    caches = [torch.zeros(NB, BS, ref.row_bytes(kv), dtype=torch.uint8) for _ in range(2)]
+    slots = torch.zeros(n, dtype=torch.int32)
+    shape, stride = (n, kv, 128), (row + 132 if n == 1 else 2 * row, 300 if kv == 1 else 128, 1)
+    rows = torch.zeros(4096, dtype=torch.bfloat16).as_strided(shape, stride)
+    assert rows.stride() == stride
+    pagedkv.store_kvcache_fp4(rows, rows, *caches, slots)
+    assert handed["pk_store_kvcache_fp4"][1] == handed["pk_store_kvcache_fp4"][3] == (row if n == 1 else 2 * row)
+    q = torch.zeros(1 << 26, dtype=torch.bfloat16).as_strided((n, kv, 128), (1 << 25 if n == 1 else 2 * row, stride[1], 1))
+    cu = torch.arange(n + 1, dtype=torch.int32)
+    pagedkv.varlen_attention_fp4(q, *caches, cu, cu, 1, 10, torch.zeros(n, 1, dtype=torch.int32))
+    assert handed["pk_varlen_attention_fp4"][1] == (row if n == 1 else 2 * row)
+    if kv > 1:
+        with pytest.raises(ValueError, match="contiguous heads"):
+            pagedkv.store_kvcache_fp4(rows.as_strided(shape, (row, 136, 1)), rows, *caches, slots)
