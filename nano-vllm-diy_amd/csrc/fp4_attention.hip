@@ -35,7 +35,6 @@
 // so there are at most two partial results a run. The lengths are on the GPU only, so a launch has work-groups of both
 // kinds wherever the call's bounds allow sequences of more than 16 columns; those without any end at once.
 #include <algorithm>
-#include <type_traits>
 
 #include "fp4.h"
 
@@ -868,9 +867,9 @@ struct Columns {
 };
 
 // Few rows: HEADS slots of kv heads from head0 on, of which `heads` are heads, and 8 / HEADS wavefronts to each, which
-// take 32 keys of every step in turn. Bound by HBM where there is enough to read: 208 to 220 us for 256 sequences of
-// 1k-8k keys of 8 kv heads, 5.6 to 5.9 TB/s; 35 us for 128 of 100-2048 (4 TB/s), 5 of them before the first step is
-// there. Sequences of at most 16 columns, what one tile holds, come here: 48 of 4 to 16 columns and 300-4000 keys of 4 kv
+// take 32 keys of every step in turn. Bound by HBM where there is enough to read: 217 us a call for 256 sequences of
+// 1k-8k keys of 8 kv heads, 5.65 TB/s (the kernel 209 at best, where a stream that is only read reaches 6.34); 34 us for
+// 128 of 100-2048 (4.2 TB/s), 5 of them before the first step is there. Sequences of at most 16 columns, what one tile holds, come here: 48 of 4 to 16 columns and 300-4000 keys of 4 kv
 // heads took 22 us and 6 for the merge; with those of more than 8 columns in the other kernel 15 + 36 + 11, of more
 // than 4 columns 8 + 50 + 12.
 template <int HEADS>
@@ -977,10 +976,10 @@ __device__ __forceinline__ void attend_few(const Fp4AttnArgs& a, const Partials&
 // convert them to bf16 tiles once (16 values of K and of V each), and its 8 wavefronts read these. (With each
 // wavefront converting the rows for its own 32 columns the kernel was bound by its vector instructions, 282 for 32
 // keys and 32 columns, 106 of them conversions.) Step s + 1 is converted after step s's products, in their shadow
-// (before them: 712 us in place of 698 for 16 chunks of 1024 rows behind 4096 keys), steps s + 2 and s + 3 are on their way.
+// (before them 16 chunks of 1024 rows behind 4096 keys took 2% longer), steps s + 2 and s + 3 are on their way.
 //
-// Bound by the vector instructions and the products together: the matrix cores are busy for 42% of a SIMD's time,
-// the vector units for 48%. Two other forms ran within 3% of this one: step s's exponentials between the products of
+// Bound by the vector instructions and the products together: the matrix cores are busy for 43% of a SIMD's time,
+// the vector units for 48%. The 16 chunks take 629 us a call, 985 TFLOP/s. Two other forms ran within 3% of this one: step s's exponentials between the products of
 // step s + 1, and that with four wavefronts of 64 columns, half the reads of LDS.
 //
 // The tiles have 256-byte rows, 16 chunks of 16 bytes. K: chunk c of row r in slot c ^ (r & 15): the 16 lanes of a
@@ -1083,8 +1082,8 @@ __device__ __forceinline__ void many_nan(State<T>& st, uint32_t s, const int (&r
 // large: the lane's row has a scale byte of V from kLargeScale on.
 // The reads are kept ahead of the products that use them (the compiler's own order reads each operand right before
 // its product and waits for it.) A wavefront goes first while it has products: otherwise the two on a SIMD fall into step
-// in some builds, and wait for the same units (16 chunks: 770 to 785 us in place of 748, with 3, 4, 5, 6 or 8 reads
-// of K ahead, whichever way the registers came to lie; with the priorities 751 and 746 for 3 and 4).
+// in some builds, and wait for the same units (16 chunks took 3 to 5% longer in those, with 3, 4, 5, 6 or 8 reads of K
+// ahead, whichever way the registers came to lie; with the priorities 3 and 4 of them differ by less than 1%).
 template <int T>
 __device__ __forceinline__ void many_take(State<T>& st, const lds_u8* tiles, const int (&k)[4], const int (&v)[8],
                                           bool large, bool masked, const int (&rel)[T], float c2, int lane) {
@@ -1251,7 +1250,7 @@ __global__ __launch_bounds__(kFewWaves* kWave, 2) void attend_few_kernel(const F
 }
 
 // Both kinds of sequences: the work-groups of one kind begin where those of the other end. (In two launches a mixed step's
-// kernels took 38.3 and 37.4 us in place of 70.4; 16 chunks alone 745 and 4.8 in place of 757.)
+// kernels took 38.3 and 37.4 us in place of 70.4; 16 chunks alone took 1% less.)
 template <int HEADS>
 __global__ __launch_bounds__(kFewWaves* kWave, 2) void attend_mixed_kernel(const Fp4AttnArgs a, const Partials few,
                                                                            const Partials many, int few_runs, int many_runs,
@@ -1292,7 +1291,7 @@ __device__ __forceinline__ void merge(const Fp4AttnArgs& a, const Partials& part
     if (pair < pairs) {
       const auto at = [&](int j) { return part.at(2 * (int64_t)(run + j) + (j == 0 ? 1 : 0), MANY ? 0 : head, col); };
       // four at a time, all of their loads at once: a round trip less than with the maximum found ahead (a mixed step's
-      // 68 MB 14.1 us in place of 17.3, 8 sequences 5.0 in place of 6.0)
+      // 42 MB 14.1 us in place of 17.3, 8 sequences 5.0 in place of 6.0)
       for (int j0 = slice; j0 < pieces; j0 += 4 * slices) {
         float2 ml[4];
         f32x4 o[4];

@@ -43,7 +43,7 @@ __device__ __forceinline__ void put_head(uint8_t* row, int heads, int h, int c, 
 
 // Head rows that a 16-lane row has in flight: a work-group takes 64 head rows at once, whole tokens (`tokens` of them;
 // one token where it has more). One row at a time, with its own division and its slot's load before its own, stored
-// 8191 tokens of 8 kv heads in 14.7 us, this takes 12.2 (8.7 at a large copy's rate).
+// 11406 tokens of 8 kv heads in 14.7 us, this takes 11.8 (12.1 at a large copy's rate).
 constexpr int kRowsAhead = 4;
 constexpr int kRowsAtOnce = kRowsPerGroup * kRowsAhead;
 inline int tokens_at_once(int rows) { return rows < kRowsAtOnce ? kRowsAtOnce / rows : 1; }
@@ -191,7 +191,8 @@ __global__ __launch_bounds__(kRowThreads) void append_fp4_kernel(const Fp4Append
 }
 
 // Sequence blockIdx.y's rows through its table, `tokens` keys at once as store_fp4_kernel takes tokens (one head row at
-// a time: 9.3 us for 8191 keys of 8 kv heads; this: 8.4).
+// a time: 9.3 us for 11406 keys of 8 kv heads in five sequences, this: 8.4 to 8.7; 6.0 at a large copy's rate. What is over
+// is the start of the launch and the chain of lengths, table entry and row.)
 __global__ __launch_bounds__(kRowThreads) void gather_fp4_kernel(const Fp4GatherArgs a, int tokens) {
   const int b = blockIdx.y;
   const int c = threadIdx.x & 15;
