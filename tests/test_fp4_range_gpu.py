@@ -22,10 +22,12 @@ def _raise_v(c, heads, by, rows=None):
 def _check(c, got, scale=D ** -0.5):
     """As test_fp4_attention_gpu's, with what the larger reference costs: weights and sums are held relative to a
     largest weight of at least 2^-32, so what vanishes below fp32's smallest normal value, 2^-126, is up to 2^-94 of
-    max |v| a key."""
+    max |v| a key. And with the weights' rounding in the sum below: p (1 + d), |d| <= 2^-8, moves o = sum p v / sum p by
+    sum d p (v - o) / sum p, at most 2^-8 (A + |o|). One key's V far above the others' comes near to that: of two keys
+    with weights w and 1 - w and V only at the first, 2^-7 |o| (1 - w)."""
     want, bound = ref.attention(c["q"], c["kc"], c["vc"], c["tables"], c["q_lens"], c["k_lens"], scale)
     top = ref.values(c["vc"], c["vc"].shape[-1] // 68).abs().amax()
-    bound = bound + 2.0 ** -94 * max(c["k_lens"]) * top
+    bound = bound + 2.0 ** -94 * max(c["k_lens"]) * top + 2.0 ** -8 * want.abs()
     over = (got.double() - want).abs() - bound
     assert torch.isfinite(got).all()
     assert over.max().item() <= 0, f"over the bound by {over.max().item():.3e} at {int(over.argmax())}"
@@ -104,3 +106,14 @@ def test_lengths_that_overlap_have_no_more_steps_than_a_call(gpu):
     pagedkv.varlen_attention_fp4(q[:64], cache, cache, cu_q[:2].clamp(max=64), cu_k[:2].clamp(max=640), 64, keys, table[:1],
                                  causal=False, out=out[:64])
     assert (out[:64] == 0).all() and (out[64:] == 7).all()
+
+
+def test_two_keys_of_which_one_has_all_the_value(gpu):
+    """V of one of two keys is 0: the roundings of both weights move what is left of the other."""
+    n = 512
+    c = _case(gpu, 16, 8, [(1, 2)] * n, seed=8)
+    kv = 8
+    for i in range(n):
+        c["vc"][int(c["tables"][i, 0]), 0, :64 * kv] = 0
+    _raise_v(c, range(4), 126)
+    _check(c, _run(c))
