@@ -610,14 +610,14 @@ int pk_compact_blocks(void* k_caches, void* v_caches, int64_t k_layer_stride, in
  *   past max_seqlen_q not written, keys past max_seqlen_k ignored; a row that sees no key (or none with a
  *   score above -infinity) is written as 0.
  *   num_rows: the rows of q and out; a sequence's rows past them are neither read nor written, and if the
- *   lengths overlap and add up to 2^31 steps (below) or more, no row is. q's row stride below 2^25. block_size a multiple
- *   of 64, GQA groups of 1, 2, 4 or 8. Softmax, sums and partial results are fp32, the
- *   weights rounded to bf16 for the product with V. V may have any values of the format; weights below 2^-126 of
- *   a row's largest are lost, below 2^-94 where the sequence has scale bytes of V from 192 (2^65) on. Scores are
- *   fp32: a row with one past its range is NaN, unless that is -infinity, which weighs nothing. NaN blocks reach the
- *   rows that see them and no others. A row's result depends on the call's other sequences by the rounding of its partial sums; equal
- *   calls give equal bits. By the call's bounds there have to be fewer than 2^31 steps: num_seqs
- *   ceil(max_seqlen_k / keys), keys = 256 / the kv heads that a work-group takes (the largest divisor of
+ *   lengths overlap and add up to 2^31 steps (below) or more, no row is. q's row stride below 2^25. block_size
+ *   a multiple of 64, GQA groups of 1, 2, 4 or 8. Softmax, sums and partial results are fp32, the weights
+ *   rounded to bf16 for the product with V. V may have any values of the format; weights below 2^-126 of a
+ *   row's largest are lost, below 2^-94 where the sequence has scale bytes of V from 192 (2^65) on. Scores are
+ *   fp32: a row with one past its range is NaN, unless that is -infinity, which weighs nothing. NaN blocks
+ *   reach the rows that see them and no others. A row's result depends on the call's other sequences by the
+ *   rounding of its partial sums; equal calls give equal bits. By the call's bounds there have to be fewer than
+ *   2^31 steps: num_seqs ceil(max_seqlen_k / keys), keys = 256 / the kv heads that a work-group takes (the largest divisor of
  *   num_kv_heads up to 8, rounded up to 1, 2, 4 or 8); and where a sequence may have more than 16 columns, rows x
  *   num_heads / num_kv_heads, (num_rows num_heads / num_kv_heads / 256 + num_seqs) ceil(max_seqlen_k / 64).
  *   workspace: pk_varlen_attention_fp4_workspace_bytes, 256-byte aligned (at most 520 bytes for 512

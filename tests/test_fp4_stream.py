@@ -80,7 +80,7 @@ def test_loads_to_lds(kernels, wanted, count):  # noqa: F811
 LOAD = "s_mov_b32 m0, s9\ns_nop 0\nglobal_load_lds_dword v1, s[2:3]\n"
 
 
-def test_checker_sees_planted_m0_uses():
+def test_planted_m0_uses_are_found():
     assert not check_m0(_code(LOAD + "s_endpgm"))
     assert check_m0(_code(LOAD + "s_mov_b32 s4, m0\ns_endpgm"))
     assert check_m0(_code("global_load_lds_dwordx4 v1, s[2:3]\ns_endpgm"))
@@ -98,5 +98,5 @@ def test_checker_sees_planted_m0_uses():
     ("s_nop 0\n" + LOAD + "v_readlane_b32 s2, v5, 1\ns_nop 1\ns_cbranch_scc1 1 -> 1\n", 0),
     # not past an end
     ("v_readlane_b32 s2, v5, 1\ns_branch 5 -> 5\n" + LOAD + "s_endpgm\n", 0)])
-def test_checker_sees_planted_bases(text, bad):
+def test_planted_bases_are_found(text, bad):
     assert len(check_bases(_code(text + "s_endpgm"))) == bad
